@@ -10,7 +10,10 @@ for the token loop:
   ``FlowLM.load_voice`` — Model.LoadVoice (pockettts/voice.go:26-63);
 * ``Streams`` — speakChunk's per-frame loop (pockettts/speak.go:146-175)
   for a batch of independent streams;
-* ``GGUF`` — the internal/gguf reader.
+* ``GGUF`` — the internal/gguf reader;
+* ``KV8`` — the 8-bit paged key/value cache (grx_kv8), on caller-owned
+  device memory: append, attend, read;
+* ``logprobs`` — log probabilities of given tokens, entropy, alternatives.
 
 There is no CPU fallback: importing works without a GPU, but every call
 that computes needs libgrx.so and a CUDA device and raises otherwise.
@@ -57,6 +60,11 @@ def _sig(lib):
         "grx_weight_free": (None, [P]),
         "grx_linear": (I, [P, P, I, P, P]),
         "grx_linear_q8_static": (I, [P, P, I, P, P, P]),
+        "grx_kv8_append": (I, [P, P, I, P, L, L, P, L, L, P]),
+        "grx_kv8_read": (I, [P, P, I, P, L, L, P, L, L, P]),
+        "grx_kv8_attend": (I, [P, P, I, I, P, L, L, C.c_float, I, P, L, L, P, P]),
+        "grx_kv8_check": (I, [P, P, I]),
+        "grx_logprobs": (I, [I, I, P, I, I, L, P, I, P, P, P, P, P]),
         "grx_flowlm_load": (I, [P, S, I, PP]),
         "grx_flowlm_free": (None, [P]),
         "grx_flowlm_dims": (I, [P] + [C.POINTER(C.c_int)] * 8),
@@ -282,6 +290,112 @@ def linear_q8_static(w: Weight, d_x: int, m: int, d_bias: int | None, d_dst: int
     activations go to one fixed array shared by every call on the device:
     calls that may overlap on the GPU must be ordered by the caller."""
     _check(lib().grx_linear_q8_static(w._h, d_x, m, d_bias, d_dst, stream or None))
+
+
+# ------------------------------------------------ 8-bit paged KV cache
+
+TYPES = {"f32": 0, "f16": 1, "bf16": 30}  # GRX_F32, GRX_F16, GRX_BF16
+_ROPE = {"none": 0, "pairs": 1, "halves": 2}
+
+
+class _KV8(C.Structure):  # grx_kv8
+    _fields_ = [("device", C.c_int), ("pages", C.c_int), ("page_tokens", C.c_int), ("kv_heads", C.c_int),
+                ("head_dim", C.c_int), ("k", C.c_void_p), ("v", C.c_void_p), ("scale", C.c_void_p)]
+
+
+class _KV8Seqs(C.Structure):  # grx_kv8_seqs
+    _fields_ = [("n", C.c_int), ("table_width", C.c_int), ("rows", C.c_int), ("max_new", C.c_int),
+                ("max_len", C.c_int), ("table", C.c_void_p), ("len", C.c_void_p), ("row0", C.c_void_p),
+                ("first", C.c_void_p), ("rope", C.c_void_p), ("rope_positions", C.c_int), ("rope_mode", C.c_int),
+                ("status", C.c_void_p)]
+
+
+class KV8Seqs:
+    """The sequences of a call (grx_kv8_seqs), as device addresses: the page
+    table [n][table_width], the lengths d_len [n] (this call's tokens among
+    them), the row numbers d_row0 [n + 1] (None: one row for each sequence).
+    Make it once and use it for every layer of a step, and for every step
+    while the addresses and bounds stay."""
+
+    def __init__(self, n: int, d_table: int, table_width: int, d_len: int, max_len: int, d_row0: int | None = None,
+                 rows: int | None = None, max_new: int = 1, d_first: int | None = None, d_rope: int | None = None,
+                 rope_positions: int = 0, rope: str = "none", d_status: int | None = None):
+        self._s = _KV8Seqs(n, table_width, n if rows is None else rows, max_new, max_len, d_table, d_len, d_row0,
+                           d_first, d_rope, rope_positions, _ROPE[rope], d_status)
+        self._p = C.byref(self._s)
+
+
+class KV8:
+    """An 8-bit paged key/value cache (grx_kv8) in caller-owned device memory
+    (addresses): d_k, d_v [pages][kv_heads][page_tokens][head_dim] int8,
+    d_scale [pages][kv_heads][2] float32. Calls queue work on `stream` and
+    return; strides are (row, head) in elements, None for packed rows."""
+
+    def __init__(self, d_k: int, d_v: int, d_scale: int, pages: int, page_tokens: int, kv_heads: int, head_dim: int,
+                 device: int = 0):
+        self._s = _KV8(device, pages, page_tokens, kv_heads, head_dim, d_k, d_v, d_scale)
+        self._p = C.byref(self._s)
+        self.kv_heads, self.head_dim = kv_heads, head_dim
+        self._packed = (kv_heads * head_dim, head_dim)
+        self._lib = lib()
+
+    def append(self, seqs: KV8Seqs, d_k: int, d_v: int, dtype: str = "f32", k_strides=None, v_strides=None,
+               stream: int = 0) -> None:
+        """grx_kv8_append: the rows' keys (rotated) and values into the cache."""
+        kr, kh = k_strides or self._packed
+        vr, vh = v_strides or self._packed
+        rc = self._lib.grx_kv8_append(self._p, seqs._p, TYPES[dtype], d_k, kr, kh, d_v, vr, vh, stream or None)
+        if rc < 0:
+            _check(rc)
+
+    def read(self, seqs: KV8Seqs, d_k: int | None, d_v: int | None, dtype: str = "f32", k_strides=None,
+             v_strides=None, stream: int = 0) -> None:
+        """grx_kv8_read: the stored values of the rows' tokens."""
+        kr, kh = k_strides or self._packed
+        vr, vh = v_strides or self._packed
+        rc = self._lib.grx_kv8_read(self._p, seqs._p, TYPES[dtype], d_k, kr, kh, d_v, vr, vh, stream or None)
+        if rc < 0:
+            _check(rc)
+
+    def attend(self, seqs: KV8Seqs, heads: int, d_q: int, d_out: int, dtype: str = "f32", scale: float | None = None,
+               window: int = 0, d_lse: int | None = None, q_strides=None, out_strides=None, stream: int = 0) -> None:
+        """grx_kv8_attend: attention of the rows' queries over their
+        sequences; scale defaults to head_dim ** -0.5."""
+        d = self.head_dim
+        qr, qh = q_strides or (heads * d, d)
+        orow, oh = out_strides or (heads * d, d)
+        rc = self._lib.grx_kv8_attend(self._p, seqs._p, TYPES[dtype], heads, d_q, qr, qh,
+                                      d ** -0.5 if scale is None else scale, window, d_out, orow, oh, d_lse,
+                                      stream or None)
+        if rc < 0:
+            _check(rc)
+
+    def check(self, table: np.ndarray, lens, row0=None, rows: int | None = None, max_new: int = 1,
+              rope_positions: int | None = None, writes: bool = False) -> None:
+        """grx_kv8_check on host copies of a call's arrays; raises GrxError
+        with what does not fit."""
+        t = np.ascontiguousarray(table, np.int32)
+        ln = np.ascontiguousarray(lens, np.int32)
+        r0 = None if row0 is None else np.ascontiguousarray(row0, np.int32)
+        n = ln.size
+        if t.ndim != 2 or t.shape[0] != n or (r0 is not None and r0.size != n + 1):
+            raise ValueError(f"check: a table of shape {t.shape} and {n} lengths")
+        s = _KV8Seqs(n, t.shape[1], n if rows is None else rows, max_new, int(ln.max(initial=0)) if n else 0,
+                     t.ctypes.data, ln.ctypes.data, None if r0 is None else r0.ctypes.data, None, None,
+                     rope_positions or 0, 0 if rope_positions is None else 1, None)
+        _check(self._lib.grx_kv8_check(self._p, C.byref(s), int(writes)))
+
+
+def logprobs(d_logits: int, rows: int, vocab: int, dtype: str = "f32", row_stride: int | None = None,
+             d_targets: int | None = None, top: int = 0, d_logprob: int | None = None, d_entropy: int | None = None,
+             d_top_ids: int | None = None, d_top_logprobs: int | None = None, device: int = 0,
+             stream: int = 0) -> None:
+    """grx_logprobs on device addresses: log probabilities of the targets,
+    entropies, and the `top` most likely tokens of each row of logits."""
+    rc = lib().grx_logprobs(device, TYPES[dtype], d_logits, rows, vocab, vocab if row_stride is None else row_stride,
+                            d_targets, top, d_logprob, d_entropy, d_top_ids, d_top_logprobs, stream or None)
+    if rc < 0:
+        _check(rc)
 
 
 class FlowLM:

@@ -5,6 +5,7 @@
 #include <mutex>
 
 #include "gguf.h"
+#include "kv8.h"
 
 namespace grx {
 void q8_kernels_init();
@@ -37,6 +38,7 @@ int device_init(int dev) {
     mimi_kernels_init();
     attn_kernels_init();
     fconf_kernels_init();
+    kv8_kernels_init();
     cudaError_t e = cudaGetLastError();  // attribute calls report here; clear it
     if (e != cudaSuccess) return fail(GRX_ECUDA, std::string("kernel attributes: ") + cudaGetErrorString(e));
     done[size_t(dev)] = true;

@@ -1,0 +1,857 @@
+// The 8-bit paged key/value cache: appending tokens to it (with the position
+// rotation of the keys), reading them back, and attention over it.
+//
+// A page holds the keys and values of `page` tokens for every head,
+// [pages][heads][page][head_dim] bytes each, and two scales per page and
+// head; a byte q stands for q·scale. All three kernels take rows through
+// kv8_span and pages through kv8_page (kv8.h), which bound every access; a
+// sequence or page that does not fit is left out and reported.
+#include <cuda_runtime.h>
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "kv8.h"
+
+namespace grx {
+
+namespace {
+
+constexpr uint32_t FULL = 0xffffffffu;
+constexpr int kRangeError = -5;  // GRX_ERANGE, what the status word gets
+
+enum { ROPE_NONE = 0, ROPE_PAIRS = 1, ROPE_HALVES = 2 };
+
+__device__ __forceinline__ void report(const Kv8Args& a) {
+  if (a.status) *a.status = kRangeError;
+}
+
+// Four consecutive values of a row; `vec` where their address is a multiple
+// of their size together.
+__device__ __forceinline__ void load4(const float* p, bool vec, float* x) {
+  if (vec) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = p[i];
+  }
+}
+__device__ __forceinline__ float wide(__half h) { return __half2float(h); }
+__device__ __forceinline__ float wide(__nv_bfloat16 h) { return __bfloat162float(h); }
+template <class H>
+__device__ __forceinline__ void load4(const H* p, bool vec, float* x) {
+  H h[4];
+  if (vec) {
+    *reinterpret_cast<uint2*>(h) = *reinterpret_cast<const uint2*>(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) h[i] = p[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) x[i] = wide(h[i]);
+}
+
+__device__ __forceinline__ void narrow(float x, float* p) { *p = x; }
+__device__ __forceinline__ void narrow(float x, __half* p) { *p = __float2half_rn(x); }
+__device__ __forceinline__ void narrow(float x, __nv_bfloat16* p) { *p = __float2bfloat16_rn(x); }
+
+// ------------------------------------------------------------- append ----
+//
+// A unit is one (sequence, page it writes, head, keys or values): G threads
+// that hold the page's new values in registers, find their largest
+// magnitude a, and set s' = max(s, a/127); where that grew, what the page
+// held becomes rne(q·s/s'); the new values become rne(x/s'). No two units
+// share a byte or a scale, so there are no atomics and no order.
+//
+// Rotation, quotients and roundings are in 64 bits (the products x·cos are
+// exact there): a value next to a rounding border would otherwise go to one
+// or the other side by the order of 32-bit operations, a whole step of the
+// page's scale. The scale itself is stored in 32 bits, as the reader
+// multiplies with it.
+//
+// A thread holds at most kItems items of eight values: two groups of four
+// that the rotation pairs with each other.
+constexpr int kItems = 4;
+
+template <int D, int G, class T>
+__global__ void __launch_bounds__(256) k_kv8_append(Kv8Args a, Kv8Rows kin, Kv8Rows vin, int blocks, bool vec) {
+  __shared__ double red[8];
+  const int tid = threadIdx.x % G;
+  const int64_t unit = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) / G;
+  const int hh = int(unit % (2 * a.heads)), h = hh >> 1;
+  const bool key = (hh & 1) == 0;
+  const int64_t rest = unit / (2 * a.heads);
+  const int b = int(rest % blocks);
+  const int64_t i64 = rest / blocks;
+  if (i64 >= a.n) return;
+  const int i = int(i64);
+  const Kv8Span sp = kv8_span(a, i);
+  if (!sp.ok) {
+    if (tid == 0) report(a);
+    return;
+  }
+  const int p0 = sp.len - sp.T;
+  if (p0 < 0 || sp.T == 0) return;  // a slot that holds nothing
+  const int block = (p0 >> a.plog) + b, begin = block << a.plog;
+  const int lo = max(p0, begin), hi = min(sp.len, begin + (1 << a.plog));
+  if (lo >= hi) return;
+  const int page = kv8_page(a, i, block);
+  if (page < 0) {
+    if (tid == 0) report(a);
+    return;
+  }
+  const int held = lo - begin;  // tokens that the page holds already
+  const int64_t ph = int64_t(page) * a.heads + h;
+  int8_t* base = (key ? a.k : a.v) + ((ph << a.plog) * D);
+  float* sptr = a.scale + 2 * ph + (key ? 0 : 1);
+  const float old = held > 0 ? *sptr : 0.f;
+
+  const Kv8Rows& in = key ? kin : vin;
+  const T* src = static_cast<const T*>(in.p) + int64_t(sp.row + lo - p0) * in.row + int64_t(h) * in.head;
+  const int mode = key ? a.rope_mode : ROPE_NONE;
+  constexpr int C = D / 8;  // items a token
+  const int items = (hi - lo) * C;
+  double y[kItems][8];
+  double amax = 0;
+  bool finite = true;
+#pragma unroll
+  for (int u = 0; u < kItems; u++) {
+    const int it = tid + u * G;
+    if (it < items) {
+      const int t = it / C, c = it % C;
+      const int e0 = mode == ROPE_HALVES ? 4 * c : 8 * c, e1 = mode == ROPE_HALVES ? D / 2 + 4 * c : 8 * c + 4;
+      float x[8];
+      load4(src + t * in.row + e0, vec, x);
+      load4(src + t * in.row + e1, vec, x + 4);
+      if (mode != ROPE_NONE) {
+        const float4* cs = reinterpret_cast<const float4*>(a.rope + (int64_t(lo + t) * (D / 2) + 4 * c) * 2);
+        const float4 f0 = cs[0], f1 = cs[1];
+        const float co[4] = {f0.x, f0.z, f1.x, f1.z}, si[4] = {f0.y, f0.w, f1.y, f1.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int p = mode == ROPE_PAIRS ? 2 * j : j, q = mode == ROPE_PAIRS ? 2 * j + 1 : j + 4;
+          const double xa = x[p], xb = x[q], cc = co[j], ss = si[j];
+          // the products are exact, so one rounding each
+          const double r0 = __fma_rn(xa, cc, -(xb * ss)), r1 = __fma_rn(xa, ss, xb * cc);
+          if (mode == ROPE_PAIRS)
+            y[u][2 * j] = r0, y[u][2 * j + 1] = r1;
+          else
+            y[u][j] = r0, y[u][j + 4] = r1;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) y[u][j] = x[j];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        amax = fmax(amax, fabs(y[u][j]));
+        finite = finite && isfinite(y[u][j]);
+      }
+    }
+  }
+  // a value that is no number makes the scale none either
+  if (!finite) amax = INFINITY;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmax(amax, __shfl_xor_sync(FULL, amax, o));
+  if (G > 32) {
+    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < G / 32; w++) amax = fmax(amax, red[w]);
+  }
+  float scale = fmaxf(old, float(amax / 127.0));
+  if (isinf(amax) || isnan(old)) scale = __int_as_float(0x7fc00000);
+  const bool grown = scale > old;
+  const double back = scale > 0.f ? 1.0 / double(scale) : 0.0;  // 0 for 0 and for no number
+  if (held > 0 && grown) {
+    const double r = double(old) * back;
+    uint4* w = reinterpret_cast<uint4*>(base);
+    for (int j = tid; j < held * (D / 16); j += G) {
+      uint4 q = w[j];
+      uint32_t* qw = &q.x;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        uint32_t o = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int v = int8_t(qw[e] >> (8 * k));
+          o |= uint32_t(__double2int_rn(double(v) * r) & 255) << (8 * k);
+        }
+        qw[e] = o;
+      }
+      w[j] = q;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kItems; u++) {
+    const int it = tid + u * G;
+    if (it < items) {
+      const int t = it / C, c = it % C;
+      uint32_t w[2] = {0, 0};
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const int q = back > 0.0 ? max(-127, min(127, __double2int_rn(y[u][j] * back))) : 0;
+        w[j / 4] |= uint32_t(q & 255) << (8 * (j % 4));
+      }
+      int8_t* dst = base + (held + t) * D;
+      if (mode == ROPE_HALVES) {
+        *reinterpret_cast<uint32_t*>(dst + 4 * c) = w[0];
+        *reinterpret_cast<uint32_t*>(dst + D / 2 + 4 * c) = w[1];
+      } else {
+        *reinterpret_cast<uint2*>(dst + 8 * c) = make_uint2(w[0], w[1]);
+      }
+    }
+  }
+  // every thread of the unit has read the old scale: the reductions above
+  // are behind that read
+  if (tid == 0) *sptr = scale;
+}
+
+// --------------------------------------------------------------- read ----
+//
+// The values of stored tokens: sixteen bytes of one token and head to a
+// thread, q·scale in 32 bits, rounded once to the output's type.
+template <int D, class T>
+__global__ void __launch_bounds__(256) k_kv8_read(Kv8Args a, Kv8Rows kout, Kv8Rows vout, bool vec) {
+  constexpr int C = D / 16;
+  const int i = blockIdx.y;
+  const Kv8Span sp = kv8_span(a, i);
+  if (!sp.ok) {
+    if (threadIdx.x == 0) report(a);
+    return;
+  }
+  const int p0 = sp.len - sp.T;
+  if (p0 < 0) return;
+  const int64_t idx = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const int c = int(idx % C);
+  const int64_t r = idx / C;
+  const int hh = int(r % (2 * a.heads)), h = hh % a.heads;
+  const bool key = hh < a.heads;
+  const int64_t t64 = r / (2 * a.heads);
+  if (t64 >= sp.T) return;
+  const Kv8Rows& o = key ? kout : vout;
+  if (!o.p) return;
+  const int t = int(t64), pos = p0 + t;
+  const int page = kv8_page(a, i, pos >> a.plog);
+  if (page < 0) {
+    report(a);
+    return;
+  }
+  const int64_t ph = int64_t(page) * a.heads + h;
+  const int slot = pos & ((1 << a.plog) - 1);
+  const uint4 q = *reinterpret_cast<const uint4*>((key ? a.k : a.v) + ((ph << a.plog) + slot) * D + 16 * c);
+  const float s = a.scale[2 * ph + (key ? 0 : 1)];
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  T* dst = static_cast<T*>(const_cast<void*>(o.p)) + int64_t(sp.row + t) * o.row + int64_t(h) * o.head + 16 * c;
+  __align__(16) T y[16];
+#pragma unroll
+  for (int j = 0; j < 16; j++) narrow(__fmul_rn(float(int8_t(w[j / 4] >> (8 * (j % 4)))), s), &y[j]);
+  if (vec) {
+#pragma unroll
+    for (int j = 0; j < int(sizeof(T)); j++) reinterpret_cast<uint4*>(dst)[j] = reinterpret_cast<const uint4*>(y)[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; j++) dst[j] = y[j];
+  }
+}
+
+// Whether groups of `count` elements of rows that begin at p with these
+// strides lie at multiples of their size.
+template <class T>
+bool aligned(const Kv8Rows& r, int count) {
+  const uintptr_t b = sizeof(T) * count;
+  return reinterpret_cast<uintptr_t>(r.p) % b == 0 && (r.row * sizeof(T)) % b == 0 && (r.head * sizeof(T)) % b == 0;
+}
+
+template <int D, class T>
+cudaError_t append_t(const Kv8Args& a, const Kv8Rows& k, const Kv8Rows& v, cudaStream_t st) {
+  const int page = 1 << a.plog;
+  const int blocks = (a.max_new + page - 2) / page + 1;  // pages that max_new tokens can touch
+  const int64_t units = int64_t(a.n) * blocks * 2 * a.heads;
+  const bool vec = aligned<T>(k, 4) && aligned<T>(v, 4);
+  // A warp to a unit while its registers hold the unit's new values, else
+  // eight of them: 64 tokens of 128 values are kItems items of 256 threads.
+  if (std::min(a.max_new, page) * (D / 8) <= 32 * kItems)
+    k_kv8_append<D, 32, T><<<unsigned((units + 7) / 8), 256, 0, st>>>(a, k, v, blocks, vec);
+  else
+    k_kv8_append<D, 256, T><<<unsigned(units), 256, 0, st>>>(a, k, v, blocks, vec);
+  return cudaGetLastError();
+}
+
+template <int D, class T>
+cudaError_t read_t(const Kv8Args& a, const Kv8Rows& k, const Kv8Rows& v, cudaStream_t st) {
+  const int64_t threads = int64_t(a.max_new) * 2 * a.heads * (D / 16);
+  const bool vec = (!k.p || aligned<T>(k, 16 / sizeof(T))) && (!v.p || aligned<T>(v, 16 / sizeof(T)));
+  k_kv8_read<D, T><<<dim3(unsigned((threads + 255) / 256), a.n), 256, 0, st>>>(a, k, v, vec);
+  return cudaGetLastError();
+}
+
+// ------------------------------------------------------------- attend ----
+//
+// One pass over a sequence's keys and values with the running maximum and
+// sum of the softmax, on the tensor cores' integer and bfloat16 products,
+// with sixteen keys as a product's rows and eight queries as its columns.
+//
+// Scores. A query's values become whole numbers of amax/2^22, written as
+// three signed digits in base 256, so the products with the cache's bytes
+// are exact integer products (m16n8k32) straight from the bytes as they were
+// loaded: no conversion of a key, and 32-bit accuracy (2^-23 of the largest
+// query value).
+// Values. p·s_v, with the page's value scale in it, is split into bfloat16
+// numbers: three for float32 outputs (24 bits, what a float32 weight has; two
+// measured 2.5e-6 of the outputs' norm off the 64-bit result, against 2.5e-7
+// for float32 arithmetic), two for 16-bit ones (2^-17 of each weight, far
+// below the output's own rounding). A byte is exact in bfloat16: with 0x43 above the low seven bits and 0x43 above the sign bit,
+// the difference of the two numbers (128 + low) − (128 or 256) is the byte.
+//
+// Layout. A warp takes sixteen tokens at a time, straight from global
+// memory into the registers of the product's operands: a key row's bytes
+// are spread over four lanes, sixteen consecutive ones each, a value row's
+// over eight. No shared memory in the loop and no synchronisation: four
+// warps of a block, and the blocks of a cluster, take separate stretches of
+// the keys and are joined at the end through (distributed) shared memory.
+// The maximum moves only when a score passes it by 2^8 (the weights stay
+// far from overflow), so most steps need no exchange between lanes.
+constexpr int kWarps = 4;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void mma_s8(int* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// Two floats as bfloat16s, lo in the low half.
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t y;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+  return y;
+}
+// Byte b (0..3) of x and of y as bfloat16s, x's in the low half.
+template <int B>
+__device__ __forceinline__ uint32_t bytes_bf16(uint32_t x, uint32_t y) {
+  const uint32_t p = __byte_perm(x, y, B | (4 + B) << 8);
+  const uint32_t m = (p & 0x007f007fu) | 0x43004300u, s = (p & 0x00800080u) | 0x43004300u;
+  uint32_t d;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(m), "r"(s));
+  return d;
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The float at p's place in the shared memory of the cluster's block `rank`.
+__device__ __forceinline__ float peer_f32(const float* p, uint32_t rank) {
+  uint32_t at;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(uint32_t(__cvta_generic_to_shared(p))), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at));
+  return v;
+}
+
+template <int D>
+struct Tile {  // sixteen tokens as the products take them
+  uint4 k[2][D / 64];
+  uint4 v[D / 32];  // four tokens of D/8 bytes
+  float sk, sv;
+};
+
+template <int D, int NQ>
+constexpr size_t attend_smem() {
+  return size_t(NQ) * 3 * (D / 64) * 32 * 16   // query digits
+         + size_t(8 * NQ) * (4 + 4)            // factors, positions
+         + size_t(kWarps) * 8 * NQ * (D + 2) * 4  // the warps' sums, maxima and outputs
+         + size_t(8 * NQ) * (D + 2) * 4;       // the block's
+}
+
+template <int D, int NQ, int NP>
+__global__ void __launch_bounds__(32 * kWarps, NQ == 1 ? 4 : 2)
+    k_kv8_attend(Kv8Args a, Kv8Attend t, int type, int S, int qtiles, bool vec) {
+  constexpr int NR = 8 * NQ, H2 = D / 64;
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint4* qd = reinterpret_cast<uint4*>(smem);                 // [NQ][3][H2][32]
+  float* qf = reinterpret_cast<float*>(qd + NQ * 3 * H2 * 32);  // [NR]
+  int* qpos = reinterpret_cast<int*>(qf + NR);                // [NR]
+  float* wm = reinterpret_cast<float*>(qpos + NR);            // [kWarps][NR]
+  float* wl = wm + kWarps * NR;
+  float* wo = wl + kWarps * NR;                               // [kWarps][NR][D]
+  float* bm = wo + kWarps * NR * D;                           // [NR], [NR], [NR][D]
+  float* bl = bm + NR;
+  float* bo = bl + NR;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tg = lane & 3;
+  const int rank = S > 1 ? int(cluster_rank()) : 0;
+  const int64_t unit = blockIdx.x / S;
+  const int h = int(unit % a.heads), qt = int(unit / a.heads % qtiles), i = int(unit / a.heads / qtiles);
+  const int group = t.heads / a.heads;
+  const Kv8Span sp = kv8_span(a, i);
+  if (!sp.ok) {
+    if (tid == 0) report(a);
+    return;  // every block of the cluster: it has one sequence
+  }
+  const int r0 = qt * NR, nrow = min(NR, sp.T * group - r0);  // this block's query rows
+  if (nrow <= 0) return;
+  const int p0 = sp.len - sp.T;
+  const int pmin = p0 + r0 / group, pmax = p0 + (r0 + nrow - 1) / group;
+  const int first = a.first ? max(0, a.first[i]) : 0;
+  const int klo = max(first, t.window > 0 ? pmin - t.window + 1 : 0), khi = pmax + 1;
+  const int cb = klo >> 4, ce = max(cb, (khi + 15) >> 4);
+  const int per = (ce - cb + S * kWarps - 1) / (S * kWarps);
+  const int c0 = min(ce, cb + (rank * kWarps + warp) * per), c1 = min(ce, c0 + per);
+
+  // --- the pages ahead: lane l holds page and scales of the tile wbase + l ---
+  const int cshift = a.plog - 4;
+  const float2* scales = reinterpret_cast<const float2*>(a.scale);
+  auto page_of = [&](int c) { return c < c1 ? kv8_page(a, i, c >> cshift) : -1; };
+  auto scale_of = [&](int page) {
+    return page >= 0 ? scales[int64_t(page) * a.heads + h] : make_float2(0.f, 0.f);
+  };
+  int wbase = c0;
+  int pg = page_of(c0 + lane);
+  if (pg < 0 && c0 + lane < c1) report(a);
+  float2 sc = scale_of(pg);
+  int pg1 = page_of(c0 + 32 + lane);
+
+  Tile<D> buf[2];
+  auto fetch = [&](Tile<D>& b, int c) {
+    if (c >= c1) return;
+    if (c - wbase == 32) {
+      wbase += 32;
+      pg = pg1;
+      if (pg < 0 && wbase + lane < c1) report(a);
+      sc = scale_of(pg);
+      pg1 = page_of(wbase + 32 + lane);
+    }
+    const int page = __shfl_sync(FULL, pg, c - wbase);
+    b.sk = __shfl_sync(FULL, sc.x, c - wbase);
+    b.sv = __shfl_sync(FULL, sc.y, c - wbase);
+    if (page < 0) {
+      // no such page: its tokens are not there
+      b.sk = __int_as_float(0xff800000);
+#pragma unroll
+      for (int j = 0; j < H2; j++) b.k[0][j] = b.k[1][j] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < D / 32; j++) b.v[j] = make_uint4(0, 0, 0, 0);
+      return;
+    }
+    const int slot = (c << 4) & ((1 << a.plog) - 1);
+    const int64_t at = (((int64_t(page) * a.heads + h) << a.plog) + slot) * D;
+    const int8_t* kp = a.k + at + g * D + 16 * tg;
+#pragma unroll
+    for (int r = 0; r < 2; r++)
+#pragma unroll
+      for (int j = 0; j < H2; j++)
+        b.k[r][j] = __ldg(reinterpret_cast<const uint4*>(kp + r * 8 * D + j * 64));
+    const int8_t* vp = a.v + at + 2 * tg * D + g * (D / 8);
+    if constexpr (D == 64) {
+      const uint2 x0 = __ldg(reinterpret_cast<const uint2*>(vp)), x1 = __ldg(reinterpret_cast<const uint2*>(vp + D));
+      const uint2 x2 = __ldg(reinterpret_cast<const uint2*>(vp + 8 * D)),
+                  x3 = __ldg(reinterpret_cast<const uint2*>(vp + 9 * D));
+      b.v[0] = make_uint4(x0.x, x0.y, x1.x, x1.y);
+      b.v[1] = make_uint4(x2.x, x2.y, x3.x, x3.y);
+    } else {
+      b.v[0] = __ldg(reinterpret_cast<const uint4*>(vp));
+      b.v[1] = __ldg(reinterpret_cast<const uint4*>(vp + D));
+      b.v[2] = __ldg(reinterpret_cast<const uint4*>(vp + 8 * D));
+      b.v[3] = __ldg(reinterpret_cast<const uint4*>(vp + 9 * D));
+    }
+  };
+  fetch(buf[0], c0);
+  fetch(buf[1], c0 + 1);
+
+  // --- the queries: rotated, and written as digits ---
+  for (int nq = warp; nq < NQ; nq += kWarps) {
+    const int r = nq * 8 + g;  // this lane's query
+    const bool there = r < nrow;
+    const int tq = there ? (r0 + r) / group : 0, hq = h * group + (there ? (r0 + r) % group : 0);
+    const int pos = p0 + tq;
+    float x[H2][16];
+    const int64_t off = int64_t(sp.row + tq) * t.q.row + int64_t(hq) * t.q.head + 16 * tg;
+#pragma unroll
+    for (int j = 0; j < H2; j++)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const int64_t o = off + 64 * j + e;
+        if (!there) {
+          x[j][e] = x[j][e + 1] = x[j][e + 2] = x[j][e + 3] = 0.f;
+        } else if (type == 0) {
+          load4(static_cast<const float*>(t.q.p) + o, vec, &x[j][e]);
+        } else if (type == 1) {
+          load4(static_cast<const __half*>(t.q.p) + o, vec, &x[j][e]);
+        } else {
+          load4(static_cast<const __nv_bfloat16*>(t.q.p) + o, vec, &x[j][e]);
+        }
+      }
+    if (a.rope_mode != ROPE_NONE) {
+      // a slot that holds nothing has no position; its scores are not used
+      const float2* cs = reinterpret_cast<const float2*>(a.rope) + int64_t(max(pos, 0)) * (D / 2);
+      if (a.rope_mode == ROPE_PAIRS) {
+#pragma unroll
+        for (int j = 0; j < H2; j++)
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            const float2 f = cs[(64 * j + 16 * tg + e) / 2];
+            const float p = x[j][e], q = x[j][e + 1];
+            x[j][e] = __fmaf_rn(p, f.x, -__fmul_rn(q, f.y));
+            x[j][e + 1] = __fmaf_rn(p, f.y, __fmul_rn(q, f.x));
+          }
+      } else if (D == 64) {
+        // the partner is 32 values on: two lanes away
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          const float o = __shfl_xor_sync(FULL, x[0][e], 2);
+          const float2 f = cs[(16 * tg + e) & 31];
+          x[0][e] = __fmaf_rn(x[0][e], f.x, tg < 2 ? -__fmul_rn(o, f.y) : __fmul_rn(o, f.y));
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          const float2 f = cs[16 * tg + e];
+          const float p = x[0][e], q = x[H2 - 1][e];
+          x[0][e] = __fmaf_rn(p, f.x, -__fmul_rn(q, f.y));
+          x[H2 - 1][e] = __fmaf_rn(p, f.y, __fmul_rn(q, f.x));
+        }
+      }
+    }
+    float amax = 0.f;
+    bool finite = true;
+#pragma unroll
+    for (int j = 0; j < H2; j++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        amax = fmaxf(amax, fabsf(x[j][e]));
+        finite = finite && isfinite(x[j][e]);
+      }
+    amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, 2));
+    finite = ((__ballot_sync(FULL, finite) >> (lane & ~3)) & 15) == 15;
+#pragma unroll
+    for (int j = 0; j < H2; j++) {
+      uint32_t w[3][4] = {};
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        const float y = finite && amax > 0.f ? __fmul_rn(__fdiv_rn(x[j][e], amax), 4194304.f) : 0.f;
+        const int n = __float2int_rn(y);
+        const int d0 = int8_t(n), n1 = (n - d0) >> 8, d1 = int8_t(n1), d2 = (n1 - d1) >> 8;
+        w[0][e / 4] |= uint32_t(d0 & 255) << (8 * (e % 4));
+        w[1][e / 4] |= uint32_t(d1 & 255) << (8 * (e % 4));
+        w[2][e / 4] |= uint32_t(d2 & 255) << (8 * (e % 4));
+      }
+#pragma unroll
+      for (int d = 0; d < 3; d++)
+        qd[((nq * 3 + d) * H2 + j) * 32 + lane] = make_uint4(w[d][0], w[d][1], w[d][2], w[d][3]);
+    }
+    if (tg == 0) {
+      // scores in units of log 2; a query that is no number has no score
+      const float f = __fmul_rn(__fmul_rn(amax, 1.f / 4194304.f), __fmul_rn(t.scale, 1.44269504f));
+      qf[r] = finite ? f : __int_as_float(0x7fc00000);
+      qpos[r] = there ? pos : -1;
+    }
+  }
+  __syncthreads();
+
+  // --- the pass over the keys ---
+  float o[NQ][D / 16][4] = {};
+  float m[NQ][2], l[NQ][2] = {}, f[NQ][2];
+#pragma unroll
+  for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      m[nq][j] = __int_as_float(0xff800000);
+      f[nq][j] = qf[nq * 8 + 2 * tg + j];
+    }
+  // tiles that every query of the block sees whole
+  const int in_lo = max(first, t.window > 0 ? pmax - t.window + 1 : 0), in_hi = pmin;
+  auto step = [&](const Tile<D>& b, int c) {
+    const bool edge = c * 16 < in_lo || c * 16 + 15 > in_hi || nrow < NR || b.sk == __int_as_float(0xff800000);
+    uint32_t pw[NQ][NP][2];  // the weights, transposed: queries in rows
+#pragma unroll
+    for (int nq = 0; nq < NQ; nq++) {
+      int acc[3][4];
+#pragma unroll
+      for (int d = 0; d < 3; d++) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[d][j] = MAGIC_BITS;
+#pragma unroll
+        for (int j = 0; j < H2; j++) {
+          const uint4 q = qd[((nq * 3 + d) * H2 + j) * 32 + lane];
+          mma_s8(acc[d], b.k[0][j].x, b.k[1][j].x, b.k[0][j].y, b.k[1][j].y, q.x, q.y);
+          mma_s8(acc[d], b.k[0][j].z, b.k[1][j].z, b.k[0][j].w, b.k[1][j].w, q.z, q.w);
+        }
+      }
+      float s[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const float a0 = __fsub_rn(__int_as_float(acc[0][j]), MAGIC), a1 = __fsub_rn(__int_as_float(acc[1][j]), MAGIC),
+                    a2 = __fsub_rn(__int_as_float(acc[2][j]), MAGIC);
+        s[j] = __fmul_rn(__fmaf_rn(65536.f, a2, __fmaf_rn(256.f, a1, a0)), __fmul_rn(f[nq][j & 1], b.sk));
+      }
+      bool hide[4] = {false, false, false, false};
+      if (edge) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int p = qpos[nq * 8 + 2 * tg + (j & 1)], key = c * 16 + g + (j >> 1) * 8;
+          hide[j] = key > p || key < first || (t.window > 0 && key <= p - t.window) ||
+                    b.sk == __int_as_float(0xff800000);
+          if (hide[j]) s[j] = __int_as_float(0xff800000);
+        }
+      }
+      const float over = fmaxf(fmaxf(__fsub_rn(s[0], m[nq][0]), __fsub_rn(s[2], m[nq][0])),
+                               fmaxf(__fsub_rn(s[1], m[nq][1]), __fsub_rn(s[3], m[nq][1])));
+      if (__any_sync(FULL, over > 8.f)) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          float x = fmaxf(s[j], s[j + 2]);
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(FULL, x, d));
+          x = fmaxf(x, m[nq][j]);
+          const float r = m[nq][j] == x ? 1.f : ex2(__fsub_rn(m[nq][j], x));
+          m[nq][j] = x;
+          l[nq][j] = __fmul_rn(l[nq][j], r);
+#pragma unroll
+          for (int mt = 0; mt < D / 16; mt++) {
+            o[nq][mt][j] = __fmul_rn(o[nq][mt][j], r);
+            o[nq][mt][j + 2] = __fmul_rn(o[nq][mt][j + 2], r);
+          }
+        }
+      }
+      float w[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        // before the first key that it sees a query has no maximum
+        const float ref = m[nq][j & 1] == __int_as_float(0xff800000) ? 0.f : m[nq][j & 1];
+        const float p = ex2(__fsub_rn(s[j], ref));
+        l[nq][j & 1] = __fadd_rn(l[nq][j & 1], p);
+        w[j] = hide[j] ? 0.f : __fmul_rn(p, b.sv);
+      }
+#pragma unroll
+      for (int n = 0; n < NP; n++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const uint32_t h = pack_bf16(w[2 * j], w[2 * j + 1]);
+          w[2 * j] = __fsub_rn(w[2 * j], bits_f(h << 16));
+          w[2 * j + 1] = __fsub_rn(w[2 * j + 1], bits_f(h & 0xffff0000u));
+          pw[nq][n][j] = transpose8(h);
+        }
+    }
+    const uint32_t* vw = &b.v[0].x;  // four tokens of D/32 words
+    constexpr int W = D / 32;
+    auto values = [&](auto MT) {
+      constexpr int mt = decltype(MT)::value, wd = mt / 2, by = 2 * (mt % 2);
+      const uint32_t a0 = bytes_bf16<by>(vw[wd], vw[W + wd]), a1 = bytes_bf16<by + 1>(vw[wd], vw[W + wd]);
+      const uint32_t a2 = bytes_bf16<by>(vw[2 * W + wd], vw[3 * W + wd]),
+                     a3 = bytes_bf16<by + 1>(vw[2 * W + wd], vw[3 * W + wd]);
+#pragma unroll
+      for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+        for (int n = 0; n < NP; n++) mma_bf16(o[nq][mt], a0, a1, a2, a3, pw[nq][n][0], pw[nq][n][1]);
+    };
+    values(std::integral_constant<int, 0>());
+    values(std::integral_constant<int, 1>());
+    values(std::integral_constant<int, 2>());
+    values(std::integral_constant<int, 3>());
+    if constexpr (D == 128) {
+      values(std::integral_constant<int, 4>());
+      values(std::integral_constant<int, 5>());
+      values(std::integral_constant<int, 6>());
+      values(std::integral_constant<int, 7>());
+    }
+  };
+  for (int c = c0; c < c1; c += 2) {
+    step(buf[0], c);
+    fetch(buf[0], c + 2);
+    if (c + 1 < c1) {
+      step(buf[1], c + 1);
+      fetch(buf[1], c + 3);
+    }
+  }
+
+  // --- the warps' shares joined ---
+#pragma unroll
+  for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) l[nq][j] = __fadd_rn(l[nq][j], __shfl_xor_sync(FULL, l[nq][j], d));
+      const int r = nq * 8 + 2 * tg + j;
+      if (g == 0) {
+        wm[warp * NR + r] = m[nq][j];
+        wl[warp * NR + r] = l[nq][j];
+      }
+      float* dst = wo + (warp * NR + r) * D + g * (D / 8);
+#pragma unroll
+      for (int mt = 0; mt < D / 16; mt++)
+        *reinterpret_cast<float2*>(dst + 2 * mt) = make_float2(o[nq][mt][j], o[nq][mt][j + 2]);
+    }
+  __syncthreads();
+  // Item: 32 values of one row, a lane each. The weight of a share is
+  // 2^(its maximum − the largest); one without keys counts 0 (its maximum
+  // is −inf), and where all are, the sums are 0 or no number already.
+  auto weight = [](float mi, float top) { return mi == top ? 1.f : ex2(__fsub_rn(mi, top)); };
+  auto finish = [&](int r, int d, float top, float sum, float val) {
+    const int tq = (r0 + r) / group, hq = h * group + (r0 + r) % group;
+    const float y = sum == 0.f ? 0.f : __fdiv_rn(val, sum);
+    if (t.out.p) {
+      const int64_t at = int64_t(sp.row + tq) * t.out.row + int64_t(hq) * t.out.head + d;
+      void* op = const_cast<void*>(t.out.p);
+      if (type == 0)
+        static_cast<float*>(op)[at] = y;
+      else if (type == 1)
+        static_cast<__half*>(op)[at] = __float2half_rn(y);
+      else
+        static_cast<__nv_bfloat16*>(op)[at] = __float2bfloat16_rn(y);
+    }
+    if (t.q8) {
+      const int64_t at = int64_t(sp.row + tq) * t.heads * D + hq * D + d;
+      float s;
+      t.q8[at] = quant_lane(y, &s);
+      if (lane == 0) t.q8s[at / QK] = make_float2(s, s);
+    }
+    if (t.lse && d == 0)
+      t.lse[int64_t(sp.row + tq) * t.heads + hq] =
+          sum == 0.f ? __int_as_float(0xff800000) : __fmaf_rn(top, 0.693147181f, logf(sum));
+  };
+  const int items = nrow * (D / 32);
+  for (int it = warp; it < items; it += kWarps) {
+    const int r = it / (D / 32), d = it % (D / 32) * 32 + lane;
+    float top = wm[r], sum = 0.f, val = 0.f;
+#pragma unroll
+    for (int w = 1; w < kWarps; w++) top = fmaxf(top, wm[w * NR + r]);
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) {
+      const float k = weight(wm[w * NR + r], top);
+      sum = __fmaf_rn(k, wl[w * NR + r], sum);
+      val = __fmaf_rn(k, wo[(w * NR + r) * D + d], val);
+    }
+    if (S == 1) {
+      finish(r, d, top, sum, val);
+    } else {
+      bo[r * D + d] = val;
+      if (d == 0) {
+        bm[r] = top;
+        bl[r] = sum;
+      }
+    }
+  }
+  if (S == 1) return;
+  cluster_sync();
+  for (int it = rank * kWarps + warp; it < items; it += S * kWarps) {
+    const int r = it / (D / 32), d = it % (D / 32) * 32 + lane;
+    float top = __int_as_float(0xff800000), sum = 0.f, val = 0.f;
+    for (int b = 0; b < S; b++) top = fmaxf(top, peer_f32(bm + r, b));
+    for (int b = 0; b < S; b++) {
+      const float k = weight(peer_f32(bm + r, b), top);
+      sum = __fmaf_rn(k, peer_f32(bl + r, b), sum);
+      val = __fmaf_rn(k, peer_f32(bo + r * D + d, b), val);
+    }
+    finish(r, d, top, sum, val);
+  }
+  cluster_sync();  // no block leaves while another reads its shared memory
+}
+
+constexpr int kSMs = 148;
+
+template <int D, int NQ, int NP>
+cudaError_t attend_t(const Kv8Args& a, int type, const Kv8Attend& t, cudaStream_t st) {
+  const int group = t.heads / a.heads;
+  const int qtiles = int((int64_t(a.max_new) * group + 8 * NQ - 1) / (8 * NQ));
+  const int64_t units = int64_t(a.n) * a.heads * qtiles;
+  // Blocks of one unit's keys: enough to fill the GPU four blocks deep,
+  // while each warp keeps two tiles of sixteen keys.
+  int S = 1;
+  while (S < 16 && units * S < 4 * kSMs && a.max_len >= 16 * kWarps * 2 * S * 2) S *= 2;
+  const bool vec = type == 0 ? aligned<float>(t.q, 4) : aligned<__half>(t.q, 4);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(units * S));
+  cfg.blockDim = dim3(32 * kWarps);
+  cfg.dynamicSmemBytes = attend_smem<D, NQ>();
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = unsigned(S);
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = S > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, k_kv8_attend<D, NQ, NP>, a, t, type, S, qtiles, vec);
+}
+
+template <int D, int NP>
+cudaError_t attend_d(const Kv8Args& a, int type, const Kv8Attend& t, cudaStream_t st) {
+  const int64_t rows = int64_t(a.max_new) * (t.heads / a.heads);  // queries that share a head's keys
+  if (rows <= 8) return attend_t<D, 1, NP>(a, type, t, st);
+  if (rows <= 16) return attend_t<D, 2, NP>(a, type, t, st);
+  return attend_t<D, 4, NP>(a, type, t, st);
+}
+
+template <int D, int NQ, int NP>
+void attend_attrs() {
+  cudaFuncSetAttribute(k_kv8_attend<D, NQ, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                       int(attend_smem<D, NQ>()));
+  cudaFuncSetAttribute(k_kv8_attend<D, NQ, NP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+}
+template <int D, int NP>
+void attend_init() {
+  attend_attrs<D, 1, NP>();
+  attend_attrs<D, 2, NP>();
+  attend_attrs<D, 4, NP>();
+}
+
+}  // namespace
+
+cudaError_t launch_kv8_append(const Kv8Args& a, int head_dim, int type, const Kv8Rows& k, const Kv8Rows& v,
+                              cudaStream_t st) {
+  if (head_dim == 64)
+    return type == 0   ? append_t<64, float>(a, k, v, st)
+           : type == 1 ? append_t<64, __half>(a, k, v, st)
+                       : append_t<64, __nv_bfloat16>(a, k, v, st);
+  return type == 0   ? append_t<128, float>(a, k, v, st)
+         : type == 1 ? append_t<128, __half>(a, k, v, st)
+                     : append_t<128, __nv_bfloat16>(a, k, v, st);
+}
+
+cudaError_t launch_kv8_read(const Kv8Args& a, int head_dim, int type, const Kv8Rows& k, const Kv8Rows& v,
+                            cudaStream_t st) {
+  if (head_dim == 64)
+    return type == 0   ? read_t<64, float>(a, k, v, st)
+           : type == 1 ? read_t<64, __half>(a, k, v, st)
+                       : read_t<64, __nv_bfloat16>(a, k, v, st);
+  return type == 0   ? read_t<128, float>(a, k, v, st)
+         : type == 1 ? read_t<128, __half>(a, k, v, st)
+                     : read_t<128, __nv_bfloat16>(a, k, v, st);
+}
+
+cudaError_t launch_kv8_attend(const Kv8Args& a, int head_dim, int type, const Kv8Attend& t, cudaStream_t st) {
+  if (head_dim == 64) return type == 0 ? attend_d<64, 3>(a, type, t, st) : attend_d<64, 2>(a, type, t, st);
+  return type == 0 ? attend_d<128, 3>(a, type, t, st) : attend_d<128, 2>(a, type, t, st);
+}
+
+void kv8_kernels_init() {
+  attend_init<64, 2>();
+  attend_init<64, 3>();
+  attend_init<128, 2>();
+  attend_init<128, 3>();
+}
+
+}  // namespace grx

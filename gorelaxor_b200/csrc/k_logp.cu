@@ -1,0 +1,514 @@
+// Log probabilities of given tokens, with the entropy of each row and its
+// most likely tokens, in one pass over the logits.
+//
+// With m the row's largest logit (at one index) and the sums over the other
+// indices
+//   z = Σ e^(x_j − m),   t = Σ (m − x_j)·e^(x_j − m),
+// the log probability of token j is (x_j − m) − log1p(z) and the entropy is
+// log1p(z) + t/(1 + z). Every term is positive and the 1 is kept apart, so a
+// row whose model is sure loses nothing to cancellation. A share of a row is
+// (m, z, t) in 32 bits; two with m1 >= m2 and e = e^(m2 − m1) join as
+//   z = z1 + e·(1 + z2),   t = t1 + e·(t2 + (m1 − m2)·(1 + z2)).
+//
+// The most likely tokens: each thread knows the largest of its own values
+// from the pass. The `top`-th largest of these is a bound that the answer
+// does not go below, so only the threads at or above it (about `top` of
+// hundreds) have their values looked at again, and the few values above the
+// bound are ranked. Values compare as (value, lower index first), each as
+// one 64-bit number; NaN counts below −inf.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "common.cuh"
+#include "logp.h"
+
+namespace grx {
+
+namespace {
+
+constexpr uint32_t FULL = 0xffffffffu;
+constexpr float kLog2e = 1.44269504f;
+constexpr float kFar = -200.f;  // e^kFar is 0 in 32 bits; stands for −inf where a product with 0 follows
+typedef unsigned long long u64;
+
+__device__ __forceinline__ float ninf() { return __int_as_float(0xff800000); }
+__device__ __forceinline__ float qnan() { return __int_as_float(0x7fc00000); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The larger, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+__device__ __forceinline__ float wide(float x) { return x; }
+__device__ __forceinline__ float wide(__half h) { return __half2float(h); }
+__device__ __forceinline__ float wide(__nv_bfloat16 h) { return __bfloat162float(h); }
+
+// A value as a whole number of the same order; −0 as 0, NaN below all.
+__device__ __forceinline__ uint32_t order(float x) {
+  if (isnan(x)) return 0;
+  const uint32_t u = __float_as_uint(__fadd_rn(x, 0.f));
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float unorder(uint32_t u) {
+  if (u == 0) return qnan();
+  return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+// (value, lower index first) as one number; 0 is no token.
+__device__ __forceinline__ u64 key_of(float x, int i) { return u64(order(x)) << 32 | uint32_t(0x7fffffff - i); }
+
+// A share of a row: the largest value (−inf: none), and the sums over the
+// others.
+struct Share {
+  float m, z, t;
+};
+
+__device__ __forceinline__ Share join(Share a, Share b) {
+  if (b.m > a.m) {
+    const Share c = a;
+    a = b;
+    b = c;
+  }
+  if (b.m == ninf()) {
+    // nothing that counts, unless a NaN is in its sums
+    a.z = __fadd_rn(a.z, b.z);
+    return a;
+  }
+  const float d = fmaxf(__fsub_rn(b.m, a.m), kFar), e = ex2(__fmul_rn(d, kLog2e)), n = __fadd_rn(1.f, b.z);
+  a.z = __fmaf_rn(e, n, a.z);
+  a.t = __fmaf_rn(e, __fmaf_rn(-d, n, b.t), a.t);
+  return a;
+}
+
+// All 32 lanes' shares; every lane gets the same bits.
+__device__ __forceinline__ Share warp_join(Share s) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Share b;
+    b.m = __shfl_xor_sync(FULL, s.m, o);
+    b.z = __shfl_xor_sync(FULL, s.z, o);
+    b.t = __shfl_xor_sync(FULL, s.t, o);
+    s = threadIdx.x & o ? join(b, s) : join(s, b);
+  }
+  return s;
+}
+
+__device__ __forceinline__ u64 warp_max(u64 k) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) k = max(k, __shfl_xor_sync(FULL, k, o));
+  return k;
+}
+
+// One value other than the largest into the sums of a share.
+__device__ __forceinline__ void add(Share& s, float x) {
+  const float d = max_nan(__fsub_rn(x, s.m), kFar), e = ex2(__fmul_rn(d, kLog2e));
+  s.z = __fadd_rn(s.z, e);
+  s.t = __fmaf_rn(-d, e, s.t);
+}
+
+// A thread's values as they come: their share, and the first of the largest.
+struct Run {
+  Share s = {ninf(), 0.f, 0.f};
+  float top = 0.f;
+  int at = -1;
+};
+
+// U groups of V values; group u begins at the index i0 + u·step.
+template <int V, int U>
+__device__ __forceinline__ void take(Run& r, const float (&x)[U][V], int i0, int step) {
+  float c = x[0][0];
+#pragma unroll
+  for (int u = 0; u < U; u++)
+#pragma unroll
+    for (int j = 0; j < V; j++) c = fmaxf(c, x[u][j]);
+  if (r.at < 0 || !(c < r.top)) {
+    // a new largest value or its equal, or no number: one by one
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        const float v = x[u][j];
+        if (v > r.s.m)
+          r.s = join(Share{v, 0.f, 0.f}, r.s);
+        else if (v != ninf())
+          add(r.s, v);
+        if (r.at < 0 || order(v) > order(r.top)) {
+          r.top = v;
+          r.at = i0 + u * step + j;
+        }
+      }
+    return;
+  }
+#pragma unroll
+  for (int u = 0; u < U; u++)
+#pragma unroll
+    for (int j = 0; j < V; j++) add(r.s, x[u][j]);
+}
+
+template <class T>
+__device__ __forceinline__ void load16(const T* p, float* x) {
+  constexpr int V = 16 / sizeof(T);
+  T h[V];
+  *reinterpret_cast<uint4*>(h) = __ldg(reinterpret_cast<const uint4*>(p));
+#pragma unroll
+  for (int j = 0; j < V; j++) x[j] = wide(h[j]);
+}
+
+// What the row's outputs are made of, by one thread.
+template <class T>
+__device__ __forceinline__ void row_out(const LogpArgs& a, int row, const T* x, Share s) {
+  // no largest number, no distribution
+  const bool fine = isfinite(s.m);
+  const float lz = log1pf(s.z);
+  if (a.logprob) {
+    const int t = a.targets[row];
+    a.logprob[row] = fine && t >= 0 && t < a.vocab ? __fsub_rn(__fsub_rn(wide(x[t]), s.m), lz) : qnan();
+  }
+  if (a.entropy) a.entropy[row] = fine ? __fadd_rn(lz, __fdiv_rn(s.t, __fadd_rn(1.f, s.z))) : qnan();
+}
+
+__device__ __forceinline__ void top_out(const LogpArgs& a, int row, int r, u64 key, Share s) {
+  if (a.ids) a.ids[int64_t(row) * a.top + r] = 0x7fffffff - int(uint32_t(key));
+  if (a.lps)
+    a.lps[int64_t(row) * a.top + r] =
+        isfinite(s.m) ? __fsub_rn(__fsub_rn(unorder(uint32_t(key >> 32)), s.m), log1pf(s.z)) : qnan();
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+template <class V>
+__device__ __forceinline__ V peer(const V* p, uint32_t rank) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(uint32_t(__cvta_generic_to_shared(p))), "r"(rank));
+  V v;
+  if constexpr (sizeof(V) == 8)
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at));
+  else
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at));
+  return v;
+}
+
+// ---- a row to a cluster of S blocks of NT threads ----
+//
+// Bound by the bytes of the logits. Loads are 16 bytes wide from the first
+// aligned value on, four to a thread in flight; few rows are split over a
+// cluster, whose first block joins the shares through distributed shared
+// memory.
+constexpr int kCand = 1024;
+
+template <class T, int NT>
+__global__ void __launch_bounds__(NT) k_logp(LogpArgs a, int S) {
+  constexpr int V = 16 / sizeof(T), U = 4, NW = NT / 32;
+  __shared__ Share ws[NW];
+  __shared__ u64 wk[NW];
+  __shared__ u64 cand[kCand];
+  __shared__ u64 best[kLogpMaxTop];
+  __shared__ int sel[NT];
+  __shared__ int nsel, ncand;
+  __shared__ Share mine, whole;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int rank = S > 1 ? int(cluster_rank()) : 0, row = blockIdx.x / S, k = a.top;
+  const T* x = static_cast<const T*>(a.x) + int64_t(row) * a.stride;
+  const int head = min(a.vocab, int((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / int(sizeof(T)));
+  const int nv = (a.vocab - head) / V, tail = a.vocab - head - nv * V;
+  const T* xv = x + head;
+  const int vb = int(int64_t(nv) * rank / S), ve = int(int64_t(nv) * (rank + 1) / S);
+  // the values before and behind the vectors, one to a thread
+  const bool in_head = rank == 0 && tid < head, in_tail = rank == S - 1 && tid < tail;
+  const int at_tail = a.vocab - tail + tid;
+  if (tid == 0) nsel = ncand = 0;
+
+  Run r;
+  int v = vb + tid;
+  for (; v + (U - 1) * NT < ve; v += U * NT) {
+    float f[U][V];
+#pragma unroll
+    for (int u = 0; u < U; u++) load16(xv + int64_t(v + u * NT) * V, f[u]);
+    take<V, U>(r, f, head + v * V, NT * V);
+  }
+  for (; v < ve; v += NT) {
+    float f[1][V];
+    load16(xv + int64_t(v) * V, f[0]);
+    take<V, 1>(r, f, head + v * V, 0);
+  }
+  if (in_head) {
+    const float f[1][1] = {{wide(x[tid])}};
+    // an earlier index than the vectors': it wins a tie
+    const float t0 = r.top;
+    const int a0 = r.at;
+    take<1, 1>(r, f, tid, 0);
+    if (a0 >= 0 && order(f[0][0]) == order(t0)) r.at = tid;
+  }
+  if (in_tail) {
+    const float f[1][1] = {{wide(x[at_tail])}};
+    take<1, 1>(r, f, at_tail, 0);
+  }
+  {
+    const Share s = warp_join(r.s);
+    if (lane == 0) ws[warp] = s;
+  }
+  const u64 mykey = r.at >= 0 ? key_of(r.top, r.at) : 0;
+  if (k == 1) {
+    const u64 m = warp_max(mykey);
+    if (lane == 0) wk[warp] = m;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    Share s = lane < NW ? ws[lane] : Share{ninf(), 0.f, 0.f};
+    s = warp_join(s);
+    if (lane == 0) mine = s;
+    if (k == 1) {
+      const u64 m = warp_max(lane < NW ? wk[lane] : 0);
+      if (lane == 0) best[0] = m;
+    }
+  }
+  if (k > 1) {
+    // a bound: the largest found, bit by bit, that `k` threads reach
+    const uint32_t u = uint32_t(mykey >> 32);
+    uint32_t bound = 0;
+    for (int bit = 31; bit >= 0; bit--) {
+      const uint32_t c = bound | 1u << bit;
+      const int n = __syncthreads_count(r.at >= 0 && u >= c);
+      if (n >= k) {
+        bound = c;
+        if (n <= k + 8) break;
+      }
+    }
+    if (tid < k) best[tid] = 0;
+    if (r.at >= 0 && u >= bound) sel[atomicAdd(&nsel, 1)] = tid;
+    auto offer = [&](float f, int i) {
+      if (order(f) >= bound) {
+        const int p = atomicAdd(&ncand, 1);
+        if (p < kCand) cand[p] = key_of(f, i);
+      }
+    };
+    __syncthreads();
+    if (in_head) offer(wide(x[tid]), tid);
+    if (in_tail) offer(wide(x[at_tail]), at_tail);
+    for (int j = warp; j < nsel; j += NW)
+      for (int w = vb + sel[j] + lane * NT; w < ve; w += 32 * NT) {
+        float f[V];
+        load16(xv + int64_t(w) * V, f);
+#pragma unroll
+        for (int e = 0; e < V; e++) offer(f[e], head + w * V + e);
+      }
+    __syncthreads();
+    if (ncand <= kCand) {
+      for (int c = tid; c < ncand; c += NT) {
+        const u64 mk = cand[c];
+        int above = 0;
+        for (int d = 0; d < ncand; d++) above += cand[d] > mk;
+        if (above < k) best[above] = mk;
+      }
+    } else {
+      // more equals than the list takes: the largest below the last, k times
+      u64 last = ~u64(0);
+      for (int n = 0; n < k; n++) {
+        u64 m = 0;
+        auto see = [&](float f, int i) {
+          const u64 q = key_of(f, i);
+          if (q < last && q > m) m = q;
+        };
+        if (in_head) see(wide(x[tid]), tid);
+        if (in_tail) see(wide(x[at_tail]), at_tail);
+        for (int w = vb + tid; w < ve; w += NT) {
+          float f[V];
+          load16(xv + int64_t(w) * V, f);
+#pragma unroll
+          for (int e = 0; e < V; e++) see(f[e], head + w * V + e);
+        }
+        m = warp_max(m);
+        if (lane == 0) wk[warp] = m;
+        __syncthreads();
+        last = 0;
+        for (int w = 0; w < NW; w++) last = max(last, wk[w]);
+        __syncthreads();
+        if (tid == 0) best[n] = last;
+      }
+    }
+  }
+  if (S == 1) {
+    __syncthreads();
+    if (tid == 0) row_out(a, row, x, mine);
+    if (tid < k) top_out(a, row, tid, best[tid], mine);
+    return;
+  }
+  cluster_sync();
+  if (rank == 0) {
+    if (warp == 0) {
+      Share s = {ninf(), 0.f, 0.f};
+      if (lane < S) s = Share{peer(&mine.m, lane), peer(&mine.z, lane), peer(&mine.t, lane)};
+      s = warp_join(s);
+      if (lane == 0) whole = s;
+    }
+    for (int j = tid; j < S * k; j += NT) cand[j] = peer(&best[j % k], j / k);
+  }
+  cluster_sync();  // no block leaves while its shared memory is read
+  if (rank != 0) return;
+  if (tid == 0) row_out(a, row, x, whole);
+  for (int j = tid; j < S * k; j += NT) {
+    const u64 mk = cand[j];
+    int above = 0;
+    for (int d = 0; d < S * k; d++) above += cand[d] > mk;
+    if (mk && above < k) top_out(a, row, above, mk, whole);
+  }
+}
+
+// ---- short rows: a warp each, the row in its registers ----
+constexpr int kWarpCand = 128, kRowsPerBlock = 8;
+
+template <class T, int NE>
+__global__ void __launch_bounds__(32 * kRowsPerBlock) k_logp_warp(LogpArgs a) {
+  __shared__ u64 cands[kRowsPerBlock][kWarpCand];
+  __shared__ int counts[kRowsPerBlock];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, k = a.top;
+  const int64_t row64 = int64_t(blockIdx.x) * kRowsPerBlock + warp;
+  if (row64 >= a.rows) return;
+  const int row = int(row64);
+  const T* x = static_cast<const T*>(a.x) + row64 * a.stride;
+  float f[NE];
+#pragma unroll
+  for (int j = 0; j < NE; j++) {
+    const int i = lane + 32 * j;
+    f[j] = i < a.vocab ? wide(x[i]) : 0.f;
+  }
+  u64 mykey = 0;
+  {
+    float top = 0.f;
+    int at = -1;
+#pragma unroll
+    for (int j = 0; j < NE; j++) {
+      const int i = lane + 32 * j;
+      if (i < a.vocab && (at < 0 || !(f[j] <= top))) {
+        if (at < 0 || order(f[j]) > order(top)) {
+          top = f[j];
+          at = i;
+        }
+      }
+    }
+    if (at >= 0) mykey = key_of(top, at);
+  }
+  const u64 first = warp_max(mykey);
+  Share s = {unorder(uint32_t(first >> 32)), 0.f, 0.f};
+  const int skip = 0x7fffffff - int(uint32_t(first));
+#pragma unroll
+  for (int j = 0; j < NE; j++) {
+    const int i = lane + 32 * j;
+    if (i < a.vocab && i != skip) add(s, f[j]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s.z = __fadd_rn(s.z, __shfl_xor_sync(FULL, s.z, o));
+    s.t = __fadd_rn(s.t, __shfl_xor_sync(FULL, s.t, o));
+  }
+  if (lane == 0) row_out(a, row, x, s);
+  if (k == 0) return;
+  if (k == 1) {
+    if (lane == 0) top_out(a, row, 0, first, s);
+    return;
+  }
+  const uint32_t u = uint32_t(mykey >> 32);
+  uint32_t bound = 0;
+  for (int bit = 31; bit >= 0; bit--) {
+    const uint32_t c = bound | 1u << bit;
+    const int n = __popc(__ballot_sync(FULL, mykey != 0 && u >= c));
+    if (n >= k) {
+      bound = c;
+      if (n <= k + 4) break;
+    }
+  }
+  if (lane == 0) counts[warp] = 0;
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < NE; j++) {
+    const int i = lane + 32 * j;
+    if (i < a.vocab && order(f[j]) >= bound) {
+      const int p = atomicAdd(&counts[warp], 1);
+      if (p < kWarpCand) cands[warp][p] = key_of(f[j], i);
+    }
+  }
+  __syncwarp();
+  const int n = counts[warp];
+  if (n <= kWarpCand) {
+    for (int c = lane; c < n; c += 32) {
+      const u64 mk = cands[warp][c];
+      int above = 0;
+      for (int d = 0; d < n; d++) above += cands[warp][d] > mk;
+      if (above < k) top_out(a, row, above, mk, s);
+    }
+  } else {
+    u64 last = ~u64(0);
+    for (int r = 0; r < k; r++) {
+      u64 m = 0;
+#pragma unroll
+      for (int j = 0; j < NE; j++) {
+        const int i = lane + 32 * j;
+        const u64 q = i < a.vocab ? key_of(f[j], i) : 0;
+        if (q < last && q > m) m = q;
+      }
+      last = warp_max(m);
+      if (lane == 0) top_out(a, row, r, last, s);
+    }
+  }
+}
+
+constexpr int kSMs = 148;
+
+template <class T, int NT>
+cudaError_t rows_t(const LogpArgs& a, cudaStream_t st) {
+  // few rows: up to eight blocks to a row, each with a few vectors a thread
+  int S = 1;
+  while (S < 8 && int64_t(a.rows) * S < 2 * kSMs && a.vocab >= 2 * S * NT * int(16 / sizeof(T))) S *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(a.rows) * S);
+  cfg.blockDim = dim3(NT);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = unsigned(S);
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = S > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, k_logp<T, NT>, a, S);
+}
+
+template <class T>
+cudaError_t logp_t(const LogpArgs& a, cudaStream_t st) {
+  const unsigned blocks = unsigned((a.rows + kRowsPerBlock - 1) / kRowsPerBlock);
+  if (a.vocab <= 32 * 16)
+    k_logp_warp<T, 16><<<blocks, 32 * kRowsPerBlock, 0, st>>>(a);
+  else if (a.vocab <= 32 * 40)
+    k_logp_warp<T, 40><<<blocks, 32 * kRowsPerBlock, 0, st>>>(a);
+  else if (a.vocab <= 32 * 64)
+    k_logp_warp<T, 64><<<blocks, 32 * kRowsPerBlock, 0, st>>>(a);
+  else if (a.vocab < 16384)
+    return rows_t<T, 256>(a, st);
+  else
+    return rows_t<T, 512>(a, st);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_logp(const LogpArgs& a, int type, cudaStream_t st) {
+  return type == 0   ? logp_t<float>(a, st)
+         : type == 1 ? logp_t<__half>(a, st)
+                     : logp_t<__nv_bfloat16>(a, st);
+}
+
+}  // namespace grx

@@ -109,6 +109,129 @@ int grx_linear(const grx_weight* w, const float* x, int m, const float* bias, fl
 int grx_linear_q8_static(const grx_weight* w, const float* d_x, int m, const float* d_bias, float* d_dst,
                          void* stream);
 
+/* ------------------------------------------ 8-bit paged KV cache -------
+ * A key/value cache in pages, a byte a value: for hosts that run their own
+ * layers around the token loops' products (grx_linear) and keep many or
+ * long sequences, at a quarter of a float32 cache's memory and reads. No
+ * counterpart in the reference, whose caches are contiguous float32
+ * (pockettts/nn.go:113). grx_streams_create_kv8 runs the flow LM on one.
+ *
+ * Pages hold page_tokens tokens of every key/value head. The sequence i's
+ * token at position p lies in the page table[i·table_width + p/page_tokens]
+ * at the slot p % page_tokens; pages of a common beginning may stand in
+ * several rows of the table. A page and head has two scales, one for its
+ * keys and one for its values, and a byte q stands for q·scale.
+ *
+ * Device memory is the caller's: k and v [pages][kv_heads][page_tokens]
+ * [head_dim] int8 from 16-byte boundaries, scale [pages][kv_heads][2]
+ * float32 (keys, values) from an 8-byte boundary. Nothing needs clearing.
+ * head_dim is 64 or 128, page_tokens 16, 32 or 64. */
+#define GRX_F32 0 /* types of rows, numbered as in GGUF files */
+#define GRX_F16 1
+#define GRX_BF16 30
+typedef struct grx_kv8 {
+  int device;
+  int pages, page_tokens, kv_heads, head_dim;
+  int8_t *k, *v;
+  float* scale;
+} grx_kv8;
+
+/* The sequences of one call. Sequence i holds len[i] tokens, the new ones
+ * of this call among them; the call's rows row0[i] .. row0[i+1] − 1 are its
+ * last row0[i+1] − row0[i] tokens, in order. row0 NULL: one row for each
+ * sequence, row i for sequence i, and len[i] = 0 is a slot without tokens
+ * (nothing is appended; attention answers zeros). All arrays are device
+ * memory of the cache's device, read when the kernels run.
+ *
+ * rows bounds the row numbers, max_new a sequence's rows in the call (1 with
+ * row0 NULL). max_len is about how long the longest sequence is: it decides
+ * how the work is split, and no result depends on it. Rows behind the last
+ * sequence's are left as they are.
+ *
+ * The rotation, if rope is given: the pair of values (a, b) of a row at the
+ * position p becomes (a·c − b·s, a·s + b·c) with (c, s) = rope[p][j], j the
+ * pair's number: values 2j and 2j+1 (GRX_ROPE_PAIRS, as the flow LM pairs
+ * them, pockettts/nn.go:80-95) or j and j + head_dim/2 (GRX_ROPE_HALVES).
+ *
+ * Entries that do not fit (a row number or count outside what rows, max_new
+ * and len allow, a len past table_width pages or rope_positions, a page that
+ * is none of the cache's) touch no memory: the sequence, or the page's
+ * tokens, are left out, and *status, if given (device memory), becomes
+ * GRX_ERANGE. It is never cleared by a call. */
+#define GRX_ROPE_NONE 0
+#define GRX_ROPE_PAIRS 1
+#define GRX_ROPE_HALVES 2
+typedef struct grx_kv8_seqs {
+  int n;                     /* sequences, up to 65535 */
+  int table_width;           /* pages in a row of the table */
+  int rows, max_new, max_len;
+  const int* table;          /* [n][table_width] */
+  const int* len;            /* [n] */
+  const int* row0;           /* [n + 1], or NULL */
+  const int* first;          /* [n] or NULL (attention only): keys before first[i] are not seen */
+  const float* rope;         /* [rope_positions][head_dim/2][2] cos, sin, from a 16-byte boundary */
+  int rope_positions, rope_mode;
+  int* status;               /* one int, or NULL */
+} grx_kv8_seqs;
+
+/* Rows in memory: element e of head h of row r at r·row + h·head + e, in
+ * elements (any strides; multiples of 16 bytes load fastest). */
+
+/* Appends the rows' keys (rotated) and values to the cache. A page that
+ * gets new tokens has, for its keys and its values of each head, the new
+ * scale s' = max(s, a/127), a the largest magnitude among the new values
+ * and s the scale so far (0 when the page's first token is among the new);
+ * where s' > s, the bytes it held become rne(q·s/s'); the new ones are
+ * rne(x/s'). Quotients and roundings are done in 64 bits, so the bytes do
+ * not depend on how tokens of one call are spread over threads; a value
+ * that is not finite makes its page's scale NaN, until the page begins
+ * anew. A page that is written must belong to one sequence of the call
+ * (grx_kv8_check finds out). Work is queued on `stream` and not waited for;
+ * nothing is allocated and the caller's current device stays. The first
+ * call on a device sets up its kernels: make it outside a stream capture. */
+int grx_kv8_append(const grx_kv8* kv, const grx_kv8_seqs* s, int type, const void* k, int64_t k_row, int64_t k_head,
+                   const void* v, int64_t v_row, int64_t v_head, void* stream);
+/* The stored values of the rows' tokens (keys as rotated): q·scale rounded
+ * to the type. k or v may be NULL. */
+int grx_kv8_read(const grx_kv8* kv, const grx_kv8_seqs* s, int type, void* k, int64_t k_row, int64_t k_head, void* v,
+                 int64_t v_row, int64_t v_head, void* stream);
+/* Attention of the rows' queries over their sequences: heads query heads, a
+ * multiple of kv_heads (query head h reads key head h·kv_heads/heads), each
+ * query seeing the keys up to its own position, from first[i] on and, with
+ * window > 0, the last `window` of them. out = softmax(scale·q·k)·v, sums in
+ * 32 bits; the queries are rotated as the keys were. lse [rows][heads] (may
+ * be NULL) gets log Σ e^(scale·q·k). A query that sees no key answers zeros
+ * and −inf; one that is not finite, or sees a page whose scale is not,
+ * answers NaN. Results do not depend on timing. Queued on `stream`. */
+int grx_kv8_attend(const grx_kv8* kv, const grx_kv8_seqs* s, int type, int heads, const void* q, int64_t q_row,
+                   int64_t q_head, float scale, int window, void* out, int64_t out_row, int64_t out_head, float* lse,
+                   void* stream);
+/* The checks that the kernels make, on the host, with a message: here the
+ * arrays of s are HOST memory (rope and status are not read; needs no
+ * device). With writes != 0 also that no page this call would append to
+ * stands elsewhere in the table. 0, GRX_EINVAL or GRX_ERANGE. */
+int grx_kv8_check(const grx_kv8* kv, const grx_kv8_seqs* s, int writes);
+
+/* ------------------------------------------ token log probabilities ----
+ * What a model's logits say of given tokens: for scoring texts, for the
+ * confidence of a transcript, for alternatives. logits is device memory of
+ * `device`: `rows` rows of `vocab` values of `type`, row r at
+ * r·row_stride elements. Each of the outputs (device) may be NULL:
+ *   logprob [rows]: log softmax at targets[r] (NaN for a target outside the
+ *     vocabulary); needs targets [rows];
+ *   entropy [rows]: −Σ p log p, in nats;
+ *   top_ids, top_logprobs [rows][top]: the largest logits, the lower index
+ *     first among equals (NaN below −inf); top is 0 to 32 and at most vocab.
+ * A logit of −inf has probability 0. A row with a NaN, or whose largest
+ * logit is not finite, has no distribution: its numbers are NaN. Sums are
+ * 32 bits, of positive terms only (a sure row keeps its small numbers).
+ * Queued on `stream`; allocates nothing; the first call on a device outside
+ * a stream capture. grx_whisper_score asks this of a Whisper batch. */
+#define GRX_LOGPROBS_MAX_TOP 32
+int grx_logprobs(int device, int type, const void* logits, int rows, int vocab, int64_t row_stride,
+                 const int* targets, int top, float* logprob, float* entropy, int* top_ids, float* top_logprobs,
+                 void* stream);
+
 /* ------------------------------------------- Pocket TTS FlowLM ---------
  * pockettts.Model (pockettts/model.go:14) restricted to the flow LM and
  * its flow head; Mimi and the text path stay with the caller. */
