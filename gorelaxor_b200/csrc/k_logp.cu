@@ -6,16 +6,21 @@
 //   z = Σ e^(x_j − m),   t = Σ (m − x_j)·e^(x_j − m),
 // the log probability of token j is (x_j − m) − log1p(z) and the entropy is
 // log1p(z) + t/(1 + z). Every term is positive and the 1 is kept apart, so a
-// row whose model is sure loses nothing to cancellation. A share of a row is
-// (m, z, t) in 32 bits; two with m1 >= m2 and e = e^(m2 − m1) join as
-//   z = z1 + e·(1 + z2),   t = t1 + e·(t2 + (m1 − m2)·(1 + z2)).
+// row whose model is sure loses nothing to cancellation.
 //
-// The most likely tokens: each thread knows the largest of its own values
-// from the pass. The `top`-th largest of these is a bound that the answer
-// does not go below, so only the threads at or above it (about `top` of
-// hundreds) have their values looked at again, and the few values above the
-// bound are ranked. Values compare as (value, lower index first), each as
-// one 64-bit number; NaN counts below −inf.
+// In the pass each thread keeps the largest value m' of its own and sums over
+// all of them, largest included, moved to a new m' once for every few vectors
+// (no branch: a branch "only where the largest grows" is taken by some lane
+// of nearly every warp). Its sums hold a 1 that hides small terms only where
+// m' is about m. The threads with the largest m' are looked at a second time
+// anyway, for the most likely tokens, and their sums are then made anew
+// without the values equal to m.
+//
+// The most likely tokens: the `top`-th largest of the threads' m' is a bound
+// that the answer does not go below, so only the threads at or above it
+// (about `top` of hundreds) have their values looked at again, and the few
+// values above the bound are ranked. Values compare as (value, lower index
+// first), each as one 64-bit number; NaN counts below −inf.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -66,12 +71,14 @@ __device__ __forceinline__ float unorder(uint32_t u) {
 // (value, lower index first) as one number; 0 is no token.
 __device__ __forceinline__ u64 key_of(float x, int i) { return u64(order(x)) << 32 | uint32_t(0x7fffffff - i); }
 
-// A share of a row: the largest value (−inf: none), and the sums over the
+// A share of a row: its largest value (−inf: none), and the sums over the
 // others.
 struct Share {
   float m, z, t;
 };
 
+// Two shares with m1 >= m2 and e = e^(m2 − m1):
+//   z = z1 + e·(1 + z2),   t = t1 + e·(t2 + (m1 − m2)·(1 + z2)).
 __device__ __forceinline__ Share join(Share a, Share b) {
   if (b.m > a.m) {
     const Share c = a;
@@ -107,51 +114,62 @@ __device__ __forceinline__ u64 warp_max(u64 k) {
   for (int o = 16; o > 0; o >>= 1) k = max(k, __shfl_xor_sync(FULL, k, o));
   return k;
 }
-
-// One value other than the largest into the sums of a share.
-__device__ __forceinline__ void add(Share& s, float x) {
-  const float d = max_nan(__fsub_rn(x, s.m), kFar), e = ex2(__fmul_rn(d, kLog2e));
-  s.z = __fadd_rn(s.z, e);
-  s.t = __fmaf_rn(-d, e, s.t);
+__device__ __forceinline__ float warp_max(float m) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
+  return m;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(FULL, v, o));
+  return v;
 }
 
-// A thread's values as they come: their share, and the first of the largest.
+// One value into sums over e^(x − m), x <= m (or NaN: the sums become NaN).
+__device__ __forceinline__ void add(float& z, float& t, float x, float m) {
+  const float d = max_nan(__fsub_rn(x, m), kFar), e = ex2(__fmul_rn(d, kLog2e));
+  z = __fadd_rn(z, e);
+  t = __fmaf_rn(-d, e, t);
+}
+
+// A thread's values: the largest, and z and t over all of them.
 struct Run {
-  Share s = {ninf(), 0.f, 0.f};
-  float top = 0.f;
-  int at = -1;
+  float m = ninf(), z = 0.f, t = 0.f;
 };
 
-// U groups of V values; group u begins at the index i0 + u·step.
-template <int V, int U>
-__device__ __forceinline__ void take(Run& r, const float (&x)[U][V], int i0, int step) {
-  float c = x[0][0];
+// Values two by two, the sums in two halves: packed 32-bit operations, each
+// half rounded as one alone.
+template <int N>
+__device__ __forceinline__ void take(Run& r, const float (&x)[N]) {
+  float c = r.m;
 #pragma unroll
-  for (int u = 0; u < U; u++)
+  for (int j = 0; j < N; j++) c = fmaxf(c, x[j]);
+  // the sums so far, from r.m to c; without a finite value so far they are 0
+  // (or NaN), and without one now they stay that
+  const float up = r.m == c ? 0.f : fmaxf(__fsub_rn(r.m, c), kFar), k = ex2(__fmul_rn(up, kLog2e));
+  r.t = __fmul_rn(k, __fmaf_rn(-up, r.z, r.t));
+  r.z = __fmul_rn(k, r.z);
+  r.m = c;
+  const float mm = c == ninf() ? 0.f : c;
+  if constexpr (N % 2 == 0) {
+    f2 z = 0, t = 0;
+    const f2 nm = f2dup(-mm), l = f2dup(kLog2e), one = f2dup(-1.f);
 #pragma unroll
-    for (int j = 0; j < V; j++) c = fmaxf(c, x[u][j]);
-  if (r.at < 0 || !(c < r.top)) {
-    // a new largest value or its equal, or no number: one by one
+    for (int j = 0; j < N; j += 2) {
+      const f2 d = f2add(f2make(x[j], x[j + 1]), nm);
+      const f2 dc = f2make(max_nan(f2lo(d), kFar), max_nan(f2hi(d), kFar));
+      const f2 y = f2mul(dc, l);
+      const f2 e = f2make(ex2(f2lo(y)), ex2(f2hi(y)));
+      z = f2add(z, e);
+      t = f2fma(dc, e, t);
+    }
+    t = f2mul(t, one);
+    r.z = __fadd_rn(r.z, __fadd_rn(f2lo(z), f2hi(z)));
+    r.t = __fadd_rn(r.t, __fadd_rn(f2lo(t), f2hi(t)));
+  } else {
 #pragma unroll
-    for (int u = 0; u < U; u++)
-#pragma unroll
-      for (int j = 0; j < V; j++) {
-        const float v = x[u][j];
-        if (v > r.s.m)
-          r.s = join(Share{v, 0.f, 0.f}, r.s);
-        else if (v != ninf())
-          add(r.s, v);
-        if (r.at < 0 || order(v) > order(r.top)) {
-          r.top = v;
-          r.at = i0 + u * step + j;
-        }
-      }
-    return;
+    for (int j = 0; j < N; j++) add(r.z, r.t, x[j], mm);
   }
-#pragma unroll
-  for (int u = 0; u < U; u++)
-#pragma unroll
-    for (int j = 0; j < V; j++) add(r.s, x[u][j]);
 }
 
 template <class T>
@@ -214,12 +232,11 @@ constexpr int kCand = 1024;
 template <class T, int NT>
 __global__ void __launch_bounds__(NT) k_logp(LogpArgs a, int S) {
   constexpr int V = 16 / sizeof(T), U = 4, NW = NT / 32;
-  __shared__ Share ws[NW];
+  __shared__ float wm[NW], wz[NW], wt[NW];
   __shared__ u64 wk[NW];
   __shared__ u64 cand[kCand];
   __shared__ u64 best[kLogpMaxTop];
-  __shared__ int sel[NT];
-  __shared__ int nsel, ncand;
+  __shared__ int ncand, nties;
   __shared__ Share mine, whole;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int rank = S > 1 ? int(cluster_rank()) : 0, row = blockIdx.x / S, k = a.top;
@@ -231,98 +248,123 @@ __global__ void __launch_bounds__(NT) k_logp(LogpArgs a, int S) {
   // the values before and behind the vectors, one to a thread
   const bool in_head = rank == 0 && tid < head, in_tail = rank == S - 1 && tid < tail;
   const int at_tail = a.vocab - tail + tid;
-  if (tid == 0) nsel = ncand = 0;
+  if (tid == 0) ncand = nties = 0;
 
   Run r;
   int v = vb + tid;
   for (; v + (U - 1) * NT < ve; v += U * NT) {
-    float f[U][V];
+    float f[U * V];
 #pragma unroll
-    for (int u = 0; u < U; u++) load16(xv + int64_t(v + u * NT) * V, f[u]);
-    take<V, U>(r, f, head + v * V, NT * V);
+    for (int u = 0; u < U; u++) load16(xv + int64_t(v + u * NT) * V, f + u * V);
+    take(r, f);
   }
   for (; v < ve; v += NT) {
-    float f[1][V];
-    load16(xv + int64_t(v) * V, f[0]);
-    take<V, 1>(r, f, head + v * V, 0);
+    float f[V];
+    load16(xv + int64_t(v) * V, f);
+    take(r, f);
   }
   if (in_head) {
-    const float f[1][1] = {{wide(x[tid])}};
-    // an earlier index than the vectors': it wins a tie
-    const float t0 = r.top;
-    const int a0 = r.at;
-    take<1, 1>(r, f, tid, 0);
-    if (a0 >= 0 && order(f[0][0]) == order(t0)) r.at = tid;
+    const float f[1] = {wide(x[tid])};
+    take(r, f);
   }
   if (in_tail) {
-    const float f[1][1] = {{wide(x[at_tail])}};
-    take<1, 1>(r, f, at_tail, 0);
+    const float f[1] = {wide(x[at_tail])};
+    take(r, f);
   }
+  const bool some = vb + tid < ve || in_head || in_tail;
   {
-    const Share s = warp_join(r.s);
-    if (lane == 0) ws[warp] = s;
-  }
-  const u64 mykey = r.at >= 0 ? key_of(r.top, r.at) : 0;
-  if (k == 1) {
-    const u64 m = warp_max(mykey);
-    if (lane == 0) wk[warp] = m;
+    const float m = warp_max(r.m);
+    if (lane == 0) wm[warp] = m;
   }
   __syncthreads();
-  if (warp == 0) {
-    Share s = lane < NW ? ws[lane] : Share{ninf(), 0.f, 0.f};
-    s = warp_join(s);
-    if (lane == 0) mine = s;
-    if (k == 1) {
-      const u64 m = warp_max(lane < NW ? wk[lane] : 0);
-      if (lane == 0) best[0] = m;
-    }
-  }
+  float m = wm[0];
+#pragma unroll
+  for (int w = 1; w < NW; w++) m = fmaxf(m, wm[w]);
+  // the bound: the largest value, or the largest found, bit by bit, that
+  // `top` threads reach
+  const uint32_t u = order(r.m);
+  uint32_t bound = order(m);
   if (k > 1) {
-    // a bound: the largest found, bit by bit, that `k` threads reach
-    const uint32_t u = uint32_t(mykey >> 32);
-    uint32_t bound = 0;
+    bound = 0;
     for (int bit = 31; bit >= 0; bit--) {
       const uint32_t c = bound | 1u << bit;
-      const int n = __syncthreads_count(r.at >= 0 && u >= c);
+      const int n = __syncthreads_count(some && u >= c);
       if (n >= k) {
         bound = c;
         if (n <= k + 8) break;
       }
     }
-    if (tid < k) best[tid] = 0;
-    if (r.at >= 0 && u >= bound) sel[atomicAdd(&nsel, 1)] = tid;
-    auto offer = [&](float f, int i) {
-      if (order(f) >= bound) {
-        const int p = atomicAdd(&ncand, 1);
-        if (p < kCand) cand[p] = key_of(f, i);
-      }
-    };
-    __syncthreads();
-    if (in_head) offer(wide(x[tid]), tid);
-    if (in_tail) offer(wide(x[at_tail]), at_tail);
-    for (int j = warp; j < nsel; j += NW)
-      for (int w = vb + sel[j] + lane * NT; w < ve; w += 32 * NT) {
-        float f[V];
-        load16(xv + int64_t(w) * V, f);
+  }
+  const bool again = some && u >= bound;
+  if (tid < k) best[tid] = 0;
+  // The chosen threads' values once more, their warp to a thread's: where m
+  // is among them, their sums without the values equal to it (so no number
+  // depends on `top`); and the values that reach the bound.
+  const bool owner = some && r.m == m;
+  float z = 0.f, t = 0.f;
+  int ties = 0;
+  auto look = [&](float f, int i, bool sums) {
+    if (sums) {
+      if (f == m)
+        ties++;
+      else if (f != ninf())
+        add(z, t, f, m);
+    }
+    if (k && order(f) >= bound) {
+      const int p = atomicAdd(&ncand, 1);
+      if (p < kCand) cand[p] = key_of(f, i);
+    }
+  };
+  if (!owner) {
+    const float d = r.m == ninf() ? 0.f : fmaxf(__fsub_rn(r.m, m), kFar), e = ex2(__fmul_rn(d, kLog2e));
+    t = __fmul_rn(e, __fmaf_rn(-d, r.z, r.t));
+    z = __fmul_rn(e, r.z);
+  }
+  if (again && in_head) look(wide(x[tid]), tid, owner);
+  if (again && in_tail) look(wide(x[at_tail]), at_tail, owner);
+  const uint32_t owners = __ballot_sync(FULL, owner);
+  for (uint32_t chosen = __ballot_sync(FULL, again); chosen; chosen &= chosen - 1) {
+    const int j = __ffs(chosen) - 1;
+    const bool sums = owners >> j & 1;
+    for (int w = vb + warp * 32 + j + lane * NT; w < ve; w += 32 * NT) {
+      float f[V];
+      load16(xv + int64_t(w) * V, f);
 #pragma unroll
-        for (int e = 0; e < V; e++) offer(f[e], head + w * V + e);
-      }
-    __syncthreads();
-    if (ncand <= kCand) {
-      for (int c = tid; c < ncand; c += NT) {
+      for (int e = 0; e < V; e++) look(f[e], head + w * V + e, sums);
+    }
+  }
+  z = warp_sum(z);
+  t = warp_sum(t);
+  if (ties) atomicAdd(&nties, ties);
+  if (lane == 0) {
+    wz[warp] = z;
+    wt[warp] = t;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    z = warp_sum(lane < NW ? wz[lane] : 0.f);
+    t = warp_sum(lane < NW ? wt[lane] : 0.f);
+    // equals of m but one count 1 each, with no gap; −inf counts nothing
+    if (lane == 0) mine = Share{m, m == ninf() ? z : __fadd_rn(z, float(max(nties, 1) - 1)), t};
+  }
+  if (k) {
+    const int n = ncand, all = (ve - vb) * V + (rank == 0 ? head : 0) + (rank == S - 1 ? tail : 0);
+    if (n >= min(k, all) && n <= kCand) {
+      for (int c = tid; c < n; c += NT) {
         const u64 mk = cand[c];
         int above = 0;
-        for (int d = 0; d < ncand; d++) above += cand[d] > mk;
+        for (int d = 0; d < n; d++) above += cand[d] > mk;
         if (above < k) best[above] = mk;
       }
     } else {
-      // more equals than the list takes: the largest below the last, k times
+      // More equals than the list takes (or values that are no number among
+      // the threads' counted): the largest below the last, k times.
       u64 last = ~u64(0);
-      for (int n = 0; n < k; n++) {
-        u64 m = 0;
+      for (int c = 0; c < k; c++) {
+        u64 q = 0;
         auto see = [&](float f, int i) {
-          const u64 q = key_of(f, i);
-          if (q < last && q > m) m = q;
+          const u64 y = key_of(f, i);
+          if (y < last && y > q) q = y;
         };
         if (in_head) see(wide(x[tid]), tid);
         if (in_tail) see(wide(x[at_tail]), at_tail);
@@ -332,13 +374,13 @@ __global__ void __launch_bounds__(NT) k_logp(LogpArgs a, int S) {
 #pragma unroll
           for (int e = 0; e < V; e++) see(f[e], head + w * V + e);
         }
-        m = warp_max(m);
-        if (lane == 0) wk[warp] = m;
+        q = warp_max(q);
+        if (lane == 0) wk[warp] = q;
         __syncthreads();
         last = 0;
         for (int w = 0; w < NW; w++) last = max(last, wk[w]);
         __syncthreads();
-        if (tid == 0) best[n] = last;
+        if (tid == 0) best[c] = last;
       }
     }
   }
@@ -373,7 +415,7 @@ __global__ void __launch_bounds__(NT) k_logp(LogpArgs a, int S) {
 constexpr int kWarpCand = 128, kRowsPerBlock = 8;
 
 template <class T, int NE>
-__global__ void __launch_bounds__(32 * kRowsPerBlock) k_logp_warp(LogpArgs a) {
+__global__ void __launch_bounds__(32 * kRowsPerBlock, 2) k_logp_warp(LogpArgs a) {
   __shared__ u64 cands[kRowsPerBlock][kWarpCand];
   __shared__ int counts[kRowsPerBlock];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, k = a.top;
@@ -381,52 +423,47 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock) k_logp_warp(LogpArgs a) {
   if (row64 >= a.rows) return;
   const int row = int(row64);
   const T* x = static_cast<const T*>(a.x) + row64 * a.stride;
+  // values behind the row are −inf: they count nothing anywhere but among
+  // the candidates, which look at the index
   float f[NE];
 #pragma unroll
-  for (int j = 0; j < NE; j++) {
-    const int i = lane + 32 * j;
-    f[j] = i < a.vocab ? wide(x[i]) : 0.f;
-  }
-  u64 mykey = 0;
-  {
-    float top = 0.f;
-    int at = -1;
+  for (int j = 0; j < NE; j++) f[j] = lane + 32 * j < a.vocab ? wide(x[lane + 32 * j]) : ninf();
+  float mine = f[0];
 #pragma unroll
-    for (int j = 0; j < NE; j++) {
-      const int i = lane + 32 * j;
-      if (i < a.vocab && (at < 0 || !(f[j] <= top))) {
-        if (at < 0 || order(f[j]) > order(top)) {
-          top = f[j];
-          at = i;
-        }
-      }
+  for (int j = 1; j < NE; j++) mine = fmaxf(mine, f[j]);
+  if (isnan(mine)) mine = ninf();
+  const float m = warp_max(mine);
+  Share s = {m, 0.f, 0.f};
+  int ties = 0, at = 0x7fffffff;
+#pragma unroll
+  for (int j = NE - 1; j >= 0; j--) {
+    if (32 * j >= a.vocab) continue;
+    const float d = max_nan(__fsub_rn(f[j], m), kFar);
+    const bool tie = f[j] == m;
+    const float e = tie ? 0.f : ex2(__fmul_rn(d, kLog2e));
+    s.z = __fadd_rn(s.z, e);
+    s.t = __fmaf_rn(-d, e, s.t);
+    if (tie) {
+      ties++;
+      at = lane + 32 * j;
     }
-    if (at >= 0) mykey = key_of(top, at);
   }
-  const u64 first = warp_max(mykey);
-  Share s = {unorder(uint32_t(first >> 32)), 0.f, 0.f};
-  const int skip = 0x7fffffff - int(uint32_t(first));
-#pragma unroll
-  for (int j = 0; j < NE; j++) {
-    const int i = lane + 32 * j;
-    if (i < a.vocab && i != skip) add(s, f[j]);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    s.z = __fadd_rn(s.z, __shfl_xor_sync(FULL, s.z, o));
-    s.t = __fadd_rn(s.t, __shfl_xor_sync(FULL, s.t, o));
-  }
+  s.z = warp_sum(s.z);
+  s.t = warp_sum(s.t);
+  ties = __reduce_add_sync(FULL, ties);
+  s.z = __fadd_rn(s.z, float(max(ties, 1) - 1));
   if (lane == 0) row_out(a, row, x, s);
   if (k == 0) return;
-  if (k == 1) {
-    if (lane == 0) top_out(a, row, 0, first, s);
+  if (k == 1 && isfinite(m)) {
+    at = __reduce_min_sync(FULL, at);
+    if (lane == 0) top_out(a, row, 0, key_of(m, at), s);
     return;
   }
-  const uint32_t u = uint32_t(mykey >> 32);
+  const uint32_t u = order(mine);
   uint32_t bound = 0;
   for (int bit = 31; bit >= 0; bit--) {
     const uint32_t c = bound | 1u << bit;
-    const int n = __popc(__ballot_sync(FULL, mykey != 0 && u >= c));
+    const int n = __popc(__ballot_sync(FULL, lane < a.vocab && u >= c));
     if (n >= k) {
       bound = c;
       if (n <= k + 4) break;
@@ -444,7 +481,7 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock) k_logp_warp(LogpArgs a) {
   }
   __syncwarp();
   const int n = counts[warp];
-  if (n <= kWarpCand) {
+  if (n >= k && n <= kWarpCand) {
     for (int c = lane; c < n; c += 32) {
       const u64 mk = cands[warp][c];
       int above = 0;
@@ -454,14 +491,14 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock) k_logp_warp(LogpArgs a) {
   } else {
     u64 last = ~u64(0);
     for (int r = 0; r < k; r++) {
-      u64 m = 0;
+      u64 q = 0;
 #pragma unroll
       for (int j = 0; j < NE; j++) {
         const int i = lane + 32 * j;
-        const u64 q = i < a.vocab ? key_of(f[j], i) : 0;
-        if (q < last && q > m) m = q;
+        const u64 y = i < a.vocab ? key_of(f[j], i) : 0;
+        if (y < last && y > q) q = y;
       }
-      last = warp_max(m);
+      last = warp_max(q);
       if (lane == 0) top_out(a, row, r, last, s);
     }
   }
