@@ -291,31 +291,32 @@ cudaError_t read_t(const Kv8Args& a, const Kv8Rows& k, const Kv8Rows& v, cudaStr
 // ------------------------------------------------------------- attend ----
 //
 // One pass over a sequence's keys and values with the running maximum and
-// sum of the softmax, on the tensor cores' integer and bfloat16 products,
-// with sixteen keys as a product's rows and eight queries as its columns.
+// sum of the softmax, on the tensor cores' integer and half products, with
+// sixteen keys as a product's rows and eight queries as its columns.
 //
 // Scores. A query's values become whole numbers of amax/2^22, written as
-// three signed digits in base 256, so the products with the cache's bytes
-// are exact integer products (m16n8k32) straight from the bytes as they were
-// loaded: no conversion of a key, and 32-bit accuracy (2^-23 of the largest
-// query value).
-// Values. p·s_v, with the page's value scale in it, is split into bfloat16
-// numbers: three for float32 outputs (24 bits, what a float32 weight has; two
-// measured 2.5e-6 of the outputs' norm off the 64-bit result, against 2.5e-7
-// for float32 arithmetic), two for 16-bit ones (2^-17 of each weight, far
-// below the output's own rounding). A byte is exact in bfloat16: with 0x43 above the low seven bits and 0x43 above the sign bit,
-// the difference of the two numbers (128 + low) − (128 or 256) is the byte.
+// three signed digits in base 256, so the products with the cache's bytes are
+// exact integer products (m16n8k32) straight from the bytes as they were
+// loaded: no conversion of a key, and 32-bit scores. (Two digits would do
+// for 16-bit outputs, not for lse.)
+// Values. A byte is exact in float16: below 0x64 its bits ^ 0x80 are the
+// number 1024 + 128 + byte, and one subtraction leaves it. The weight
+// w = p·s_v/W, with W the largest value scale so far, is a float16 for 16-bit
+// outputs (2^-11 of each weight, what a float16 output is rounded by) and the
+// sum of two for float32 ones (2^-25 of the largest weight).
 //
 // Layout. A warp takes sixteen tokens at a time, straight from global
 // memory into the registers of the product's operands: a key row's bytes
 // are spread over four lanes, sixteen consecutive ones each, a value row's
-// over eight. No shared memory in the loop and no synchronisation: four
-// warps of a block, and the blocks of a cluster, take separate stretches of
-// the keys and are joined at the end through (distributed) shared memory.
-// The maximum moves only when a score passes it by 2^8 (the weights stay
-// far from overflow), so most steps need no exchange between lanes.
-constexpr int kWarps = 4;
+// over eight. No shared memory in the loop and no synchronisation: WU warps
+// of a block, and the blocks of a cluster, take separate stretches of the
+// keys and are joined at the end through (distributed) shared memory; with
+// WU = 1 each warp has a unit of its own and writes it out. The maximum
+// moves only when a score passes it by 2^8 (the weights stay far from
+// overflow), so most steps need no exchange between lanes.
 
+__device__ __forceinline__ float ninf() { return __int_as_float(0xff800000); }
+__device__ __forceinline__ float qnan() { return __int_as_float(0x7fc00000); }
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -327,9 +328,9 @@ __device__ __forceinline__ void mma_s8(int* c, uint32_t a0, uint32_t a1, uint32_
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_bf16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+__device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -338,19 +339,18 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// Two floats as bfloat16s, lo in the low half.
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+// Two floats as float16s, lo in the low half.
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t y;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
   return y;
 }
-// Byte b (0..3) of x and of y as bfloat16s, x's in the low half.
+// Byte b (0..3) of x and of y as float16s, x's in the low half.
 template <int B>
-__device__ __forceinline__ uint32_t bytes_bf16(uint32_t x, uint32_t y) {
-  const uint32_t p = __byte_perm(x, y, B | (4 + B) << 8);
-  const uint32_t m = (p & 0x007f007fu) | 0x43004300u, s = (p & 0x00800080u) | 0x43004300u;
+__device__ __forceinline__ uint32_t bytes_f16(uint32_t x, uint32_t y) {
+  const uint32_t u = (__byte_perm(x, y, B | (4 + B) << 8) & 0x00ff00ffu) ^ 0x64806480u;
   uint32_t d;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(m), "r"(s));
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(u), "r"(0xe480e480u));
   return d;
 }
 
@@ -378,63 +378,76 @@ struct Tile {  // sixteen tokens as the products take them
   float sk, sv;
 };
 
-template <int D, int NQ>
-constexpr size_t attend_smem() {
-  return size_t(NQ) * 3 * (D / 64) * 32 * 16   // query digits
-         + size_t(8 * NQ) * (4 + 4)            // factors, positions
-         + size_t(kWarps) * 8 * NQ * (D + 2) * 4  // the warps' sums, maxima and outputs
-         + size_t(8 * NQ) * (D + 2) * 4;       // the block's
-}
+// Warps of a block, tiles that a warp has under way, blocks that an SM
+// shall hold: by the registers that a tile and the outputs take.
+template <int D, int NQ, int WU>
+struct Shape {
+  static constexpr int warps = WU == 1 ? 4 : WU;
+  static constexpr int ahead = D == 64 && NQ == 1 ? 3 : 2;
+  static constexpr int blocks = WU > 4 ? 1 : NQ > 1 ? 2 : D == 64 ? 4 : 3;
+  static constexpr size_t digits = size_t(NQ) * 3 * (D / 64) * 32 * 16;  // bytes, a unit's
+  static constexpr size_t smem =
+      (WU == 1 ? warps : 1) * (digits + size_t(8 * NQ) * 8) + (WU == 1 ? 0 : size_t(warps + 1) * 8 * NQ * (D + 2) * 4);
+};
 
-template <int D, int NQ, int NP>
-__global__ void __launch_bounds__(32 * kWarps, NQ == 1 ? 4 : 2)
-    k_kv8_attend(Kv8Args a, Kv8Attend t, int type, int S, int qtiles, bool vec) {
-  constexpr int NR = 8 * NQ, H2 = D / 64;
+// NP: float16s of a weight.
+template <int D, int NQ, int NP, int WU>
+__global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>::blocks)
+    k_kv8_attend(Kv8Args a, Kv8Attend t, int type, int S, int qtiles, int units, bool vec, bool ovec) {
+  using Sh = Shape<D, NQ, WU>;
+  constexpr int NR = 8 * NQ, H2 = D / 64, PF = Sh::ahead;
   extern __shared__ __align__(16) uint8_t smem[];
-  uint4* qd = reinterpret_cast<uint4*>(smem);                 // [NQ][3][H2][32]
-  float* qf = reinterpret_cast<float*>(qd + NQ * 3 * H2 * 32);  // [NR]
-  int* qpos = reinterpret_cast<int*>(qf + NR);                // [NR]
-  float* wm = reinterpret_cast<float*>(qpos + NR);            // [kWarps][NR]
-  float* wl = wm + kWarps * NR;
-  float* wo = wl + kWarps * NR;                               // [kWarps][NR][D]
-  float* bm = wo + kWarps * NR * D;                           // [NR], [NR], [NR][D]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tg = lane & 3;
+  uint8_t* mine = smem + (WU == 1 ? warp * (Sh::digits + NR * 8) : 0);
+  uint4* qd = reinterpret_cast<uint4*>(mine);                       // [NQ][3][H2][32]
+  float* qf = reinterpret_cast<float*>(mine + Sh::digits);          // [NR]
+  int* qpos = reinterpret_cast<int*>(qf + NR);                      // [NR]
+  float* wm = reinterpret_cast<float*>(qpos + NR);                  // [WU][NR], WU > 1
+  float* wl = wm + WU * NR;
+  float* wo = wl + WU * NR;                                         // [WU][NR][D]
+  float* bm = wo + WU * NR * D;                                     // [NR], [NR], [NR][D]
   float* bl = bm + NR;
   float* bo = bl + NR;
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tg = lane & 3;
   const int rank = S > 1 ? int(cluster_rank()) : 0;
-  const int64_t unit = blockIdx.x / S;
-  const int h = int(unit % a.heads), qt = int(unit / a.heads % qtiles), i = int(unit / a.heads / qtiles);
+  const int unit = WU == 1 ? blockIdx.x * Sh::warps + warp : blockIdx.x / S;
+  if (unit >= units) return;
+  const int h = unit % a.heads, qt = unit / a.heads % qtiles, i = unit / a.heads / qtiles;
   const int group = t.heads / a.heads;
   const Kv8Span sp = kv8_span(a, i);
   if (!sp.ok) {
-    if (tid == 0) report(a);
+    if ((WU == 1 ? lane : tid) == 0) report(a);
     return;  // every block of the cluster: it has one sequence
   }
-  const int r0 = qt * NR, nrow = min(NR, sp.T * group - r0);  // this block's query rows
+  const int r0 = qt * NR, nrow = min(NR, sp.T * group - r0);  // this unit's query rows
   if (nrow <= 0) return;
   const int p0 = sp.len - sp.T;
   const int pmin = p0 + r0 / group, pmax = p0 + (r0 + nrow - 1) / group;
   const int first = a.first ? max(0, a.first[i]) : 0;
   const int klo = max(first, t.window > 0 ? pmin - t.window + 1 : 0), khi = pmax + 1;
   const int cb = klo >> 4, ce = max(cb, (khi + 15) >> 4);
-  const int per = (ce - cb + S * kWarps - 1) / (S * kWarps);
-  const int c0 = min(ce, cb + (rank * kWarps + warp) * per), c1 = min(ce, c0 + per);
+  const int per = (ce - cb + S * WU - 1) / (S * WU);
+  const int c0 = min(ce, cb + (WU == 1 ? 0 : rank * WU + warp) * per), c1 = min(ce, c0 + per);
 
   // --- the pages ahead: lane l holds page and scales of the tile wbase + l ---
   const int cshift = a.plog - 4;
-  const float2* scales = reinterpret_cast<const float2*>(a.scale);
+  const float2* scales = reinterpret_cast<const float2*>(a.scale) + h;
   auto page_of = [&](int c) { return c < c1 ? kv8_page(a, i, c >> cshift) : -1; };
-  auto scale_of = [&](int page) {
-    return page >= 0 ? scales[int64_t(page) * a.heads + h] : make_float2(0.f, 0.f);
+  auto scale_of = [&](int page) {  // one that is not finite as NaN; −inf stands for no page
+    if (page < 0) return make_float2(ninf(), 0.f);
+    const float2 s = scales[int64_t(page) * a.heads];
+    return make_float2(isfinite(s.x) ? s.x : qnan(), isfinite(s.y) ? s.y : qnan());
   };
   int wbase = c0;
   int pg = page_of(c0 + lane);
   if (pg < 0 && c0 + lane < c1) report(a);
   float2 sc = scale_of(pg);
   int pg1 = page_of(c0 + 32 + lane);
+  const int8_t* kbase = a.k + ((int64_t(h) << a.plog) + g) * D + 16 * tg;
+  const int8_t* vbase = a.v + ((int64_t(h) << a.plog) + 2 * tg) * D + g * (D / 8);
+  const int64_t pbytes = (int64_t(a.heads) << a.plog) * D;
 
-  Tile<D> buf[2];
+  Tile<D> buf[PF];
   auto fetch = [&](Tile<D>& b, int c) {
     if (c >= c1) return;
     if (c - wbase == 32) {
@@ -447,24 +460,20 @@ __global__ void __launch_bounds__(32 * kWarps, NQ == 1 ? 4 : 2)
     const int page = __shfl_sync(FULL, pg, c - wbase);
     b.sk = __shfl_sync(FULL, sc.x, c - wbase);
     b.sv = __shfl_sync(FULL, sc.y, c - wbase);
-    if (page < 0) {
-      // no such page: its tokens are not there
-      b.sk = __int_as_float(0xff800000);
+    if (page < 0) {  // no such page: its tokens are not there (sk is −inf)
 #pragma unroll
       for (int j = 0; j < H2; j++) b.k[0][j] = b.k[1][j] = make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int j = 0; j < D / 32; j++) b.v[j] = make_uint4(0, 0, 0, 0);
       return;
     }
-    const int slot = (c << 4) & ((1 << a.plog) - 1);
-    const int64_t at = (((int64_t(page) * a.heads + h) << a.plog) + slot) * D;
-    const int8_t* kp = a.k + at + g * D + 16 * tg;
+    const int64_t at = page * pbytes + ((c << 4) & ((1 << a.plog) - 1)) * D;
+    const int8_t *kp = kbase + at, *vp = vbase + at;
 #pragma unroll
     for (int r = 0; r < 2; r++)
 #pragma unroll
       for (int j = 0; j < H2; j++)
         b.k[r][j] = __ldg(reinterpret_cast<const uint4*>(kp + r * 8 * D + j * 64));
-    const int8_t* vp = a.v + at + 2 * tg * D + g * (D / 8);
     if constexpr (D == 64) {
       const uint2 x0 = __ldg(reinterpret_cast<const uint2*>(vp)), x1 = __ldg(reinterpret_cast<const uint2*>(vp + D));
       const uint2 x2 = __ldg(reinterpret_cast<const uint2*>(vp + 8 * D)),
@@ -478,11 +487,12 @@ __global__ void __launch_bounds__(32 * kWarps, NQ == 1 ? 4 : 2)
       b.v[3] = __ldg(reinterpret_cast<const uint4*>(vp + 9 * D));
     }
   };
-  fetch(buf[0], c0);
-  fetch(buf[1], c0 + 1);
+#pragma unroll
+  for (int u = 0; u < PF; u++) fetch(buf[u], c0 + u);
 
   // --- the queries: rotated, and written as digits ---
-  for (int nq = warp; nq < NQ; nq += kWarps) {
+  constexpr float kUnits = 4194304.f;
+  for (int nq = WU == 1 ? 0 : warp; nq < NQ; nq += WU) {
     const int r = nq * 8 + g;  // this lane's query
     const bool there = r < nrow;
     const int tq = there ? (r0 + r) / group : 0, hq = h * group + (there ? (r0 + r) % group : 0);
@@ -547,17 +557,21 @@ __global__ void __launch_bounds__(32 * kWarps, NQ == 1 ? 4 : 2)
     amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, 2));
     finite = ((__ballot_sync(FULL, finite) >> (lane & ~3)) & 15) == 15;
+    // tiny rows are lifted first, so that neither quotient leaves the range
+    const float lift = amax < 1e-30f ? 1e30f : 1.f;
+    const float to = finite && amax > 0.f ? __fdiv_rn(kUnits, __fmul_rn(amax, lift)) : 0.f;
 #pragma unroll
     for (int j = 0; j < H2; j++) {
       uint32_t w[3][4] = {};
 #pragma unroll
       for (int e = 0; e < 16; e++) {
-        const float y = finite && amax > 0.f ? __fmul_rn(__fdiv_rn(x[j][e], amax), 4194304.f) : 0.f;
-        const int n = __float2int_rn(y);
-        const int d0 = int8_t(n), n1 = (n - d0) >> 8, d1 = int8_t(n1), d2 = (n1 - d1) >> 8;
-        w[0][e / 4] |= uint32_t(d0 & 255) << (8 * (e % 4));
-        w[1][e / 4] |= uint32_t(d1 & 255) << (8 * (e % 4));
-        w[2][e / 4] |= uint32_t(d2 & 255) << (8 * (e % 4));
+        int n = finite ? __float2int_rn(__fmul_rn(__fmul_rn(x[j][e], lift), to)) : 0;
+#pragma unroll
+        for (int d = 0; d < 3; d++) {
+          const int digit = d < 2 ? int(int8_t(n)) : n;
+          n = (n - digit) >> 8;
+          w[d][e / 4] |= uint32_t(digit & 255) << (8 * (e % 4));
+        }
       }
 #pragma unroll
       for (int d = 0; d < 3; d++)
@@ -565,108 +579,132 @@ __global__ void __launch_bounds__(32 * kWarps, NQ == 1 ? 4 : 2)
     }
     if (tg == 0) {
       // scores in units of log 2; a query that is no number has no score
-      const float f = __fmul_rn(__fmul_rn(amax, 1.f / 4194304.f), __fmul_rn(t.scale, 1.44269504f));
-      qf[r] = finite ? f : __int_as_float(0x7fc00000);
+      const float f = __fmul_rn(__fmul_rn(amax, 1.f / kUnits), __fmul_rn(t.scale, 1.44269504f));
+      qf[r] = finite ? f : qnan();
       qpos[r] = there ? pos : -1;
     }
   }
-  __syncthreads();
+  if (WU == 1)
+    __syncwarp();
+  else
+    __syncthreads();
 
   // --- the pass over the keys ---
   float o[NQ][D / 16][4] = {};
-  float m[NQ][2], l[NQ][2] = {}, f[NQ][2];
+  float ref[NQ][2], l[NQ][2] = {}, f[NQ][2];
+  float W = 0.f, toW = 0.f;  // the value scales' reference, and 1/W
 #pragma unroll
   for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-      m[nq][j] = __int_as_float(0xff800000);
+      ref[nq][j] = ninf();
       f[nq][j] = qf[nq * 8 + 2 * tg + j];
     }
-  // tiles that every query of the block sees whole
+  // tiles that every query of the unit sees whole
   const int in_lo = max(first, t.window > 0 ? pmax - t.window + 1 : 0), in_hi = pmin;
   auto step = [&](const Tile<D>& b, int c) {
-    const bool edge = c * 16 < in_lo || c * 16 + 15 > in_hi || nrow < NR || b.sk == __int_as_float(0xff800000);
+    const bool edge = c * 16 < in_lo || c * 16 + 15 > in_hi || b.sk == ninf();
+    if (fabsf(b.sv) > W) {  // a larger scale, in every lane alike: twice it, to move less often
+      const float w = fminf(fmaxf(__fmul_rn(2.f, fabsf(b.sv)), 1.17549435e-38f), 3.4e38f), k = __fdiv_rn(W, w);
+      W = w;
+      toW = __fdiv_rn(1.f, w);
+#pragma unroll
+      for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+        for (int mt = 0; mt < D / 16; mt++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) o[nq][mt][j] = __fmul_rn(o[nq][mt][j], k);
+    }
+    const float sv = __fmul_rn(b.sv, toW);
     uint32_t pw[NQ][NP][2];  // the weights, transposed: queries in rows
 #pragma unroll
     for (int nq = 0; nq < NQ; nq++) {
-      int acc[3][4];
-#pragma unroll
-      for (int d = 0; d < 3; d++) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) acc[d][j] = MAGIC_BITS;
+      int hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+      auto digit = [&](int* acc, int d) {
 #pragma unroll
         for (int j = 0; j < H2; j++) {
           const uint4 q = qd[((nq * 3 + d) * H2 + j) * 32 + lane];
-          mma_s8(acc[d], b.k[0][j].x, b.k[1][j].x, b.k[0][j].y, b.k[1][j].y, q.x, q.y);
-          mma_s8(acc[d], b.k[0][j].z, b.k[1][j].z, b.k[0][j].w, b.k[1][j].w, q.z, q.w);
+          mma_s8(acc, b.k[0][j].x, b.k[1][j].x, b.k[0][j].y, b.k[1][j].y, q.x, q.y);
+          mma_s8(acc, b.k[0][j].z, b.k[1][j].z, b.k[0][j].w, b.k[1][j].w, q.z, q.w);
         }
-      }
-      float s[4];
+      };
+      // the two upper digits share an accumulator: 128·128·16512 < 2^31
+      digit(hi, 2);
+#pragma unroll
+      for (int j = 0; j < 4; j++) hi[j] <<= 8;
+      digit(hi, 1);
+      digit(lo, 0);
+      float s[4], x[4];
+      const float fs[2] = {__fmul_rn(f[nq][0], b.sk), __fmul_rn(f[nq][1], b.sk)};
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const float a0 = __fsub_rn(__int_as_float(acc[0][j]), MAGIC), a1 = __fsub_rn(__int_as_float(acc[1][j]), MAGIC),
-                    a2 = __fsub_rn(__int_as_float(acc[2][j]), MAGIC);
-        s[j] = __fmul_rn(__fmaf_rn(65536.f, a2, __fmaf_rn(256.f, a1, a0)), __fmul_rn(f[nq][j & 1], b.sk));
+        s[j] = __fmaf_rn(256.f, float(hi[j]), float(lo[j]));
+        x[j] = __fmaf_rn(s[j], fs[j & 1], -ref[nq][j & 1]);
       }
       bool hide[4] = {false, false, false, false};
       if (edge) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           const int p = qpos[nq * 8 + 2 * tg + (j & 1)], key = c * 16 + g + (j >> 1) * 8;
-          hide[j] = key > p || key < first || (t.window > 0 && key <= p - t.window) ||
-                    b.sk == __int_as_float(0xff800000);
-          if (hide[j]) s[j] = __int_as_float(0xff800000);
+          hide[j] = key > p || key < first || (t.window > 0 && key <= p - t.window) || b.sk == ninf();
+          if (hide[j]) x[j] = ninf();
         }
       }
-      const float over = fmaxf(fmaxf(__fsub_rn(s[0], m[nq][0]), __fsub_rn(s[2], m[nq][0])),
-                               fmaxf(__fsub_rn(s[1], m[nq][1]), __fsub_rn(s[3], m[nq][1])));
-      if (__any_sync(FULL, over > 8.f)) {
+      // before its first key a query's reference is −inf, and any score above
+      if (__any_sync(FULL, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > 8.f)) {
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-          float x = fmaxf(s[j], s[j + 2]);
+          float m = fmaxf(hide[j] ? ninf() : __fmul_rn(s[j], fs[j]), hide[j + 2] ? ninf() : __fmul_rn(s[j + 2], fs[j]));
 #pragma unroll
-          for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(FULL, x, d));
-          x = fmaxf(x, m[nq][j]);
-          const float r = m[nq][j] == x ? 1.f : ex2(__fsub_rn(m[nq][j], x));
-          m[nq][j] = x;
+          for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, d));
+          m = fmaxf(m, ref[nq][j]);
+          const float r = ref[nq][j] == m ? 1.f : ex2(__fsub_rn(ref[nq][j], m));
+          ref[nq][j] = m;
           l[nq][j] = __fmul_rn(l[nq][j], r);
 #pragma unroll
           for (int mt = 0; mt < D / 16; mt++) {
             o[nq][mt][j] = __fmul_rn(o[nq][mt][j], r);
             o[nq][mt][j + 2] = __fmul_rn(o[nq][mt][j + 2], r);
           }
+          x[j] = hide[j] ? ninf() : __fmaf_rn(s[j], fs[j], -m);
+          x[j + 2] = hide[j + 2] ? ninf() : __fmaf_rn(s[j + 2], fs[j], -m);
         }
       }
       float w[4];
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        // before the first key that it sees a query has no maximum
-        const float ref = m[nq][j & 1] == __int_as_float(0xff800000) ? 0.f : m[nq][j & 1];
-        const float p = ex2(__fsub_rn(s[j], ref));
+        const float p = ex2(x[j]);
         l[nq][j & 1] = __fadd_rn(l[nq][j & 1], p);
-        w[j] = hide[j] ? 0.f : __fmul_rn(p, b.sv);
+        w[j] = __fmul_rn(p, sv);
+      }
+      if (edge) {  // what is not seen counts nothing, whatever its page's scale
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (hide[j]) w[j] = 0.f;
       }
 #pragma unroll
       for (int n = 0; n < NP; n++)
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-          const uint32_t h = pack_bf16(w[2 * j], w[2 * j + 1]);
-          w[2 * j] = __fsub_rn(w[2 * j], bits_f(h << 16));
-          w[2 * j + 1] = __fsub_rn(w[2 * j + 1], bits_f(h & 0xffff0000u));
-          pw[nq][n][j] = transpose8(h);
+          const uint32_t y = pack_f16(w[2 * j], w[2 * j + 1]);
+          if (n + 1 < NP) {
+            w[2 * j] = __fsub_rn(w[2 * j], __half2float(__ushort_as_half(y & 0xffff)));
+            w[2 * j + 1] = __fsub_rn(w[2 * j + 1], __half2float(__ushort_as_half(y >> 16)));
+          }
+          pw[nq][n][j] = transpose8(y);
         }
     }
     const uint32_t* vw = &b.v[0].x;  // four tokens of D/32 words
-    constexpr int W = D / 32;
+    constexpr int WV = D / 32;
     auto values = [&](auto MT) {
       constexpr int mt = decltype(MT)::value, wd = mt / 2, by = 2 * (mt % 2);
-      const uint32_t a0 = bytes_bf16<by>(vw[wd], vw[W + wd]), a1 = bytes_bf16<by + 1>(vw[wd], vw[W + wd]);
-      const uint32_t a2 = bytes_bf16<by>(vw[2 * W + wd], vw[3 * W + wd]),
-                     a3 = bytes_bf16<by + 1>(vw[2 * W + wd], vw[3 * W + wd]);
+      const uint32_t a0 = bytes_f16<by>(vw[wd], vw[WV + wd]), a1 = bytes_f16<by + 1>(vw[wd], vw[WV + wd]);
+      const uint32_t a2 = bytes_f16<by>(vw[2 * WV + wd], vw[3 * WV + wd]),
+                     a3 = bytes_f16<by + 1>(vw[2 * WV + wd], vw[3 * WV + wd]);
 #pragma unroll
       for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
-        for (int n = 0; n < NP; n++) mma_bf16(o[nq][mt], a0, a1, a2, a3, pw[nq][n][0], pw[nq][n][1]);
+        for (int n = 0; n < NP; n++) mma_f16(o[nq][mt], a0, a1, a2, a3, pw[nq][n][0], pw[nq][n][1]);
     };
     values(std::integral_constant<int, 0>());
     values(std::integral_constant<int, 1>());
@@ -679,114 +717,179 @@ __global__ void __launch_bounds__(32 * kWarps, NQ == 1 ? 4 : 2)
       values(std::integral_constant<int, 7>());
     }
   };
-  for (int c = c0; c < c1; c += 2) {
-    step(buf[0], c);
-    fetch(buf[0], c + 2);
-    if (c + 1 < c1) {
-      step(buf[1], c + 1);
-      fetch(buf[1], c + 3);
-    }
+  for (int c = c0; c < c1; c += PF) {
+#pragma unroll
+    for (int u = 0; u < PF; u++)
+      if (c + u < c1) {
+        step(buf[u], c + u);
+        fetch(buf[u], c + u + PF);
+      }
   }
-
-  // --- the warps' shares joined ---
 #pragma unroll
   for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
+    for (int j = 0; j < 2; j++)
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) l[nq][j] = __fadd_rn(l[nq][j], __shfl_xor_sync(FULL, l[nq][j], d));
-      const int r = nq * 8 + 2 * tg + j;
-      if (g == 0) {
-        wm[warp * NR + r] = m[nq][j];
-        wl[warp * NR + r] = l[nq][j];
-      }
-      float* dst = wo + (warp * NR + r) * D + g * (D / 8);
-#pragma unroll
-      for (int mt = 0; mt < D / 16; mt++)
-        *reinterpret_cast<float2*>(dst + 2 * mt) = make_float2(o[nq][mt][j], o[nq][mt][j + 2]);
-    }
-  __syncthreads();
-  // Item: 32 values of one row, a lane each. The weight of a share is
-  // 2^(its maximum − the largest); one without keys counts 0 (its maximum
-  // is −inf), and where all are, the sums are 0 or no number already.
-  auto weight = [](float mi, float top) { return mi == top ? 1.f : ex2(__fsub_rn(mi, top)); };
-  auto finish = [&](int r, int d, float top, float sum, float val) {
-    const int tq = (r0 + r) / group, hq = h * group + (r0 + r) % group;
-    const float y = sum == 0.f ? 0.f : __fdiv_rn(val, sum);
-    if (t.out.p) {
-      const int64_t at = int64_t(sp.row + tq) * t.out.row + int64_t(hq) * t.out.head + d;
-      void* op = const_cast<void*>(t.out.p);
-      if (type == 0)
-        static_cast<float*>(op)[at] = y;
-      else if (type == 1)
-        static_cast<__half*>(op)[at] = __float2half_rn(y);
-      else
-        static_cast<__nv_bfloat16*>(op)[at] = __float2bfloat16_rn(y);
-    }
-    if (t.q8) {
-      const int64_t at = int64_t(sp.row + tq) * t.heads * D + hq * D + d;
-      float s;
-      t.q8[at] = quant_lane(y, &s);
-      if (lane == 0) t.q8s[at / QK] = make_float2(s, s);
-    }
-    if (t.lse && d == 0)
-      t.lse[int64_t(sp.row + tq) * t.heads + hq] =
-          sum == 0.f ? __int_as_float(0xff800000) : __fmaf_rn(top, 0.693147181f, logf(sum));
+
+  auto put = [&](int64_t at, float y) {
+    void* op = const_cast<void*>(t.out.p);
+    if (type == 0)
+      static_cast<float*>(op)[at] = y;
+    else if (type == 1)
+      static_cast<__half*>(op)[at] = __float2half_rn(y);
+    else
+      static_cast<__nv_bfloat16*>(op)[at] = __float2bfloat16_rn(y);
   };
-  const int items = nrow * (D / 32);
-  for (int it = warp; it < items; it += kWarps) {
-    const int r = it / (D / 32), d = it % (D / 32) * 32 + lane;
-    float top = wm[r], sum = 0.f, val = 0.f;
+  auto lse_of = [](float top, float sum) { return sum == 0.f ? ninf() : __fmaf_rn(top, 0.693147181f, logf(sum)); };
+
+  if constexpr (WU == 1) {
+    // a lane's D/8 values of two queries, straight out
+    constexpr int E = D / 8;
 #pragma unroll
-    for (int w = 1; w < kWarps; w++) top = fmaxf(top, wm[w * NR + r]);
+    for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
-    for (int w = 0; w < kWarps; w++) {
-      const float k = weight(wm[w * NR + r], top);
-      sum = __fmaf_rn(k, wl[w * NR + r], sum);
-      val = __fmaf_rn(k, wo[(w * NR + r) * D + d], val);
-    }
-    if (S == 1) {
-      finish(r, d, top, sum, val);
-    } else {
-      bo[r * D + d] = val;
-      if (d == 0) {
-        bm[r] = top;
-        bl[r] = sum;
+      for (int j = 0; j < 2; j++) {
+        const int r = nq * 8 + 2 * tg + j;
+        const bool there = r < nrow;
+        const int tq = there ? (r0 + r) / group : 0, hq = h * group + (there ? (r0 + r) % group : 0);
+        const float inv = l[nq][j] == 0.f ? 0.f : __fdiv_rn(W, l[nq][j]);
+        float y[E];
+#pragma unroll
+        for (int mt = 0; mt < D / 16; mt++) {
+          y[2 * mt] = __fmul_rn(o[nq][mt][j], inv);
+          y[2 * mt + 1] = __fmul_rn(o[nq][mt][j + 2], inv);
+        }
+        if (t.q8) {
+          // blocks of 32 values: over 32/E of the eight lanes of a query
+          float m = 0.f;
+#pragma unroll
+          for (int e = 0; e < E; e++) m = fmaxf(m, fabsf(y[e]));
+#pragma unroll
+          for (int d = 4; d < 4 * 32 / E; d <<= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, d));
+          if (there) {
+            const int64_t at = (int64_t(sp.row + tq) * t.heads + hq) * D + g * E;
+#pragma unroll
+            for (int e = 0; e < E; e += 4) {
+              char4 c4;
+              c4.x = quant_val(y[e], m), c4.y = quant_val(y[e + 1], m);
+              c4.z = quant_val(y[e + 2], m), c4.w = quant_val(y[e + 3], m);
+              *reinterpret_cast<char4*>(t.q8 + at + e) = c4;
+            }
+            if (g * E % 32 == 0) t.q8s[at / QK] = make_float2(quant_scale(m), quant_scale(m));
+          }
+        }
+        if (!there) continue;
+        if (t.out.p) {
+          const int64_t at = int64_t(sp.row + tq) * t.out.row + int64_t(hq) * t.out.head + g * E;
+          if (ovec && type == 0) {
+            float4* op = reinterpret_cast<float4*>(static_cast<float*>(const_cast<void*>(t.out.p)) + at);
+#pragma unroll
+            for (int e = 0; e < E; e += 4) op[e / 4] = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+          } else if (ovec) {
+            uint16_t hy[E];
+#pragma unroll
+            for (int e = 0; e < E; e++)
+              hy[e] = type == 1 ? __half_as_ushort(__float2half_rn(y[e]))
+                                : __bfloat16_as_ushort(__float2bfloat16_rn(y[e]));
+            uint4* op = reinterpret_cast<uint4*>(static_cast<uint16_t*>(const_cast<void*>(t.out.p)) + at);
+#pragma unroll
+            for (int e = 0; e < E; e += 8)
+              op[e / 8] = make_uint4(hy[e] | hy[e + 1] << 16, hy[e + 2] | hy[e + 3] << 16, hy[e + 4] | hy[e + 5] << 16,
+                                     hy[e + 6] | hy[e + 7] << 16);
+          } else {
+#pragma unroll
+            for (int e = 0; e < E; e++) put(at + e, y[e]);
+          }
+        }
+        if (t.lse && g == 0) t.lse[int64_t(sp.row + tq) * t.heads + hq] = lse_of(ref[nq][j], l[nq][j]);
+      }
+  } else {
+    // --- the warps' shares joined ---
+#pragma unroll
+    for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const int r = nq * 8 + 2 * tg + j;
+        if (r >= nrow) continue;
+        if (g == 0) {
+          wm[warp * NR + r] = ref[nq][j];
+          wl[warp * NR + r] = l[nq][j];
+        }
+        float* dst = wo + (warp * NR + r) * D + g * (D / 8);
+#pragma unroll
+        for (int mt = 0; mt < D / 16; mt++)
+          *reinterpret_cast<float2*>(dst + 2 * mt) =
+              make_float2(__fmul_rn(o[nq][mt][j], W), __fmul_rn(o[nq][mt][j + 2], W));
+      }
+    __syncthreads();
+    // Item: 32 values of one row, a lane each. The weight of a share is
+    // 2^(its reference − the largest); one without keys counts 0 (its
+    // reference is −inf), and where all are, the sums are 0 or no number.
+    auto weight = [](float mi, float top) { return mi == top ? 1.f : ex2(__fsub_rn(mi, top)); };
+    auto finish = [&](int r, int d, float top, float sum, float val) {
+      const int tq = (r0 + r) / group, hq = h * group + (r0 + r) % group;
+      const float y = sum == 0.f ? 0.f : __fdiv_rn(val, sum);
+      if (t.out.p) put(int64_t(sp.row + tq) * t.out.row + int64_t(hq) * t.out.head + d, y);
+      if (t.q8) {
+        const int64_t at = int64_t(sp.row + tq) * t.heads * D + hq * D + d;
+        float s;
+        t.q8[at] = quant_lane(y, &s);
+        if (lane == 0) t.q8s[at / QK] = make_float2(s, s);
+      }
+      if (t.lse && d == 0) t.lse[int64_t(sp.row + tq) * t.heads + hq] = lse_of(top, sum);
+    };
+    const int items = nrow * (D / 32);
+    for (int it = warp; it < items; it += WU) {
+      const int r = it / (D / 32), d = it % (D / 32) * 32 + lane;
+      float top = wm[r], sum = 0.f, val = 0.f;
+#pragma unroll
+      for (int w = 1; w < WU; w++) top = fmaxf(top, wm[w * NR + r]);
+#pragma unroll
+      for (int w = 0; w < WU; w++) {
+        const float k = weight(wm[w * NR + r], top);
+        sum = __fmaf_rn(k, wl[w * NR + r], sum);
+        val = __fmaf_rn(k, wo[(w * NR + r) * D + d], val);
+      }
+      if (S == 1) {
+        finish(r, d, top, sum, val);
+      } else {
+        bo[r * D + d] = val;
+        if (d == 0) {
+          bm[r] = top;
+          bl[r] = sum;
+        }
       }
     }
-  }
-  if (S == 1) return;
-  cluster_sync();
-  for (int it = rank * kWarps + warp; it < items; it += S * kWarps) {
-    const int r = it / (D / 32), d = it % (D / 32) * 32 + lane;
-    float top = __int_as_float(0xff800000), sum = 0.f, val = 0.f;
-    for (int b = 0; b < S; b++) top = fmaxf(top, peer_f32(bm + r, b));
-    for (int b = 0; b < S; b++) {
-      const float k = weight(peer_f32(bm + r, b), top);
-      sum = __fmaf_rn(k, peer_f32(bl + r, b), sum);
-      val = __fmaf_rn(k, peer_f32(bo + r * D + d, b), val);
+    if (S == 1) return;
+    cluster_sync();
+    for (int it = rank * WU + warp; it < items; it += S * WU) {
+      const int r = it / (D / 32), d = it % (D / 32) * 32 + lane;
+      float top = ninf(), sum = 0.f, val = 0.f;
+      for (int b = 0; b < S; b++) top = fmaxf(top, peer_f32(bm + r, b));
+      for (int b = 0; b < S; b++) {
+        const float k = weight(peer_f32(bm + r, b), top);
+        sum = __fmaf_rn(k, peer_f32(bl + r, b), sum);
+        val = __fmaf_rn(k, peer_f32(bo + r * D + d, b), val);
+      }
+      finish(r, d, top, sum, val);
     }
-    finish(r, d, top, sum, val);
+    cluster_sync();  // no block leaves while another reads its shared memory
   }
-  cluster_sync();  // no block leaves while another reads its shared memory
 }
 
 constexpr int kSMs = 148;
 
-template <int D, int NQ, int NP>
-cudaError_t attend_t(const Kv8Args& a, int type, const Kv8Attend& t, cudaStream_t st) {
-  const int group = t.heads / a.heads;
-  const int qtiles = int((int64_t(a.max_new) * group + 8 * NQ - 1) / (8 * NQ));
-  const int64_t units = int64_t(a.n) * a.heads * qtiles;
-  // Blocks of one unit's keys: enough to fill the GPU four blocks deep,
-  // while each warp keeps two tiles of sixteen keys.
-  int S = 1;
-  while (S < 16 && units * S < 4 * kSMs && a.max_len >= 16 * kWarps * 2 * S * 2) S *= 2;
+template <int D, int NQ, int NP, int WU>
+cudaError_t attend_launch(const Kv8Args& a, int type, const Kv8Attend& t, int64_t units, int qtiles, int S,
+                          cudaStream_t st) {
+  using Sh = Shape<D, NQ, WU>;
   const bool vec = type == 0 ? aligned<float>(t.q, 4) : aligned<__half>(t.q, 4);
+  const bool ovec = type == 0 ? aligned<float>(t.out, 4) : aligned<__half>(t.out, 8);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(units * S));
-  cfg.blockDim = dim3(32 * kWarps);
-  cfg.dynamicSmemBytes = attend_smem<D, NQ>();
+  cfg.gridDim = dim3(unsigned(WU == 1 ? (units + Sh::warps - 1) / Sh::warps : units * S));
+  cfg.blockDim = dim3(32 * Sh::warps);
+  cfg.dynamicSmemBytes = Sh::smem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -794,7 +897,33 @@ cudaError_t attend_t(const Kv8Args& a, int type, const Kv8Attend& t, cudaStream_
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = S > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, k_kv8_attend<D, NQ, NP>, a, t, type, S, qtiles, vec);
+  return cudaLaunchKernelEx(&cfg, k_kv8_attend<D, NQ, NP, WU>, a, t, type, S, qtiles, int(units), vec, ovec);
+}
+
+// Warps of a block where a unit's keys are split over many.
+template <int D>
+constexpr int kWide = D == 64 ? 16 : 12;
+
+template <int D, int NQ, int NP>
+cudaError_t attend_t(const Kv8Args& a, int type, const Kv8Attend& t, cudaStream_t st) {
+  const int group = t.heads / a.heads;
+  const int qtiles = int((int64_t(a.max_new) * group + 8 * NQ - 1) / (8 * NQ));
+  const int64_t units = int64_t(a.n) * a.heads * qtiles;
+  // Stretches of a unit's keys: enough warps for the GPU, at most 64 tiles
+  // of sixteen keys to one, at least two.
+  const int64_t tiles = (std::max(a.max_len, 1) + 15) / 16, most = std::max<int64_t>(1, tiles / 2);
+  const int64_t parts = std::min(most, std::max((tiles + 63) / 64, (int64_t(kSMs) * 16 + units - 1) / units));
+  if (parts == 1) return attend_launch<D, NQ, NP, 1>(a, type, t, units, qtiles, 1, st);
+  int S = 1;
+  if constexpr (NQ == 1) {
+    constexpr int WU = kWide<D>;
+    if (parts > 4 && units <= kSMs) {
+      while (S < 16 && S * WU < parts && units * S * 2 <= kSMs) S *= 2;
+      return attend_launch<D, NQ, NP, WU>(a, type, t, units, qtiles, S, st);
+    }
+  }
+  while (S < 16 && S * 4 < parts) S *= 2;
+  return attend_launch<D, NQ, NP, 4>(a, type, t, units, qtiles, S, st);
 }
 
 template <int D, int NP>
@@ -805,17 +934,21 @@ cudaError_t attend_d(const Kv8Args& a, int type, const Kv8Attend& t, cudaStream_
   return attend_t<D, 4, NP>(a, type, t, st);
 }
 
-template <int D, int NQ, int NP>
+template <int D, int NQ, int NP, int WU>
 void attend_attrs() {
-  cudaFuncSetAttribute(k_kv8_attend<D, NQ, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                       int(attend_smem<D, NQ>()));
-  cudaFuncSetAttribute(k_kv8_attend<D, NQ, NP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  const auto k = k_kv8_attend<D, NQ, NP, WU>;
+  cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Shape<D, NQ, WU>::smem));
+  cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
 }
 template <int D, int NP>
 void attend_init() {
-  attend_attrs<D, 1, NP>();
-  attend_attrs<D, 2, NP>();
-  attend_attrs<D, 4, NP>();
+  attend_attrs<D, 1, NP, 1>();
+  attend_attrs<D, 1, NP, 4>();
+  attend_attrs<D, 1, NP, kWide<D>>();
+  attend_attrs<D, 2, NP, 1>();
+  attend_attrs<D, 2, NP, 4>();
+  attend_attrs<D, 4, NP, 1>();
+  attend_attrs<D, 4, NP, 4>();
 }
 
 }  // namespace
@@ -843,15 +976,15 @@ cudaError_t launch_kv8_read(const Kv8Args& a, int head_dim, int type, const Kv8R
 }
 
 cudaError_t launch_kv8_attend(const Kv8Args& a, int head_dim, int type, const Kv8Attend& t, cudaStream_t st) {
-  if (head_dim == 64) return type == 0 ? attend_d<64, 3>(a, type, t, st) : attend_d<64, 2>(a, type, t, st);
-  return type == 0 ? attend_d<128, 3>(a, type, t, st) : attend_d<128, 2>(a, type, t, st);
+  if (head_dim == 64) return type == 0 ? attend_d<64, 2>(a, type, t, st) : attend_d<64, 1>(a, type, t, st);
+  return type == 0 ? attend_d<128, 2>(a, type, t, st) : attend_d<128, 1>(a, type, t, st);
 }
 
 void kv8_kernels_init() {
   attend_init<64, 2>();
-  attend_init<64, 3>();
+  attend_init<64, 1>();
   attend_init<128, 2>();
-  attend_init<128, 3>();
+  attend_init<128, 1>();
 }
 
 }  // namespace grx

@@ -79,7 +79,7 @@ class Cache:
         return x.transpose(1, 0, 2, 3).reshape(self.heads, -1, self.d)[:, :length]
 
 
-def attend(cache, pages, length, q, table=None, mode="none", scale=None, window=0, first=0):
+def attend(cache, pages, length, q, table=None, mode="none", scale=None, window=0, first=0, half=False):
     """q [t][heads][d] of the last t tokens → out [t][heads][d], lse, and a
     bound on a float32 kernel's error of out (see below)."""
     t, heads, d = q.shape
@@ -111,4 +111,10 @@ def attend(cache, pages, length, q, table=None, mode="none", scale=None, window=
                 ds = (2.0**-22 * np.abs(x[r, h]).max() * np.abs(kk).sum(1).max() * abs(scale)
                       + 4 * 2.0**-24 * np.abs(s).max())
                 tol[r, h] = np.abs(vv).max() * (2 * ds + 2.0**-21 + ((hi - lo) / 16 + 32) * 2.0**-23)
+                # The weights of 16-bit outputs are float16 (half a step 2^-11
+                # of each, or 2^-25 of the reference below its smallest normal
+                # number; the reference is at most 2·3 times a page's scale
+                # where the scales are in 0.5..1.5, and counts 1 in the sum).
+                if half:
+                    tol[r, h] += np.abs(vv).max() * (2.0**-11 + (hi - lo) * 6 * 2.0**-25)
     return out, lse, tol

@@ -102,7 +102,7 @@ class Side:
             if b == a:
                 continue
             want, wl, tol = attend(self.ref, self.table[i], m, qs[a:b], self.rope, self.mode, window=window,
-                                   first=first[i] if first is not None else 0)
+                                   first=first[i] if first is not None else 0, half=dtype != "f32")
             tol = tol[..., None] + EPS2[dtype] * np.abs(want) * (dtype != "f32") + 2.0**-24 * (dtype == "f16")
             bad = ~(np.abs(got[a:b] - want) <= tol * want_tol)
             bad &= ~(np.isnan(want) & np.isnan(got[a:b]))
