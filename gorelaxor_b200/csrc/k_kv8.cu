@@ -371,6 +371,67 @@ __device__ __forceinline__ float peer_f32(const float* p, uint32_t rank) {
   return v;
 }
 
+// Values 16·tg .. 16·tg + 15 of each 64 of a query at the position `pos`,
+// rotated, by four lanes together.
+template <int D>
+__device__ __forceinline__ void rotate16(float (&x)[D / 64][16], const Kv8Args& a, int pos, int tg) {
+  constexpr int H2 = D / 64;
+  if (a.rope_mode == ROPE_NONE) return;
+  // a slot that holds nothing has no position; its scores are not used
+  const float2* cs = reinterpret_cast<const float2*>(a.rope) + int64_t(max(pos, 0)) * (D / 2);
+  if (a.rope_mode == ROPE_PAIRS) {
+#pragma unroll
+    for (int j = 0; j < H2; j++)
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const float2 f = cs[(64 * j + 16 * tg + e) / 2];
+        const float p = x[j][e], q = x[j][e + 1];
+        x[j][e] = __fmaf_rn(p, f.x, -__fmul_rn(q, f.y));
+        x[j][e + 1] = __fmaf_rn(p, f.y, __fmul_rn(q, f.x));
+      }
+  } else if (D == 64) {
+    // the partner is 32 values on: two lanes away
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      const float o = __shfl_xor_sync(FULL, x[0][e], 2);
+      const float2 f = cs[(16 * tg + e) & 31];
+      x[0][e] = __fmaf_rn(x[0][e], f.x, tg < 2 ? -__fmul_rn(o, f.y) : __fmul_rn(o, f.y));
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      const float2 f = cs[16 * tg + e];
+      const float p = x[0][e], q = x[H2 - 1][e];
+      x[0][e] = __fmaf_rn(p, f.x, -__fmul_rn(q, f.y));
+      x[H2 - 1][e] = __fmaf_rn(p, f.y, __fmul_rn(q, f.x));
+    }
+  }
+}
+
+constexpr float kQueryUnits = 4194304.f;  // a query's largest value
+
+__device__ __forceinline__ void put(const Kv8Attend& t, int type, int64_t at, float y) {
+  void* op = const_cast<void*>(t.out.p);
+  if (type == 0)
+    static_cast<float*>(op)[at] = y;
+  else if (type == 1)
+    static_cast<__half*>(op)[at] = __float2half_rn(y);
+  else
+    static_cast<__nv_bfloat16*>(op)[at] = __float2bfloat16_rn(y);
+}
+__device__ __forceinline__ float lse_of(float top, float sum) {
+  return sum == 0.f ? ninf() : __fmaf_rn(top, 0.693147181f, logf(sum));
+}
+
+// Which bytes of a transposed pair of weights the column g takes into word
+// n of its operand: `bytes` (two selectors) at the place of the column's
+// keys, 0 elsewhere. Keys t = g/2: word t/2, bytes 2·(t % 2).
+__device__ __forceinline__ uint32_t column_bytes(int g, int n, uint32_t bytes) {
+  const int t = g >> 1;
+  if (t >> 1 != n) return 0x4444;
+  return t & 1 ? bytes << 8 | 0x44 : 0x4400 | bytes;
+}
+
 template <int D>
 struct Tile {  // sixteen tokens as the products take them
   uint4 k[2][D / 64];
@@ -491,7 +552,6 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
   for (int u = 0; u < PF; u++) fetch(buf[u], c0 + u);
 
   // --- the queries: rotated, and written as digits ---
-  constexpr float kUnits = 4194304.f;
   for (int nq = WU == 1 ? 0 : warp; nq < NQ; nq += WU) {
     const int r = nq * 8 + g;  // this lane's query
     const bool there = r < nrow;
@@ -514,37 +574,7 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
           load4(static_cast<const __nv_bfloat16*>(t.q.p) + o, vec, &x[j][e]);
         }
       }
-    if (a.rope_mode != ROPE_NONE) {
-      // a slot that holds nothing has no position; its scores are not used
-      const float2* cs = reinterpret_cast<const float2*>(a.rope) + int64_t(max(pos, 0)) * (D / 2);
-      if (a.rope_mode == ROPE_PAIRS) {
-#pragma unroll
-        for (int j = 0; j < H2; j++)
-#pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            const float2 f = cs[(64 * j + 16 * tg + e) / 2];
-            const float p = x[j][e], q = x[j][e + 1];
-            x[j][e] = __fmaf_rn(p, f.x, -__fmul_rn(q, f.y));
-            x[j][e + 1] = __fmaf_rn(p, f.y, __fmul_rn(q, f.x));
-          }
-      } else if (D == 64) {
-        // the partner is 32 values on: two lanes away
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-          const float o = __shfl_xor_sync(FULL, x[0][e], 2);
-          const float2 f = cs[(16 * tg + e) & 31];
-          x[0][e] = __fmaf_rn(x[0][e], f.x, tg < 2 ? -__fmul_rn(o, f.y) : __fmul_rn(o, f.y));
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-          const float2 f = cs[16 * tg + e];
-          const float p = x[0][e], q = x[H2 - 1][e];
-          x[0][e] = __fmaf_rn(p, f.x, -__fmul_rn(q, f.y));
-          x[H2 - 1][e] = __fmaf_rn(p, f.y, __fmul_rn(q, f.x));
-        }
-      }
-    }
+    rotate16<D>(x, a, pos, tg);
     float amax = 0.f;
     bool finite = true;
 #pragma unroll
@@ -559,7 +589,7 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
     finite = ((__ballot_sync(FULL, finite) >> (lane & ~3)) & 15) == 15;
     // tiny rows are lifted first, so that neither quotient leaves the range
     const float lift = amax < 1e-30f ? 1e30f : 1.f;
-    const float to = finite && amax > 0.f ? __fdiv_rn(kUnits, __fmul_rn(amax, lift)) : 0.f;
+    const float to = finite && amax > 0.f ? __fdiv_rn(kQueryUnits, __fmul_rn(amax, lift)) : 0.f;
 #pragma unroll
     for (int j = 0; j < H2; j++) {
       uint32_t w[3][4] = {};
@@ -579,7 +609,7 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
     }
     if (tg == 0) {
       // scores in units of log 2; a query that is no number has no score
-      const float f = __fmul_rn(__fmul_rn(amax, 1.f / kUnits), __fmul_rn(t.scale, 1.44269504f));
+      const float f = __fmul_rn(__fmul_rn(amax, 1.f / kQueryUnits), __fmul_rn(t.scale, 1.44269504f));
       qf[r] = finite ? f : qnan();
       qpos[r] = there ? pos : -1;
     }
@@ -732,17 +762,6 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) l[nq][j] = __fadd_rn(l[nq][j], __shfl_xor_sync(FULL, l[nq][j], d));
 
-  auto put = [&](int64_t at, float y) {
-    void* op = const_cast<void*>(t.out.p);
-    if (type == 0)
-      static_cast<float*>(op)[at] = y;
-    else if (type == 1)
-      static_cast<__half*>(op)[at] = __float2half_rn(y);
-    else
-      static_cast<__nv_bfloat16*>(op)[at] = __float2bfloat16_rn(y);
-  };
-  auto lse_of = [](float top, float sum) { return sum == 0.f ? ninf() : __fmaf_rn(top, 0.693147181f, logf(sum)); };
-
   if constexpr (WU == 1) {
     // a lane's D/8 values of two queries, straight out
     constexpr int E = D / 8;
@@ -799,7 +818,7 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
                                      hy[e + 6] | hy[e + 7] << 16);
           } else {
 #pragma unroll
-            for (int e = 0; e < E; e++) put(at + e, y[e]);
+            for (int e = 0; e < E; e++) put(t, type, at + e, y[e]);
           }
         }
         if (t.lse && g == 0) t.lse[int64_t(sp.row + tq) * t.heads + hq] = lse_of(ref[nq][j], l[nq][j]);
@@ -830,7 +849,7 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
     auto finish = [&](int r, int d, float top, float sum, float val) {
       const int tq = (r0 + r) / group, hq = h * group + (r0 + r) % group;
       const float y = sum == 0.f ? 0.f : __fdiv_rn(val, sum);
-      if (t.out.p) put(int64_t(sp.row + tq) * t.out.row + int64_t(hq) * t.out.head + d, y);
+      if (t.out.p) put(t, type, int64_t(sp.row + tq) * t.out.row + int64_t(hq) * t.out.head + d, y);
       if (t.q8) {
         const int64_t at = int64_t(sp.row + tq) * t.heads * D + hq * D + d;
         float s;
@@ -878,7 +897,411 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
   }
 }
 
+// ---------------------------------------------- attend, one query a head ----
+//
+// Where a sequence's key head has one query (a single token, as many query
+// heads as key heads: the flow LM's step), seven of a product's eight
+// columns would be empty. Here they hold the digits instead, and a warp
+// takes 32 tokens at a time:
+//  * the query's digits stand in the columns (the lowest in even ones, the
+//    middle in odd ones, the highest added to odd ones), so every lane has
+//    the digits of four keys and takes one of them: one score, one
+//    exponential and one weight a lane for 32 keys;
+//  * the weight is a whole number of 2^-22 of the reference weight, whose
+//    three bytes are taken as they lie in the float n + 2^23; one 8x8
+//    transposition brings the bytes of all 32 keys to the columns of an
+//    integer product with the values' bytes (m16n8k32, unsigned weights):
+//    the four keys of a row group in columns of their own, lowest and
+//    highest digits in one product, middle ones in another;
+//  * the values' bytes need a 4x4 byte transposition (eight byte
+//    permutations for sixteen bytes) and no conversion.
+// Sums are exact integers until the reference moves (a score 2^1 above it,
+// a larger value scale) or 32768 keys have gone by; then they go into
+// float32 sums. About 60 instructions for sixteen tokens where eight columns
+// of queries take 260: bound by the cache's bytes.
+template <int D>
+struct Tile2 {  // 32 tokens: two tiles of sixteen
+  uint4 k[2][2][D / 64];
+  uint4 v[2][D / 32];
+};
+
+__device__ __forceinline__ void mma_s8u8(int* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <int D, int WU>
+struct Shape1 {
+  static constexpr int warps = WU == 1 ? 4 : WU;
+  static constexpr int per_sm = D == 64 ? 16 : 8;  // warps, by their registers
+  static constexpr int blocks = per_sm / warps < 1 ? 1 : per_sm / warps;
+  static constexpr size_t smem = WU == 1 ? 0 : size_t(warps + 1) * (D + 2) * 4;
+};
+
+template <int D, int WU>
+__global__ void __launch_bounds__(32 * Shape1<D, WU>::warps, Shape1<D, WU>::blocks)
+    k_kv8_attend1(Kv8Args a, Kv8Attend t, int type, int S, int units, bool vec) {
+  constexpr int H2 = D / 64, M = D / 16, WV = D / 32;
+  constexpr float kOne = 4194303.f;  // of a weight of 1; weights go to 2
+  extern __shared__ __align__(16) float part[];  // [WU][D + 2], and the block's
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tg = lane & 3;
+  const int rank = S > 1 ? int(cluster_rank()) : 0;
+  const int unit = WU == 1 ? blockIdx.x * Shape1<D, WU>::warps + warp : blockIdx.x / S;
+  if (unit >= units) return;
+  const int h = unit % a.heads, i = unit / a.heads;
+  const Kv8Span sp = kv8_span(a, i);
+  if (!sp.ok) {
+    if ((WU == 1 ? lane : tid) == 0) report(a);
+    return;
+  }
+  if (sp.T == 0) return;
+  const int p = sp.len - 1;  // the query's position
+  const int first = max(a.first ? max(0, a.first[i]) : 0, t.window > 0 ? p - t.window + 1 : 0);
+  const int cb = first >> 4, ce = max(cb, (p + 16) >> 4);
+  const int per = (ce - cb + S * WU - 1) / (S * WU);
+  const int c0 = min(ce, cb + (WU == 1 ? 0 : rank * WU + warp) * per), c1 = min(ce, c0 + per);
+
+  // --- the pages ahead: lane l holds page and scales of the tile wbase + l ---
+  const int cshift = a.plog - 4;
+  const float2* scales = reinterpret_cast<const float2*>(a.scale) + h;
+  auto page_of = [&](int c) { return c < c1 ? kv8_page(a, i, c >> cshift) : -1; };
+  auto scale_of = [&](int page) {
+    if (page < 0) return make_float2(0.f, 0.f);
+    const float2 s = scales[int64_t(page) * a.heads];
+    return make_float2(isfinite(s.x) ? s.x : qnan(), s.y >= 0.f && isfinite(s.y) ? s.y : qnan());
+  };
+  int wbase = c0;
+  int pg = page_of(c0 + lane);
+  if (pg < 0 && c0 + lane < c1) report(a);
+  float2 sc = scale_of(pg);
+  int pg1 = page_of(c0 + 32 + lane);
+  const int8_t* kbase = a.k + ((int64_t(h) << a.plog) + g) * D + 16 * tg;
+  const int8_t* vbase = a.v + ((int64_t(h) << a.plog) + 2 * tg) * D + g * (D / 8);
+  const int64_t pbytes = (int64_t(a.heads) << a.plog) * D;
+  const int smask = (1 << a.plog) - 1;
+
+  Tile2<D> b;
+  // loads of the step at tile c, by pages pa and pb (−1: its tokens are not there)
+  auto load_k = [&](int c, int pa, int pb) {
+#pragma unroll
+    for (int n = 0; n < 2; n++) {
+      const int page = n ? pb : pa;
+      const int8_t* kp = kbase + page * pbytes + (((c + n) << 4) & smask) * D;
+#pragma unroll
+      for (int r = 0; r < 2; r++)
+#pragma unroll
+        for (int j = 0; j < H2; j++)
+          b.k[n][r][j] = page < 0 ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(kp + r * 8 * D + j * 64));
+    }
+  };
+  auto load_v = [&](int c, int pa, int pb) {
+#pragma unroll
+    for (int n = 0; n < 2; n++) {
+      const int page = n ? pb : pa;
+      const int8_t* vp = vbase + page * pbytes + (((c + n) << 4) & smask) * D;
+      if constexpr (D == 64) {
+        uint2 x[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+          x[r] = page < 0 ? make_uint2(0, 0)
+                          : __ldg(reinterpret_cast<const uint2*>(vp + ((r & 1) + (r >> 1) * 8) * D));
+        b.v[n][0] = make_uint4(x[0].x, x[0].y, x[1].x, x[1].y);
+        b.v[n][1] = make_uint4(x[2].x, x[2].y, x[3].x, x[3].y);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+          b.v[n][r] = page < 0 ? make_uint4(0, 0, 0, 0)
+                               : __ldg(reinterpret_cast<const uint4*>(vp + ((r & 1) + (r >> 1) * 8) * D));
+      }
+    }
+  };
+  int pa = __shfl_sync(FULL, pg, 0), pb = __shfl_sync(FULL, pg, 1);
+  load_k(c0, pa, pb);
+  load_v(c0, pa, pb);
+
+  // --- the query: rotated, and written as digits ---
+  uint32_t q01[H2][4], q2[H2][4];
+  float f;
+  {
+    float x[H2][16];
+    const int64_t off = int64_t(sp.row) * t.q.row + int64_t(h) * t.q.head + 16 * tg;
+#pragma unroll
+    for (int j = 0; j < H2; j++)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const int64_t o = off + 64 * j + e;
+        if (type == 0)
+          load4(static_cast<const float*>(t.q.p) + o, vec, &x[j][e]);
+        else if (type == 1)
+          load4(static_cast<const __half*>(t.q.p) + o, vec, &x[j][e]);
+        else
+          load4(static_cast<const __nv_bfloat16*>(t.q.p) + o, vec, &x[j][e]);
+      }
+    rotate16<D>(x, a, p, tg);
+    float amax = 0.f;
+    bool finite = true;
+#pragma unroll
+    for (int j = 0; j < H2; j++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        amax = fmaxf(amax, fabsf(x[j][e]));
+        finite = finite && isfinite(x[j][e]);
+      }
+    amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, 2));
+    finite = __all_sync(FULL, finite);
+    const float lift = amax < 1e-30f ? 1e30f : 1.f;
+    const float to = finite && amax > 0.f ? __fdiv_rn(kQueryUnits, __fmul_rn(amax, lift)) : 0.f;
+#pragma unroll
+    for (int j = 0; j < H2; j++)
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        uint32_t lo = 0, up = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int n = finite ? __float2int_rn(__fmul_rn(__fmul_rn(x[j][4 * w + e], lift), to)) : 0;
+          const int d0 = int8_t(n), n1 = (n - d0) >> 8, d1 = int8_t(n1), d2 = (n1 - d1) >> 8;
+          lo |= uint32_t((g & 1 ? d1 : d0) & 255) << (8 * e);
+          up |= uint32_t((g & 1 ? d2 : 0) & 255) << (8 * e);
+        }
+        q01[j][w] = lo;
+        q2[j][w] = up;
+      }
+    f = finite ? __fmul_rn(__fmul_rn(amax, 1.f / kQueryUnits), __fmul_rn(t.scale, 1.44269504f)) : qnan();
+  }
+
+  // --- the pass over the keys: lane (g, tg) has key g + 8·(tg & 1) of tile tg >> 1 ---
+  const uint32_t at0 = column_bytes(g, 0, 0x20), at1 = column_bytes(g, 1, 0x20);
+  const uint32_t mid0 = g & 1 ? 0x4444 : column_bytes(g, 0, 0x31), mid1 = g & 1 ? 0x4444 : column_bytes(g, 1, 0x31);
+  int lh[M][4] = {}, md[M][4] = {};  // lowest (even columns) and highest (odd) digits; middle ones
+  float o[M][2] = {};
+  float ref = ninf(), l = 0.f, W = 0.f, toW = 0.f;
+  auto flush = [&]() {
+#pragma unroll
+    for (int mt = 0; mt < M; mt++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const float lo = __fmaf_rn(256.f, float(md[mt][2 * e]), float(lh[mt][2 * e]));
+        o[mt][e] = __fadd_rn(o[mt][e], __fmaf_rn(65536.f, float(lh[mt][2 * e + 1]), lo));
+        lh[mt][2 * e] = lh[mt][2 * e + 1] = md[mt][2 * e] = 0;
+      }
+  };
+  auto rescale = [&](float r) {
+#pragma unroll
+    for (int mt = 0; mt < M; mt++) {
+      o[mt][0] = __fmul_rn(o[mt][0], r);
+      o[mt][1] = __fmul_rn(o[mt][1], r);
+    }
+  };
+  int held = 0;  // steps in the integer sums
+  for (int c = c0; c < c1; c += 2) {
+    // this step's scales, the next one's pages
+    const int j = c - wbase;
+    const float sk = __shfl_sync(FULL, sc.x, j + (tg >> 1));
+    const float sva = __shfl_sync(FULL, sc.y, j), svb = __shfl_sync(FULL, sc.y, j + 1);
+    const bool gone = pa < 0 || pb < 0, mygone = (tg < 2 ? pa : pb) < 0;
+    const bool edge = gone || c * 16 < first || c * 16 + 31 > p;
+    if (j == 30) {
+      wbase += 32;
+      pg = pg1;
+      if (pg < 0 && wbase + lane < c1) report(a);
+      sc = scale_of(pg);
+      pg1 = page_of(wbase + 32 + lane);
+    }
+    pa = __shfl_sync(FULL, pg, c + 2 - wbase);
+    pb = __shfl_sync(FULL, pg, c + 3 - wbase);
+
+    // the highest digit's sums, then the lower ones' on top: even columns
+    // the lowest digit, odd ones 256·highest + middle (below 2^31)
+    int s0[4] = {0, 0, 0, 0}, s1[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < H2; e++) {
+      mma_s8(s0, b.k[0][0][e].x, b.k[0][1][e].x, b.k[0][0][e].y, b.k[0][1][e].y, q2[e][0], q2[e][1]);
+      mma_s8(s1, b.k[1][0][e].x, b.k[1][1][e].x, b.k[1][0][e].y, b.k[1][1][e].y, q2[e][0], q2[e][1]);
+      mma_s8(s0, b.k[0][0][e].z, b.k[0][1][e].z, b.k[0][0][e].w, b.k[0][1][e].w, q2[e][2], q2[e][3]);
+      mma_s8(s1, b.k[1][0][e].z, b.k[1][1][e].z, b.k[1][0][e].w, b.k[1][1][e].w, q2[e][2], q2[e][3]);
+    }
+    s0[1] <<= 8, s0[3] <<= 8, s1[1] <<= 8, s1[3] <<= 8;
+#pragma unroll
+    for (int e = 0; e < H2; e++) {
+      mma_s8(s0, b.k[0][0][e].x, b.k[0][1][e].x, b.k[0][0][e].y, b.k[0][1][e].y, q01[e][0], q01[e][1]);
+      mma_s8(s1, b.k[1][0][e].x, b.k[1][1][e].x, b.k[1][0][e].y, b.k[1][1][e].y, q01[e][0], q01[e][1]);
+      mma_s8(s0, b.k[0][0][e].z, b.k[0][1][e].z, b.k[0][0][e].w, b.k[0][1][e].w, q01[e][2], q01[e][3]);
+      mma_s8(s1, b.k[1][0][e].z, b.k[1][1][e].z, b.k[1][0][e].w, b.k[1][1][e].w, q01[e][2], q01[e][3]);
+    }
+    if (c + 2 < c1) load_k(c + 2, pa, pb);
+    const int lo = tg & 2 ? (tg & 1 ? s1[2] : s1[0]) : (tg & 1 ? s0[2] : s0[0]);
+    const int up = tg & 2 ? (tg & 1 ? s1[3] : s1[1]) : (tg & 1 ? s0[3] : s0[1]);
+    const float s = __fmaf_rn(256.f, float(up), float(lo)), fs = __fmul_rn(f, sk);
+    float x = __fmaf_rn(s, fs, -ref), sv = tg < 2 ? sva : svb;
+    bool hide = false;
+    if (edge) {
+      const int key = (c + (tg >> 1)) * 16 + g + 8 * (tg & 1);
+      hide = key > p || key < first || mygone;
+      if (hide) x = ninf(), sv = 0.f;
+    }
+    // The reference moves: a larger value scale (an eighth above it, to move
+    // less often), or a score 2 above (any, before the first key).
+    const float wide = fmaxf(sva, svb);
+    if (wide > W) {
+      flush();
+      held = 0;
+      const float w = fminf(fmaxf(__fmul_rn(1.125f, wide), 1.17549435e-38f), 3.4e38f);
+      rescale(__fdiv_rn(W, w));
+      W = w;
+      toW = __fdiv_rn(1.f, w);
+    }
+    if (__any_sync(FULL, x > 1.f)) {
+      flush();
+      held = 0;
+      float m = hide ? ninf() : __fmul_rn(s, fs);
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, d));
+      m = fmaxf(m, ref);
+      const float r = ref == m ? 1.f : ex2(__fsub_rn(ref, m));
+      ref = m;
+      l = __fmul_rn(l, r);
+      rescale(r);
+      x = hide ? ninf() : __fmaf_rn(s, fs, -m);
+    }
+    const float w = ex2(x);
+    l = __fadd_rn(l, __fmaf_rn(0.f, sv, w));  // a scale that is no number makes the sum none
+    // n + 2^23: the bytes of n as they lie
+    const uint32_t y = __float_as_uint(__fmaf_rn(__fmul_rn(w, __fmul_rn(sv, toW)), kOne, 8388608.f));
+    const uint32_t yt = transpose8(y);
+    const uint32_t b0 = __byte_perm(yt, 0, at0), b1 = __byte_perm(yt, 0, at1);
+    const uint32_t m0 = __byte_perm(yt, 0, mid0), m1 = __byte_perm(yt, 0, mid1);
+    const uint32_t *va = &b.v[0][0].x, *vb = &b.v[1][0].x;
+#pragma unroll
+    for (int wd = 0; wd < WV; wd++) {
+      // four tokens' words of four values each → four words of a value each
+      uint32_t d[2][4];
+#pragma unroll
+      for (int n = 0; n < 2; n++) {
+        const uint32_t* v = n ? vb : va;
+        const uint32_t l01 = __byte_perm(v[wd], v[WV + wd], 0x5140), h01 = __byte_perm(v[wd], v[WV + wd], 0x7362);
+        const uint32_t l23 = __byte_perm(v[2 * WV + wd], v[3 * WV + wd], 0x5140),
+                       h23 = __byte_perm(v[2 * WV + wd], v[3 * WV + wd], 0x7362);
+        d[n][0] = __byte_perm(l01, l23, 0x5410);
+        d[n][1] = __byte_perm(l01, l23, 0x7632);
+        d[n][2] = __byte_perm(h01, h23, 0x5410);
+        d[n][3] = __byte_perm(h01, h23, 0x7632);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const uint32_t av[4] = {d[0][2 * e], d[0][2 * e + 1], d[1][2 * e], d[1][2 * e + 1]};
+        mma_s8u8(lh[2 * wd + e], av, b0, b1);
+        mma_s8u8(md[2 * wd + e], av, m0, m1);
+      }
+    }
+    if (c + 2 < c1) load_v(c + 2, pa, pb);
+    if (++held == 1024) {  // 32768 keys: 255·128·32768 < 2^31
+      flush();
+      held = 0;
+    }
+  }
+  flush();
+  // sums over the columns (the lanes of a row group), and over all lanes
+#pragma unroll
+  for (int mt = 0; mt < M; mt++)
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      o[mt][e] = __fadd_rn(o[mt][e], __shfl_xor_sync(FULL, o[mt][e], 1));
+      o[mt][e] = __fadd_rn(o[mt][e], __shfl_xor_sync(FULL, o[mt][e], 2));
+    }
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) l = __fadd_rn(l, __shfl_xor_sync(FULL, l, d));
+
+  // lane (g, tg) goes on with D/32 of row group g's D/8 values
+  constexpr int E = D / 32;
+  float y[E];
+  const float unit_w = __fmul_rn(W, 1.f / kOne);
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    float v = o[e / 2][e % 2];
+#pragma unroll
+    for (int n = 1; n < 4; n++)
+      if (tg == n) v = o[(n * E + e) / 2][e % 2];
+    y[e] = __fmul_rn(v, unit_w);
+  }
+  const int d0 = g * (D / 8) + tg * E;
+  auto finish = [&](float top, float sum, const float* val) {
+    float r[E], m = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      r[e] = sum == 0.f ? 0.f : __fdiv_rn(val[e], sum);
+      m = fmaxf(m, fabsf(r[e]));
+    }
+    if (t.out.p) {
+      const int64_t at = int64_t(sp.row) * t.out.row + int64_t(h) * t.out.head + d0;
+#pragma unroll
+      for (int e = 0; e < E; e++) put(t, type, at + e, r[e]);
+    }
+    if (t.q8) {  // blocks of 32 values: 32/E lanes
+#pragma unroll
+      for (int d = 1; d < 32 / E; d <<= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, d));
+      const int64_t at = (int64_t(sp.row) * t.heads + h) * D + d0;
+#pragma unroll
+      for (int e = 0; e < E; e++) t.q8[at + e] = quant_val(r[e], m);
+      if (d0 % QK == 0) t.q8s[at / QK] = make_float2(quant_scale(m), quant_scale(m));
+    }
+    if (t.lse && lane == 0) t.lse[int64_t(sp.row) * t.heads + h] = lse_of(top, sum);
+  };
+  if constexpr (WU == 1) {
+    finish(ref, l, y);
+  } else {
+    float* mine = part + warp * (D + 2);
+    if (lane == 0) mine[D] = ref, mine[D + 1] = l;
+#pragma unroll
+    for (int e = 0; e < E; e++) mine[d0 + e] = y[e];
+    __syncthreads();
+    if (warp != 0 && S == 1) return;
+    float* block = part + WU * (D + 2);
+    if (warp == 0) {
+      float top = ninf(), sum = 0.f, val[E] = {};
+      for (int w = 0; w < WU; w++) top = fmaxf(top, part[w * (D + 2) + D]);
+      for (int w = 0; w < WU; w++) {
+        const float* o1 = part + w * (D + 2);
+        const float k = o1[D] == top ? 1.f : ex2(__fsub_rn(o1[D], top));
+        sum = __fmaf_rn(k, o1[D + 1], sum);
+#pragma unroll
+        for (int e = 0; e < E; e++) val[e] = __fmaf_rn(k, o1[d0 + e], val[e]);
+      }
+      if (S == 1) {
+        finish(top, sum, val);
+        return;
+      }
+      if (lane == 0) block[D] = top, block[D + 1] = sum;
+#pragma unroll
+      for (int e = 0; e < E; e++) block[d0 + e] = val[e];
+    }
+    cluster_sync();
+    if (rank == 0 && warp == 0) {
+      float top = ninf(), sum = 0.f, val[E] = {};
+      for (int n = 0; n < S; n++) top = fmaxf(top, peer_f32(block + D, n));
+      for (int n = 0; n < S; n++) {
+        const float m = peer_f32(block + D, n), k = m == top ? 1.f : ex2(__fsub_rn(m, top));
+        sum = __fmaf_rn(k, peer_f32(block + D + 1, n), sum);
+#pragma unroll
+        for (int e = 0; e < E; e++) val[e] = __fmaf_rn(k, peer_f32(block + d0 + e, n), val[e]);
+      }
+      finish(top, sum, val);
+    }
+    cluster_sync();  // no block leaves while another reads its shared memory
+  }
+}
+
 constexpr int kSMs = 148;
+
+// Blocks and warps for a unit's keys: the stretches that they are cut into
+// give the GPU enough warps, at most `longest` tiles of sixteen keys to one
+// and at least two.
+inline int64_t stretches(const Kv8Args& a, int64_t units, int warps_per_sm, int longest) {
+  const int64_t tiles = (std::max(a.max_len, 1) + 15) / 16, most = std::max<int64_t>(1, tiles / 2);
+  return std::min(most, std::max((tiles + longest - 1) / longest, (int64_t(kSMs) * warps_per_sm + units - 1) / units));
+}
+
 
 template <int D, int NQ, int NP, int WU>
 cudaError_t attend_launch(const Kv8Args& a, int type, const Kv8Attend& t, int64_t units, int qtiles, int S,
@@ -909,10 +1332,7 @@ cudaError_t attend_t(const Kv8Args& a, int type, const Kv8Attend& t, cudaStream_
   const int group = t.heads / a.heads;
   const int qtiles = int((int64_t(a.max_new) * group + 8 * NQ - 1) / (8 * NQ));
   const int64_t units = int64_t(a.n) * a.heads * qtiles;
-  // Stretches of a unit's keys: enough warps for the GPU, at most 64 tiles
-  // of sixteen keys to one, at least two.
-  const int64_t tiles = (std::max(a.max_len, 1) + 15) / 16, most = std::max<int64_t>(1, tiles / 2);
-  const int64_t parts = std::min(most, std::max((tiles + 63) / 64, (int64_t(kSMs) * 16 + units - 1) / units));
+  const int64_t parts = stretches(a, units, 16, 64);
   if (parts == 1) return attend_launch<D, NQ, NP, 1>(a, type, t, units, qtiles, 1, st);
   int S = 1;
   if constexpr (NQ == 1) {
@@ -926,9 +1346,39 @@ cudaError_t attend_t(const Kv8Args& a, int type, const Kv8Attend& t, cudaStream_
   return attend_launch<D, NQ, NP, 4>(a, type, t, units, qtiles, S, st);
 }
 
+template <int D, int WU>
+cudaError_t attend1_launch(const Kv8Args& a, int type, const Kv8Attend& t, int S, cudaStream_t st) {
+  using Sh = Shape1<D, WU>;
+  const int units = a.n * a.heads;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(WU == 1 ? (units + Sh::warps - 1) / Sh::warps : units * S));
+  cfg.blockDim = dim3(32 * Sh::warps);
+  cfg.dynamicSmemBytes = Sh::smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = unsigned(S);
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = S > 1 ? 1 : 0;
+  const bool vec = type == 0 ? aligned<float>(t.q, 4) : aligned<__half>(t.q, 4);
+  return cudaLaunchKernelEx(&cfg, k_kv8_attend1<D, WU>, a, t, type, S, units, vec);
+}
+
+template <int D>
+cudaError_t attend1_d(const Kv8Args& a, int type, const Kv8Attend& t, cudaStream_t st) {
+  const int64_t units = int64_t(a.n) * a.heads, parts = stretches(a, units, Shape1<D, 1>::per_sm, 64);
+  if (parts == 1) return attend1_launch<D, 1>(a, type, t, 1, st);
+  if (parts <= 4) return attend1_launch<D, 4>(a, type, t, 1, st);
+  int S = 1;
+  while (S < 16 && S * 8 < parts) S *= 2;
+  return attend1_launch<D, 8>(a, type, t, S, st);
+}
+
 template <int D, int NP>
 cudaError_t attend_d(const Kv8Args& a, int type, const Kv8Attend& t, cudaStream_t st) {
   const int64_t rows = int64_t(a.max_new) * (t.heads / a.heads);  // queries that share a head's keys
+  if (rows == 1) return attend1_d<D>(a, type, t, st);
   if (rows <= 8) return attend_t<D, 1, NP>(a, type, t, st);
   if (rows <= 16) return attend_t<D, 2, NP>(a, type, t, st);
   return attend_t<D, 4, NP>(a, type, t, st);
@@ -939,6 +1389,10 @@ void attend_attrs() {
   const auto k = k_kv8_attend<D, NQ, NP, WU>;
   cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Shape<D, NQ, WU>::smem));
   cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+}
+template <int D>
+void attend1_init() {
+  cudaFuncSetAttribute(k_kv8_attend1<D, 8>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
 }
 template <int D, int NP>
 void attend_init() {
@@ -981,6 +1435,8 @@ cudaError_t launch_kv8_attend(const Kv8Args& a, int head_dim, int type, const Kv
 }
 
 void kv8_kernels_init() {
+  attend1_init<64>();
+  attend1_init<128>();
   attend_init<64, 2>();
   attend_init<64, 1>();
   attend_init<128, 2>();
