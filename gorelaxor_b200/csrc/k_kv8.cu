@@ -410,6 +410,48 @@ __device__ __forceinline__ void rotate16(float (&x)[D / 64][16], const Kv8Args& 
 
 constexpr float kQueryUnits = 4194304.f;  // a query's largest value
 
+// The largest magnitude of the values that four lanes hold, NaN where one is
+// not finite. `lanes`: those that take part.
+template <int D>
+__device__ __forceinline__ float group_amax(const float (&x)[D / 64][16], uint32_t lanes) {
+  float m = 0.f, nan = 0.f;
+#pragma unroll
+  for (int j = 0; j < D / 64; j++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      m = fmaxf(m, fabsf(x[j][e]));
+      nan = __fmaf_rn(0.f, x[j][e], nan);  // 0·inf and 0·NaN
+    }
+  m = __fadd_rn(m, nan);
+  const float a = __shfl_xor_sync(lanes, m, 1);
+  m = m > a || isnan(m) ? m : a;
+  const float b = __shfl_xor_sync(lanes, m, 2);
+  return m > b || isnan(m) ? m : b;
+}
+// The factor that makes the largest value kQueryUnits (0 for rows of zeros
+// or of no numbers); tiny rows are lifted first, so that it stays in range.
+template <int D>
+__device__ __forceinline__ float lift_row(float (&x)[D / 64][16], float amax) {
+  if (amax < 1e-30f) {
+    amax = __fmul_rn(amax, 1e30f);
+#pragma unroll
+    for (int j = 0; j < D / 64; j++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) x[j][e] = __fmul_rn(x[j][e], 1e30f);
+  }
+  return amax > 0.f ? __fdiv_rn(kQueryUnits, amax) : 0.f;
+}
+// n + 1.5·2^23 → n's three signed digits in base 256, a byte each: with 128
+// added to every digit they are the bytes of n + 0x808080.
+__device__ __forceinline__ uint32_t digits_of(float y) {
+  return (__float_as_uint(y) - MAGIC_BITS + 0x808080u) ^ 0x808080u;
+}
+// Byte `at` of four words.
+__device__ __forceinline__ uint32_t take_bytes(const uint32_t* n, int at) {
+  const uint32_t pick = at | (at + 4) << 4;
+  return __byte_perm(__byte_perm(n[0], n[1], pick), __byte_perm(n[2], n[3], pick), 0x5410);
+}
+
 __device__ __forceinline__ void put(const Kv8Attend& t, int type, int64_t at, float y) {
   void* op = const_cast<void*>(t.out.p);
   if (type == 0)
@@ -432,23 +474,138 @@ __device__ __forceinline__ uint32_t column_bytes(int g, int n, uint32_t bytes) {
   return t & 1 ? bytes << 8 | 0x44 : 0x4400 | bytes;
 }
 
+// Tiles of sixteen tokens come from the cache into a warp's own ring in
+// shared memory by 16-byte asynchronous copies: what is under way is bounded
+// by shared memory, not by registers (loads straight into the products'
+// registers, with one step of 32 tokens ahead, read 5.5 TB/s of long
+// sequences and 3.3 of short ones). The chunks of a tile are placed so that
+// the products' loads meet no bank twice.
 template <int D>
-struct Tile {  // sixteen tokens as the products take them
-  uint4 k[2][D / 64];
-  uint4 v[D / 32];  // four tokens of D/8 bytes
-  float sk, sv;
-};
+struct Ring {
+  static constexpr int half = 16 * D, tile = 2 * half;  // bytes of a tile's keys (or values), and of both
+  uint32_t base;                 // the ring
+  uint32_t kdst, vdst[2];        // this lane's first chunk of a tile's keys and values (even, odd ones)
+  uint32_t ksrc[D / 64], vsrc[2];  // what it reads as operands: of the tokens g, and 2·tg (+ 1)
+  const int8_t *k, *v;           // the head's bytes in page 0, at this lane's chunk
+  int pbytes, smask;
 
-// Warps of a block, tiles that a warp has under way, blocks that an SM
-// shall hold: by the registers that a tile and the outputs take.
+  __device__ __forceinline__ Ring(const Kv8Args& a, int h, const void* at, int lane) {
+    const int g = lane >> 2, tg = lane & 3;
+    base = uint32_t(__cvta_generic_to_shared(at));
+    const int c = lane % (D / 16), t = lane / (D / 16);  // chunk, token
+    if constexpr (D == 64) {
+      kdst = 16 * lane;
+      vdst[0] = vdst[1] = 64 * (t ^ (t >> 1 & 1)) + 16 * (c ^ (t >> 2 & 1) << 1);
+      ksrc[0] = 64 * g + 16 * tg;
+#pragma unroll
+      for (int r = 0; r < 2; r++)
+        vsrc[r] = half + 64 * (2 * tg + (r ^ (tg & 1))) + 16 * (g >> 1 ^ (tg >> 1) << 1) + 8 * (g & 1);
+    } else {
+      kdst = 128 * t + 16 * (c ^ (t & 1) << 2);
+#pragma unroll
+      for (int r = 0; r < 2; r++) vdst[r] = 128 * t + 16 * (c ^ (t & 2) ^ r << 2);
+#pragma unroll
+      for (int j = 0; j < D / 64; j++) ksrc[j] = 128 * g + 16 * (tg + 4 * j ^ (g & 1) << 2);
+#pragma unroll
+      for (int r = 0; r < 2; r++) vsrc[r] = half + 128 * (2 * tg + r) + 16 * (g ^ 2 * tg);
+    }
+    k = a.k + ((int64_t(h) << a.plog) * D) + 16 * lane;
+    v = a.v + ((int64_t(h) << a.plog) * D) + 16 * lane;
+    pbytes = (a.heads << a.plog) * D;  // at most 2^23
+    smask = (1 << a.plog) - 1;
+  }
+  // Tile c of its sequence, of the page `page` (no page: any bytes will do,
+  // the tile's keys are hidden), into the ring's place n.
+  __device__ __forceinline__ void fetch(int n, int page, int c) const {
+    const int64_t off = int64_t(max(page, 0)) * pbytes + ((c << 4) & smask) * D;
+    const uint32_t to = base + n * tile;
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + kdst + 512 * i), "l"(k + off + 512 * i));
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + half + vdst[i & 1] + 512 * i),
+                   "l"(v + off + 512 * i));
+    }
+  }
+  // Sixteen bytes 16·tg .. of each 64 of the keys g and g + 8.
+  __device__ __forceinline__ void keys(int n, uint4 (&x)[2][D / 64]) const {
+    const uint32_t from = base + n * tile;
+#pragma unroll
+    for (int r = 0; r < 2; r++)
+#pragma unroll
+      for (int j = 0; j < D / 64; j++)
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(x[r][j].x), "=r"(x[r][j].y), "=r"(x[r][j].z), "=r"(x[r][j].w)
+                     : "r"(from + ksrc[j] + 8 * r * D));
+  }
+  // Values g·D/8 .. of the tokens 2tg, 2tg + 1, 2tg + 8, 2tg + 9: D/32 words each.
+  __device__ __forceinline__ void values(int n, uint32_t (&x)[4][D / 32]) const {
+    const uint32_t from = base + n * tile;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const uint32_t at = from + vsrc[r & 1] + (r >> 1) * 8 * D;
+      if constexpr (D == 64)
+        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(x[r][0]), "=r"(x[r][1]) : "r"(at));
+      else
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(x[r][0]), "=r"(x[r][1]), "=r"(x[r][2]), "=r"(x[r][3])
+                     : "r"(at));
+    }
+  }
+};
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// The pages of a warp's tiles c0 .. c1 − 1 and their scales: lane l holds
+// those of the tile base + l, and the page of the tile base + 32 + l.
+struct Pages {
+  const Kv8Args& a;
+  const float2* scales;
+  int i, c1, base, page, ahead;
+  float2 scale;
+
+  // `early`: the table's entry of tile `lane`, read before the length was known.
+  __device__ __forceinline__ Pages(const Kv8Args& args, int seq, int h, int c0, int c1_, int lane, int early)
+      : a(args), scales(reinterpret_cast<const float2*>(args.scale) + h), i(seq), c1(c1_), base(c0) {
+    page = c0 == 0 ? (lane < c1 && early >= 0 && early < a.pages ? early : -1) : of(c0 + lane);
+    scale = scale_of(page);
+    if (page < 0 && c0 + lane < c1) report(a);
+    ahead = of(c0 + 32 + lane);
+  }
+  __device__ __forceinline__ int of(int c) const { return c < c1 ? kv8_page(a, i, c >> (a.plog - 4)) : -1; }
+  // A scale that is not finite (or, of values, below 0) as NaN; no page: 0.
+  __device__ __forceinline__ float2 scale_of(int p) const {
+    if (p < 0) return make_float2(0.f, 0.f);
+    const float2 s = scales[int64_t(p) * a.heads];
+    return make_float2(isfinite(s.x) ? s.x : qnan(), s.y >= 0.f && isfinite(s.y) ? s.y : qnan());
+  }
+  __device__ __forceinline__ void move(int lane) {  // to the next 32 tiles
+    base += 32;
+    page = ahead;
+    if (page < 0 && base + lane < c1) report(a);
+    scale = scale_of(page);
+    ahead = of(base + 32 + lane);
+  }
+};
+__device__ __forceinline__ int early_page(const Kv8Args& a, int i, int lane) {
+  const int b = lane >> (a.plog - 4);
+  return b < a.width ? a.table[int64_t(i) * a.width + b] : -1;
+}
+
+// Warps of a block, tiles of a warp's ring, blocks that an SM shall hold: by
+// registers and by the rings (about 200 KB an SM).
 template <int D, int NQ, int WU>
 struct Shape {
   static constexpr int warps = WU == 1 ? 4 : WU;
-  static constexpr int ahead = D == 64 && NQ == 1 ? 3 : 2;
-  static constexpr int blocks = WU > 4 ? 1 : NQ > 1 ? 2 : D == 64 ? 4 : 3;
+  static constexpr int ring = D == 64 ? 5 : 4;
+  static constexpr int blocks = NQ > 1 || WU > 4 ? 2 : D == 64 ? 4 : 3;
   static constexpr size_t digits = size_t(NQ) * 3 * (D / 64) * 32 * 16;  // bytes, a unit's
-  static constexpr size_t smem =
-      (WU == 1 ? warps : 1) * (digits + size_t(8 * NQ) * 8) + (WU == 1 ? 0 : size_t(warps + 1) * 8 * NQ * (D + 2) * 4);
+  static constexpr size_t rings = size_t(warps) * ring * Ring<D>::tile;
+  // the joined outputs take the rings' place
+  static constexpr size_t join = WU == 1 ? 0 : size_t(warps + 1) * 8 * NQ * (D + 2) * 4;
+  static constexpr size_t smem = (WU == 1 ? warps : 1) * (digits + size_t(8 * NQ) * 8) + (rings > join ? rings : join);
 };
 
 // NP: float16s of a weight.
@@ -456,17 +613,19 @@ template <int D, int NQ, int NP, int WU>
 __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>::blocks)
     k_kv8_attend(Kv8Args a, Kv8Attend t, int type, int S, int qtiles, int units, bool vec, bool ovec) {
   using Sh = Shape<D, NQ, WU>;
-  constexpr int NR = 8 * NQ, H2 = D / 64, PF = Sh::ahead;
+  constexpr int NR = 8 * NQ, H2 = D / 64, R = Sh::ring;
   extern __shared__ __align__(16) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tg = lane & 3;
+  constexpr int kUnits = WU == 1 ? Sh::warps : 1;
+  uint8_t* rings = smem + kUnits * (Sh::digits + NR * 8);
   uint8_t* mine = smem + (WU == 1 ? warp * (Sh::digits + NR * 8) : 0);
-  uint4* qd = reinterpret_cast<uint4*>(mine);                       // [NQ][3][H2][32]
-  float* qf = reinterpret_cast<float*>(mine + Sh::digits);          // [NR]
-  int* qpos = reinterpret_cast<int*>(qf + NR);                      // [NR]
-  float* wm = reinterpret_cast<float*>(qpos + NR);                  // [WU][NR], WU > 1
+  uint4* qd = reinterpret_cast<uint4*>(mine);               // [NQ][3][H2][32]
+  float* qf = reinterpret_cast<float*>(mine + Sh::digits);  // [NR]
+  int* qpos = reinterpret_cast<int*>(qf + NR);              // [NR]
+  float* wm = reinterpret_cast<float*>(rings);              // [WU][NR], WU > 1, when the rings are done
   float* wl = wm + WU * NR;
-  float* wo = wl + WU * NR;                                         // [WU][NR][D]
-  float* bm = wo + WU * NR * D;                                     // [NR], [NR], [NR][D]
+  float* wo = wl + WU * NR;                                 // [WU][NR][D]
+  float* bm = wo + WU * NR * D;                             // [NR], [NR], [NR][D]
   float* bl = bm + NR;
   float* bo = bl + NR;
 
@@ -475,6 +634,7 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
   if (unit >= units) return;
   const int h = unit % a.heads, qt = unit / a.heads % qtiles, i = unit / a.heads / qtiles;
   const int group = t.heads / a.heads;
+  const int early = early_page(a, i, lane);
   const Kv8Span sp = kv8_span(a, i);
   if (!sp.ok) {
     if ((WU == 1 ? lane : tid) == 0) report(a);
@@ -490,66 +650,17 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
   const int per = (ce - cb + S * WU - 1) / (S * WU);
   const int c0 = min(ce, cb + (WU == 1 ? 0 : rank * WU + warp) * per), c1 = min(ce, c0 + per);
 
-  // --- the pages ahead: lane l holds page and scales of the tile wbase + l ---
-  const int cshift = a.plog - 4;
-  const float2* scales = reinterpret_cast<const float2*>(a.scale) + h;
-  auto page_of = [&](int c) { return c < c1 ? kv8_page(a, i, c >> cshift) : -1; };
-  auto scale_of = [&](int page) {  // one that is not finite as NaN; −inf stands for no page
-    if (page < 0) return make_float2(ninf(), 0.f);
-    const float2 s = scales[int64_t(page) * a.heads];
-    return make_float2(isfinite(s.x) ? s.x : qnan(), isfinite(s.y) ? s.y : qnan());
-  };
-  int wbase = c0;
-  int pg = page_of(c0 + lane);
-  if (pg < 0 && c0 + lane < c1) report(a);
-  float2 sc = scale_of(pg);
-  int pg1 = page_of(c0 + 32 + lane);
-  const int8_t* kbase = a.k + ((int64_t(h) << a.plog) + g) * D + 16 * tg;
-  const int8_t* vbase = a.v + ((int64_t(h) << a.plog) + 2 * tg) * D + g * (D / 8);
-  const int64_t pbytes = (int64_t(a.heads) << a.plog) * D;
-
-  Tile<D> buf[PF];
-  auto fetch = [&](Tile<D>& b, int c) {
-    if (c >= c1) return;
-    if (c - wbase == 32) {
-      wbase += 32;
-      pg = pg1;
-      if (pg < 0 && wbase + lane < c1) report(a);
-      sc = scale_of(pg);
-      pg1 = page_of(wbase + 32 + lane);
-    }
-    const int page = __shfl_sync(FULL, pg, c - wbase);
-    b.sk = __shfl_sync(FULL, sc.x, c - wbase);
-    b.sv = __shfl_sync(FULL, sc.y, c - wbase);
-    if (page < 0) {  // no such page: its tokens are not there (sk is −inf)
-#pragma unroll
-      for (int j = 0; j < H2; j++) b.k[0][j] = b.k[1][j] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int j = 0; j < D / 32; j++) b.v[j] = make_uint4(0, 0, 0, 0);
-      return;
-    }
-    const int64_t at = page * pbytes + ((c << 4) & ((1 << a.plog) - 1)) * D;
-    const int8_t *kp = kbase + at, *vp = vbase + at;
-#pragma unroll
-    for (int r = 0; r < 2; r++)
-#pragma unroll
-      for (int j = 0; j < H2; j++)
-        b.k[r][j] = __ldg(reinterpret_cast<const uint4*>(kp + r * 8 * D + j * 64));
-    if constexpr (D == 64) {
-      const uint2 x0 = __ldg(reinterpret_cast<const uint2*>(vp)), x1 = __ldg(reinterpret_cast<const uint2*>(vp + D));
-      const uint2 x2 = __ldg(reinterpret_cast<const uint2*>(vp + 8 * D)),
-                  x3 = __ldg(reinterpret_cast<const uint2*>(vp + 9 * D));
-      b.v[0] = make_uint4(x0.x, x0.y, x1.x, x1.y);
-      b.v[1] = make_uint4(x2.x, x2.y, x3.x, x3.y);
-    } else {
-      b.v[0] = __ldg(reinterpret_cast<const uint4*>(vp));
-      b.v[1] = __ldg(reinterpret_cast<const uint4*>(vp + D));
-      b.v[2] = __ldg(reinterpret_cast<const uint4*>(vp + 8 * D));
-      b.v[3] = __ldg(reinterpret_cast<const uint4*>(vp + 9 * D));
-    }
+  Pages pages(a, i, h, c0, c1, lane, early);
+  const Ring<D> ring(a, h, rings + warp * R * Ring<D>::tile, lane);
+  // tiles are fetched in order, R − 1 ahead of the one in use, a group of copies each
+  int fc = c0;
+  auto fetch = [&](int n, int page) {
+    if (fc < c1) ring.fetch(n, page, fc);
+    copies_commit();
+    fc++;
   };
 #pragma unroll
-  for (int u = 0; u < PF; u++) fetch(buf[u], c0 + u);
+  for (int u = 0; u < R - 1; u++) fetch(u, __shfl_sync(FULL, pages.page, u));
 
   // --- the queries: rotated, and written as digits ---
   for (int nq = WU == 1 ? 0 : warp; nq < NQ; nq += WU) {
@@ -575,42 +686,21 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
         }
       }
     rotate16<D>(x, a, pos, tg);
-    float amax = 0.f;
-    bool finite = true;
-#pragma unroll
-    for (int j = 0; j < H2; j++)
-#pragma unroll
-      for (int e = 0; e < 16; e++) {
-        amax = fmaxf(amax, fabsf(x[j][e]));
-        finite = finite && isfinite(x[j][e]);
-      }
-    amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, 2));
-    finite = ((__ballot_sync(FULL, finite) >> (lane & ~3)) & 15) == 15;
-    // tiny rows are lifted first, so that neither quotient leaves the range
-    const float lift = amax < 1e-30f ? 1e30f : 1.f;
-    const float to = finite && amax > 0.f ? __fdiv_rn(kQueryUnits, __fmul_rn(amax, lift)) : 0.f;
+    const float amax = group_amax<D>(x, FULL);  // NaN where a value is none
+    const float to = lift_row<D>(x, amax);
 #pragma unroll
     for (int j = 0; j < H2; j++) {
-      uint32_t w[3][4] = {};
+      uint32_t y[16];
 #pragma unroll
-      for (int e = 0; e < 16; e++) {
-        int n = finite ? __float2int_rn(__fmul_rn(__fmul_rn(x[j][e], lift), to)) : 0;
-#pragma unroll
-        for (int d = 0; d < 3; d++) {
-          const int digit = d < 2 ? int(int8_t(n)) : n;
-          n = (n - digit) >> 8;
-          w[d][e / 4] |= uint32_t(digit & 255) << (8 * (e % 4));
-        }
-      }
+      for (int e = 0; e < 16; e++) y[e] = digits_of(__fmaf_rn(x[j][e], to, MAGIC));
 #pragma unroll
       for (int d = 0; d < 3; d++)
-        qd[((nq * 3 + d) * H2 + j) * 32 + lane] = make_uint4(w[d][0], w[d][1], w[d][2], w[d][3]);
+        qd[((nq * 3 + d) * H2 + j) * 32 + lane] =
+            make_uint4(take_bytes(y, d), take_bytes(y + 4, d), take_bytes(y + 8, d), take_bytes(y + 12, d));
     }
     if (tg == 0) {
       // scores in units of log 2; a query that is no number has no score
-      const float f = __fmul_rn(__fmul_rn(amax, 1.f / kQueryUnits), __fmul_rn(t.scale, 1.44269504f));
-      qf[r] = finite ? f : qnan();
+      qf[r] = __fmul_rn(__fmul_rn(amax, 1.f / kQueryUnits), __fmul_rn(t.scale, 1.44269504f));
       qpos[r] = there ? pos : -1;
     }
   }
@@ -632,10 +722,13 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
     }
   // tiles that every query of the unit sees whole
   const int in_lo = max(first, t.window > 0 ? pmax - t.window + 1 : 0), in_hi = pmin;
-  auto step = [&](const Tile<D>& b, int c) {
-    const bool edge = c * 16 < in_lo || c * 16 + 15 > in_hi || b.sk == ninf();
-    if (fabsf(b.sv) > W) {  // a larger scale, in every lane alike: twice it, to move less often
-      const float w = fminf(fmaxf(__fmul_rn(2.f, fabsf(b.sv)), 1.17549435e-38f), 3.4e38f), k = __fdiv_rn(W, w);
+  auto step = [&](int n, int c) {
+    const int j = c - pages.base;
+    const int page = __shfl_sync(FULL, pages.page, j);
+    const float bsk = __shfl_sync(FULL, pages.scale.x, j), bsv = __shfl_sync(FULL, pages.scale.y, j);
+    const bool edge = page < 0 || c * 16 < in_lo || c * 16 + 15 > in_hi;
+    if (bsv > W) {  // a larger scale, in every lane alike: twice it, to move less often
+      const float w = fminf(fmaxf(__fmul_rn(2.f, bsv), 1.17549435e-38f), 3.4e38f), k = __fdiv_rn(W, w);
       W = w;
       toW = __fdiv_rn(1.f, w);
 #pragma unroll
@@ -645,7 +738,9 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
 #pragma unroll
           for (int j = 0; j < 4; j++) o[nq][mt][j] = __fmul_rn(o[nq][mt][j], k);
     }
-    const float sv = __fmul_rn(b.sv, toW);
+    uint4 bk[2][H2];
+    ring.keys(n, bk);
+    const float sv = __fmul_rn(bsv, toW);
     uint32_t pw[NQ][NP][2];  // the weights, transposed: queries in rows
 #pragma unroll
     for (int nq = 0; nq < NQ; nq++) {
@@ -654,8 +749,8 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
 #pragma unroll
         for (int j = 0; j < H2; j++) {
           const uint4 q = qd[((nq * 3 + d) * H2 + j) * 32 + lane];
-          mma_s8(acc, b.k[0][j].x, b.k[1][j].x, b.k[0][j].y, b.k[1][j].y, q.x, q.y);
-          mma_s8(acc, b.k[0][j].z, b.k[1][j].z, b.k[0][j].w, b.k[1][j].w, q.z, q.w);
+          mma_s8(acc, bk[0][j].x, bk[1][j].x, bk[0][j].y, bk[1][j].y, q.x, q.y);
+          mma_s8(acc, bk[0][j].z, bk[1][j].z, bk[0][j].w, bk[1][j].w, q.z, q.w);
         }
       };
       // the two upper digits share an accumulator: 128·128·16512 < 2^31
@@ -665,7 +760,7 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
       digit(hi, 1);
       digit(lo, 0);
       float s[4], x[4];
-      const float fs[2] = {__fmul_rn(f[nq][0], b.sk), __fmul_rn(f[nq][1], b.sk)};
+      const float fs[2] = {__fmul_rn(f[nq][0], bsk), __fmul_rn(f[nq][1], bsk)};
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         s[j] = __fmaf_rn(256.f, float(hi[j]), float(lo[j]));
@@ -676,7 +771,7 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           const int p = qpos[nq * 8 + 2 * tg + (j & 1)], key = c * 16 + g + (j >> 1) * 8;
-          hide[j] = key > p || key < first || (t.window > 0 && key <= p - t.window) || b.sk == ninf();
+          hide[j] = key > p || key < first || (t.window > 0 && key <= p - t.window) || page < 0;
           if (hide[j]) x[j] = ninf();
         }
       }
@@ -724,13 +819,12 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
           pw[nq][n][j] = transpose8(y);
         }
     }
-    const uint32_t* vw = &b.v[0].x;  // four tokens of D/32 words
-    constexpr int WV = D / 32;
+    uint32_t bv[4][D / 32];
+    ring.values(n, bv);
     auto values = [&](auto MT) {
       constexpr int mt = decltype(MT)::value, wd = mt / 2, by = 2 * (mt % 2);
-      const uint32_t a0 = bytes_f16<by>(vw[wd], vw[WV + wd]), a1 = bytes_f16<by + 1>(vw[wd], vw[WV + wd]);
-      const uint32_t a2 = bytes_f16<by>(vw[2 * WV + wd], vw[3 * WV + wd]),
-                     a3 = bytes_f16<by + 1>(vw[2 * WV + wd], vw[3 * WV + wd]);
+      const uint32_t a0 = bytes_f16<by>(bv[0][wd], bv[1][wd]), a1 = bytes_f16<by + 1>(bv[0][wd], bv[1][wd]);
+      const uint32_t a2 = bytes_f16<by>(bv[2][wd], bv[3][wd]), a3 = bytes_f16<by + 1>(bv[2][wd], bv[3][wd]);
 #pragma unroll
       for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
@@ -747,13 +841,23 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
       values(std::integral_constant<int, 7>());
     }
   };
-  for (int c = c0; c < c1; c += PF) {
-#pragma unroll
-    for (int u = 0; u < PF; u++)
-      if (c + u < c1) {
-        step(buf[u], c + u);
-        fetch(buf[u], c + u + PF);
-      }
+  int n = 0;
+  for (int c = c0; c < c1; c++) {
+    if (c - pages.base == 32) pages.move(lane);
+    copies_wait<R - 2>();
+    __syncwarp();  // every lane's copies of this tile, and its reads of the one before
+    {
+      // the tile R − 1 further on, into the place that the last step left;
+      // its page may be among the next 32 tiles'
+      const int j = fc - pages.base, pn = __shfl_sync(FULL, j < 32 ? pages.page : pages.ahead, j & 31);
+      fetch(n == 0 ? R - 1 : n - 1, pn);
+    }
+    step(n, c);
+    n = n + 1 == R ? 0 : n + 1;
+  }
+  if (WU > 1) {
+    copies_wait<0>();
+    __syncthreads();  // the rings are done: their place is used again
   }
 #pragma unroll
   for (int nq = 0; nq < NQ; nq++)
@@ -919,37 +1023,43 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
 // a larger value scale) or 32768 keys have gone by; then they go into
 // float32 sums. About 60 instructions for sixteen tokens where eight columns
 // of queries take 260: bound by the cache's bytes.
-template <int D>
-struct Tile2 {  // 32 tokens: two tiles of sixteen
-  uint4 k[2][2][D / 64];
-  uint4 v[2][D / 32];
-};
-
 __device__ __forceinline__ void mma_s8u8(int* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+#ifndef KV8_STEPS64
+#define KV8_STEPS64 3
+#define KV8_WARPS64 16
+#endif
+#ifndef KV8_STEPS128
+#define KV8_STEPS128 2
+#define KV8_WARPS128 12
+#endif
 template <int D, int WU>
 struct Shape1 {
   static constexpr int warps = WU == 1 ? 4 : WU;
-  static constexpr int per_sm = D == 64 ? 16 : 8;  // warps, by their registers
+  static constexpr int ring = D == 64 ? KV8_STEPS64 : KV8_STEPS128;  // steps of 32 tokens
+  static constexpr int per_sm = D == 64 ? KV8_WARPS64 : KV8_WARPS128;  // warps, by registers and rings
   static constexpr int blocks = per_sm / warps < 1 ? 1 : per_sm / warps;
-  static constexpr size_t smem = WU == 1 ? 0 : size_t(warps + 1) * (D + 2) * 4;
+  static constexpr size_t rings = size_t(warps) * ring * 2 * Ring<D>::tile;
+  static constexpr size_t smem = rings;  // the joined outputs, smaller, take their place
 };
 
 template <int D, int WU>
 __global__ void __launch_bounds__(32 * Shape1<D, WU>::warps, Shape1<D, WU>::blocks)
     k_kv8_attend1(Kv8Args a, Kv8Attend t, int type, int S, int units, bool vec) {
-  constexpr int H2 = D / 64, M = D / 16, WV = D / 32;
+  constexpr int H2 = D / 64, M = D / 16, WV = D / 32, R = Shape1<D, WU>::ring;
   constexpr float kOne = 4194303.f;  // of a weight of 1; weights go to 2
-  extern __shared__ __align__(16) float part[];  // [WU][D + 2], and the block's
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* part = reinterpret_cast<float*>(smem);  // [WU][D + 2], and the block's, when the rings are done
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tg = lane & 3;
   const int rank = S > 1 ? int(cluster_rank()) : 0;
   const int unit = WU == 1 ? blockIdx.x * Shape1<D, WU>::warps + warp : blockIdx.x / S;
   if (unit >= units) return;
   const int h = unit % a.heads, i = unit / a.heads;
+  const int early = early_page(a, i, lane);
   const Kv8Span sp = kv8_span(a, i);
   if (!sp.ok) {
     if ((WU == 1 ? lane : tid) == 0) report(a);
@@ -959,66 +1069,24 @@ __global__ void __launch_bounds__(32 * Shape1<D, WU>::warps, Shape1<D, WU>::bloc
   const int p = sp.len - 1;  // the query's position
   const int first = max(a.first ? max(0, a.first[i]) : 0, t.window > 0 ? p - t.window + 1 : 0);
   const int cb = first >> 4, ce = max(cb, (p + 16) >> 4);
-  const int per = (ce - cb + S * WU - 1) / (S * WU);
+  const int per = ((ce - cb + S * WU - 1) / (S * WU) + 1) & ~1;  // whole steps
   const int c0 = min(ce, cb + (WU == 1 ? 0 : rank * WU + warp) * per), c1 = min(ce, c0 + per);
 
-  // --- the pages ahead: lane l holds page and scales of the tile wbase + l ---
-  const int cshift = a.plog - 4;
-  const float2* scales = reinterpret_cast<const float2*>(a.scale) + h;
-  auto page_of = [&](int c) { return c < c1 ? kv8_page(a, i, c >> cshift) : -1; };
-  auto scale_of = [&](int page) {
-    if (page < 0) return make_float2(0.f, 0.f);
-    const float2 s = scales[int64_t(page) * a.heads];
-    return make_float2(isfinite(s.x) ? s.x : qnan(), s.y >= 0.f && isfinite(s.y) ? s.y : qnan());
-  };
-  int wbase = c0;
-  int pg = page_of(c0 + lane);
-  if (pg < 0 && c0 + lane < c1) report(a);
-  float2 sc = scale_of(pg);
-  int pg1 = page_of(c0 + 32 + lane);
-  const int8_t* kbase = a.k + ((int64_t(h) << a.plog) + g) * D + 16 * tg;
-  const int8_t* vbase = a.v + ((int64_t(h) << a.plog) + 2 * tg) * D + g * (D / 8);
-  const int64_t pbytes = (int64_t(a.heads) << a.plog) * D;
-  const int smask = (1 << a.plog) - 1;
-
-  Tile2<D> b;
-  // loads of the step at tile c, by pages pa and pb (−1: its tokens are not there)
-  auto load_k = [&](int c, int pa, int pb) {
-#pragma unroll
-    for (int n = 0; n < 2; n++) {
-      const int page = n ? pb : pa;
-      const int8_t* kp = kbase + page * pbytes + (((c + n) << 4) & smask) * D;
-#pragma unroll
-      for (int r = 0; r < 2; r++)
-#pragma unroll
-        for (int j = 0; j < H2; j++)
-          b.k[n][r][j] = page < 0 ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(kp + r * 8 * D + j * 64));
+  Pages pages(a, i, h, c0, c1, lane, early);
+  const Ring<D> ring(a, h, smem + warp * R * 2 * Ring<D>::tile, lane);
+  // steps of two tiles are fetched in order, R − 1 ahead of the one in use, a group of copies each
+  int fc = c0;
+  auto fetch = [&](int n, int pa, int pb) {
+    if (fc < c1) {
+      ring.fetch(2 * n, pa, fc);
+      ring.fetch(2 * n + 1, pb, fc + 1);
     }
+    copies_commit();
+    fc += 2;
   };
-  auto load_v = [&](int c, int pa, int pb) {
 #pragma unroll
-    for (int n = 0; n < 2; n++) {
-      const int page = n ? pb : pa;
-      const int8_t* vp = vbase + page * pbytes + (((c + n) << 4) & smask) * D;
-      if constexpr (D == 64) {
-        uint2 x[4];
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-          x[r] = page < 0 ? make_uint2(0, 0)
-                          : __ldg(reinterpret_cast<const uint2*>(vp + ((r & 1) + (r >> 1) * 8) * D));
-        b.v[n][0] = make_uint4(x[0].x, x[0].y, x[1].x, x[1].y);
-        b.v[n][1] = make_uint4(x[2].x, x[2].y, x[3].x, x[3].y);
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-          b.v[n][r] = page < 0 ? make_uint4(0, 0, 0, 0)
-                               : __ldg(reinterpret_cast<const uint4*>(vp + ((r & 1) + (r >> 1) * 8) * D));
-      }
-    }
-  };
-  int pa = __shfl_sync(FULL, pg, 0), pb = __shfl_sync(FULL, pg, 1);
-  load_k(c0, pa, pb);
-  load_v(c0, pa, pb);
+  for (int u = 0; u < R - 1; u++)
+    fetch(u, __shfl_sync(FULL, pages.page, 2 * u), __shfl_sync(FULL, pages.page, 2 * u + 1));
 
   // --- the query: rotated, and written as digits ---
   uint32_t q01[H2][4], q2[H2][4];
@@ -1039,36 +1107,19 @@ __global__ void __launch_bounds__(32 * Shape1<D, WU>::warps, Shape1<D, WU>::bloc
           load4(static_cast<const __nv_bfloat16*>(t.q.p) + o, vec, &x[j][e]);
       }
     rotate16<D>(x, a, p, tg);
-    float amax = 0.f;
-    bool finite = true;
-#pragma unroll
-    for (int j = 0; j < H2; j++)
-#pragma unroll
-      for (int e = 0; e < 16; e++) {
-        amax = fmaxf(amax, fabsf(x[j][e]));
-        finite = finite && isfinite(x[j][e]);
-      }
-    amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, 2));
-    finite = __all_sync(FULL, finite);
-    const float lift = amax < 1e-30f ? 1e30f : 1.f;
-    const float to = finite && amax > 0.f ? __fdiv_rn(kQueryUnits, __fmul_rn(amax, lift)) : 0.f;
+    const float amax = group_amax<D>(x, FULL);  // NaN where a value is none
+    const float to = lift_row<D>(x, amax);
 #pragma unroll
     for (int j = 0; j < H2; j++)
 #pragma unroll
       for (int w = 0; w < 4; w++) {
-        uint32_t lo = 0, up = 0;
+        uint32_t n[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const int n = finite ? __float2int_rn(__fmul_rn(__fmul_rn(x[j][4 * w + e], lift), to)) : 0;
-          const int d0 = int8_t(n), n1 = (n - d0) >> 8, d1 = int8_t(n1), d2 = (n1 - d1) >> 8;
-          lo |= uint32_t((g & 1 ? d1 : d0) & 255) << (8 * e);
-          up |= uint32_t((g & 1 ? d2 : 0) & 255) << (8 * e);
-        }
-        q01[j][w] = lo;
-        q2[j][w] = up;
+        for (int e = 0; e < 4; e++) n[e] = digits_of(__fmaf_rn(x[j][4 * w + e], to, MAGIC));
+        q01[j][w] = take_bytes(n, g & 1);
+        q2[j][w] = g & 1 ? take_bytes(n, 2) : 0;
       }
-    f = finite ? __fmul_rn(__fmul_rn(amax, 1.f / kQueryUnits), __fmul_rn(t.scale, 1.44269504f)) : qnan();
+    f = __fmul_rn(__fmul_rn(amax, 1.f / kQueryUnits), __fmul_rn(t.scale, 1.44269504f));
   }
 
   // --- the pass over the keys: lane (g, tg) has key g + 8·(tg & 1) of tile tg >> 1 ---
@@ -1077,92 +1128,75 @@ __global__ void __launch_bounds__(32 * Shape1<D, WU>::warps, Shape1<D, WU>::bloc
   int lh[M][4] = {}, md[M][4] = {};  // lowest (even columns) and highest (odd) digits; middle ones
   float o[M][2] = {};
   float ref = ninf(), l = 0.f, W = 0.f, toW = 0.f;
-  auto flush = [&]() {
+  int held = 0;  // steps in the integer sums
+  // the integer sums into the float ones, and these times r
+  auto flush = [&](float r) {
 #pragma unroll
     for (int mt = 0; mt < M; mt++)
 #pragma unroll
       for (int e = 0; e < 2; e++) {
         const float lo = __fmaf_rn(256.f, float(md[mt][2 * e]), float(lh[mt][2 * e]));
-        o[mt][e] = __fadd_rn(o[mt][e], __fmaf_rn(65536.f, float(lh[mt][2 * e + 1]), lo));
+        o[mt][e] = __fmul_rn(r, __fadd_rn(o[mt][e], __fmaf_rn(65536.f, float(lh[mt][2 * e + 1]), lo)));
         lh[mt][2 * e] = lh[mt][2 * e + 1] = md[mt][2 * e] = 0;
       }
+    held = 0;
   };
-  auto rescale = [&](float r) {
-#pragma unroll
-    for (int mt = 0; mt < M; mt++) {
-      o[mt][0] = __fmul_rn(o[mt][0], r);
-      o[mt][1] = __fmul_rn(o[mt][1], r);
-    }
-  };
-  int held = 0;  // steps in the integer sums
-  for (int c = c0; c < c1; c += 2) {
-    // this step's scales, the next one's pages
-    const int j = c - wbase;
-    const float sk = __shfl_sync(FULL, sc.x, j + (tg >> 1));
-    const float sva = __shfl_sync(FULL, sc.y, j), svb = __shfl_sync(FULL, sc.y, j + 1);
-    const bool gone = pa < 0 || pb < 0, mygone = (tg < 2 ? pa : pb) < 0;
-    const bool edge = gone || c * 16 < first || c * 16 + 31 > p;
-    if (j == 30) {
-      wbase += 32;
-      pg = pg1;
-      if (pg < 0 && wbase + lane < c1) report(a);
-      sc = scale_of(pg);
-      pg1 = page_of(wbase + 32 + lane);
-    }
-    pa = __shfl_sync(FULL, pg, c + 2 - wbase);
-    pb = __shfl_sync(FULL, pg, c + 3 - wbase);
-
+  auto step = [&](int n, int c) {
+    const int j = c - pages.base;
+    const int pa = __shfl_sync(FULL, pages.page, j), pb = __shfl_sync(FULL, pages.page, j + 1);
+    const float sva = __shfl_sync(FULL, pages.scale.y, j), svb = __shfl_sync(FULL, pages.scale.y, j + 1);
+    const float fs = __fmul_rn(f, __shfl_sync(FULL, pages.scale.x, j + (tg >> 1)));
+    float sv = tg < 2 ? sva : svb;
+    const float wide = fmaxf(sva, svb);
+    const bool edge = (pa | pb) < 0 || c * 16 < first || c * 16 + 31 > p;
     // the highest digit's sums, then the lower ones' on top: even columns
     // the lowest digit, odd ones 256·highest + middle (below 2^31)
+    uint4 ka[2][H2], kb[2][H2];
+    ring.keys(2 * n, ka);
+    ring.keys(2 * n + 1, kb);
     int s0[4] = {0, 0, 0, 0}, s1[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int e = 0; e < H2; e++) {
-      mma_s8(s0, b.k[0][0][e].x, b.k[0][1][e].x, b.k[0][0][e].y, b.k[0][1][e].y, q2[e][0], q2[e][1]);
-      mma_s8(s1, b.k[1][0][e].x, b.k[1][1][e].x, b.k[1][0][e].y, b.k[1][1][e].y, q2[e][0], q2[e][1]);
-      mma_s8(s0, b.k[0][0][e].z, b.k[0][1][e].z, b.k[0][0][e].w, b.k[0][1][e].w, q2[e][2], q2[e][3]);
-      mma_s8(s1, b.k[1][0][e].z, b.k[1][1][e].z, b.k[1][0][e].w, b.k[1][1][e].w, q2[e][2], q2[e][3]);
+      mma_s8(s0, ka[0][e].x, ka[1][e].x, ka[0][e].y, ka[1][e].y, q2[e][0], q2[e][1]);
+      mma_s8(s1, kb[0][e].x, kb[1][e].x, kb[0][e].y, kb[1][e].y, q2[e][0], q2[e][1]);
+      mma_s8(s0, ka[0][e].z, ka[1][e].z, ka[0][e].w, ka[1][e].w, q2[e][2], q2[e][3]);
+      mma_s8(s1, kb[0][e].z, kb[1][e].z, kb[0][e].w, kb[1][e].w, q2[e][2], q2[e][3]);
     }
     s0[1] <<= 8, s0[3] <<= 8, s1[1] <<= 8, s1[3] <<= 8;
 #pragma unroll
     for (int e = 0; e < H2; e++) {
-      mma_s8(s0, b.k[0][0][e].x, b.k[0][1][e].x, b.k[0][0][e].y, b.k[0][1][e].y, q01[e][0], q01[e][1]);
-      mma_s8(s1, b.k[1][0][e].x, b.k[1][1][e].x, b.k[1][0][e].y, b.k[1][1][e].y, q01[e][0], q01[e][1]);
-      mma_s8(s0, b.k[0][0][e].z, b.k[0][1][e].z, b.k[0][0][e].w, b.k[0][1][e].w, q01[e][2], q01[e][3]);
-      mma_s8(s1, b.k[1][0][e].z, b.k[1][1][e].z, b.k[1][0][e].w, b.k[1][1][e].w, q01[e][2], q01[e][3]);
+      mma_s8(s0, ka[0][e].x, ka[1][e].x, ka[0][e].y, ka[1][e].y, q01[e][0], q01[e][1]);
+      mma_s8(s1, kb[0][e].x, kb[1][e].x, kb[0][e].y, kb[1][e].y, q01[e][0], q01[e][1]);
+      mma_s8(s0, ka[0][e].z, ka[1][e].z, ka[0][e].w, ka[1][e].w, q01[e][2], q01[e][3]);
+      mma_s8(s1, kb[0][e].z, kb[1][e].z, kb[0][e].w, kb[1][e].w, q01[e][2], q01[e][3]);
     }
-    if (c + 2 < c1) load_k(c + 2, pa, pb);
     const int lo = tg & 2 ? (tg & 1 ? s1[2] : s1[0]) : (tg & 1 ? s0[2] : s0[0]);
     const int up = tg & 2 ? (tg & 1 ? s1[3] : s1[1]) : (tg & 1 ? s0[3] : s0[1]);
-    const float s = __fmaf_rn(256.f, float(up), float(lo)), fs = __fmul_rn(f, sk);
-    float x = __fmaf_rn(s, fs, -ref), sv = tg < 2 ? sva : svb;
+    const float s = __fmaf_rn(256.f, float(up), float(lo));
+    float x = __fmaf_rn(s, fs, -ref);
     bool hide = false;
     if (edge) {
       const int key = (c + (tg >> 1)) * 16 + g + 8 * (tg & 1);
-      hide = key > p || key < first || mygone;
+      hide = key > p || key < first || (tg < 2 ? pa : pb) < 0;
       if (hide) x = ninf(), sv = 0.f;
     }
     // The reference moves: a larger value scale (an eighth above it, to move
     // less often), or a score 2 above (any, before the first key).
-    const float wide = fmaxf(sva, svb);
     if (wide > W) {
-      flush();
-      held = 0;
       const float w = fminf(fmaxf(__fmul_rn(1.125f, wide), 1.17549435e-38f), 3.4e38f);
-      rescale(__fdiv_rn(W, w));
+      flush(__fdiv_rn(W, w));
       W = w;
       toW = __fdiv_rn(1.f, w);
     }
     if (__any_sync(FULL, x > 1.f)) {
-      flush();
-      held = 0;
       float m = hide ? ninf() : __fmul_rn(s, fs);
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, d));
       m = fmaxf(m, ref);
       const float r = ref == m ? 1.f : ex2(__fsub_rn(ref, m));
+      flush(r);
       ref = m;
       l = __fmul_rn(l, r);
-      rescale(r);
       x = hide ? ninf() : __fmaf_rn(s, fs, -m);
     }
     const float w = ex2(x);
@@ -1172,21 +1206,23 @@ __global__ void __launch_bounds__(32 * Shape1<D, WU>::warps, Shape1<D, WU>::bloc
     const uint32_t yt = transpose8(y);
     const uint32_t b0 = __byte_perm(yt, 0, at0), b1 = __byte_perm(yt, 0, at1);
     const uint32_t m0 = __byte_perm(yt, 0, mid0), m1 = __byte_perm(yt, 0, mid1);
-    const uint32_t *va = &b.v[0][0].x, *vb = &b.v[1][0].x;
+    uint32_t v[2][4][WV];
+    ring.values(2 * n, v[0]);
+    ring.values(2 * n + 1, v[1]);
 #pragma unroll
     for (int wd = 0; wd < WV; wd++) {
       // four tokens' words of four values each → four words of a value each
       uint32_t d[2][4];
 #pragma unroll
-      for (int n = 0; n < 2; n++) {
-        const uint32_t* v = n ? vb : va;
-        const uint32_t l01 = __byte_perm(v[wd], v[WV + wd], 0x5140), h01 = __byte_perm(v[wd], v[WV + wd], 0x7362);
-        const uint32_t l23 = __byte_perm(v[2 * WV + wd], v[3 * WV + wd], 0x5140),
-                       h23 = __byte_perm(v[2 * WV + wd], v[3 * WV + wd], 0x7362);
-        d[n][0] = __byte_perm(l01, l23, 0x5410);
-        d[n][1] = __byte_perm(l01, l23, 0x7632);
-        d[n][2] = __byte_perm(h01, h23, 0x5410);
-        d[n][3] = __byte_perm(h01, h23, 0x7632);
+      for (int m = 0; m < 2; m++) {
+        const uint32_t l01 = __byte_perm(v[m][0][wd], v[m][1][wd], 0x5140),
+                       h01 = __byte_perm(v[m][0][wd], v[m][1][wd], 0x7362);
+        const uint32_t l23 = __byte_perm(v[m][2][wd], v[m][3][wd], 0x5140),
+                       h23 = __byte_perm(v[m][2][wd], v[m][3][wd], 0x7362);
+        d[m][0] = __byte_perm(l01, l23, 0x5410);
+        d[m][1] = __byte_perm(l01, l23, 0x7632);
+        d[m][2] = __byte_perm(h01, h23, 0x5410);
+        d[m][3] = __byte_perm(h01, h23, 0x7632);
       }
 #pragma unroll
       for (int e = 0; e < 2; e++) {
@@ -1195,13 +1231,28 @@ __global__ void __launch_bounds__(32 * Shape1<D, WU>::warps, Shape1<D, WU>::bloc
         mma_s8u8(md[2 * wd + e], av, m0, m1);
       }
     }
-    if (c + 2 < c1) load_v(c + 2, pa, pb);
-    if (++held == 1024) {  // 32768 keys: 255·128·32768 < 2^31
-      flush();
-      held = 0;
+    if (++held == 1024) flush(1.f);  // 32768 keys: 255·128·32768 < 2^31
+  };
+  int n = 0;
+  for (int c = c0; c < c1; c += 2) {
+    if (c - pages.base == 32) pages.move(lane);
+    copies_wait<R - 2>();
+    __syncwarp();  // every lane's copies of this step, and its reads of the one before
+    {
+      // the step R − 1 further on, into the place that the last one left; its
+      // pages may be among the next 32 tiles'
+      const int j = fc - pages.base, from = j < 32 ? pages.page : pages.ahead;
+      const int pa = __shfl_sync(FULL, from, j & 31), pb = __shfl_sync(FULL, from, (j & 31) + 1);
+      fetch(n == 0 ? R - 1 : n - 1, pa, pb);
     }
+    step(n, c);
+    n = n + 1 == R ? 0 : n + 1;
   }
-  flush();
+  if (WU > 1) {
+    copies_wait<0>();
+    __syncthreads();  // the rings are done: their place is used again
+  }
+  flush(1.f);
   // sums over the columns (the lanes of a row group), and over all lanes
 #pragma unroll
   for (int mt = 0; mt < M; mt++)
@@ -1325,7 +1376,7 @@ cudaError_t attend_launch(const Kv8Args& a, int type, const Kv8Attend& t, int64_
 
 // Warps of a block where a unit's keys are split over many.
 template <int D>
-constexpr int kWide = D == 64 ? 16 : 12;
+constexpr int kWide = D == 64 ? 8 : 6;
 
 template <int D, int NQ, int NP>
 cudaError_t attend_t(const Kv8Args& a, int type, const Kv8Attend& t, cudaStream_t st) {
@@ -1338,7 +1389,7 @@ cudaError_t attend_t(const Kv8Args& a, int type, const Kv8Attend& t, cudaStream_
   if constexpr (NQ == 1) {
     constexpr int WU = kWide<D>;
     if (parts > 4 && units <= kSMs) {
-      while (S < 16 && S * WU < parts && units * S * 2 <= kSMs) S *= 2;
+      while (S < 16 && S * WU < parts) S *= 2;
       return attend_launch<D, NQ, NP, WU>(a, type, t, units, qtiles, S, st);
     }
   }
@@ -1390,9 +1441,16 @@ void attend_attrs() {
   cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Shape<D, NQ, WU>::smem));
   cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
 }
+template <int D, int WU>
+void attend1_attrs() {
+  cudaFuncSetAttribute(k_kv8_attend1<D, WU>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Shape1<D, WU>::smem));
+  cudaFuncSetAttribute(k_kv8_attend1<D, WU>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+}
 template <int D>
 void attend1_init() {
-  cudaFuncSetAttribute(k_kv8_attend1<D, 8>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  attend1_attrs<D, 1>();
+  attend1_attrs<D, 4>();
+  attend1_attrs<D, 8>();
 }
 template <int D, int NP>
 void attend_init() {
