@@ -38,6 +38,7 @@ __device__ __forceinline__ void load4(const float* p, bool vec, float* x) {
     for (int i = 0; i < 4; i++) x[i] = p[i];
   }
 }
+__device__ __forceinline__ float wide(float x) { return x; }
 __device__ __forceinline__ float wide(__half h) { return __half2float(h); }
 __device__ __forceinline__ float wide(__nv_bfloat16 h) { return __bfloat162float(h); }
 template <class H>
@@ -60,140 +61,239 @@ __device__ __forceinline__ void narrow(float x, __nv_bfloat16* p) { *p = __float
 // ------------------------------------------------------------- append ----
 //
 // A unit is one (sequence, page it writes, head, keys or values): G threads
-// that hold the page's new values in registers, find their largest
-// magnitude a, and set s' = max(s, a/127); where that grew, what the page
-// held becomes rne(q·s/s'); the new values become rne(x/s'). No two units
-// share a byte or a scale, so there are no atomics and no order.
+// that hold the page's new values, find the largest magnitude a, and set
+// s' = max(s, a/127); where that grew, what the page held becomes
+// rne(q·s/s'); the new values become rne(x/s'). No two units share a byte or
+// a scale, so there are no atomics and no order.
 //
-// Rotation, quotients and roundings are in 64 bits (the products x·cos are
-// exact there): a value next to a rounding border would otherwise go to one
-// or the other side by the order of 32-bit operations, a whole step of the
-// page's scale. The scale itself is stored in 32 bits, as the reader
-// multiplies with it.
+// The definition's rotations, quotients and roundings are in 64 bits: a
+// value next to a rounding border goes to one or the other side by less
+// than 32 bits hold, a whole step of the page's scale. They are computed in
+// 32 bits, which is off by less than 4e-5 of a step (127 steps times a few
+// 2^-24), and again in 64 where a value comes within kNear of a border, as
+// 2 in 10000 do. The scale's largest magnitude likewise: the values within
+// 2^-19 of the largest are formed again in 64 bits. Pages of very small or
+// very large numbers (kTiny, kHuge) take 64 bits throughout.
 //
 // A thread holds at most kItems items of eight values: two groups of four
-// that the rotation pairs with each other.
+// that the rotation pairs with each other. Bound by latency for single
+// tokens, by the bytes of the rows for prompts.
 constexpr int kItems = 4;
+constexpr float kNear = 0.4999f;
+constexpr float kTiny = 1e-30f, kHuge = 1e37f;
+
+// One item's eight values in 64 bits: elements e0 .. e0 + 3 and e1 .. e1 + 3
+// of a row, rotated by the angles at cs.
+template <class T>
+__device__ void item64(const T* src, int e0, int e1, int mode, const float* cs, double* y) {
+#pragma unroll
+  for (int j = 0; j < 8; j++) y[j] = wide(src[j < 4 ? e0 + j : e1 + j - 4]);
+  if (mode == ROPE_NONE) return;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const int p = mode == ROPE_PAIRS ? 2 * j : j, q = mode == ROPE_PAIRS ? 2 * j + 1 : j + 4;
+    const double xa = y[p], xb = y[q], cc = cs[2 * j], ss = cs[2 * j + 1];
+    // the products are exact, so one rounding each
+    y[p] = __fma_rn(xa, cc, -(xb * ss));
+    y[q] = __fma_rn(xa, ss, xb * cc);
+  }
+}
+
+// Four signed bytes times r, rounded, and whether any came near a border.
+__device__ __forceinline__ uint32_t scaled_bytes(uint32_t q, float r, bool* near) {
+  const uint32_t u = q ^ 0x80808080u;
+  float t[4], off = 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    const float v = __fsub_rn(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 | k)), 8388736.f);
+    t[k] = __fmaf_rn(v, r, MAGIC);
+    off = fmaxf(off, fabsf(__fmaf_rn(v, r, -__fsub_rn(t[k], MAGIC))));
+  }
+  *near = *near || off > kNear;
+  return __byte_perm(__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040),
+                     __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
+}
 
 template <int D, int G, class T>
-__global__ void __launch_bounds__(256) k_kv8_append(Kv8Args a, Kv8Rows kin, Kv8Rows vin, int blocks, bool vec) {
-  __shared__ double red[8];
+__global__ void __launch_bounds__(256, G == D / 8 ? 4 : 3) k_kv8_append(Kv8Args a, Kv8Rows kin, Kv8Rows vin, int blocks, bool vec) {
+  constexpr int C = D / 8;                // items a token
+  constexpr int N = G == C ? 1 : kItems;  // items a thread
+  __shared__ uint32_t red[16];
   const int tid = threadIdx.x % G;
-  const int64_t unit = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) / G;
-  const int hh = int(unit % (2 * a.heads)), h = hh >> 1;
-  const bool key = (hh & 1) == 0;
-  const int64_t rest = unit / (2 * a.heads);
-  const int b = int(rest % blocks);
-  const int64_t i64 = rest / blocks;
-  if (i64 >= a.n) return;
-  const int i = int(i64);
-  const Kv8Span sp = kv8_span(a, i);
-  if (!sp.ok) {
-    if (tid == 0) report(a);
-    return;
+  const uint32_t unit = (blockIdx.x * 256u + threadIdx.x) / G;  // the launch has fewer than 2^31
+  const uint32_t rest = unit / (2 * a.heads);
+  const int hh = int(unit - rest * (2 * a.heads)), h = hh < a.heads ? hh : hh - a.heads;
+  const bool key = hh < a.heads;
+  const int i = min(int(rest / blocks), a.n), b = int(rest % blocks);
+  // every thread stays for the exchanges between lanes; `live` ones have work
+  bool live = i < a.n;
+  Kv8Span sp = {0, 0, 0, false};
+  if (live) {
+    sp = kv8_span(a, i);
+    if (!sp.ok && tid == 0) report(a);
+    live = sp.ok;
   }
-  const int p0 = sp.len - sp.T;
-  if (p0 < 0 || sp.T == 0) return;  // a slot that holds nothing
-  const int block = (p0 >> a.plog) + b, begin = block << a.plog;
+  const int p0 = sp.len - sp.T;  // below 0: a slot that holds nothing
+  const int block = (max(p0, 0) >> a.plog) + b, begin = block << a.plog;
   const int lo = max(p0, begin), hi = min(sp.len, begin + (1 << a.plog));
-  if (lo >= hi) return;
-  const int page = kv8_page(a, i, block);
-  if (page < 0) {
-    if (tid == 0) report(a);
-    return;
-  }
-  const int held = lo - begin;  // tokens that the page holds already
-  const int64_t ph = int64_t(page) * a.heads + h;
-  int8_t* base = (key ? a.k : a.v) + ((ph << a.plog) * D);
-  float* sptr = a.scale + 2 * ph + (key ? 0 : 1);
-  const float old = held > 0 ? *sptr : 0.f;
+  live = live && p0 >= 0 && lo < hi;
+  if (G > 32 && !live) return;  // a block is one unit
+  // the page's number comes while the rows do
+  const int page = live ? kv8_page(a, i, block) : 0;
 
   const Kv8Rows& in = key ? kin : vin;
   const T* src = static_cast<const T*>(in.p) + int64_t(sp.row + lo - p0) * in.row + int64_t(h) * in.head;
   const int mode = key ? a.rope_mode : ROPE_NONE;
-  constexpr int C = D / 8;  // items a token
-  const int items = (hi - lo) * C;
-  double y[kItems][8];
-  double amax = 0;
-  bool finite = true;
+  int items = live ? (hi - lo) * C : 0;
+  const auto at0 = [&](int c) { return mode == ROPE_HALVES ? 4 * c : 8 * c; };
+  const auto at1 = [&](int c) { return mode == ROPE_HALVES ? D / 2 + 4 * c : 8 * c + 4; };
+  const auto angles = [&](int t, int c) { return a.rope + (int64_t(lo + t) * (D / 2) + 4 * c) * 2; };
+  float y[N][8];
+  float most = 0.f, nan = 0.f;
 #pragma unroll
-  for (int u = 0; u < kItems; u++) {
+  for (int u = 0; u < N; u++) {
     const int it = tid + u * G;
     if (it < items) {
       const int t = it / C, c = it % C;
-      const int e0 = mode == ROPE_HALVES ? 4 * c : 8 * c, e1 = mode == ROPE_HALVES ? D / 2 + 4 * c : 8 * c + 4;
-      float x[8];
-      load4(src + t * in.row + e0, vec, x);
-      load4(src + t * in.row + e1, vec, x + 4);
+      const T* row = src + int64_t(t) * in.row;
+      load4(row + at0(c), vec, y[u]);
+      load4(row + at1(c), vec, y[u] + 4);
       if (mode != ROPE_NONE) {
-        const float4* cs = reinterpret_cast<const float4*>(a.rope + (int64_t(lo + t) * (D / 2) + 4 * c) * 2);
+        const float4* cs = reinterpret_cast<const float4*>(angles(t, c));
         const float4 f0 = cs[0], f1 = cs[1];
         const float co[4] = {f0.x, f0.z, f1.x, f1.z}, si[4] = {f0.y, f0.w, f1.y, f1.w};
+        if (mode == ROPE_PAIRS) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const int p = mode == ROPE_PAIRS ? 2 * j : j, q = mode == ROPE_PAIRS ? 2 * j + 1 : j + 4;
-          const double xa = x[p], xb = x[q], cc = co[j], ss = si[j];
-          // the products are exact, so one rounding each
-          const double r0 = __fma_rn(xa, cc, -(xb * ss)), r1 = __fma_rn(xa, ss, xb * cc);
-          if (mode == ROPE_PAIRS)
-            y[u][2 * j] = r0, y[u][2 * j + 1] = r1;
-          else
-            y[u][j] = r0, y[u][j + 4] = r1;
+          for (int j = 0; j < 4; j++) {
+            const float xa = y[u][2 * j], xb = y[u][2 * j + 1];
+            y[u][2 * j] = __fmaf_rn(xa, co[j], -__fmul_rn(xb, si[j]));
+            y[u][2 * j + 1] = __fmaf_rn(xa, si[j], __fmul_rn(xb, co[j]));
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const float xa = y[u][j], xb = y[u][j + 4];
+            y[u][j] = __fmaf_rn(xa, co[j], -__fmul_rn(xb, si[j]));
+            y[u][j + 4] = __fmaf_rn(xa, si[j], __fmul_rn(xb, co[j]));
+          }
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++) y[u][j] = x[j];
       }
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        amax = fmax(amax, fabs(y[u][j]));
-        finite = finite && isfinite(y[u][j]);
+        most = fmaxf(most, fabsf(y[u][j]));
+        nan = __fmaf_rn(0.f, y[u][j], nan);  // 0·inf and 0·NaN
       }
     }
   }
-  // a value that is no number makes the scale none either
-  if (!finite) amax = INFINITY;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmax(amax, __shfl_xor_sync(FULL, amax, o));
-  if (G > 32) {
-    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = amax;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < G / 32; w++) amax = fmax(amax, red[w]);
+  if (page < 0) {
+    if (live && tid == 0) report(a);
+    live = false;
+    items = 0;
+    most = nan = 0.f;
   }
-  float scale = fmaxf(old, float(amax / 127.0));
-  if (isinf(amax) || isnan(old)) scale = __int_as_float(0x7fc00000);
-  const bool grown = scale > old;
-  const double back = scale > 0.f ? 1.0 / double(scale) : 0.0;  // 0 for 0 and for no number
-  if (held > 0 && grown) {
-    const double r = double(old) * back;
+  const int held = live ? lo - begin : 0;  // tokens that the page holds already
+  const int64_t ph = int64_t(max(page, 0)) * a.heads + h;
+  int8_t* base = (key ? a.k : a.v) + ((ph << a.plog) * D);
+  float* sptr = a.scale + 2 * ph + (key ? 0 : 1);
+  const float old = held > 0 ? *sptr : 0.f;
+  // the unit's largest of numbers that are not negative, as their bits
+  // compare (NaN above all); `round` picks the place of its exchange
+  auto largest = [&](float m, int round) {
+    uint32_t v = __float_as_uint(m) & 0x7fffffffu;
+    if constexpr (G < 32) {
+#pragma unroll
+      for (int o = G / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(FULL, v, o));
+    } else {
+      v = __reduce_max_sync(FULL, v);
+      if constexpr (G > 32) {
+        if (threadIdx.x % 32 == 0) red[8 * round + threadIdx.x / 32] = v;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < G / 32; w++) v = max(v, red[8 * round + w]);
+      }
+    }
+    return __uint_as_float(v);
+  };
+  const float top = largest(__fadd_rn(most, nan), 0);
+  bool slow = !(top < kHuge) || (top > 0.f && top < kTiny);
+  float mine = 0.f;  // a/127 as stored, of this thread's candidates
+  const float bound = slow ? 0.f : __fmul_rn(top, 1.f - 0x1p-19f);
+  if (top != 0.f && (slow || most >= bound)) {
+#pragma unroll
+    for (int u = 0; u < N; u++) {
+      const int it = tid + u * G;
+      float m32 = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; j++) m32 = fmaxf(m32, fabsf(y[u][j]));
+      if (it >= items || !(slow || m32 >= bound)) continue;
+      if (mode == ROPE_NONE && !slow) {  // not rotated: exact as it is
+        mine = fmaxf(mine, float(double(m32) / 127.0));
+        continue;
+      }
+      const int t = it / C, c = it % C;
+      double x[8];
+      item64(src + int64_t(t) * in.row, at0(c), at1(c), mode, angles(t, c), x);
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const double m = fabs(x[j]);
+        if (!(m <= 1.7976931348623157e308))
+          mine = __int_as_float(0x7fc00000);
+        else if (m >= bound && !isnan(mine))
+          mine = fmaxf(mine, float(m / 127.0));
+      }
+    }
+  }
+  const float fresh = largest(mine, 1);
+  const float scale = isnan(old) || isnan(fresh) ? __int_as_float(0x7fc00000) : fmaxf(old, fresh);
+  const bool some = scale > 0.f;  // not 0, and a number
+  slow = slow || scale < kTiny;
+  const float back = some ? __fdiv_rn(1.f, scale) : 0.f;
+  if (held > 0 && scale > old) {
+    const float r = __fmul_rn(old, back);
     uint4* w = reinterpret_cast<uint4*>(base);
     for (int j = tid; j < held * (D / 16); j += G) {
-      uint4 q = w[j];
-      uint32_t* qw = &q.x;
+      const uint4 q = w[j];
+      bool near = slow;
+      uint4 z = make_uint4(scaled_bytes(q.x, r, &near), scaled_bytes(q.y, r, &near), scaled_bytes(q.z, r, &near),
+                           scaled_bytes(q.w, r, &near));
+      if (near) {
+        const double r64 = double(old) * (1.0 / double(scale));
+        const uint32_t qw[4] = {q.x, q.y, q.z, q.w};
+        uint32_t zw[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        uint32_t o = 0;
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const int v = int8_t(qw[e] >> (8 * k));
-          o |= uint32_t(__double2int_rn(double(v) * r) & 255) << (8 * k);
-        }
-        qw[e] = o;
+        for (int e = 0; e < 16; e++)
+          zw[e / 4] |= uint32_t(__double2int_rn(double(int8_t(qw[e / 4] >> (8 * (e % 4)))) * r64) & 255) << (8 * (e % 4));
+        z = make_uint4(zw[0], zw[1], zw[2], zw[3]);
       }
-      w[j] = q;
+      w[j] = z;
     }
   }
 #pragma unroll
-  for (int u = 0; u < kItems; u++) {
+  for (int u = 0; u < N; u++) {
     const int it = tid + u * G;
     if (it < items) {
       const int t = it / C, c = it % C;
-      uint32_t w[2] = {0, 0};
+      float q[8], off = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        const int q = back > 0.0 ? max(-127, min(127, __double2int_rn(y[u][j] * back))) : 0;
-        w[j / 4] |= uint32_t(q & 255) << (8 * (j % 4));
+        q[j] = __fmaf_rn(y[u][j], back, MAGIC);
+        off = fmaxf(off, fabsf(__fmaf_rn(y[u][j], back, -__fsub_rn(q[j], MAGIC))));
+      }
+      uint32_t w[2];
+#pragma unroll
+      for (int k = 0; k < 2; k++)
+        w[k] = __byte_perm(__byte_perm(__float_as_uint(q[4 * k]), __float_as_uint(q[4 * k + 1]), 0x0040),
+                           __byte_perm(__float_as_uint(q[4 * k + 2]), __float_as_uint(q[4 * k + 3]), 0x0040), 0x5410);
+      if (!some) {
+        w[0] = w[1] = 0;
+      } else if (slow || off > kNear) {
+        double x[8];
+        item64(src + int64_t(t) * in.row, at0(c), at1(c), mode, angles(t, c), x);
+        const double back64 = 1.0 / double(scale);
+        w[0] = w[1] = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          w[j / 4] |= uint32_t(max(-127, min(127, __double2int_rn(x[j] * back64))) & 255) << (8 * (j % 4));
       }
       int8_t* dst = base + (held + t) * D;
       if (mode == ROPE_HALVES) {
@@ -204,56 +304,70 @@ __global__ void __launch_bounds__(256) k_kv8_append(Kv8Args a, Kv8Rows kin, Kv8R
       }
     }
   }
-  // every thread of the unit has read the old scale: the reductions above
-  // are behind that read
-  if (tid == 0) *sptr = scale;
+  // every thread of the unit has read the old scale: the exchanges above are
+  // behind that read
+  if (live && tid == 0) *sptr = scale;
 }
 
 // --------------------------------------------------------------- read ----
 //
-// The values of stored tokens: sixteen bytes of one token and head to a
-// thread, q·scale in 32 bits, rounded once to the output's type.
+// The values of stored tokens: q·scale in 32 bits, rounded once to the
+// output's type. A thread has sixteen bytes of outputs of up to kReads
+// tokens at a time, neighbours' next to its own: X threads over a token's
+// heads, keys and values, 256/X tokens side by side. Bound by the bytes
+// written.
+constexpr int kReads = 4;
+
 template <int D, class T>
-__global__ void __launch_bounds__(256) k_kv8_read(Kv8Args a, Kv8Rows kout, Kv8Rows vout, bool vec) {
-  constexpr int C = D / 16;
+__global__ void __launch_bounds__(256) k_kv8_read(Kv8Args a, Kv8Rows kout, Kv8Rows vout, int xlog, bool vec) {
+  constexpr int V = 16 / sizeof(T), C = D / V;  // values a thread, threads a token and head
   const int i = blockIdx.y;
   const Kv8Span sp = kv8_span(a, i);
   if (!sp.ok) {
     if (threadIdx.x == 0) report(a);
     return;
   }
-  const int p0 = sp.len - sp.T;
-  if (p0 < 0) return;
-  const int64_t idx = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  const int c = int(idx % C);
-  const int64_t r = idx / C;
-  const int hh = int(r % (2 * a.heads)), h = hh % a.heads;
-  const bool key = hh < a.heads;
-  const int64_t t64 = r / (2 * a.heads);
-  if (t64 >= sp.T) return;
-  const Kv8Rows& o = key ? kout : vout;
-  if (!o.p) return;
-  const int t = int(t64), pos = p0 + t;
-  const int page = kv8_page(a, i, pos >> a.plog);
-  if (page < 0) {
-    report(a);
-    return;
+  const int p0 = sp.len - sp.T, X = 1 << xlog, Y = 256 >> xlog;
+  const int t0 = blockIdx.x * (kReads * Y) + (threadIdx.x >> xlog);
+  if (p0 < 0 || t0 >= sp.T) return;
+  int page[kReads];
+#pragma unroll
+  for (int u = 0; u < kReads; u++) {
+    const int t = t0 + u * Y;
+    page[u] = t < sp.T ? kv8_page(a, i, (p0 + t) >> a.plog) : -2;
+    if (page[u] == -1) report(a);
   }
-  const int64_t ph = int64_t(page) * a.heads + h;
-  const int slot = pos & ((1 << a.plog) - 1);
-  const uint4 q = *reinterpret_cast<const uint4*>((key ? a.k : a.v) + ((ph << a.plog) + slot) * D + 16 * c);
-  const float s = a.scale[2 * ph + (key ? 0 : 1)];
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-  T* dst = static_cast<T*>(const_cast<void*>(o.p)) + int64_t(sp.row + t) * o.row + int64_t(h) * o.head + 16 * c;
-  __align__(16) T y[16];
+  for (int x = threadIdx.x & (X - 1); x < 2 * a.heads * C; x += X) {
+    const int hh = x / C, e = x % C * V;
+    const bool key = hh < a.heads;
+    const int h = key ? hh : hh - a.heads;
+    const Kv8Rows& o = key ? kout : vout;
+    if (!o.p) continue;
+    uint32_t q[kReads][V / 4];
+    float s[kReads];
 #pragma unroll
-  for (int j = 0; j < 16; j++) narrow(__fmul_rn(float(int8_t(w[j / 4] >> (8 * (j % 4)))), s), &y[j]);
-  if (vec) {
+    for (int u = 0; u < kReads; u++) {
+      const int64_t ph = int64_t(max(page[u], 0)) * a.heads + h;
+      const int slot = (p0 + t0 + u * Y) & ((1 << a.plog) - 1);
+      const int8_t* from = (key ? a.k : a.v) + ((ph << a.plog) + slot) * D + e;
+      s[u] = a.scale[2 * ph + (key ? 0 : 1)];
 #pragma unroll
-    for (int j = 0; j < int(sizeof(T)); j++) reinterpret_cast<uint4*>(dst)[j] = reinterpret_cast<const uint4*>(y)[j];
-  } else {
+      for (int w = 0; w < V / 4; w++) q[u][w] = reinterpret_cast<const uint32_t*>(from)[w];
+    }
+    T* dst = static_cast<T*>(const_cast<void*>(o.p)) + int64_t(sp.row + t0) * o.row + int64_t(h) * o.head + e;
 #pragma unroll
-    for (int j = 0; j < 16; j++) dst[j] = y[j];
+    for (int u = 0; u < kReads; u++, dst += Y * o.row) {
+      if (page[u] < 0) continue;
+      __align__(16) T y[V];
+#pragma unroll
+      for (int j = 0; j < V; j++) narrow(__fmul_rn(float(int8_t(q[u][j / 4] >> (8 * (j % 4)))), s[u]), &y[j]);
+      if (vec) {
+        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(y);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; j++) dst[j] = y[j];
+      }
+    }
   }
 }
 
@@ -271,20 +385,26 @@ cudaError_t append_t(const Kv8Args& a, const Kv8Rows& k, const Kv8Rows& v, cudaS
   const int blocks = (a.max_new + page - 2) / page + 1;  // pages that max_new tokens can touch
   const int64_t units = int64_t(a.n) * blocks * 2 * a.heads;
   const bool vec = aligned<T>(k, 4) && aligned<T>(v, 4);
-  // A warp to a unit while its registers hold the unit's new values, else
-  // eight of them: 64 tokens of 128 values are kItems items of 256 threads.
-  if (std::min(a.max_new, page) * (D / 8) <= 32 * kItems)
-    k_kv8_append<D, 32, T><<<unsigned((units + 7) / 8), 256, 0, st>>>(a, k, v, blocks, vec);
+  // One token to a sequence: as many threads as hold it. A warp while its
+  // registers hold a unit's new values, else eight: 64 tokens of 128 values
+  // are kItems items of 256 threads.
+  const auto grid = [&](int g) { return unsigned((units * g + 255) / 256); };
+  if (a.max_new == 1)
+    k_kv8_append<D, D / 8, T><<<grid(D / 8), 256, 0, st>>>(a, k, v, blocks, vec);
+  else if (std::min(a.max_new, page) * (D / 8) <= 32 * kItems)
+    k_kv8_append<D, 32, T><<<grid(32), 256, 0, st>>>(a, k, v, blocks, vec);
   else
-    k_kv8_append<D, 256, T><<<unsigned(units), 256, 0, st>>>(a, k, v, blocks, vec);
+    k_kv8_append<D, 256, T><<<grid(256), 256, 0, st>>>(a, k, v, blocks, vec);
   return cudaGetLastError();
 }
 
 template <int D, class T>
 cudaError_t read_t(const Kv8Args& a, const Kv8Rows& k, const Kv8Rows& v, cudaStream_t st) {
-  const int64_t threads = int64_t(a.max_new) * 2 * a.heads * (D / 16);
   const bool vec = (!k.p || aligned<T>(k, 16 / sizeof(T))) && (!v.p || aligned<T>(v, 16 / sizeof(T)));
-  k_kv8_read<D, T><<<dim3(unsigned((threads + 255) / 256), a.n), 256, 0, st>>>(a, k, v, vec);
+  int xlog = 4;  // threads over a token
+  while (xlog < 8 && 1 << xlog < 2 * a.heads * (D / int(16 / sizeof(T)))) xlog++;
+  const int tokens = kReads * (256 >> xlog);
+  k_kv8_read<D, T><<<dim3(unsigned((a.max_new - 1) / tokens + 1), a.n), 256, 0, st>>>(a, k, v, xlog, vec);
   return cudaGetLastError();
 }
 
