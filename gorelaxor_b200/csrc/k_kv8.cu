@@ -19,6 +19,7 @@ namespace grx {
 namespace {
 
 constexpr uint32_t FULL = 0xffffffffu;
+constexpr int kSMs = 148;
 constexpr int kRangeError = -5;  // GRX_ERANGE, what the status word gets
 
 enum { ROPE_NONE = 0, ROPE_PAIRS = 1, ROPE_HALVES = 2 };
@@ -66,64 +67,144 @@ __device__ __forceinline__ void narrow(float x, __nv_bfloat16* p) { *p = __float
 // rne(q·s/s'); the new values become rne(x/s'). No two units share a byte or
 // a scale, so there are no atomics and no order.
 //
-// The definition's rotations, quotients and roundings are in 64 bits: a
-// value next to a rounding border goes to one or the other side by less
-// than 32 bits hold, a whole step of the page's scale. They are computed in
-// 32 bits, which is off by less than 4e-5 of a step (127 steps times a few
-// 2^-24), and again in 64 where a value comes within kNear of a border, as
-// 2 in 10000 do. The scale's largest magnitude likewise: the values within
-// 2^-19 of the largest are formed again in 64 bits. Pages of very small or
-// very large numbers (kTiny, kHuge) take 64 bits throughout.
+// The definition's rotations and quotients are exact to 64 bits: a value
+// next to a rounding border goes to one or the other side by less than 32
+// bits hold, a whole step of the page's scale. They are computed in 32 bits,
+// which is off by less than 3e-5 of a step (127 steps times 3.4·2^-24), and
+// where a value comes within 4e-5 of a border (one in 12000) it is formed
+// again in 64 bits and compared with the border, (k ± 1/2)·s', itself: that
+// product is exact. The scale's largest magnitude likewise: the values within
+// 2^-19 of the largest are formed again in 64 bits (not rotated ones: they
+// are exact). Pages of very small or very large numbers (kTiny, kHuge) take
+// 64 bits throughout.
 //
 // A thread holds at most kItems items of eight values: two groups of four
 // that the rotation pairs with each other. Bound by latency for single
 // tokens, by the bytes of the rows for prompts.
 constexpr int kItems = 4;
-constexpr float kNear = 0.4999f;
+constexpr float kNear = 0.49996f;
 constexpr float kTiny = 1e-30f, kHuge = 1e37f;
 
-// One item's eight values in 64 bits: elements e0 .. e0 + 3 and e1 .. e1 + 3
-// of a row, rotated by the angles at cs.
+// Element j (0..7) of an item in 64 bits: elements e0 .. e0 + 3 and e1 ..
+// e1 + 3 of a row, rotated by the angles at cs.
 template <class T>
-__device__ void item64(const T* src, int e0, int e1, int mode, const float* cs, double* y) {
-#pragma unroll
-  for (int j = 0; j < 8; j++) y[j] = wide(src[j < 4 ? e0 + j : e1 + j - 4]);
-  if (mode == ROPE_NONE) return;
-#pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const int p = mode == ROPE_PAIRS ? 2 * j : j, q = mode == ROPE_PAIRS ? 2 * j + 1 : j + 4;
-    const double xa = y[p], xb = y[q], cc = cs[2 * j], ss = cs[2 * j + 1];
-    // the products are exact, so one rounding each
-    y[p] = __fma_rn(xa, cc, -(xb * ss));
-    y[q] = __fma_rn(xa, ss, xb * cc);
-  }
+__device__ __forceinline__ double value64(const T* src, int e0, int e1, int mode, const float* cs, int j) {
+  const auto at = [&](int n) { return double(wide(src[n < 4 ? e0 + n : e1 + n - 4])); };
+  if (mode == ROPE_NONE) return at(j);
+  const int n = mode == ROPE_PAIRS ? j >> 1 : j & 3, second = mode == ROPE_PAIRS ? j & 1 : j >> 2;
+  const double xa = at(mode == ROPE_PAIRS ? 2 * n : n), xb = at(mode == ROPE_PAIRS ? 2 * n + 1 : n + 4);
+  const double cc = cs[2 * n], ss = cs[2 * n + 1];
+  // the products are exact, so one rounding
+  return second ? __fma_rn(xa, ss, xb * cc) : __fma_rn(xa, cc, -(xb * ss));
 }
+// rne(x/s) for a quotient within a step of k: x against the borders of k.
+__device__ __forceinline__ int settle(double x, double s, int k) {
+  const double up = (k + 0.5) * s, dn = (k - 0.5) * s;
+  if (x > up || (x == up && (k & 1))) return k + 1;
+  if (x < dn || (x == dn && (k & 1))) return k - 1;
+  return k;
+}
+__device__ __noinline__ double divided(double x, double y) { return x / y; }
+// |x|/127 in 32 bits (NaN for what is not finite): the quotient's rounding,
+// which a product with 1/127 gives but where it lies on a border as far as 64
+// bits tell.
+__device__ __forceinline__ float over127(double x) {
+  const double m = fabs(x), q = m * (1.0 / 127.0), e = q * 0x1p-51;
+  const float lo = float(q - e), hi = float(q + e);
+  if (!isfinite(m)) return __int_as_float(0x7fc00000);
+  return lo == hi ? lo : float(divided(m, 127.0));
+}
+// rne(x/s) where neither is known to be in the range of 32-bit reciprocals.
+__device__ __noinline__ int rounded64(double x, float s) { return max(-127, min(127, __double2int_rn(x / double(s)))); }
 
-// Four signed bytes times r, rounded, and whether any came near a border.
-__device__ __forceinline__ uint32_t scaled_bytes(uint32_t q, float r, bool* near) {
-  const uint32_t u = q ^ 0x80808080u;
-  float t[4], off = 0.f;
-#pragma unroll
-  for (int k = 0; k < 4; k++) {
-    const float v = __fsub_rn(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 | k)), 8388736.f);
-    t[k] = __fmaf_rn(v, r, MAGIC);
-    off = fmaxf(off, fabsf(__fmaf_rn(v, r, -__fsub_rn(t[k], MAGIC))));
-  }
-  *near = *near || off > kNear;
+// Four floats n + 1.5·2^23 as bytes n.
+__device__ __forceinline__ uint32_t low_bytes(const float* t) {
   return __byte_perm(__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040),
                      __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
 }
+// x·r rounded, as n + 1.5·2^23, and whether a border is near.
+__device__ __forceinline__ float rounded(float x, float r, bool* near) {
+  const float t = __fmaf_rn(x, r, MAGIC);
+  *near = fabsf(__fmaf_rn(x, r, -__fsub_rn(t, MAGIC))) > kNear;
+  return t;
+}
 
+// Four signed bytes times s/s1 (about r), rounded.
+__device__ __forceinline__ uint32_t scaled_bytes(uint32_t q, float r, float s, float s1, bool slow) {
+  const uint32_t u = q ^ 0x80808080u;
+  float t[4];
+  uint32_t redo = slow ? 15 : 0;
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    bool near;
+    t[k] = rounded(__fsub_rn(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 | k)), 8388736.f), r, &near);
+    if (near) redo |= 1 << k;
+  }
+  uint32_t w = low_bytes(t);
+  for (; redo; redo &= redo - 1) {
+    const int at = 8 * (__ffs(redo) - 1);
+    const double x = double(int8_t(q >> at)) * double(s);
+    const int v = slow ? rounded64(x, s1) : settle(x, double(s1), int8_t(w >> at));
+    w = (w & ~(255u << at)) | uint32_t(v & 255) << at;
+  }
+  return w;
+}
+
+// Eight values of a row as they are in memory.
+template <class T>
+struct Raw {
+  uint32_t w[2 * sizeof(T)];
+};
+template <class T>
+__device__ __forceinline__ void load_raw(const T* p0, const T* p1, bool vec, Raw<T>& r) {
+  if (vec) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<uint4*>(r.w) = *reinterpret_cast<const uint4*>(p0);
+      *reinterpret_cast<uint4*>(r.w + 4) = *reinterpret_cast<const uint4*>(p1);
+    } else {
+      *reinterpret_cast<uint2*>(r.w) = *reinterpret_cast<const uint2*>(p0);
+      *reinterpret_cast<uint2*>(r.w + 2) = *reinterpret_cast<const uint2*>(p1);
+    }
+  } else {
+    T h[8];
+#pragma unroll
+    for (int j = 0; j < 4; j++) h[j] = p0[j], h[4 + j] = p1[j];
+#pragma unroll
+    for (int j = 0; j < int(2 * sizeof(T)); j++) r.w[j] = reinterpret_cast<const uint32_t*>(h)[j];
+  }
+}
+__device__ __forceinline__ void unpack(const Raw<float>& r, float* x) {
+#pragma unroll
+  for (int j = 0; j < 8; j++) x[j] = __uint_as_float(r.w[j]);
+}
+__device__ __forceinline__ void unpack(const Raw<__half>& r, float* x) {
+#pragma unroll
+  for (int j = 0; j < 8; j++) x[j] = __half2float(__ushort_as_half(uint16_t(r.w[j / 2] >> (16 * (j % 2)))));
+}
+__device__ __forceinline__ void unpack(const Raw<__nv_bfloat16>& r, float* x) {
+#pragma unroll
+  for (int j = 0; j < 8; j++) x[j] = bits_f(j % 2 ? r.w[j / 2] & 0xffff0000u : r.w[j / 2] << 16);
+}
+// The larger, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// A group of threads has `per` units of one sequence and page, heads one
+// after the other, keys before values: the next one's rows come while the
+// present one is rounded.
 template <int D, int G, class T>
-__global__ void __launch_bounds__(256, G == D / 8 ? 4 : 3) k_kv8_append(Kv8Args a, Kv8Rows kin, Kv8Rows vin, int blocks, bool vec) {
+__global__ void __launch_bounds__(256, G == D / 8 ? 4 : 3)
+    k_kv8_append(Kv8Args a, Kv8Rows kin, Kv8Rows vin, int blocks, int per, bool vec) {
   constexpr int C = D / 8;                // items a token
   constexpr int N = G == C ? 1 : kItems;  // items a thread
   __shared__ uint32_t red[16];
   const int tid = threadIdx.x % G;
-  const uint32_t unit = (blockIdx.x * 256u + threadIdx.x) / G;  // the launch has fewer than 2^31
-  const uint32_t rest = unit / (2 * a.heads);
-  const int hh = int(unit - rest * (2 * a.heads)), h = hh < a.heads ? hh : hh - a.heads;
-  const bool key = hh < a.heads;
+  const uint32_t group = (blockIdx.x * 256u + threadIdx.x) / G;  // the launch has fewer than 2^31 units
+  const uint32_t parts = (2 * a.heads + per - 1) / per, rest = group / parts;
+  const int hb = int(group - rest * parts) * per, he = min(hb + per, 2 * a.heads);
   const int i = min(int(rest / blocks), a.n), b = int(rest % blocks);
   // every thread stays for the exchanges between lanes; `live` ones have work
   bool live = i < a.n;
@@ -137,29 +218,76 @@ __global__ void __launch_bounds__(256, G == D / 8 ? 4 : 3) k_kv8_append(Kv8Args 
   const int block = (max(p0, 0) >> a.plog) + b, begin = block << a.plog;
   const int lo = max(p0, begin), hi = min(sp.len, begin + (1 << a.plog));
   live = live && p0 >= 0 && lo < hi;
-  if (G > 32 && !live) return;  // a block is one unit
+  if (G > 32 && !live) return;  // a block is one group
   // the page's number comes while the rows do
   const int page = live ? kv8_page(a, i, block) : 0;
-
-  const Kv8Rows& in = key ? kin : vin;
-  const T* src = static_cast<const T*>(in.p) + int64_t(sp.row + lo - p0) * in.row + int64_t(h) * in.head;
-  const int mode = key ? a.rope_mode : ROPE_NONE;
   int items = live ? (hi - lo) * C : 0;
-  const auto at0 = [&](int c) { return mode == ROPE_HALVES ? 4 * c : 8 * c; };
-  const auto at1 = [&](int c) { return mode == ROPE_HALVES ? D / 2 + 4 * c : 8 * c + 4; };
+  int held = live ? lo - begin : 0;  // tokens that the page holds already
+
+  const auto row_of = [&](int hh) {
+    const Kv8Rows& in = hh < a.heads ? kin : vin;
+    return static_cast<const T*>(in.p) + int64_t(sp.row + lo - p0) * in.row +
+           int64_t(hh < a.heads ? hh : hh - a.heads) * in.head;
+  };
+  const auto stride_of = [&](int hh) { return hh < a.heads ? kin.row : vin.row; };
+  const auto mode_of = [&](int hh) { return hh < a.heads ? a.rope_mode : int(ROPE_NONE); };
+  const auto at0 = [&](int mode, int c) { return mode == ROPE_HALVES ? 4 * c : 8 * c; };
+  const auto at1 = [&](int mode, int c) { return mode == ROPE_HALVES ? D / 2 + 4 * c : 8 * c + 4; };
   const auto angles = [&](int t, int c) { return a.rope + (int64_t(lo + t) * (D / 2) + 4 * c) * 2; };
-  float y[N][8];
-  float most = 0.f, nan = 0.f;
+  Raw<T> raw[N];
+  const auto load = [&](int hh) {
+    const T* src = row_of(hh);
+    const int64_t st = stride_of(hh);
+    const int mode = mode_of(hh);
 #pragma unroll
-  for (int u = 0; u < N; u++) {
-    const int it = tid + u * G;
-    if (it < items) {
-      const int t = it / C, c = it % C;
-      const T* row = src + int64_t(t) * in.row;
-      load4(row + at0(c), vec, y[u]);
-      load4(row + at1(c), vec, y[u] + 4);
+    for (int u = 0; u < N; u++) {
+      const int it = tid + u * G, t = it / C, c = it % C;
+      if (it < items) load_raw(src + t * st + at0(mode, c), src + t * st + at1(mode, c), vec, raw[u]);
+    }
+  };
+  load(hb);
+  if (page < 0) {
+    if (live && tid == 0) report(a);
+    if (G > 32) return;
+    live = false;
+    items = held = 0;
+  }
+  // the unit's largest of numbers that are not negative, as their bits
+  // compare (NaN above all); `round` picks the place of its exchange
+  auto largest = [&](float m, int round) {
+    uint32_t v = __float_as_uint(m) & 0x7fffffffu;
+    if constexpr (G < 32) {
+#pragma unroll
+      for (int o = G / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(FULL, v, o));
+    } else {
+      v = __reduce_max_sync(FULL, v);
+      if constexpr (G > 32) {
+        if (threadIdx.x % 32 == 0) red[8 * round + threadIdx.x / 32] = v;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < G / 32; w++) v = max(v, red[8 * round + w]);
+      }
+    }
+    return __uint_as_float(v);
+  };
+  for (int hh = hb; hh < he; hh++) {
+    const bool key = hh < a.heads;
+    const int64_t ph = int64_t(max(page, 0)) * a.heads + (key ? hh : hh - a.heads);
+    int8_t* base = (key ? a.k : a.v) + ((ph << a.plog) * D);
+    float* sptr = a.scale + 2 * ph + (key ? 0 : 1);
+    const float old = held > 0 ? *sptr : 0.f;
+    const T* src = row_of(hh);
+    const int64_t st = stride_of(hh);
+    const int mode = mode_of(hh);
+    float y[N][8];
+    float most = 0.f;
+#pragma unroll
+    for (int u = 0; u < N; u++) {
+      const int it = tid + u * G;
+      if (it >= items) continue;
+      unpack(raw[u], y[u]);
       if (mode != ROPE_NONE) {
-        const float4* cs = reinterpret_cast<const float4*>(angles(t, c));
+        const float4* cs = reinterpret_cast<const float4*>(angles(it / C, it % C));
         const float4 f0 = cs[0], f1 = cs[1];
         const float co[4] = {f0.x, f0.z, f1.x, f1.z}, si[4] = {f0.y, f0.w, f1.y, f1.w};
         if (mode == ROPE_PAIRS) {
@@ -179,134 +307,84 @@ __global__ void __launch_bounds__(256, G == D / 8 ? 4 : 3) k_kv8_append(Kv8Args 
         }
       }
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        most = fmaxf(most, fabsf(y[u][j]));
-        nan = __fmaf_rn(0.f, y[u][j], nan);  // 0·inf and 0·NaN
+      for (int j = 0; j < 8; j++) most = max_nan(most, fabsf(y[u][j]));
+    }
+    if (hh + 1 < he) load(hh + 1);
+    const float top = largest(most, 0);
+    bool slow = !(top < kHuge) || (top > 0.f && top < kTiny);
+    float mine = 0.f;  // a/127 as stored, of this thread's candidates
+    const float bound = slow ? 0.f : __fmul_rn(top, 1.f - 0x1p-19f);
+    if (top != 0.f && (slow || (mode != ROPE_NONE && most >= bound))) {
+#pragma unroll
+      for (int u = 0; u < N; u++) {
+        const int it = tid + u * G;
+        uint32_t redo = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          if (slow || fabsf(y[u][j]) >= bound) redo |= 1 << j;
+        if (it >= items) redo = 0;
+        for (; redo; redo &= redo - 1) {
+          const int t = it / C, c = it % C;
+          const float q = over127(
+              value64(src + t * st, at0(mode, c), at1(mode, c), mode, angles(t, c), __ffs(redo) - 1));
+          mine = isnan(q) || isnan(mine) ? __int_as_float(0x7fc00000) : fmaxf(mine, q);
+        }
       }
     }
-  }
-  if (page < 0) {
-    if (live && tid == 0) report(a);
-    live = false;
-    items = 0;
-    most = nan = 0.f;
-  }
-  const int held = live ? lo - begin : 0;  // tokens that the page holds already
-  const int64_t ph = int64_t(max(page, 0)) * a.heads + h;
-  int8_t* base = (key ? a.k : a.v) + ((ph << a.plog) * D);
-  float* sptr = a.scale + 2 * ph + (key ? 0 : 1);
-  const float old = held > 0 ? *sptr : 0.f;
-  // the unit's largest of numbers that are not negative, as their bits
-  // compare (NaN above all); `round` picks the place of its exchange
-  auto largest = [&](float m, int round) {
-    uint32_t v = __float_as_uint(m) & 0x7fffffffu;
-    if constexpr (G < 32) {
-#pragma unroll
-      for (int o = G / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(FULL, v, o));
-    } else {
-      v = __reduce_max_sync(FULL, v);
-      if constexpr (G > 32) {
-        if (threadIdx.x % 32 == 0) red[8 * round + threadIdx.x / 32] = v;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < G / 32; w++) v = max(v, red[8 * round + w]);
+    // what is not rotated is exact as it is (and a 32-bit number over 127 is
+    // never near the middle of two others: its digits repeat every seven bits)
+    const float fresh = mode == ROPE_NONE && !slow ? __fdiv_rn(top, 127.f) : largest(mine, 1);
+    const float scale = isnan(old) || isnan(fresh) ? __int_as_float(0x7fc00000) : fmaxf(old, fresh);
+    const bool some = scale > 0.f;  // not 0, and a number
+    slow = slow || scale < kTiny;
+    const float back = some ? __fdiv_rn(1.f, scale) : 0.f;
+    if (held > 0 && scale > old) {
+      const float r = __fmul_rn(old, back);
+      uint4* w = reinterpret_cast<uint4*>(base);
+      for (int j = tid; j < held * (D / 16); j += G) {
+        const uint4 q = w[j];
+        w[j] = make_uint4(scaled_bytes(q.x, r, old, scale, slow), scaled_bytes(q.y, r, old, scale, slow),
+                          scaled_bytes(q.z, r, old, scale, slow), scaled_bytes(q.w, r, old, scale, slow));
       }
     }
-    return __uint_as_float(v);
-  };
-  const float top = largest(__fadd_rn(most, nan), 0);
-  bool slow = !(top < kHuge) || (top > 0.f && top < kTiny);
-  float mine = 0.f;  // a/127 as stored, of this thread's candidates
-  const float bound = slow ? 0.f : __fmul_rn(top, 1.f - 0x1p-19f);
-  if (top != 0.f && (slow || most >= bound)) {
 #pragma unroll
     for (int u = 0; u < N; u++) {
       const int it = tid + u * G;
-      float m32 = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; j++) m32 = fmaxf(m32, fabsf(y[u][j]));
-      if (it >= items || !(slow || m32 >= bound)) continue;
-      if (mode == ROPE_NONE && !slow) {  // not rotated: exact as it is
-        mine = fmaxf(mine, float(double(m32) / 127.0));
-        continue;
-      }
+      if (it >= items) continue;
       const int t = it / C, c = it % C;
-      double x[8];
-      item64(src + int64_t(t) * in.row, at0(c), at1(c), mode, angles(t, c), x);
+      float q[8];
+      uint32_t redo = slow ? 255 : 0;
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        const double m = fabs(x[j]);
-        if (!(m <= 1.7976931348623157e308))
-          mine = __int_as_float(0x7fc00000);
-        else if (m >= bound && !isnan(mine))
-          mine = fmaxf(mine, float(m / 127.0));
+        bool near;
+        q[j] = rounded(y[u][j], back, &near);
+        if (near) redo |= 1 << j;
       }
-    }
-  }
-  const float fresh = largest(mine, 1);
-  const float scale = isnan(old) || isnan(fresh) ? __int_as_float(0x7fc00000) : fmaxf(old, fresh);
-  const bool some = scale > 0.f;  // not 0, and a number
-  slow = slow || scale < kTiny;
-  const float back = some ? __fdiv_rn(1.f, scale) : 0.f;
-  if (held > 0 && scale > old) {
-    const float r = __fmul_rn(old, back);
-    uint4* w = reinterpret_cast<uint4*>(base);
-    for (int j = tid; j < held * (D / 16); j += G) {
-      const uint4 q = w[j];
-      bool near = slow;
-      uint4 z = make_uint4(scaled_bytes(q.x, r, &near), scaled_bytes(q.y, r, &near), scaled_bytes(q.z, r, &near),
-                           scaled_bytes(q.w, r, &near));
-      if (near) {
-        const double r64 = double(old) * (1.0 / double(scale));
-        const uint32_t qw[4] = {q.x, q.y, q.z, q.w};
-        uint32_t zw[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int e = 0; e < 16; e++)
-          zw[e / 4] |= uint32_t(__double2int_rn(double(int8_t(qw[e / 4] >> (8 * (e % 4)))) * r64) & 255) << (8 * (e % 4));
-        z = make_uint4(zw[0], zw[1], zw[2], zw[3]);
-      }
-      w[j] = z;
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < N; u++) {
-    const int it = tid + u * G;
-    if (it < items) {
-      const int t = it / C, c = it % C;
-      float q[8], off = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        q[j] = __fmaf_rn(y[u][j], back, MAGIC);
-        off = fmaxf(off, fabsf(__fmaf_rn(y[u][j], back, -__fsub_rn(q[j], MAGIC))));
-      }
-      uint32_t w[2];
-#pragma unroll
-      for (int k = 0; k < 2; k++)
-        w[k] = __byte_perm(__byte_perm(__float_as_uint(q[4 * k]), __float_as_uint(q[4 * k + 1]), 0x0040),
-                           __byte_perm(__float_as_uint(q[4 * k + 2]), __float_as_uint(q[4 * k + 3]), 0x0040), 0x5410);
-      if (!some) {
-        w[0] = w[1] = 0;
-      } else if (slow || off > kNear) {
-        double x[8];
-        item64(src + int64_t(t) * in.row, at0(c), at1(c), mode, angles(t, c), x);
-        const double back64 = 1.0 / double(scale);
-        w[0] = w[1] = 0;
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-          w[j / 4] |= uint32_t(max(-127, min(127, __double2int_rn(x[j] * back64))) & 255) << (8 * (j % 4));
+      uint2 w = make_uint2(low_bytes(q), low_bytes(q + 4));
+      if (!some) w = make_uint2(0, 0), redo = 0;
+      for (; redo; redo &= redo - 1) {
+        const int j = __ffs(redo) - 1, at = 8 * (j & 3);
+        const double x = value64(src + t * st, at0(mode, c), at1(mode, c), mode, angles(t, c), j);
+        const uint32_t half = j < 4 ? w.x : w.y;
+        const int v = slow ? rounded64(x, scale) : settle(x, double(scale), int8_t(half >> at));
+        const uint32_t put = (half & ~(255u << at)) | uint32_t(v & 255) << at;
+        if (j < 4)
+          w.x = put;
+        else
+          w.y = put;
       }
       int8_t* dst = base + (held + t) * D;
       if (mode == ROPE_HALVES) {
-        *reinterpret_cast<uint32_t*>(dst + 4 * c) = w[0];
-        *reinterpret_cast<uint32_t*>(dst + D / 2 + 4 * c) = w[1];
+        *reinterpret_cast<uint32_t*>(dst + 4 * c) = w.x;
+        *reinterpret_cast<uint32_t*>(dst + D / 2 + 4 * c) = w.y;
       } else {
-        *reinterpret_cast<uint2*>(dst + 8 * c) = make_uint2(w[0], w[1]);
+        *reinterpret_cast<uint2*>(dst + 8 * c) = w;
       }
     }
+    // every thread of the unit has read the old scale: the exchanges above
+    // are behind that read
+    if (live && tid == 0) *sptr = scale;
   }
-  // every thread of the unit has read the old scale: the exchanges above are
-  // behind that read
-  if (live && tid == 0) *sptr = scale;
 }
 
 // --------------------------------------------------------------- read ----
@@ -387,14 +465,21 @@ cudaError_t append_t(const Kv8Args& a, const Kv8Rows& k, const Kv8Rows& v, cudaS
   const bool vec = aligned<T>(k, 4) && aligned<T>(v, 4);
   // One token to a sequence: as many threads as hold it. A warp while its
   // registers hold a unit's new values, else eight: 64 tokens of 128 values
-  // are kItems items of 256 threads.
-  const auto grid = [&](int g) { return unsigned((units * g + 255) / 256); };
-  if (a.max_new == 1)
-    k_kv8_append<D, D / 8, T><<<grid(D / 8), 256, 0, st>>>(a, k, v, blocks, vec);
-  else if (std::min(a.max_new, page) * (D / 8) <= 32 * kItems)
-    k_kv8_append<D, 32, T><<<grid(32), 256, 0, st>>>(a, k, v, blocks, vec);
-  else
-    k_kv8_append<D, 256, T><<<grid(256), 256, 0, st>>>(a, k, v, blocks, vec);
+  // are kItems items of 256 threads. These take several units in a row where
+  // there are blocks enough without.
+  int per = 1;
+  const auto grid = [&](int g) {
+    const int64_t groups = int64_t(a.n) * blocks * ((2 * a.heads + per - 1) / per);
+    return unsigned((groups * g + 255) / 256);
+  };
+  if (a.max_new == 1) {
+    k_kv8_append<D, D / 8, T><<<grid(D / 8), 256, 0, st>>>(a, k, v, blocks, per, vec);
+  } else if (std::min(a.max_new, page) * (D / 8) <= 32 * kItems) {
+    k_kv8_append<D, 32, T><<<grid(32), 256, 0, st>>>(a, k, v, blocks, per, vec);
+  } else {
+    while (per < 2 * a.heads && units >= int64_t(2 * per) * 6 * kSMs) per *= 2;
+    k_kv8_append<D, 256, T><<<grid(256), 256, 0, st>>>(a, k, v, blocks, per, vec);
+  }
   return cudaGetLastError();
 }
 
@@ -1462,8 +1547,6 @@ __global__ void __launch_bounds__(32 * Shape1<D, WU>::warps, Shape1<D, WU>::bloc
     cluster_sync();  // no block leaves while another reads its shared memory
   }
 }
-
-constexpr int kSMs = 148;
 
 // Blocks and warps for a unit's keys: the stretches that they are cut into
 // give the GPU enough warps, at most `longest` tiles of sixteen keys to one

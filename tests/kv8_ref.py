@@ -63,11 +63,10 @@ class Cache:
                         q = np.zeros_like(y)
                     else:
                         s = max(old, np.float32(np.abs(y).max() / 127.0))
-                        back = 1.0 / float(s) if s > 0 else 0.0
                         if s > old and held:
                             p = pool[pages[b], h, :held].astype(np.float64)
-                            pool[pages[b], h, :held] = np.rint(p * (float(old) * back)).astype(np.int8)
-                        q = np.clip(np.rint(y * back), -127, 127)
+                            pool[pages[b], h, :held] = np.rint(p * float(old) / float(s)).astype(np.int8)
+                        q = np.clip(np.rint(y / float(s)), -127, 127) if s > 0 else np.zeros_like(y)
                     pool[pages[b], h, held:held + hi - lo] = q.astype(np.int8)
                     self.scale[pages[b], h, j] = s
 
