@@ -74,6 +74,8 @@ def _sig(lib):
         "grx_voice_from_latents": (I, [P, P, I, PP]),
         "grx_voice_kv": (I, [P, P, P]),
         "grx_streams_create": (I, [P, I, P, I, PP]),
+        "grx_streams_create_kv8": (I, [P, I, P, I, I, PP]),
+        "grx_streams_kv": (I, [P, I, C.POINTER(C.c_int), P]),
         "grx_streams_free": (None, [P]),
         "grx_streams_reset": (I, [P]),
         "grx_streams_text": (I, [P, P, P, P]),
@@ -148,6 +150,7 @@ def _sig(lib):
         "grx_whisper_watchdog_test": (I, [P]),
         "grx_whisper_cross": (I, [P, I, I, P, P]),
         "grx_whisper_logits": (I, [P, P]),
+        "grx_whisper_score": (I, [P, P, I, P, P, P, P]),
         "grx_whisper_batch_cuda_stream": (P, [P]),
         "grx_whisper_batch_launches": (L, [P]),
     }
@@ -467,15 +470,28 @@ class Voice:
 
 
 class Streams:
-    """n independent FlowLM streams, each starting from its voice."""
+    """n independent FlowLM streams, each starting from its voice. kv8_page:
+    tokens a page (16, 32 or 64) of 8-bit caches (grx_streams_create_kv8);
+    None keeps the reference's float32 ones."""
 
-    def __init__(self, model: FlowLM, voices: list[Voice], max_frames: int):
+    def __init__(self, model: FlowLM, voices: list[Voice], max_frames: int, kv8_page: int | None = None):
         self.model, self.n = model, len(voices)
         self._voices = voices
         arr = (C.c_void_p * self.n)(*[v._h.value for v in voices])
         h = C.c_void_p()
-        _check(lib().grx_streams_create(model._h, self.n, arr, max_frames, C.byref(h)))
+        if kv8_page is None:
+            _check(lib().grx_streams_create(model._h, self.n, arr, max_frames, C.byref(h)))
+        else:
+            _check(lib().grx_streams_create_kv8(model._h, self.n, arr, max_frames, kv8_page, C.byref(h)))
         self._h = h
+
+    def kv(self, i: int) -> np.ndarray:
+        """Stream i's caches [layers][2][positions][d], as a voice's."""
+        n = C.c_int()
+        _check(lib().grx_streams_kv(self._h, i, C.byref(n), None))
+        out = np.empty((self.model.layers, 2, n.value, self.model.d), np.float32)
+        _check(lib().grx_streams_kv(self._h, i, None, _ptr(out)))
+        return out
 
     def reset(self):
         _check(lib().grx_streams_reset(self._h))
@@ -907,6 +923,17 @@ class WhisperBatch:
         out = np.empty((self.n, self.model.n_vocab), np.float32)
         _check(lib().grx_whisper_logits(self._h, _ptr(out)))
         return out
+
+    def score(self, tokens=None, top: int = 0):
+        """What the last decode's logits say (grx_whisper_score): log
+        probabilities [n] of tokens [n] (None without tokens), entropies [n],
+        the `top` most likely tokens [n][top] and their log probabilities."""
+        t = None if tokens is None else np.ascontiguousarray(np.broadcast_to(np.asarray(tokens, np.int32), (self.n,)))
+        lp = None if t is None else np.empty(self.n, np.float32)
+        en, ids = np.empty(self.n, np.float32), np.empty((self.n, top), np.int32)
+        lps = np.empty((self.n, top), np.float32)
+        _check(lib().grx_whisper_score(self._h, _ptr(t), top, _ptr(lp), _ptr(en), _ptr(ids), _ptr(lps)))
+        return lp, en, ids, lps
 
     def cuda_stream(self) -> int:
         return lib().grx_whisper_batch_cuda_stream(self._h) or 0

@@ -28,6 +28,7 @@
 #include "gguf.h"
 #include "host.h"
 #include "kernels.h"
+#include "kv8.h"
 
 using namespace grx;
 
@@ -86,10 +87,25 @@ struct grx_voice {
 // Bytes of a set's FrameIO before its noise rows in their shared device block.
 constexpr size_t kIoPad = 256;
 
+// A set's caches in 8 bits (grx_streams_create_kv8): pages of `page` tokens
+// of every layer, k and v [layers][pages][heads][page][64], scale
+// [layers][pages][heads][2], and the streams' table. A voice's whole pages
+// are shared by its streams; its last tokens, where they fill no page, are
+// kept in a page of their own that reset copies to each stream's.
+struct Kv8Set {
+  int page = 0;  // 0: the set's caches are float32
+  int pages = 0, width = 0;
+  int8_t *k = nullptr, *v = nullptr;
+  float* scale = nullptr;
+  int *table = nullptr, *from = nullptr, *to = nullptr, restored = 0;
+  float* qkv = nullptr;  // [n][3d], a step's product
+};
+
 struct grx_streams {
   Arena ar;
   grx_flowlm* m = nullptr;
   int n = 0, cap = 0;
+  Kv8Set kv8;
   cudaStream_t st = nullptr;
   float* kv = nullptr;
   int *pos = nullptr, *pos0 = nullptr;
@@ -163,6 +179,47 @@ int stream_parts_max() {
   return p < 1 ? 1 : p > 8 ? 8 : p;
 }
 
+// One layer of a set's 8-bit caches, for all its streams with one row each.
+Kv8Args kv8_layer(const grx_streams* s, int layer) {
+  const Kv8Set& c = s->kv8;
+  const size_t tokens = size_t(c.pages) * s->m->heads * c.page;
+  Kv8Args a;
+  a.k = c.k + tokens * 64 * size_t(layer);
+  a.v = c.v + tokens * 64 * size_t(layer);
+  a.scale = c.scale + size_t(c.pages) * s->m->heads * 2 * size_t(layer);
+  a.pages = c.pages;
+  a.plog = c.page == 16 ? 4 : c.page == 32 ? 5 : 6;
+  a.heads = s->m->heads;
+  a.n = a.rows = s->n;
+  a.width = c.width;
+  a.max_len = s->cap;
+  a.table = c.table;
+  a.len = s->pos;
+  a.len_add = 1;  // the token of this step too
+  a.rope = s->rope;
+  a.rope_positions = s->cap;
+  a.rope_mode = GRX_ROPE_PAIRS;
+  return a;
+}
+
+// The rows of a layer's qkv product [rows][3d]: appended to the 8-bit caches,
+// and their attention, rounded to Q8_0.
+cudaError_t kv8_attention(const Kv8Args& a, const float* qkv, int d, int8_t* q8, float2* q8s, cudaStream_t st) {
+  Kv8Rows k, v;
+  Kv8Attend t;
+  t.q.p = qkv;
+  k.p = qkv + d;
+  v.p = qkv + 2 * d;
+  t.q.row = k.row = v.row = 3 * d;
+  t.q.head = k.head = v.head = 64;
+  t.heads = a.heads;
+  t.scale = 0.125f;
+  t.q8 = q8;
+  t.q8s = q8s;
+  cudaError_t e = launch_kv8_append(a, 64, GRX_F32, k, v, st);
+  return e != cudaSuccess ? e : launch_kv8_attend(a, 64, GRX_F32, t, st);
+}
+
 // The kernel sequence of one frame for all streams (see grx.h): flowLM.step
 // (lm.go:185-195 → nn.go:142-182) then flowHead.sample (lm.go:108-160).
 // Returns the number of kernels launched.
@@ -196,31 +253,40 @@ int enqueue_frame(grx_streams* s) {
     ln.q8 = s->xq;
     ln.q8s = s->xs;
     launch_ln(ln, M, d, st);
-    EpiArgs e;
-    e.epi = EPI_ROPE_KV;
-    e.kv.q = s->q;
-    e.kv.kv = s->kv;
-    e.kv.pos = s->pos;
-    e.kv.rope = s->rope;
-    e.kv.layer = l;
-    e.kv.layers = m->L;
-    e.kv.heads = m->heads;
-    e.kv.cap = s->cap;
-    e.kv.d = d;
-    launch_q8_product(s->xq, s->xs, M, ly.qkv, e, st);
-    AttnArgs at;
-    at.q = s->q;
-    at.kv = s->kv;
-    at.pos = s->pos;
-    at.q8 = s->xq;
-    at.q8s = s->xs;
-    at.layer = l;
-    at.layers = m->L;
-    at.heads = m->heads;
-    at.cap = s->cap;
-    at.d = d;
-    at.io = s->io;
-    launch_attn(at, M, st);
+    if (s->kv8.page) {
+      EpiArgs e;
+      e.y = s->kv8.qkv;
+      e.ldy = 3 * d;
+      launch_q8_product(s->xq, s->xs, M, ly.qkv, e, st);
+      kv8_attention(kv8_layer(s, l), s->kv8.qkv, d, s->xq, s->xs, st);
+      k++;
+    } else {
+      EpiArgs e;
+      e.epi = EPI_ROPE_KV;
+      e.kv.q = s->q;
+      e.kv.kv = s->kv;
+      e.kv.pos = s->pos;
+      e.kv.rope = s->rope;
+      e.kv.layer = l;
+      e.kv.layers = m->L;
+      e.kv.heads = m->heads;
+      e.kv.cap = s->cap;
+      e.kv.d = d;
+      launch_q8_product(s->xq, s->xs, M, ly.qkv, e, st);
+      AttnArgs at;
+      at.q = s->q;
+      at.kv = s->kv;
+      at.pos = s->pos;
+      at.q8 = s->xq;
+      at.q8s = s->xs;
+      at.layer = l;
+      at.layers = m->L;
+      at.heads = m->heads;
+      at.cap = s->cap;
+      at.d = d;
+      at.io = s->io;
+      launch_attn(at, M, st);
+    }
     EpiArgs r;
     r.epi = EPI_RESID;
     r.y = s->x;
@@ -1031,6 +1097,10 @@ int grx_streams_reset(grx_streams* s) {
   CK(cudaSetDevice(s->ar.dev));
   CK(cudaMemcpyAsync(s->pos, s->pos0, sizeof(int) * size_t(s->n), cudaMemcpyDeviceToDevice, s->st));
   if (s->b1) CK(cudaMemsetAsync(s->f1_err, 0, sizeof(int), s->st));
+  if (s->kv8.restored) {
+    const Kv8Args c = kv8_layer(s, 0);
+    CK(launch_kv8_copy_pages(c, 64, m->L, s->kv8.from, s->kv8.to, s->kv8.restored, s->st));
+  }
   for (int i = 0; i < s->n; i++)
     CK(cudaMemcpyAsync(s->lat + size_t(i) * m->ldim, m->bos, sizeof(float) * size_t(m->ldim), cudaMemcpyDeviceToDevice,
                        s->st));
@@ -1081,16 +1151,23 @@ static int streams_text_one(grx_streams* q, const int* ids, const int* off, floa
   float2* xs = ar.alloc<float2>(size_t(R) * (d / 32), &rc);  // a scale per 32-value block
   int8_t* fq = ar.alloc<int8_t>(size_t(R) * ff, &rc);
   float2* fs = ar.alloc<float2>(size_t(R) * (ff / 32), &rc);
-  int* dint = ar.alloc<int>(size_t(3) * R + size_t(5) * ns, &rc);
+  int* dint = ar.alloc<int>(size_t(3) * R + size_t(5) * ns + 2 * size_t(n) + 1, &rc);
+  float* qkv = q->kv8.page ? ar.alloc<float>(size_t(R) * 3 * d, &rc) : nullptr;
   float* lo = out ? ar.alloc<float>(size_t(ns) * d, &rc) : nullptr;
   float* lrow = out ? ar.alloc<float>(size_t(ns) * d, &rc) : nullptr;
   if (rc) return rc;
+  std::vector<int> row0(1, 0), len;  // every stream's rows and tokens, these among them
+  for (int i = 0; i < n; i++) {
+    row0.push_back(row0.back() + off[i + 1] - off[i]);
+    len.push_back(pos[size_t(i)] + off[i + 1] - off[i]);
+  }
   std::vector<int> hint;
-  for (const auto* v : {&row_id, &row_slot, &row_pos, &c_row0, &c_T, &c_pos0, &c_slot, &last_row})
+  for (const auto* v : {&row_id, &row_slot, &row_pos, &c_row0, &c_T, &c_pos0, &c_slot, &last_row, &row0, &len})
     hint.insert(hint.end(), v->begin(), v->end());
   CK(cudaMemcpyAsync(dint, hint.data(), sizeof(int) * hint.size(), cudaMemcpyHostToDevice, q->st));
   const int *d_id = dint, *d_slot = dint + R, *d_pos = dint + 2 * R, *d_row0 = dint + 3 * R, *d_T = d_row0 + ns,
-            *d_pos0 = d_T + ns, *d_cslot = d_pos0 + ns, *d_last = d_cslot + ns;
+            *d_pos0 = d_T + ns, *d_cslot = d_pos0 + ns, *d_last = d_cslot + ns, *d_rows = d_last + ns,
+            *d_len = d_rows + n + 1;
   cudaStream_t st = q->st;
   if (d_xin)  // the rows themselves (voice conditioning), in row order
     CK(cudaMemcpyAsync(x, d_xin, sizeof(float) * size_t(R) * d, cudaMemcpyDeviceToDevice, st));
@@ -1107,34 +1184,48 @@ static int streams_text_one(grx_streams* q, const int* ids, const int* off, floa
     ln.q8 = xq;
     ln.q8s = xs;
     launch_ln(ln, R, d, st);
-    EpiArgs e;
-    e.epi = EPI_ROPE_KV;
-    e.kv.q = qb;
-    e.kv.kv = q->kv;
-    e.kv.pos = d_pos;
-    e.kv.row_stream = d_slot;
-    e.kv.rope = q->rope;
-    e.kv.layer = l;
-    e.kv.layers = m->L;
-    e.kv.heads = m->heads;
-    e.kv.cap = q->cap;
-    e.kv.d = d;
-    launch_q8_product(xq, xs, R, ly.qkv, e, st);
-    AttnRowsArgs at;
-    at.q = qb;
-    at.kv = q->kv;
-    at.row0 = d_row0;
-    at.T = d_T;
-    at.pos0 = d_pos0;
-    at.slot = d_cslot;
-    at.q8 = xq;
-    at.q8s = xs;
-    at.layer = l;
-    at.layers = m->L;
-    at.heads = m->heads;
-    at.cap = q->cap;
-    at.d = d;
-    launch_attn_rows(at, ns, tmax, st);
+    if (q->kv8.page) {
+      EpiArgs e;
+      e.y = qkv;
+      e.ldy = 3 * d;
+      launch_q8_product(xq, xs, R, ly.qkv, e, st);
+      Kv8Args a = kv8_layer(q, l);
+      a.row0 = d_rows;
+      a.rows = R;
+      a.max_new = tmax;
+      a.len = d_len;
+      a.len_add = 0;
+      CK(kv8_attention(a, qkv, d, xq, xs, st));
+    } else {
+      EpiArgs e;
+      e.epi = EPI_ROPE_KV;
+      e.kv.q = qb;
+      e.kv.kv = q->kv;
+      e.kv.pos = d_pos;
+      e.kv.row_stream = d_slot;
+      e.kv.rope = q->rope;
+      e.kv.layer = l;
+      e.kv.layers = m->L;
+      e.kv.heads = m->heads;
+      e.kv.cap = q->cap;
+      e.kv.d = d;
+      launch_q8_product(xq, xs, R, ly.qkv, e, st);
+      AttnRowsArgs at;
+      at.q = qb;
+      at.kv = q->kv;
+      at.row0 = d_row0;
+      at.T = d_T;
+      at.pos0 = d_pos0;
+      at.slot = d_cslot;
+      at.q8 = xq;
+      at.q8s = xs;
+      at.layer = l;
+      at.layers = m->L;
+      at.heads = m->heads;
+      at.cap = q->cap;
+      at.d = d;
+      launch_attn_rows(at, ns, tmax, st);
+    }
     EpiArgs r;
     r.epi = EPI_RESID;
     r.y = x;
@@ -1201,7 +1292,7 @@ int grx_streams_text(grx_streams* s, const int* ids, const int* offsets, float* 
 // [bos_voice; cond] through the transformer from an empty state (lm.run with
 // n + 1 rows); the caches are the voice.
 static int streams_create_one(grx_flowlm* m, int n, const grx_voice* const* voices, int max_frames,
-                              std::unique_ptr<grx_streams>* out);
+                              std::unique_ptr<grx_streams>* out, int page = 0);
 
 int grx_voice_from_latents(grx_flowlm* m, const float* latents, int n, grx_voice** out) {
   if (!m || !latents || !out) return fail(GRX_EINVAL, "grx_voice_from_latents: null argument");
@@ -1269,17 +1360,15 @@ int grx_voice_from_latents(grx_flowlm* m, const float* latents, int n, grx_voice
   return GRX_OK;
 }
 
-static int streams_create_one(grx_flowlm* m, int n, const grx_voice* const* voices, int max_frames,
-                              std::unique_ptr<grx_streams>* out);
-
-int grx_streams_create(grx_flowlm* m, int n, const grx_voice* const* voices, int max_frames, grx_streams** out) {
+static int streams_create(grx_flowlm* m, int n, const grx_voice* const* voices, int max_frames, int page,
+                          grx_streams** out) {
   if (!m || !voices || !out || n < 1 || max_frames < 1) return fail(GRX_EINVAL, "grx_streams_create: bad argument");
   int rc = device_init(m->dev);
   if (rc) return rc;
   const int nparts = std::max(1, std::min(stream_parts_max(), n / kMinPart));
   if (nparts == 1) {
     std::unique_ptr<grx_streams> s;
-    rc = streams_create_one(m, n, voices, max_frames, &s);
+    rc = streams_create_one(m, n, voices, max_frames, &s, page);
     if (rc) return rc;
     *out = s.release();
     return GRX_OK;
@@ -1293,7 +1382,7 @@ int grx_streams_create(grx_flowlm* m, int n, const grx_voice* const* voices, int
   for (int i = 0, r0 = 0; i < nparts; i++) {
     const int ni = n / nparts + (i < n % nparts ? 1 : 0);
     std::unique_ptr<grx_streams> p;
-    rc = streams_create_one(m, ni, voices + r0, max_frames, &p);
+    rc = streams_create_one(m, ni, voices + r0, max_frames, &p, page);
     if (rc) return rc;
     p->row0 = r0;
     CK(cudaEventCreateWithFlags(&p->ev, cudaEventDisableTiming));
@@ -1306,8 +1395,110 @@ int grx_streams_create(grx_flowlm* m, int n, const grx_voice* const* voices, int
   return GRX_OK;
 }
 
+int grx_streams_create(grx_flowlm* m, int n, const grx_voice* const* voices, int max_frames, grx_streams** out) {
+  return streams_create(m, n, voices, max_frames, 0, out);
+}
+
+int grx_streams_create_kv8(grx_flowlm* m, int n, const grx_voice* const* voices, int max_frames, int page_tokens,
+                           grx_streams** out) {
+  if (page_tokens != 16 && page_tokens != 32 && page_tokens != 64)
+    return fail(GRX_EINVAL, "grx_streams_create_kv8: pages of " + std::to_string(page_tokens) + " tokens (16, 32 or 64)");
+  return streams_create(m, n, voices, max_frames, page_tokens, out);
+}
+
+// The 8-bit caches of a new set: each distinct voice's tokens are appended
+// once, to pages that its streams share; what does not fill a page goes to
+// every stream's own page when the set is reset.
+static int kv8_setup(grx_streams* s, const grx_voice* const* voices, int page) {
+  grx_flowlm* m = s->m;
+  Kv8Set& c = s->kv8;
+  const int n = s->n, H = m->heads, d = m->d, L = m->L;
+  c.page = page;
+  c.width = (s->cap + page - 1) / page;
+  std::vector<const grx_voice*> each;  // the distinct voices, and their first pages
+  std::vector<int> begin, of(size_t(n), 0);
+  int64_t pages = 0;
+  for (int i = 0; i < n; i++) {
+    size_t u = 0;
+    while (u < each.size() && each[u] != voices[i]) u++;
+    if (u == each.size()) {
+      each.push_back(voices[i]);
+      begin.push_back(int(pages));
+      pages += (voices[i]->positions + page - 1) / page;
+    }
+    of[size_t(i)] = int(u);
+  }
+  std::vector<int> table(size_t(n) * c.width), from, to;
+  for (int i = 0; i < n; i++) {
+    const int u = of[size_t(i)], whole = each[size_t(u)]->positions / page;
+    for (int b = 0; b < c.width; b++) table[size_t(i) * c.width + b] = b < whole ? begin[size_t(u)] + b : int(pages++);
+    if (each[size_t(u)]->positions % page) {
+      from.push_back(begin[size_t(u)] + whole);
+      to.push_back(table[size_t(i) * c.width + whole]);
+    }
+  }
+  if (pages * H > INT32_MAX) return fail(GRX_ERANGE, "grx_streams_create_kv8: too many pages");
+  c.pages = int(pages);
+  c.restored = int(from.size());
+  int rc = 0;
+  const size_t tokens = size_t(pages) * H * page * L;
+  c.k = s->ar.alloc<int8_t>(tokens * 64, &rc);
+  c.v = s->ar.alloc<int8_t>(tokens * 64, &rc);
+  c.scale = s->ar.alloc<float>(size_t(pages) * H * 2 * L, &rc);
+  c.table = s->ar.upload(table.data(), table.size(), &rc);
+  c.from = s->ar.upload(from.data(), from.size(), &rc);
+  c.to = s->ar.upload(to.data(), to.size(), &rc);
+  c.qkv = s->ar.alloc<float>(size_t(n) * 3 * d, &rc);
+  if (rc) return rc;
+  // the voices' tokens: a sequence each, with a table of its own
+  const int nv = int(each.size());
+  std::vector<int> vtable, len, row0(1, 0);
+  int most = 0;
+  for (const grx_voice* v : each) most = std::max(most, v->positions);
+  const int width = std::max(1, (most + page - 1) / page);
+  for (int u = 0; u < nv; u++) {
+    for (int b = 0; b < width; b++) vtable.push_back(begin[size_t(u)] + b);
+    len.push_back(each[size_t(u)]->positions);
+    row0.push_back(row0.back() + len.back());
+  }
+  const size_t R = size_t(row0.back());
+  if (R == 0) return GRX_OK;
+  Arena tmp;
+  tmp.dev = s->ar.dev;
+  int *d_table = tmp.upload(vtable.data(), vtable.size(), &rc), *d_len = tmp.upload(len.data(), len.size(), &rc),
+      *d_row0 = tmp.upload(row0.data(), row0.size(), &rc);
+  float* rows = tmp.alloc<float>(2 * R * d, &rc);
+  if (rc) return rc;
+  for (int l = 0; l < L; l++) {
+    for (int u = 0; u < nv; u++)
+      for (int j = 0; j < 2; j++) {
+        const size_t P = size_t(len[size_t(u)]) * d;
+        CK(cudaMemcpy(rows + j * R * d + size_t(row0[size_t(u)]) * d, &each[size_t(u)]->kv[(size_t(l) * 2 + j) * P],
+                      sizeof(float) * P, cudaMemcpyHostToDevice));
+      }
+    Kv8Args a = kv8_layer(s, l);
+    a.n = nv;
+    a.rows = int(R);
+    a.width = width;
+    a.max_new = a.max_len = most;
+    a.table = d_table;
+    a.len = d_len;
+    a.len_add = 0;
+    a.row0 = d_row0;
+    a.rope_mode = GRX_ROPE_NONE;  // a voice's keys are turned already
+    Kv8Rows k, v;
+    k.p = rows;
+    v.p = rows + R * d;
+    k.row = v.row = d;
+    k.head = v.head = 64;
+    CK(launch_kv8_append(a, 64, GRX_F32, k, v, s->st));
+    CK(cudaStreamSynchronize(s->st));
+  }
+  return GRX_OK;
+}
+
 static int streams_create_one(grx_flowlm* m, int n, const grx_voice* const* voices, int max_frames,
-                              std::unique_ptr<grx_streams>* out) {
+                              std::unique_ptr<grx_streams>* out, int page) {
   int rc = 0;
   int maxp = 0;
   for (int i = 0; i < n; i++) {
@@ -1323,7 +1514,7 @@ static int streams_create_one(grx_flowlm* m, int n, const grx_voice* const* voic
   const int d = m->d, fd = m->fd, ld = m->ldim, H = m->heads, L = m->L, hd = 64;
   const size_t per_stream = size_t(L) * 2 * H * s->cap * hd;
   CK(cudaStreamCreateWithFlags(&s->st, cudaStreamNonBlocking));
-  s->kv = s->ar.alloc<float>(per_stream * n, &rc);
+  if (!page) s->kv = s->ar.alloc<float>(per_stream * n, &rc);
   s->pos = s->ar.alloc<int>(size_t(n), &rc);
   s->pos0 = s->ar.alloc<int>(size_t(n), &rc);
   s->x = s->ar.alloc<float>(size_t(n) * d, &rc);
@@ -1376,6 +1567,7 @@ static int streams_create_one(grx_flowlm* m, int n, const grx_voice* const* voic
   for (int i = 0; i < n; i++) {
     const grx_voice* v = voices[i];
     p0[size_t(i)] = v->positions;
+    if (page) continue;
     float* dst = s->kv + per_stream * size_t(i);
     int first = -1;
     for (int j = 0; j < i; j++)
@@ -1402,7 +1594,7 @@ static int streams_create_one(grx_flowlm* m, int n, const grx_voice* const* voic
       }
   }
   CK(cudaMemcpy(s->pos0, p0.data(), sizeof(int) * size_t(n), cudaMemcpyHostToDevice));
-  rc = frame1_setup(s.get());
+  rc = page ? kv8_setup(s.get(), voices, page) : frame1_setup(s.get());
   if (rc) return rc;
   rc = grx_streams_reset(s.get());
   if (rc) return rc;
@@ -1429,6 +1621,56 @@ int64_t grx_streams_launches(const grx_streams* s) {
   int64_t l = s->launches;
   for (const auto& p : s->parts) l += p->launches;
   return l;
+}
+
+int grx_streams_kv(grx_streams* s, int i, int* positions, float* kv) {
+  if (!s || i < 0 || i >= s->n) return fail(GRX_EINVAL, "grx_streams_kv: bad stream index");
+  for (auto& p : s->parts)
+    if (i < p->row0 + p->n) return grx_streams_kv(p.get(), i - p->row0, positions, kv);
+  CK(cudaSetDevice(s->ar.dev));
+  int P = 0;
+  CK(cudaMemcpyAsync(&P, s->pos + i, sizeof P, cudaMemcpyDeviceToHost, s->st));
+  CK(cudaStreamSynchronize(s->st));
+  if (positions) *positions = P;
+  if (!kv || P == 0) return GRX_OK;
+  const int H = s->m->heads, d = s->m->d, L = s->m->L;
+  if (!s->kv8.page) {
+    // [layer][k|v][head][position][64] → [layer][k|v][position][d]
+    const size_t head = size_t(s->cap) * 64;
+    std::vector<float> c(size_t(L) * 2 * H * head);
+    CK(cudaMemcpy(c.data(), s->kv + c.size() * size_t(i), sizeof(float) * c.size(), cudaMemcpyDeviceToHost));
+    for (int lj = 0; lj < 2 * L; lj++)
+      for (int h = 0; h < H; h++)
+        for (int p = 0; p < P; p++)
+          std::memcpy(kv + (size_t(lj) * P + p) * d + h * 64, &c[(size_t(lj) * H + h) * head + size_t(p) * 64], 256);
+    return GRX_OK;
+  }
+  int rc = 0;
+  Arena tmp;
+  tmp.dev = s->ar.dev;
+  const int row0[2] = {0, P};
+  const int* d_row0 = tmp.upload(row0, 2, &rc);
+  float* rows = tmp.alloc<float>(size_t(L) * 2 * P * d, &rc);
+  if (rc) return rc;
+  for (int l = 0; l < L; l++) {
+    Kv8Args a = kv8_layer(s, l);
+    a.n = 1;
+    a.rows = a.max_new = P;
+    a.row0 = d_row0;
+    a.table = s->kv8.table + size_t(i) * s->kv8.width;
+    a.len = s->pos + i;
+    a.len_add = 0;
+    a.rope_mode = GRX_ROPE_NONE;
+    Kv8Rows k, v;
+    k.p = rows + size_t(l) * 2 * P * d;
+    v.p = rows + (size_t(l) * 2 + 1) * P * d;
+    k.row = v.row = d;
+    k.head = v.head = 64;
+    CK(launch_kv8_read(a, 64, GRX_F32, k, v, s->st));
+  }
+  CK(cudaMemcpyAsync(kv, rows, sizeof(float) * size_t(L) * 2 * P * d, cudaMemcpyDeviceToHost, s->st));
+  CK(cudaStreamSynchronize(s->st));
+  return GRX_OK;
 }
 
 void* grx_streams_cuda_stream(const grx_streams* s) { return s ? (void*)s->st : nullptr; }
@@ -1519,6 +1761,8 @@ int grx_streams_run_device(grx_streams* s, int frames, const float* d_noise, flo
 int grx_streams_run_device_timed(grx_streams* s, int frames, const float* d_noise, float* d_latent, float* d_eos,
                                  unsigned long long* d_attn_ts) {
   if (!s || !d_noise || frames < 0) return fail(GRX_EINVAL, "grx_streams_run_device: bad argument");
+  if (d_attn_ts && (s->parts.empty() ? s : s->parts[0].get())->kv8.page)
+    return fail(GRX_EINVAL, "grx_streams_run_device_timed: the attention over 8-bit caches writes no times");
   CK(cudaSetDevice(s->ar.dev));
   int rc = check_room(s, frames);
   if (rc) return rc;

@@ -449,6 +449,22 @@ __global__ void __launch_bounds__(256) k_kv8_read(Kv8Args a, Kv8Rows kout, Kv8Ro
   }
 }
 
+// One page of one layer a block.
+__global__ void __launch_bounds__(256) k_kv8_copy_pages(Kv8Args a, int bytes, const int* from, const int* to) {
+  const int f = from[blockIdx.x], t = to[blockIdx.x];
+  if (f < 0 || t < 0 || f >= a.pages || t >= a.pages) return;
+  const int64_t layer = int64_t(blockIdx.y) * a.pages;
+  int8_t* const pool[2] = {a.k + layer * bytes, a.v + layer * bytes};
+  for (int j = 0; j < 2; j++) {
+    const uint4* src = reinterpret_cast<const uint4*>(pool[j] + int64_t(f) * bytes);
+    uint4* dst = reinterpret_cast<uint4*>(pool[j] + int64_t(t) * bytes);
+    for (int x = threadIdx.x; x < bytes / 16; x += 256) dst[x] = src[x];
+  }
+  float* scale = a.scale + layer * a.heads * 2;
+  for (int x = threadIdx.x; x < 2 * a.heads; x += 256)
+    scale[int64_t(t) * a.heads * 2 + x] = scale[int64_t(f) * a.heads * 2 + x];
+}
+
 // Whether groups of `count` elements of rows that begin at p with these
 // strides lie at multiples of their size.
 template <class T>
@@ -1693,6 +1709,12 @@ cudaError_t launch_kv8_read(const Kv8Args& a, int head_dim, int type, const Kv8R
 cudaError_t launch_kv8_attend(const Kv8Args& a, int head_dim, int type, const Kv8Attend& t, cudaStream_t st) {
   if (head_dim == 64) return type == 0 ? attend_d<64, 2>(a, type, t, st) : attend_d<64, 1>(a, type, t, st);
   return type == 0 ? attend_d<128, 2>(a, type, t, st) : attend_d<128, 1>(a, type, t, st);
+}
+
+cudaError_t launch_kv8_copy_pages(const Kv8Args& a, int head_dim, int layers, const int* from, const int* to, int count,
+                                  cudaStream_t st) {
+  k_kv8_copy_pages<<<dim3(count, layers), 256, 0, st>>>(a, (a.heads << a.plog) * head_dim, from, to);
+  return cudaGetLastError();
 }
 
 void kv8_kernels_init() {

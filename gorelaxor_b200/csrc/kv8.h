@@ -87,6 +87,10 @@ cudaError_t launch_kv8_append(const Kv8Args& a, int head_dim, int type, const Kv
 cudaError_t launch_kv8_read(const Kv8Args& a, int head_dim, int type, const Kv8Rows& k, const Kv8Rows& v,
                             cudaStream_t st);
 cudaError_t launch_kv8_attend(const Kv8Args& a, int head_dim, int type, const Kv8Attend& t, cudaStream_t st);
+// Copies the pages from[j] to to[j] of `layers` caches that lie one behind
+// the other (a is the first).
+cudaError_t launch_kv8_copy_pages(const Kv8Args& a, int head_dim, int layers, const int* from, const int* to, int count,
+                                  cudaStream_t st);
 void kv8_kernels_init();
 
 }  // namespace grx

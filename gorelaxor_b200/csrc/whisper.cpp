@@ -16,6 +16,7 @@
 #include "gguf.h"
 #include "host.h"
 #include "kernels.h"
+#include "logp.h"
 
 using namespace grx;
 
@@ -181,6 +182,7 @@ struct grx_whisper_batch {
   float *sk = nullptr, *sv = nullptr, *ck = nullptr, *cvt = nullptr;
   float *x = nullptr, *cur = nullptr, *q = nullptr, *att = nullptr, *ff = nullptr, *logits = nullptr, *scratch = nullptr;
   float *enc = nullptr, *no_speech = nullptr;
+  int* score = nullptr;  // grx_whisper_score's device side: [n][3 + 2·kLogpMaxTop]
   // the audio encoder's work buffers, made at the first encode; its
   // attention runs enc_chunk streams at a time
   float *e_mel = nullptr, *e_x1 = nullptr, *e_h1 = nullptr, *e_x2 = nullptr, *e_x = nullptr, *e_cur = nullptr;
@@ -805,6 +807,7 @@ int grx_whisper_batch_create(grx_whisper* m, int n, grx_whisper_batch** out) {
   b->scratch = b->ar.alloc<float>(size_t(n) * m->n_vocab, &rc);
   b->enc = b->ar.alloc<float>(layer_stride_cross(m, n), &rc);
   b->no_speech = b->ar.alloc<float>(n, &rc);
+  b->score = b->ar.alloc<int>(size_t(n) * (3 + 2 * kLogpMaxTop), &rc);
   b->row_stream = b->ar.alloc<int>(n, &rc);
   b->row_pos = b->ar.alloc<int>(n, &rc);
   b->row_tok = b->ar.alloc<int>(n, &rc);
@@ -1281,6 +1284,39 @@ int grx_whisper_logits(grx_whisper_batch* b, float* out) {
   CK(cudaSetDevice(b->ar.dev));
   CK(cudaStreamSynchronize(b->st));
   CK(cudaMemcpy(out, b->logits, sizeof(float) * size_t(b->n) * b->m->n_vocab, cudaMemcpyDeviceToHost));
+  return GRX_OK;
+}
+
+int grx_whisper_score(grx_whisper_batch* b, const int* tokens, int top, float* logprob, float* entropy, int* top_ids,
+                      float* top_logprobs) {
+  if (!b || (logprob && !tokens)) return fail(GRX_EINVAL, "grx_whisper_score: null argument");
+  if (top < 0 || top > kLogpMaxTop || top > b->m->n_vocab)
+    return fail(GRX_EINVAL, "grx_whisper_score: " + std::to_string(top) + " alternatives (0 to " +
+                                std::to_string(kLogpMaxTop) + ")");
+  if (b->pos == 0) return fail(GRX_EINVAL, "grx_whisper_score: nothing has been decoded");
+  CK(cudaSetDevice(b->ar.dev));
+  const size_t n = size_t(b->n), k = size_t(top);
+  int* d_tok = b->score;
+  float *d_lp = reinterpret_cast<float*>(d_tok + n), *d_en = d_lp + n, *d_top = d_en + n;
+  int* d_ids = reinterpret_cast<int*>(d_top + n * kLogpMaxTop);
+  if (tokens) CK(cudaMemcpyAsync(d_tok, tokens, sizeof(int) * n, cudaMemcpyHostToDevice, b->st));
+  LogpArgs a;
+  a.x = b->logits;
+  a.stride = a.vocab = b->m->n_vocab;
+  a.rows = b->n;
+  a.top = top;
+  a.targets = d_tok;
+  a.logprob = tokens ? d_lp : nullptr;
+  a.entropy = d_en;
+  a.ids = d_ids;
+  a.lps = d_top;
+  CK(launch_logp(a, GRX_F32, b->st));
+  b->launches++;
+  if (logprob) CK(cudaMemcpyAsync(logprob, d_lp, sizeof(float) * n, cudaMemcpyDeviceToHost, b->st));
+  if (entropy) CK(cudaMemcpyAsync(entropy, d_en, sizeof(float) * n, cudaMemcpyDeviceToHost, b->st));
+  if (top_ids && k) CK(cudaMemcpyAsync(top_ids, d_ids, sizeof(int) * n * k, cudaMemcpyDeviceToHost, b->st));
+  if (top_logprobs && k) CK(cudaMemcpyAsync(top_logprobs, d_top, sizeof(float) * n * k, cudaMemcpyDeviceToHost, b->st));
+  CK(cudaStreamSynchronize(b->st));
   return GRX_OK;
 }
 

@@ -266,6 +266,19 @@ int grx_voice_kv(const grx_voice* v, int* positions, float* kv);
 /* n streams, stream i starting from voices[i] (speakChunk's
  * v.st.clone(...), speak.go:117), each with room for max_frames frames. */
 int grx_streams_create(grx_flowlm* m, int n, const grx_voice* const* voices, int max_frames, grx_streams** out);
+/* The same streams on 8-bit paged caches (grx_kv8) of page_tokens (16, 32
+ * or 64) tokens a page: a quarter of the memory and of what a frame's
+ * attention reads, and streams of one voice share its whole pages. Keys and
+ * values are rounded as grx_kv8_append defines, attention is
+ * grx_kv8_attend's; everything else is as with grx_streams_create, and every
+ * call on the set works (but grx_streams_run_device_timed's attention
+ * times). Results are near the float32 caches', not the reference's bits.
+ * Sets of one stream run the per-kernel path. */
+int grx_streams_create_kv8(grx_flowlm* m, int n, const grx_voice* const* voices, int max_frames, int page_tokens,
+                           grx_streams** out);
+/* Stream i's caches as a voice's: its positions, and (kv may be NULL)
+ * [layers][2][positions][d], what grx_voice_raw takes. Waits for the set. */
+int grx_streams_kv(grx_streams* s, int i, int* positions, float* kv);
 void grx_streams_free(grx_streams* s);
 /* Puts every stream back at its voice prompt and the next frame at bos. */
 int grx_streams_reset(grx_streams* s);
@@ -563,6 +576,16 @@ int grx_whisper_watchdog_test(grx_whisper_batch* b);
 int grx_whisper_cross(grx_whisper_batch* b, int i, int layer, float* k, float* vt);
 /* The logits of the last decode, [n][n_vocab]. */
 int grx_whisper_logits(grx_whisper_batch* b, float* out);
+/* What the last decode's logits say (grx_logprobs, before the sampling
+ * rules of transcribe.go:370-494): logprob [n] of tokens[i] in stream i (NaN
+ * for one outside the vocabulary), entropy [n], and the `top` (0 to
+ * GRX_LOGPROBS_MAX_TOP) most likely tokens of each stream, top_ids and
+ * top_logprobs [n][top]. Host memory; every output may be NULL, tokens too
+ * without logprob. GRX_EINVAL before the first prompt of a window. No
+ * counterpart in the reference, which keeps p and plog of the token that it
+ * samples. Synchronous. */
+int grx_whisper_score(grx_whisper_batch* b, const int* tokens, int top, float* logprob, float* entropy, int* top_ids,
+                      float* top_logprobs);
 void* grx_whisper_batch_cuda_stream(const grx_whisper_batch* b);
 int64_t grx_whisper_batch_launches(const grx_whisper_batch* b);
 
