@@ -173,12 +173,22 @@ __device__ __forceinline__ void take(Run& r, const float (&x)[N]) {
 }
 
 template <class T>
-__device__ __forceinline__ void load16(const T* p, float* x) {
+__device__ __forceinline__ void unpack16(uint4 q, float* x) {
   constexpr int V = 16 / sizeof(T);
-  T h[V];
-  *reinterpret_cast<uint4*>(h) = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-  for (int j = 0; j < V; j++) x[j] = wide(h[j]);
+  for (int j = 0; j < V; j++) {
+    if constexpr (sizeof(T) == 4)
+      x[j] = __uint_as_float(w[j]);
+    else if constexpr (std::is_same<T, __half>::value)
+      x[j] = __half2float(__ushort_as_half(uint16_t(w[j / 2] >> (16 * (j % 2)))));
+    else
+      x[j] = bits_f(j % 2 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+  }
+}
+template <class T>
+__device__ __forceinline__ void load16(const T* p, float* x) {
+  unpack16<T>(__ldg(reinterpret_cast<const uint4*>(p)), x);
 }
 
 // What the row's outputs are made of, by one thread.
@@ -224,15 +234,18 @@ __device__ __forceinline__ V peer(const V* p, uint32_t rank) {
 // ---- a row to a cluster of S blocks of NT threads ----
 //
 // Bound by the bytes of the logits. Loads are 16 bytes wide from the first
-// aligned value on, four to a thread in flight; few rows are split over a
+// aligned value on, two to a thread in flight ahead of the two that are
+// summed; few rows are split over a
 // cluster, whose first block joins the shares through distributed shared
-// memory.
-constexpr int kCand = 1024;
+// memory. Three blocks of 512 threads an SM: 107 us for 2048 rows of 100003
+// bfloat16 logits (two blocks with four vectors a turn 121, five of 256
+// threads 123).
+constexpr int kCand = 1024, kBlock = 512;
 
 template <class T, int NT>
-__global__ void __launch_bounds__(NT) k_logp(LogpArgs a, int S) {
-  constexpr int V = 16 / sizeof(T), U = 4, NW = NT / 32;
-  __shared__ float wm[NW], wz[NW], wt[NW];
+__global__ void __launch_bounds__(NT, 3) k_logp(LogpArgs a, int S) {
+  constexpr int V = 16 / sizeof(T), U = 2, NW = NT / 32;
+  __shared__ float wm[NW], wn[NW], wz[NW], wt[NW];
   __shared__ u64 wk[NW];
   __shared__ u64 cand[kCand];
   __shared__ u64 best[kLogpMaxTop];
@@ -252,11 +265,24 @@ __global__ void __launch_bounds__(NT) k_logp(LogpArgs a, int S) {
 
   Run r;
   int v = vb + tid;
-  for (; v + (U - 1) * NT < ve; v += U * NT) {
-    float f[U * V];
+  if (v + (U - 1) * NT < ve) {
+    // the next vectors come while these are summed
+    uint4 raw[U];
 #pragma unroll
-    for (int u = 0; u < U; u++) load16(xv + int64_t(v + u * NT) * V, f + u * V);
-    take(r, f);
+    for (int u = 0; u < U; u++) raw[u] = __ldg(reinterpret_cast<const uint4*>(xv) + v + u * NT);
+    for (;;) {
+      float f[U * V];
+#pragma unroll
+      for (int u = 0; u < U; u++) unpack16<T>(raw[u], f + u * V);
+      v += U * NT;
+      const bool more = v + (U - 1) * NT < ve;
+      if (more) {
+#pragma unroll
+        for (int u = 0; u < U; u++) raw[u] = __ldg(reinterpret_cast<const uint4*>(xv) + v + u * NT);
+      }
+      take(r, f);
+      if (!more) break;
+    }
   }
   for (; v < ve; v += NT) {
     float f[V];
@@ -273,20 +299,24 @@ __global__ void __launch_bounds__(NT) k_logp(LogpArgs a, int S) {
   }
   const bool some = vb + tid < ve || in_head || in_tail;
   {
-    const float m = warp_max(r.m);
-    if (lane == 0) wm[warp] = m;
+    const float m = warp_max(r.m), n = -warp_max(-r.m);
+    if (lane == 0) wm[warp] = m, wn[warp] = n;
   }
   __syncthreads();
-  float m = wm[0];
+  float m = wm[0], least = wn[0];
 #pragma unroll
-  for (int w = 1; w < NW; w++) m = fmaxf(m, wm[w]);
+  for (int w = 1; w < NW; w++) m = fmaxf(m, wm[w]), least = fminf(least, wn[w]);
   // the bound: the largest value, or the largest found, bit by bit, that
   // `top` threads reach
   const uint32_t u = order(r.m);
   uint32_t bound = order(m);
   if (k > 1) {
-    bound = 0;
-    for (int bit = 31; bit >= 0; bit--) {
+    // what the largest and the least have in common is the bound's too
+    const uint32_t ul = order(least), apart = bound ^ ul;
+    const int high = apart ? 32 - __clz(apart) : 0;
+    bound = high < 32 ? ul >> high << high : 0;
+    if (__syncthreads_count(some) < k) bound = 0;  // fewer values than asked for: all
+    for (int bit = high - 1; bit >= 0; bit--) {
       const uint32_t c = bound | 1u << bit;
       const int n = __syncthreads_count(some && u >= c);
       if (n >= k) {
@@ -303,6 +333,8 @@ __global__ void __launch_bounds__(NT) k_logp(LogpArgs a, int S) {
   const bool owner = some && r.m == m;
   float z = 0.f, t = 0.f;
   int ties = 0;
+  // (bound 0: every value, those that are no number too)
+  const float reach = unorder(bound);
   auto look = [&](float f, int i, bool sums) {
     if (sums) {
       if (f == m)
@@ -310,7 +342,7 @@ __global__ void __launch_bounds__(NT) k_logp(LogpArgs a, int S) {
       else if (f != ninf())
         add(z, t, f, m);
     }
-    if (k && order(f) >= bound) {
+    if (f >= reach || bound == 0) {
       const int p = atomicAdd(&ncand, 1);
       if (p < kCand) cand[p] = key_of(f, i);
     }
@@ -415,7 +447,7 @@ __global__ void __launch_bounds__(NT) k_logp(LogpArgs a, int S) {
 constexpr int kWarpCand = 128, kRowsPerBlock = 8;
 
 template <class T, int NE>
-__global__ void __launch_bounds__(32 * kRowsPerBlock, 2) k_logp_warp(LogpArgs a) {
+__global__ void __launch_bounds__(32 * kRowsPerBlock, NE > 48 ? 2 : 4) k_logp_warp(LogpArgs a) {
   __shared__ u64 cands[kRowsPerBlock][kWarpCand];
   __shared__ int counts[kRowsPerBlock];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, k = a.top;
@@ -425,9 +457,10 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock, 2) k_logp_warp(LogpArgs a)
   const T* x = static_cast<const T*>(a.x) + row64 * a.stride;
   // values behind the row are −inf: they count nothing anywhere but among
   // the candidates, which look at the index
+  const int whole = a.vocab / 32, rest = a.vocab % 32;
   float f[NE];
 #pragma unroll
-  for (int j = 0; j < NE; j++) f[j] = lane + 32 * j < a.vocab ? wide(x[lane + 32 * j]) : ninf();
+  for (int j = 0; j < NE; j++) f[j] = j < whole || (j == whole && lane < rest) ? wide(x[lane + 32 * j]) : ninf();
   float mine = f[0];
 #pragma unroll
   for (int j = 1; j < NE; j++) mine = fmaxf(mine, f[j]);
@@ -435,18 +468,23 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock, 2) k_logp_warp(LogpArgs a)
   const float m = warp_max(mine);
   Share s = {m, 0.f, 0.f};
   int ties = 0, at = 0x7fffffff;
+  {
+    f2 z = 0, t = 0;
+    const f2 nm = f2dup(-m), l2e = f2dup(kLog2e);
 #pragma unroll
-  for (int j = NE - 1; j >= 0; j--) {
-    if (32 * j >= a.vocab) continue;
-    const float d = max_nan(__fsub_rn(f[j], m), kFar);
-    const bool tie = f[j] == m;
-    const float e = tie ? 0.f : ex2(__fmul_rn(d, kLog2e));
-    s.z = __fadd_rn(s.z, e);
-    s.t = __fmaf_rn(-d, e, s.t);
-    if (tie) {
-      ties++;
-      at = lane + 32 * j;
+    for (int j = NE - 2; j >= 0; j -= 2) {
+      if (j > whole) continue;
+      const f2 d = f2add(f2make(f[j], f[j + 1]), nm);
+      const f2 dc = f2make(max_nan(f2lo(d), kFar), max_nan(f2hi(d), kFar)), y = f2mul(dc, l2e);
+      float e0 = ex2(f2lo(y)), e1 = ex2(f2hi(y));
+      if (f[j + 1] == m) e1 = 0.f, ties++, at = lane + 32 * (j + 1);
+      if (f[j] == m) e0 = 0.f, ties++, at = lane + 32 * j;
+      const f2 e = f2make(e0, e1);
+      z = f2add(z, e);
+      t = f2fma(dc, e, t);
     }
+    s.z = __fadd_rn(f2lo(z), f2hi(z));
+    s.t = -__fadd_rn(f2lo(t), f2hi(t));
   }
   s.z = warp_sum(s.z);
   s.t = warp_sum(s.t);
@@ -524,19 +562,23 @@ cudaError_t rows_t(const LogpArgs& a, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, k_logp<T, NT>, a, S);
 }
 
+template <class T, int NE>
+void warp_rows(const LogpArgs& a, cudaStream_t st) {
+  k_logp_warp<T, NE><<<unsigned((a.rows + kRowsPerBlock - 1) / kRowsPerBlock), 32 * kRowsPerBlock, 0, st>>>(a);
+}
+
 template <class T>
 cudaError_t logp_t(const LogpArgs& a, cudaStream_t st) {
-  const unsigned blocks = unsigned((a.rows + kRowsPerBlock - 1) / kRowsPerBlock);
   if (a.vocab <= 32 * 16)
-    k_logp_warp<T, 16><<<blocks, 32 * kRowsPerBlock, 0, st>>>(a);
-  else if (a.vocab <= 32 * 40)
-    k_logp_warp<T, 40><<<blocks, 32 * kRowsPerBlock, 0, st>>>(a);
+    warp_rows<T, 16>(a, st);
+  else if (a.vocab <= 32 * 34)
+    warp_rows<T, 34>(a, st);
+  else if (a.vocab <= 32 * 48)
+    warp_rows<T, 48>(a, st);
   else if (a.vocab <= 32 * 64)
-    k_logp_warp<T, 64><<<blocks, 32 * kRowsPerBlock, 0, st>>>(a);
-  else if (a.vocab < 16384)
-    return rows_t<T, 256>(a, st);
+    warp_rows<T, 64>(a, st);
   else
-    return rows_t<T, 512>(a, st);
+    return rows_t<T, kBlock>(a, st);
   return cudaGetLastError();
 }
 
