@@ -11,49 +11,11 @@
 
 #include <algorithm>
 
-#include "common.cuh"
-#include "kv8.h"
+#include "kv8.cuh"
 
 namespace grx {
 
 namespace {
-
-constexpr uint32_t FULL = 0xffffffffu;
-constexpr int kSMs = 148;
-constexpr int kRangeError = -5;  // GRX_ERANGE, what the status word gets
-
-enum { ROPE_NONE = 0, ROPE_PAIRS = 1, ROPE_HALVES = 2 };
-
-__device__ __forceinline__ void report(const Kv8Args& a) {
-  if (a.status) *a.status = kRangeError;
-}
-
-// Four consecutive values of a row; `vec` where their address is a multiple
-// of their size together.
-__device__ __forceinline__ void load4(const float* p, bool vec, float* x) {
-  if (vec) {
-    const float4 f = *reinterpret_cast<const float4*>(p);
-    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; i++) x[i] = p[i];
-  }
-}
-__device__ __forceinline__ float wide(float x) { return x; }
-__device__ __forceinline__ float wide(__half h) { return __half2float(h); }
-__device__ __forceinline__ float wide(__nv_bfloat16 h) { return __bfloat162float(h); }
-template <class H>
-__device__ __forceinline__ void load4(const H* p, bool vec, float* x) {
-  H h[4];
-  if (vec) {
-    *reinterpret_cast<uint2*>(h) = *reinterpret_cast<const uint2*>(p);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; i++) h[i] = p[i];
-  }
-#pragma unroll
-  for (int i = 0; i < 4; i++) x[i] = wide(h[i]);
-}
 
 __device__ __forceinline__ void narrow(float x, float* p) { *p = x; }
 __device__ __forceinline__ void narrow(float x, __half* p) { *p = __float2half_rn(x); }
@@ -465,14 +427,6 @@ __global__ void __launch_bounds__(256) k_kv8_copy_pages(Kv8Args a, int bytes, co
     scale[int64_t(t) * a.heads * 2 + x] = scale[int64_t(f) * a.heads * 2 + x];
 }
 
-// Whether groups of `count` elements of rows that begin at p with these
-// strides lie at multiples of their size.
-template <class T>
-bool aligned(const Kv8Rows& r, int count) {
-  const uintptr_t b = sizeof(T) * count;
-  return reinterpret_cast<uintptr_t>(r.p) % b == 0 && (r.row * sizeof(T)) % b == 0 && (r.head * sizeof(T)) % b == 0;
-}
-
 template <int D, class T>
 cudaError_t append_t(const Kv8Args& a, const Kv8Rows& k, const Kv8Rows& v, cudaStream_t st) {
   const int page = 1 << a.plog;
@@ -536,13 +490,6 @@ cudaError_t read_t(const Kv8Args& a, const Kv8Rows& k, const Kv8Rows& v, cudaStr
 // moves only when a score passes it by 2^8 (the weights stay far from
 // overflow), so most steps need no exchange between lanes.
 
-__device__ __forceinline__ float ninf() { return __int_as_float(0xff800000); }
-__device__ __forceinline__ float qnan() { return __int_as_float(0x7fc00000); }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void mma_s8(int* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
   asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -558,12 +505,6 @@ __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
-}
-// Two floats as float16s, lo in the low half.
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  uint32_t y;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
   return y;
 }
 // Byte b (0..3) of x and of y as float16s, x's in the low half.
@@ -590,100 +531,6 @@ __device__ __forceinline__ float peer_f32(const float* p, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(uint32_t(__cvta_generic_to_shared(p))), "r"(rank));
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at));
   return v;
-}
-
-// Values 16·tg .. 16·tg + 15 of each 64 of a query at the position `pos`,
-// rotated, by four lanes together.
-template <int D>
-__device__ __forceinline__ void rotate16(float (&x)[D / 64][16], const Kv8Args& a, int pos, int tg) {
-  constexpr int H2 = D / 64;
-  if (a.rope_mode == ROPE_NONE) return;
-  // a slot that holds nothing has no position; its scores are not used
-  const float2* cs = reinterpret_cast<const float2*>(a.rope) + int64_t(max(pos, 0)) * (D / 2);
-  if (a.rope_mode == ROPE_PAIRS) {
-#pragma unroll
-    for (int j = 0; j < H2; j++)
-#pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        const float2 f = cs[(64 * j + 16 * tg + e) / 2];
-        const float p = x[j][e], q = x[j][e + 1];
-        x[j][e] = __fmaf_rn(p, f.x, -__fmul_rn(q, f.y));
-        x[j][e + 1] = __fmaf_rn(p, f.y, __fmul_rn(q, f.x));
-      }
-  } else if (D == 64) {
-    // the partner is 32 values on: two lanes away
-#pragma unroll
-    for (int e = 0; e < 16; e++) {
-      const float o = __shfl_xor_sync(FULL, x[0][e], 2);
-      const float2 f = cs[(16 * tg + e) & 31];
-      x[0][e] = __fmaf_rn(x[0][e], f.x, tg < 2 ? -__fmul_rn(o, f.y) : __fmul_rn(o, f.y));
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 16; e++) {
-      const float2 f = cs[16 * tg + e];
-      const float p = x[0][e], q = x[H2 - 1][e];
-      x[0][e] = __fmaf_rn(p, f.x, -__fmul_rn(q, f.y));
-      x[H2 - 1][e] = __fmaf_rn(p, f.y, __fmul_rn(q, f.x));
-    }
-  }
-}
-
-constexpr float kQueryUnits = 4194304.f;  // a query's largest value
-
-// The largest magnitude of the values that four lanes hold, NaN where one is
-// not finite. `lanes`: those that take part.
-template <int D>
-__device__ __forceinline__ float group_amax(const float (&x)[D / 64][16], uint32_t lanes) {
-  float m = 0.f, nan = 0.f;
-#pragma unroll
-  for (int j = 0; j < D / 64; j++)
-#pragma unroll
-    for (int e = 0; e < 16; e++) {
-      m = fmaxf(m, fabsf(x[j][e]));
-      nan = __fmaf_rn(0.f, x[j][e], nan);  // 0·inf and 0·NaN
-    }
-  m = __fadd_rn(m, nan);
-  const float a = __shfl_xor_sync(lanes, m, 1);
-  m = m > a || isnan(m) ? m : a;
-  const float b = __shfl_xor_sync(lanes, m, 2);
-  return m > b || isnan(m) ? m : b;
-}
-// The factor that makes the largest value kQueryUnits (0 for rows of zeros
-// or of no numbers); tiny rows are lifted first, so that it stays in range.
-template <int D>
-__device__ __forceinline__ float lift_row(float (&x)[D / 64][16], float amax) {
-  if (amax < 1e-30f) {
-    amax = __fmul_rn(amax, 1e30f);
-#pragma unroll
-    for (int j = 0; j < D / 64; j++)
-#pragma unroll
-      for (int e = 0; e < 16; e++) x[j][e] = __fmul_rn(x[j][e], 1e30f);
-  }
-  return amax > 0.f ? __fdiv_rn(kQueryUnits, amax) : 0.f;
-}
-// n + 1.5·2^23 → n's three signed digits in base 256, a byte each: with 128
-// added to every digit they are the bytes of n + 0x808080.
-__device__ __forceinline__ uint32_t digits_of(float y) {
-  return (__float_as_uint(y) - MAGIC_BITS + 0x808080u) ^ 0x808080u;
-}
-// Byte `at` of four words.
-__device__ __forceinline__ uint32_t take_bytes(const uint32_t* n, int at) {
-  const uint32_t pick = at | (at + 4) << 4;
-  return __byte_perm(__byte_perm(n[0], n[1], pick), __byte_perm(n[2], n[3], pick), 0x5410);
-}
-
-__device__ __forceinline__ void put(const Kv8Attend& t, int type, int64_t at, float y) {
-  void* op = const_cast<void*>(t.out.p);
-  if (type == 0)
-    static_cast<float*>(op)[at] = y;
-  else if (type == 1)
-    static_cast<__half*>(op)[at] = __float2half_rn(y);
-  else
-    static_cast<__nv_bfloat16*>(op)[at] = __float2bfloat16_rn(y);
-}
-__device__ __forceinline__ float lse_of(float top, float sum) {
-  return sum == 0.f ? ninf() : __fmaf_rn(top, 0.693147181f, logf(sum));
 }
 
 // Which bytes of a transposed pair of weights the column g takes into word
@@ -1650,6 +1497,10 @@ cudaError_t attend_d(const Kv8Args& a, int type, const Kv8Attend& t, cudaStream_
   const int64_t rows = int64_t(a.max_new) * (t.heads / a.heads);  // queries that share a head's keys
   if (rows == 1) return attend1_d<D>(a, type, t, st);
   if (rows <= 8) return attend_t<D, 1, NP>(a, type, t, st);
+  // Many queries go to the 5th-generation tensor core, 128 a block, unless
+  // few blocks would have long stretches of keys that these kernels split.
+  const int64_t blocks = int64_t(a.n) * a.heads * ((rows + 127) / 128);
+  if (rows > 32 && (blocks >= kSMs / 4 || a.max_len <= 1024)) return launch_kv8_prompt(a, D, type, t, st);
   if (rows <= 16) return attend_t<D, 2, NP>(a, type, t, st);
   return attend_t<D, 4, NP>(a, type, t, st);
 }
@@ -1718,6 +1569,7 @@ cudaError_t launch_kv8_copy_pages(const Kv8Args& a, int head_dim, int layers, co
 }
 
 void kv8_kernels_init() {
+  kv8_prompt_init();
   attend1_init<64>();
   attend1_init<128>();
   attend_init<64, 2>();

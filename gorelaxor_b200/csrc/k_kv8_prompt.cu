@@ -1,0 +1,601 @@
+// Attention over the 8-bit paged cache for prompts: many queries of a
+// sequence share a key head, so the products belong on the 5th-generation
+// tensor core (tcgen05.mma, accumulators in Tensor Memory).
+//
+// A block takes 128 query rows (token by token, the heads of a group side by
+// side) against tiles of 64 keys, one pass with the running maximum and sum:
+//  * warps 4-7 turn a tile's bytes into float16 operands (exact): the keys as
+//    they lie, [key][value], the values turned, [value][key], both in the
+//    128-byte swizzle that the tensor core reads; the next tile's bytes come
+//    into registers meanwhile;
+//  * warp 8 issues the products: scores S = Q·Kᵀ into one of two TMEM tiles,
+//    Q being the sum of two float16s of a row scaled to 2^14 (22 bits and
+//    more: 32-bit scores), and O += P·V with P from TMEM, one float16 for
+//    16-bit outputs and the sum of two for float32 ones. The scores of tile
+//    j + 1 are issued ahead of the outputs of tile j;
+//  * warps 0-3, a row a thread: a row's 64 scores from TMEM, weights
+//    p·s_v/W, written back as P. The maximum moves only when a score passes
+//    it by 2^8; then, and when a larger value scale comes, the row of O in
+//    TMEM is multiplied.
+// Blocks with the most keys start first. Every wait is bounded (about a
+// second of clocks); one that runs out sets the block's `dead` word, every
+// role leaves its loop, the block frees its TMEM, and the status word gets
+// GRX_ETIMEDOUT.
+//
+// What bounds it is the exponentials and the rows' instructions between two
+// tiles' products (64 of each a thread and tile); the products take about
+// 800 clocks a tile of 128 x 64 at 128 values.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "kv8.cuh"
+
+namespace grx {
+
+namespace {
+
+constexpr int kTimedOut = -7;  // GRX_ETIMEDOUT
+constexpr int kRows = 128, kKeys = 64;
+constexpr float kTo14 = 1.f / 256.f;  // from kQueryUnits to 2^14
+
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded; false once about 2^31 clocks have passed or another role gave up.
+// All lanes of a warp get the same answer.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
+  bool ok = bar_try(bar, parity);
+  if (!ok) {
+    const long long t0 = clock64();
+    while (!(ok = bar_try(bar, parity))) {
+      if (*dead) break;
+      if (clock64() - t0 > (1LL << 31)) {
+        *dead = 1;
+        break;
+      }
+    }
+  }
+  return __all_sync(FULL, ok);
+}
+__device__ __forceinline__ void bar_init(uint32_t bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+// Executed by a whole warp in step, issued by the one lane elect.sync picks.
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile(
+      "{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n"
+      "@p tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar)
+      : "memory");
+}
+// K-major operand in the 128-byte swizzle: rows of 128 bytes, groups of 8
+// rows 1024 bytes apart.
+__device__ __forceinline__ uint64_t operand(uint32_t addr) {
+  return uint64_t((addr >> 4) & 0x3FFF) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
+         (uint64_t(2) << 61);
+}
+// D (+)= A·Bᵀ, float16 operands, float32 sums; A in shared memory or TMEM.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(int(add))
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(int(add))
+      : "memory");
+}
+// 32 consecutive columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t* d) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]), "=r"(d[4]), "=r"(d[5]), "=r"(d[6]), "=r"(d[7]), "=r"(d[8]),
+        "=r"(d[9]), "=r"(d[10]), "=r"(d[11]), "=r"(d[12]), "=r"(d[13]), "=r"(d[14]), "=r"(d[15]), "=r"(d[16]),
+        "=r"(d[17]), "=r"(d[18]), "=r"(d[19]), "=r"(d[20]), "=r"(d[21]), "=r"(d[22]), "=r"(d[23]), "=r"(d[24]),
+        "=r"(d[25]), "=r"(d[26]), "=r"(d[27]), "=r"(d[28]), "=r"(d[29]), "=r"(d[30]), "=r"(d[31])
+      : "r"(at)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t* d) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(at),
+      "r"(d[0]), "r"(d[1]), "r"(d[2]), "r"(d[3]), "r"(d[4]), "r"(d[5]), "r"(d[6]), "r"(d[7]), "r"(d[8]), "r"(d[9]),
+      "r"(d[10]), "r"(d[11]), "r"(d[12]), "r"(d[13]), "r"(d[14]), "r"(d[15]), "r"(d[16]), "r"(d[17]), "r"(d[18]),
+      "r"(d[19]), "r"(d[20]), "r"(d[21]), "r"(d[22]), "r"(d[23]), "r"(d[24]), "r"(d[25]), "r"(d[26]), "r"(d[27]),
+      "r"(d[28]), "r"(d[29]), "r"(d[30]), "r"(d[31])
+      : "memory");
+}
+__device__ __forceinline__ uint32_t to_f16(uint32_t u) {
+  uint32_t d;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(u ^ 0x64806480u), "r"(0xe480e480u));
+  return d;
+}
+__device__ __forceinline__ void sts16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// NP: float16s of a weight.
+template <int D, int NP>
+struct Prompt {
+  static constexpr int threads = 288;
+  // shared memory: bytes of the two halves of Q, of a tile's keys and values
+  static constexpr int q = kRows * D * 2, k = kKeys * D * 2, v = D * kKeys * 2;
+  static constexpr int off_k = 2 * q, off_v = off_k + 2 * k, off_s = off_v + 2 * v;  // scales: [2][4] pairs
+  static constexpr int off_f = off_s + 2 * 4 * 8, off_bar = off_f + kRows * 4, used = off_bar + 8 * 8 + 16;
+  // TMEM columns: two score tiles, two weight tiles, the outputs
+  static constexpr int c_p = 2 * kKeys, c_o = c_p + 2 * NP * kKeys / 2, columns = c_o + D <= 256 ? 256 : 512;
+  // Blocks that share an SM fit in its 512 columns together: one, or two.
+  static constexpr int room = columns == 512 ? 116 * 1024 : 78 * 1024;
+  static constexpr int smem = 1024 + (used > room ? used : room);
+};
+
+template <int D, int NP>
+__global__ void __launch_bounds__(288, 1)
+    k_kv8_prompt(Kv8Args a, Kv8Attend t, int type, int qtiles, bool vec, bool ovec) {
+  using C = Prompt<D, NP>;
+  constexpr int H2 = D / 64;
+  extern __shared__ uint8_t raw_smem[];
+  const uint32_t raw = smem_at(raw_smem), base = (raw + 1023) & ~1023u;
+  uint8_t* mem = raw_smem + (base - raw);
+  float2* scales = reinterpret_cast<float2*>(mem + C::off_s);  // [stage][16 keys]
+  float* rowf = reinterpret_cast<float*>(mem + C::off_f);
+  const uint32_t bars = base + C::off_bar;
+  const auto conv = [&](int b) { return bars + 8 * b; };         // a tile's operands are in stage b
+  const auto scored = [&](int b) { return bars + 8 * (2 + b); };  // its scores are in S b
+  const auto weighed = [&](int b) { return bars + 8 * (4 + b); }; // its weights are in P b
+  const auto added = [&](int b) { return bars + 8 * (6 + b); };   // its outputs are in O
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mem + C::off_bar + 64);
+  volatile int* dead = reinterpret_cast<volatile int*>(mem + C::off_bar + 68);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  // heads of one tile side by side, the last queries (the most keys) first
+  const int h = blockIdx.x % a.heads, rest = blockIdx.x / a.heads, i = rest % a.n, qt = qtiles - 1 - rest / a.n;
+  const int group = t.heads / a.heads;
+  const Kv8Span sp = kv8_span(a, i);
+  if (!sp.ok) {
+    if (tid == 0) report(a);
+    return;
+  }
+  const int r0 = qt * kRows, nrow = min(kRows, sp.T * group - r0);
+  if (nrow <= 0) return;
+  const int p0 = sp.len - sp.T;
+  const int pmin = p0 + r0 / group, pmax = p0 + (r0 + nrow - 1) / group;
+  const int first = a.first ? max(0, a.first[i]) : 0;
+  const int klo = max(first, t.window > 0 ? pmin - t.window + 1 : 0);
+  const int tb = klo / kKeys, nt = max(0, (pmax + kKeys) / kKeys - tb);  // tiles tb .. tb + nt − 1
+
+  if (tid == 0) {
+    *dead = 0;
+    for (int b = 0; b < 2; b++) {
+      bar_init(conv(b), 4);
+      bar_init(scored(b), 1);
+      bar_init(weighed(b), 4);
+      bar_init(added(b), 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (warp == 8) {
+    asm volatile(
+        "tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n"
+        "tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::"r"(smem_at(tmem_slot)),
+        "r"(C::columns)
+        : "memory");
+  }
+
+  // --- the queries: rotated, scaled, as the sum of two float16s; four lanes
+  // to a row, warps 0-7 eight rows at a time ---
+  if (warp < 8) {
+    const int g = lane >> 2, tg = lane & 3;
+#pragma unroll 1
+    for (int r = warp * 8 + g; r < kRows; r += 64) {
+      const bool there = r < nrow;
+      const int tq = there ? (r0 + r) / group : 0, hq = h * group + (there ? (r0 + r) % group : 0);
+      float x[H2][16];
+      const int64_t off = int64_t(sp.row + tq) * t.q.row + int64_t(hq) * t.q.head + 16 * tg;
+#pragma unroll
+      for (int j = 0; j < H2; j++)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const int64_t o = off + 64 * j + e;
+          if (!there)
+            x[j][e] = x[j][e + 1] = x[j][e + 2] = x[j][e + 3] = 0.f;
+          else if (type == 0)
+            load4(static_cast<const float*>(t.q.p) + o, vec, &x[j][e]);
+          else if (type == 1)
+            load4(static_cast<const __half*>(t.q.p) + o, vec, &x[j][e]);
+          else
+            load4(static_cast<const __nv_bfloat16*>(t.q.p) + o, vec, &x[j][e]);
+        }
+      rotate16<D>(x, a, p0 + tq, tg);
+      const float amax = group_amax<D>(x, FULL);
+      const float to = __fmul_rn(lift_row<D>(x, amax), kTo14);
+#pragma unroll
+      for (int j = 0; j < H2; j++) {
+        uint32_t hi[8], lo[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          // a row that is no number: 0 here, and its factor is none
+          const float y0 = to > 0.f ? __fmul_rn(x[j][2 * e], to) : 0.f, y1 = to > 0.f ? __fmul_rn(x[j][2 * e + 1], to) : 0.f;
+          hi[e] = pack_f16(y0, y1);
+          lo[e] = pack_f16(__fsub_rn(y0, __half2float(__ushort_as_half(hi[e] & 0xffff))),
+                           __fsub_rn(y1, __half2float(__ushort_as_half(hi[e] >> 16))));
+        }
+        const uint32_t at = base + j * (kRows * 128) + r * 128;
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          const uint32_t o = at + ((2 * tg + c) ^ (r & 7)) * 16;
+          sts16(o, hi[4 * c], hi[4 * c + 1], hi[4 * c + 2], hi[4 * c + 3]);
+          sts16(o + C::q, lo[4 * c], lo[4 * c + 1], lo[4 * c + 2], lo[4 * c + 3]);
+        }
+      }
+      if (tg == 0)
+        rowf[r] = __fmul_rn(__fmul_rn(amax, 256.f / kQueryUnits), __fmul_rn(t.scale, 1.44269504f));
+    }
+    fence_async();
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 8) {
+    // ---- the products
+    const uint32_t idesc_s = (1u << 4) | (uint32_t(kKeys >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
+    const uint32_t idesc_o = (1u << 4) | (uint32_t(D >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
+    const auto outputs = [&](int j) {
+      const int b = j & 1;
+      fence_after();
+#pragma unroll
+      for (int n = 0; n < NP; n++)
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; kk++)
+          mma_ts(tmem + C::c_o, tmem + C::c_p + (b * NP + n) * (kKeys / 2) + kk * 8,
+                 operand(base + C::off_v + b * C::v + kk * 32), idesc_o, j > 0 || n > 0 || kk > 0);
+      commit(added(b));
+    };
+    int done = 0;
+    bool ok = true;
+    for (int j = 0; j < nt && ok; j++) {
+      const int b = j & 1;
+      ok = bar_wait(conv(b), (j >> 1) & 1, dead);
+      if (!ok) break;
+      fence_after();
+#pragma unroll
+      for (int n = 0; n < 2; n++)
+#pragma unroll
+        for (int kk = 0; kk < D / 16; kk++)
+          mma_ss(tmem + b * kKeys, operand(base + n * C::q + (kk / 4) * (kRows * 128) + (kk % 4) * 32),
+                 operand(base + C::off_k + b * C::k + (kk / 4) * (kKeys * 128) + (kk % 4) * 32), idesc_s,
+                 n > 0 || kk > 0);
+      commit(scored(b));
+      if (j > 0) {
+        ok = bar_wait(weighed(b ^ 1), ((j - 1) >> 1) & 1, dead);
+        if (ok) outputs(j - 1), done = j;
+      }
+    }
+    if (ok && nt > 0 && bar_wait(weighed((nt - 1) & 1), ((nt - 1) >> 1) & 1, dead)) outputs(nt - 1), done = nt;
+    if (done < nt && nt > 0) {
+      // given up: what was issued ends before the TMEM is released
+      commit(added(0));
+      const long long t0 = clock64();
+      while (clock64() - t0 < (1LL << 24)) {
+      }
+    }
+  } else if (warp >= 4) {
+    // ---- a tile's operands
+    const int ct = tid - 128;  // 0 .. 127
+    constexpr int KU = D / 32;  // sixteen-byte units of keys a thread
+    constexpr int VU = D / 64;  // units of eight tokens by four values
+    const int cshift = a.plog, plast = (sp.len + (1 << a.plog) - 1) >> a.plog;
+    const int64_t pbytes = int64_t(a.heads << a.plog) * D;
+    const int8_t* kh = a.k + (int64_t(h) << a.plog) * D;
+    const int8_t* vh = a.v + (int64_t(h) << a.plog) * D;
+    // where token key of the sequence lies (some page's bytes where there is none)
+    const auto where = [&](int key) {
+      const int b = key >> cshift;
+      const int page = b < plast ? kv8_page(a, i, b) : -1;
+      return int64_t(max(page, 0)) * pbytes + int64_t(key & ((1 << a.plog) - 1)) * D;
+    };
+    uint4 kr[KU];
+    uint32_t vr[VU][8];
+    float2 sc = make_float2(0.f, 0.f);
+    const auto load = [&](int j) {
+      const int key0 = (tb + j) * kKeys;
+#pragma unroll
+      for (int u = 0; u < KU; u++) {
+        const int n = ct + 128 * u;  // unit: key n / (D/16), sixteen values n % (D/16)
+        kr[u] = __ldg(reinterpret_cast<const uint4*>(kh + where(key0 + n / (D / 16)) + n % (D / 16) * 16));
+      }
+#pragma unroll
+      for (int u = 0; u < VU; u++) {
+        const int n = ct + 128 * u;  // unit: tokens 8·(n / (D/4)) .., values 4·(n % (D/4)) ..
+        const int8_t* from = vh + where(key0 + 8 * (n / (D / 4))) + n % (D / 4) * 4;
+#pragma unroll
+        for (int e = 0; e < 8; e++) vr[u][e] = __ldg(reinterpret_cast<const uint32_t*>(from + e * D));
+      }
+      if (ct < 4) {  // sixteen keys' scales: −inf where there is no page, NaN for what is no scale
+        const int b = (key0 + 16 * ct) >> cshift, page = b < plast ? kv8_page(a, i, b) : -1;
+        if (page < 0) {
+          if (b < plast) report(a);
+          sc = make_float2(ninf(), 0.f);
+        } else {
+          const float2 s = reinterpret_cast<const float2*>(a.scale)[int64_t(page) * a.heads + h];
+          sc = make_float2(isfinite(s.x) ? s.x : qnan(), s.y >= 0.f && isfinite(s.y) ? s.y : qnan());
+        }
+      }
+    };
+    if (nt > 0) load(0);
+    for (int j = 0; j < nt; j++) {
+      const int b = j & 1;
+      if (j > 1 && !bar_wait(added(b), ((j - 2) >> 1) & 1, dead)) break;
+      if (ct < 4) scales[b * 4 + ct] = sc;
+#pragma unroll
+      for (int u = 0; u < KU; u++) {
+        const int n = ct + 128 * u, key = n / (D / 16), c = n % (D / 16);  // values 16c .. : chunks 2c and 2c + 1
+        const uint32_t at = base + C::off_k + b * C::k + (c / 4) * (kKeys * 128) + key * 128;
+        const int swap = D == 128 ? c >> 2 & 1 : key & 1;  // neighbours write different banks
+        const uint32_t w[4] = {kr[u].x, kr[u].y, kr[u].z, kr[u].w};
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const int s = e ^ swap;
+          const uint32_t x = s ? w[2] : w[0], y = s ? w[3] : w[1];
+          sts16(at + ((2 * (c % 4) + s) ^ (key & 7)) * 16, to_f16(__byte_perm(x, 0, 0x4140)),
+                to_f16(__byte_perm(x, 0, 0x4342)), to_f16(__byte_perm(y, 0, 0x4140)), to_f16(__byte_perm(y, 0, 0x4342)));
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < VU; u++) {
+        const int n = ct + 128 * u, grp = n / (D / 4), w = n % (D / 4);
+        const uint32_t at = base + C::off_v + b * C::v + 4 * w * 128;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int v = (e + (w >> 1)) & 3;  // the order in which neighbours write different banks
+          const uint32_t pick = v | (4 + v) << 8;
+          uint32_t y[4];
+#pragma unroll
+          for (int m = 0; m < 4; m++) y[m] = to_f16(__byte_perm(vr[u][2 * m], vr[u][2 * m + 1], pick) & 0x00ff00ffu);
+          sts16(at + v * 128 + (grp ^ ((4 * w + v) & 7)) * 16, y[0], y[1], y[2], y[3]);
+        }
+      }
+      if (j + 1 < nt) load(j + 1);
+      fence_async();
+      __syncwarp();
+      if (lane == 0) bar_arrive(conv(b));
+    }
+  } else {
+    // ---- the rows
+    const int r = tid;
+    const bool there = r < nrow;
+    const int tq = there ? (r0 + r) / group : 0, hq = h * group + (there ? (r0 + r) % group : 0);
+    const int p = there ? p0 + tq : pmax;
+    const int lo = max(first, t.window > 0 ? p - t.window + 1 : 0);  // sees lo .. p
+    const int in_lo = max(first, t.window > 0 ? pmax - t.window + 1 : 0);
+    const float f = rowf[r];
+    const uint32_t lanes = tmem + (uint32_t(warp * 32) << 16);
+    float ref = ninf(), l = 0.f, W = 0.f, toW = 0.f;
+    bool ok = true;
+    for (int j = 0; j < nt; j++) {
+      const int b = j & 1, key0 = (tb + j) * kKeys;
+      ok = bar_wait(conv(b), (j >> 1) & 1, dead) && bar_wait(scored(b), (j >> 1) & 1, dead);
+      if (!ok) break;
+      fence_after();
+      uint32_t s[kKeys];
+      tmem_ld32(lanes + b * kKeys, s);
+      tmem_ld32(lanes + b * kKeys + 32, s + 32);
+      float sk[4], sv[4];
+      bool gone = false;
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const float2 c = scales[b * 4 + u];
+        gone = gone || c.x == ninf();
+        sk[u] = c.x;
+        sv[u] = c.y;
+      }
+      wait_ld();
+      const bool edge = gone || key0 < in_lo || key0 + kKeys - 1 > pmin;
+      f2* x2 = reinterpret_cast<f2*>(s);
+      float* x = reinterpret_cast<float*>(s);
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const f2 c = f2dup(__fmul_rn(f, sk[u]));
+#pragma unroll
+        for (int e = 0; e < 8; e++) x2[8 * u + e] = f2mul(x2[8 * u + e], c);
+      }
+      if (edge) {
+#pragma unroll
+        for (int e = 0; e < kKeys; e++)
+          if (key0 + e < lo || key0 + e > p || sk[e / 16] == ninf()) x[e] = ninf();
+      }
+      float top = x[0];
+#pragma unroll
+      for (int e = 1; e < kKeys; e++) top = fmaxf(top, x[e]);
+      float wide = sv[0];
+#pragma unroll
+      for (int u = 1; u < 4; u++) wide = fmaxf(wide, sv[u]);
+      // the references move: a score 2^8 above the row's (any, before its
+      // first key), a larger value scale
+      const bool over = top > __fadd_rn(ref, 8.f);
+      if (__any_sync(FULL, over) || wide > W) {
+        float k = 1.f;
+        if (wide > W) {
+          const float w = fminf(fmaxf(__fmul_rn(2.f, wide), 1.17549435e-38f), 3.4e38f);
+          k = __fdiv_rn(W, w);
+          W = w;
+          toW = __fdiv_rn(1.f, w);
+        }
+        if (over) {
+          const float up = ex2(__fsub_rn(ref, top));
+          ref = top;
+          l = __fmul_rn(l, up);
+          k = __fmul_rn(k, up);
+        }
+        if (j > 0) {
+          ok = bar_wait(added(b ^ 1), ((j - 1) >> 1) & 1, dead);
+          if (!ok) break;
+          fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(lanes + C::c_o + c, o);
+            wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__fmul_rn(__uint_as_float(o[e]), k));
+            tmem_st32(lanes + C::c_o + c, o);
+          }
+          wait_st();
+        }
+      }
+      const f2 m = f2dup(ref == ninf() ? 0.f : -ref);
+      f2 sum = 0;
+#pragma unroll
+      for (int e = 0; e < kKeys / 2; e++) {
+        const f2 y = f2add(x2[e], m);
+        x2[e] = f2make(ex2(f2lo(y)), ex2(f2hi(y)));
+        sum = f2add(sum, x2[e]);
+      }
+      l = __fadd_rn(l, __fadd_rn(f2lo(sum), f2hi(sum)));
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const f2 c = f2dup(__fmul_rn(sv[u], toW));
+#pragma unroll
+        for (int e = 0; e < 8; e++) x2[8 * u + e] = f2mul(x2[8 * u + e], c);
+      }
+      if (edge) {  // what is not seen counts nothing, whatever its page's scale
+#pragma unroll
+        for (int e = 0; e < kKeys; e++)
+          if (key0 + e < lo || key0 + e > p || sk[e / 16] == ninf()) x[e] = 0.f;
+      }
+      if (j > 1) {
+        ok = bar_wait(added(b), ((j - 2) >> 1) & 1, dead);  // P b is free
+        if (!ok) break;
+      }
+#pragma unroll
+      for (int n = 0; n < NP; n++) {
+        uint32_t w[kKeys / 2];
+#pragma unroll
+        for (int e = 0; e < kKeys / 2; e++) {
+          w[e] = pack_f16(x[2 * e], x[2 * e + 1]);
+          if (n + 1 < NP) {
+            x[2 * e] = __fsub_rn(x[2 * e], __half2float(__ushort_as_half(w[e] & 0xffff)));
+            x[2 * e + 1] = __fsub_rn(x[2 * e + 1], __half2float(__ushort_as_half(w[e] >> 16)));
+          }
+        }
+        tmem_st32(lanes + C::c_p + (b * NP + n) * (kKeys / 2), w);
+      }
+      wait_st();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(weighed(b));
+    }
+    if (ok && nt > 0) ok = bar_wait(added((nt - 1) & 1), ((nt - 1) >> 1) & 1, dead);
+    if (ok) {
+      fence_after();
+      const float inv = l == 0.f ? 0.f : __fdiv_rn(W, l);
+      const int64_t at = int64_t(sp.row + tq) * t.out.row + int64_t(hq) * t.out.head;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        if (nt > 0) {
+          tmem_ld32(lanes + C::c_o + c, o);
+          wait_ld();
+        }
+        float y[32], most = 0.f;
+#pragma unroll
+        for (int e = 0; e < 32; e++) {
+          y[e] = l == 0.f ? 0.f : __fmul_rn(__uint_as_float(o[e]), inv);
+          most = fmaxf(most, fabsf(y[e]));
+        }
+        if (!there) continue;
+        if (t.out.p && ovec && type == 0) {
+          float4* op = reinterpret_cast<float4*>(static_cast<float*>(const_cast<void*>(t.out.p)) + at + c);
+#pragma unroll
+          for (int e = 0; e < 8; e++) op[e] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
+        } else if (t.out.p && ovec) {
+          uint32_t hy[16];
+#pragma unroll
+          for (int e = 0; e < 16; e++)
+            hy[e] = type == 1 ? pack_f16(y[2 * e], y[2 * e + 1])
+                              : uint32_t(__bfloat16_as_ushort(__float2bfloat16_rn(y[2 * e]))) |
+                                    uint32_t(__bfloat16_as_ushort(__float2bfloat16_rn(y[2 * e + 1]))) << 16;
+          uint4* op = reinterpret_cast<uint4*>(static_cast<uint16_t*>(const_cast<void*>(t.out.p)) + at + c);
+#pragma unroll
+          for (int e = 0; e < 4; e++) op[e] = make_uint4(hy[4 * e], hy[4 * e + 1], hy[4 * e + 2], hy[4 * e + 3]);
+        } else if (t.out.p) {
+#pragma unroll
+          for (int e = 0; e < 32; e++) put(t, type, at + c + e, y[e]);
+        }
+        if (t.q8) {  // one Q8_0 block
+          const int64_t to = (int64_t(sp.row + tq) * t.heads + hq) * D + c;
+          uint32_t w[8] = {};
+#pragma unroll
+          for (int e = 0; e < 32; e++) w[e / 4] |= uint32_t(uint8_t(quant_val(y[e], most))) << (8 * (e % 4));
+          uint4* op = reinterpret_cast<uint4*>(t.q8 + to);
+          op[0] = make_uint4(w[0], w[1], w[2], w[3]);
+          op[1] = make_uint4(w[4], w[5], w[6], w[7]);
+          t.q8s[to / QK] = make_float2(quant_scale(most), quant_scale(most));
+        }
+      }
+      if (there && t.lse) t.lse[int64_t(sp.row + tq) * t.heads + hq] = lse_of(ref, l);
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(C::columns) : "memory");
+  }
+  if (tid == 0 && *dead && a.status) *a.status = kTimedOut;
+}
+
+template <int D, int NP>
+cudaError_t launch_t(const Kv8Args& a, int type, const Kv8Attend& t, cudaStream_t st) {
+  using C = Prompt<D, NP>;
+  const int qtiles = int((int64_t(a.max_new) * (t.heads / a.heads) + kRows - 1) / kRows);
+  const bool vec = type == 0 ? aligned<float>(t.q, 4) : aligned<__half>(t.q, 4);
+  const bool ovec = type == 0 ? aligned<float>(t.out, 4) : aligned<__half>(t.out, 8);
+  k_kv8_prompt<D, NP><<<unsigned(int64_t(qtiles) * a.n * a.heads), C::threads, C::smem, st>>>(a, t, type, qtiles, vec, ovec);
+  return cudaGetLastError();
+}
+
+template <int D, int NP>
+void init_t() {
+  cudaFuncSetAttribute(k_kv8_prompt<D, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Prompt<D, NP>::smem);
+}
+
+}  // namespace
+
+cudaError_t launch_kv8_prompt(const Kv8Args& a, int head_dim, int type, const Kv8Attend& t, cudaStream_t st) {
+  if (head_dim == 64) return type == 0 ? launch_t<64, 2>(a, type, t, st) : launch_t<64, 1>(a, type, t, st);
+  return type == 0 ? launch_t<128, 2>(a, type, t, st) : launch_t<128, 1>(a, type, t, st);
+}
+
+void kv8_prompt_init() {
+  init_t<64, 1>();
+  init_t<64, 2>();
+  init_t<128, 1>();
+  init_t<128, 2>();
+}
+
+}  // namespace grx

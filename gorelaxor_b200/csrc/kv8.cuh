@@ -1,0 +1,168 @@
+// Device helpers that the 8-bit cache's kernels share (k_kv8.cu,
+// k_kv8_prompt.cu).
+#pragma once
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+#include "kv8.h"
+
+namespace grx {
+
+namespace {
+
+constexpr uint32_t FULL = 0xffffffffu;
+constexpr int kSMs = 148;
+constexpr int kRangeError = -5;  // GRX_ERANGE, what the status word gets
+
+enum { ROPE_NONE = 0, ROPE_PAIRS = 1, ROPE_HALVES = 2 };
+
+__device__ __forceinline__ void report(const Kv8Args& a) {
+  if (a.status) *a.status = kRangeError;
+}
+
+// Four consecutive values of a row; `vec` where their address is a multiple
+// of their size together.
+__device__ __forceinline__ void load4(const float* p, bool vec, float* x) {
+  if (vec) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = p[i];
+  }
+}
+__device__ __forceinline__ float wide(float x) { return x; }
+__device__ __forceinline__ float wide(__half h) { return __half2float(h); }
+__device__ __forceinline__ float wide(__nv_bfloat16 h) { return __bfloat162float(h); }
+template <class H>
+__device__ __forceinline__ void load4(const H* p, bool vec, float* x) {
+  H h[4];
+  if (vec) {
+    *reinterpret_cast<uint2*>(h) = *reinterpret_cast<const uint2*>(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) h[i] = p[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) x[i] = wide(h[i]);
+}
+
+__device__ __forceinline__ float ninf() { return __int_as_float(0xff800000); }
+__device__ __forceinline__ float qnan() { return __int_as_float(0x7fc00000); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two floats as float16s, lo in the low half.
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t y;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+  return y;
+}
+// Values 16·tg .. 16·tg + 15 of each 64 of a query at the position `pos`,
+// rotated, by four lanes together.
+template <int D>
+__device__ __forceinline__ void rotate16(float (&x)[D / 64][16], const Kv8Args& a, int pos, int tg) {
+  constexpr int H2 = D / 64;
+  if (a.rope_mode == ROPE_NONE) return;
+  // a slot that holds nothing has no position; its scores are not used
+  const float2* cs = reinterpret_cast<const float2*>(a.rope) + int64_t(max(pos, 0)) * (D / 2);
+  if (a.rope_mode == ROPE_PAIRS) {
+#pragma unroll
+    for (int j = 0; j < H2; j++)
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const float2 f = cs[(64 * j + 16 * tg + e) / 2];
+        const float p = x[j][e], q = x[j][e + 1];
+        x[j][e] = __fmaf_rn(p, f.x, -__fmul_rn(q, f.y));
+        x[j][e + 1] = __fmaf_rn(p, f.y, __fmul_rn(q, f.x));
+      }
+  } else if (D == 64) {
+    // the partner is 32 values on: two lanes away
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      const float o = __shfl_xor_sync(FULL, x[0][e], 2);
+      const float2 f = cs[(16 * tg + e) & 31];
+      x[0][e] = __fmaf_rn(x[0][e], f.x, tg < 2 ? -__fmul_rn(o, f.y) : __fmul_rn(o, f.y));
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      const float2 f = cs[16 * tg + e];
+      const float p = x[0][e], q = x[H2 - 1][e];
+      x[0][e] = __fmaf_rn(p, f.x, -__fmul_rn(q, f.y));
+      x[H2 - 1][e] = __fmaf_rn(p, f.y, __fmul_rn(q, f.x));
+    }
+  }
+}
+
+constexpr float kQueryUnits = 4194304.f;  // a query's largest value
+
+// The largest magnitude of the values that four lanes hold, NaN where one is
+// not finite. `lanes`: those that take part.
+template <int D>
+__device__ __forceinline__ float group_amax(const float (&x)[D / 64][16], uint32_t lanes) {
+  float m = 0.f, nan = 0.f;
+#pragma unroll
+  for (int j = 0; j < D / 64; j++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      m = fmaxf(m, fabsf(x[j][e]));
+      nan = __fmaf_rn(0.f, x[j][e], nan);  // 0·inf and 0·NaN
+    }
+  m = __fadd_rn(m, nan);
+  const float a = __shfl_xor_sync(lanes, m, 1);
+  m = m > a || isnan(m) ? m : a;
+  const float b = __shfl_xor_sync(lanes, m, 2);
+  return m > b || isnan(m) ? m : b;
+}
+// The factor that makes the largest value kQueryUnits (0 for rows of zeros
+// or of no numbers); tiny rows are lifted first, so that it stays in range.
+template <int D>
+__device__ __forceinline__ float lift_row(float (&x)[D / 64][16], float amax) {
+  if (amax < 1e-30f) {
+    amax = __fmul_rn(amax, 1e30f);
+#pragma unroll
+    for (int j = 0; j < D / 64; j++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) x[j][e] = __fmul_rn(x[j][e], 1e30f);
+  }
+  return amax > 0.f ? __fdiv_rn(kQueryUnits, amax) : 0.f;
+}
+// n + 1.5·2^23 → n's three signed digits in base 256, a byte each: with 128
+// added to every digit they are the bytes of n + 0x808080.
+__device__ __forceinline__ uint32_t digits_of(float y) {
+  return (__float_as_uint(y) - MAGIC_BITS + 0x808080u) ^ 0x808080u;
+}
+// Byte `at` of four words.
+__device__ __forceinline__ uint32_t take_bytes(const uint32_t* n, int at) {
+  const uint32_t pick = at | (at + 4) << 4;
+  return __byte_perm(__byte_perm(n[0], n[1], pick), __byte_perm(n[2], n[3], pick), 0x5410);
+}
+
+__device__ __forceinline__ void put(const Kv8Attend& t, int type, int64_t at, float y) {
+  void* op = const_cast<void*>(t.out.p);
+  if (type == 0)
+    static_cast<float*>(op)[at] = y;
+  else if (type == 1)
+    static_cast<__half*>(op)[at] = __float2half_rn(y);
+  else
+    static_cast<__nv_bfloat16*>(op)[at] = __float2bfloat16_rn(y);
+}
+__device__ __forceinline__ float lse_of(float top, float sum) {
+  return sum == 0.f ? ninf() : __fmaf_rn(top, 0.693147181f, logf(sum));
+}
+
+
+// Whether groups of `count` elements of rows that begin at p with these
+// strides lie at multiples of their size.
+template <class T>
+bool aligned(const Kv8Rows& r, int count) {
+  const uintptr_t b = sizeof(T) * count;
+  return reinterpret_cast<uintptr_t>(r.p) % b == 0 && (r.row * sizeof(T)) % b == 0 && (r.head * sizeof(T)) % b == 0;
+}
+
+}  // namespace
+
+}  // namespace grx

@@ -91,6 +91,10 @@ cudaError_t launch_kv8_attend(const Kv8Args& a, int head_dim, int type, const Kv
 // the other (a is the first).
 cudaError_t launch_kv8_copy_pages(const Kv8Args& a, int head_dim, int layers, const int* from, const int* to, int count,
                                   cudaStream_t st);
+// launch_kv8_attend's form for many queries of a sequence to a key head
+// (k_kv8_prompt.cu).
+cudaError_t launch_kv8_prompt(const Kv8Args& a, int head_dim, int type, const Kv8Attend& t, cudaStream_t st);
+void kv8_prompt_init();
 void kv8_kernels_init();
 
 }  // namespace grx
