@@ -142,8 +142,9 @@ struct Prompt {
   static constexpr int threads = 288;
   // shared memory: bytes of the two halves of Q, of a tile's keys and values
   static constexpr int q = kRows * D * 2, k = kKeys * D * 2, v = D * kKeys * 2;
-  static constexpr int off_k = 2 * q, off_v = off_k + 2 * k, off_s = off_v + 2 * v;  // scales: [2][4] pairs
-  static constexpr int off_f = off_s + 2 * 4 * 8, off_bar = off_f + kRows * 4, used = off_bar + 8 * 8 + 16;
+  static constexpr int stages = 3;  // tiles of operands
+  static constexpr int off_k = 2 * q, off_v = off_k + stages * k, off_s = off_v + stages * v;  // scales: [4][4] pairs
+  static constexpr int off_f = off_s + 4 * 4 * 8, off_bar = off_f + kRows * 4, used = off_bar + 12 * 8 + 16;
   // TMEM columns: two score tiles, two weight tiles, the outputs
   static constexpr int c_p = 2 * kKeys, c_o = c_p + 2 * NP * kKeys / 2, columns = c_o + D <= 256 ? 256 : 512;
   // Blocks that share an SM fit in its 512 columns together: one, or two.
@@ -159,15 +160,20 @@ __global__ void __launch_bounds__(288, 1)
   extern __shared__ uint8_t raw_smem[];
   const uint32_t raw = smem_at(raw_smem), base = (raw + 1023) & ~1023u;
   uint8_t* mem = raw_smem + (base - raw);
-  float2* scales = reinterpret_cast<float2*>(mem + C::off_s);  // [stage][16 keys]
+  float2* scales = reinterpret_cast<float2*>(mem + C::off_s);  // [tile & 3][sixteen keys]
   float* rowf = reinterpret_cast<float*>(mem + C::off_f);
   const uint32_t bars = base + C::off_bar;
-  const auto conv = [&](int b) { return bars + 8 * b; };         // a tile's operands are in stage b
-  const auto scored = [&](int b) { return bars + 8 * (2 + b); };  // its scores are in S b
-  const auto weighed = [&](int b) { return bars + 8 * (4 + b); }; // its weights are in P b
-  const auto added = [&](int b) { return bars + 8 * (6 + b); };   // its outputs are in O
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mem + C::off_bar + 64);
-  volatile int* dead = reinterpret_cast<volatile int*>(mem + C::off_bar + 68);
+  // Barriers of tile j, and the parity that they end with: its operands and
+  // scales are in shared memory; its scores in S j & 1; its weights in P j & 1;
+  // its outputs in O. No role is four tiles ahead of another.
+  const auto conv = [&](int j) { return bars + 8 * (j & 3); };
+  const auto added = [&](int j) { return bars + 8 * (4 + (j & 3)); };
+  const auto scored = [&](int j) { return bars + 8 * (8 + (j & 1)); };
+  const auto weighed = [&](int j) { return bars + 8 * (10 + (j & 1)); };
+  const auto of4 = [](int j) { return uint32_t(j >> 2) & 1u; };
+  const auto of2 = [](int j) { return uint32_t(j >> 1) & 1u; };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mem + C::off_bar + 96);
+  volatile int* dead = reinterpret_cast<volatile int*>(mem + C::off_bar + 100);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   // heads of one tile side by side, the last queries (the most keys) first
@@ -188,11 +194,13 @@ __global__ void __launch_bounds__(288, 1)
 
   if (tid == 0) {
     *dead = 0;
-    for (int b = 0; b < 2; b++) {
-      bar_init(conv(b), 4);
-      bar_init(scored(b), 1);
-      bar_init(weighed(b), 4);
-      bar_init(added(b), 1);
+    for (int j = 0; j < 4; j++) {
+      bar_init(conv(j), 4);
+      bar_init(added(j), 1);
+    }
+    for (int j = 0; j < 2; j++) {
+      bar_init(scored(j), 1);
+      bar_init(weighed(j), 4);
     }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
@@ -272,14 +280,14 @@ __global__ void __launch_bounds__(288, 1)
 #pragma unroll
         for (int kk = 0; kk < kKeys / 16; kk++)
           mma_ts(tmem + C::c_o, tmem + C::c_p + (b * NP + n) * (kKeys / 2) + kk * 8,
-                 operand(base + C::off_v + b * C::v + kk * 32), idesc_o, j > 0 || n > 0 || kk > 0);
-      commit(added(b));
+                 operand(base + C::off_v + j % C::stages * C::v + kk * 32), idesc_o, j > 0 || n > 0 || kk > 0);
+      commit(added(j));
     };
     int done = 0;
     bool ok = true;
     for (int j = 0; j < nt && ok; j++) {
       const int b = j & 1;
-      ok = bar_wait(conv(b), (j >> 1) & 1, dead);
+      ok = bar_wait(conv(j), of4(j), dead);
       if (!ok) break;
       fence_after();
 #pragma unroll
@@ -287,15 +295,16 @@ __global__ void __launch_bounds__(288, 1)
 #pragma unroll
         for (int kk = 0; kk < D / 16; kk++)
           mma_ss(tmem + b * kKeys, operand(base + n * C::q + (kk / 4) * (kRows * 128) + (kk % 4) * 32),
-                 operand(base + C::off_k + b * C::k + (kk / 4) * (kKeys * 128) + (kk % 4) * 32), idesc_s,
+                 operand(base + C::off_k + j % C::stages * C::k + (kk / 4) * (kKeys * 128) + (kk % 4) * 32),
+                 idesc_s,
                  n > 0 || kk > 0);
-      commit(scored(b));
+      commit(scored(j));
       if (j > 0) {
-        ok = bar_wait(weighed(b ^ 1), ((j - 1) >> 1) & 1, dead);
+        ok = bar_wait(weighed(j - 1), of2(j - 1), dead);
         if (ok) outputs(j - 1), done = j;
       }
     }
-    if (ok && nt > 0 && bar_wait(weighed((nt - 1) & 1), ((nt - 1) >> 1) & 1, dead)) outputs(nt - 1), done = nt;
+    if (ok && nt > 0 && bar_wait(weighed(nt - 1), of2(nt - 1), dead)) outputs(nt - 1), done = nt;
     if (done < nt && nt > 0) {
       // given up: what was issued ends before the TMEM is released
       commit(added(0));
@@ -308,55 +317,81 @@ __global__ void __launch_bounds__(288, 1)
     const int ct = tid - 128;  // 0 .. 127
     constexpr int KU = D / 32;  // sixteen-byte units of keys a thread
     constexpr int VU = D / 64;  // units of eight tokens by four values
-    const int cshift = a.plog, plast = (sp.len + (1 << a.plog) - 1) >> a.plog;
     const int64_t pbytes = int64_t(a.heads << a.plog) * D;
     const int8_t* kh = a.k + (int64_t(h) << a.plog) * D;
     const int8_t* vh = a.v + (int64_t(h) << a.plog) * D;
-    // where token key of the sequence lies (some page's bytes where there is none)
-    const auto where = [&](int key) {
-      const int b = key >> cshift;
-      const int page = b < plast ? kv8_page(a, i, b) : -1;
-      return int64_t(max(page, 0)) * pbytes + int64_t(key & ((1 << a.plog) - 1)) * D;
+    // lane l holds page and scales of the sixteen keys 16·(base + l) .., eight
+    // tiles at a time, and the pages of the next eight
+    const int plast = (sp.len + 15) >> 4;
+    const auto page_of = [&](int c) { return c < plast ? kv8_page(a, i, c >> (a.plog - 4)) : -1; };
+    // −inf where there is no page, NaN for what is no scale
+    const auto scale_of = [&](int page) {
+      if (page < 0) return make_float2(ninf(), 0.f);
+      const float2 s = reinterpret_cast<const float2*>(a.scale)[int64_t(page) * a.heads + h];
+      return make_float2(isfinite(s.x) ? s.x : qnan(), s.y >= 0.f && isfinite(s.y) ? s.y : qnan());
     };
+    int c0 = tb * 4, page = page_of(c0 + lane), ahead = page_of(c0 + 32 + lane);
+    if (page < 0 && c0 + lane < plast && c0 + lane <= pmax >> 4) report(a);
+    float2 scale = scale_of(page), next_scale = scale;
+    int64_t at16[4];  // where the next tile's four groups of sixteen keys lie (some page's bytes where there is none)
     uint4 kr[KU];
     uint32_t vr[VU][8];
-    float2 sc = make_float2(0.f, 0.f);
+    float2 sc;
     const auto load = [&](int j) {
-      const int key0 = (tb + j) * kKeys;
+      const int c = (tb + j) * 4;
+      if (c - c0 == 32) {
+        c0 += 32;
+        page = ahead;
+        if (page < 0 && c0 + lane < plast && c0 + lane <= pmax >> 4) report(a);
+        scale = scale_of(page);
+        ahead = page_of(c0 + 32 + lane);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int pg = __shfl_sync(FULL, page, c - c0 + u);
+        at16[u] = int64_t(max(pg, 0)) * pbytes + ((c + u) * 16 & ((1 << a.plog) - 1)) * D;
+      }
+      next_scale.x = __shfl_sync(FULL, scale.x, c - c0 + (lane & 3));
+      next_scale.y = __shfl_sync(FULL, scale.y, c - c0 + (lane & 3));
 #pragma unroll
       for (int u = 0; u < KU; u++) {
-        const int n = ct + 128 * u;  // unit: key n / (D/16), sixteen values n % (D/16)
-        kr[u] = __ldg(reinterpret_cast<const uint4*>(kh + where(key0 + n / (D / 16)) + n % (D / 16) * 16));
+        const int n = ct + 128 * u, key = n / (D / 16);  // unit: key, sixteen values n % (D/16)
+        // (128·u keys on: the group is known when this is compiled, but for D = 64's two)
+        const int64_t at = D == 128 ? at16[u] : key & 16 ? at16[2 * u + 1] : at16[2 * u];
+        kr[u] = __ldg(reinterpret_cast<const uint4*>(kh + at + (key & 15) * D + n % (D / 16) * 16));
       }
 #pragma unroll
       for (int u = 0; u < VU; u++) {
-        const int n = ct + 128 * u;  // unit: tokens 8·(n / (D/4)) .., values 4·(n % (D/4)) ..
-        const int8_t* from = vh + where(key0 + 8 * (n / (D / 4))) + n % (D / 4) * 4;
+        const int n = ct + 128 * u, grp = n / (D / 4);  // unit: tokens 8·grp .., values 4·(n % (D/4)) ..
+        const int g16 = grp >> 1;
+        const int64_t at = D == 128 ? (g16 & 1 ? at16[2 * u + 1] : at16[2 * u])
+                                    : (g16 & 2 ? (g16 & 1 ? at16[3] : at16[2]) : (g16 & 1 ? at16[1] : at16[0]));
+        const int8_t* from = vh + at + (grp & 1) * 8 * D + n % (D / 4) * 4;
 #pragma unroll
         for (int e = 0; e < 8; e++) vr[u][e] = __ldg(reinterpret_cast<const uint32_t*>(from + e * D));
-      }
-      if (ct < 4) {  // sixteen keys' scales: −inf where there is no page, NaN for what is no scale
-        const int b = (key0 + 16 * ct) >> cshift, page = b < plast ? kv8_page(a, i, b) : -1;
-        if (page < 0) {
-          if (b < plast) report(a);
-          sc = make_float2(ninf(), 0.f);
-        } else {
-          const float2 s = reinterpret_cast<const float2*>(a.scale)[int64_t(page) * a.heads + h];
-          sc = make_float2(isfinite(s.x) ? s.x : qnan(), s.y >= 0.f && isfinite(s.y) ? s.y : qnan());
-        }
       }
     };
     if (nt > 0) load(0);
     for (int j = 0; j < nt; j++) {
-      const int b = j & 1;
-      if (j > 1 && !bar_wait(added(b), ((j - 2) >> 1) & 1, dead)) break;
-      if (ct < 4) scales[b * 4 + ct] = sc;
+      uint4 kc[KU];
+      uint32_t vc[VU][8];
+#pragma unroll
+      for (int u = 0; u < KU; u++) kc[u] = kr[u];
+#pragma unroll
+      for (int u = 0; u < VU; u++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) vc[u][e] = vr[u][e];
+      sc = next_scale;
+      if (j + 1 < nt) load(j + 1);
+      if (j >= C::stages && !bar_wait(added(j - C::stages), of4(j - C::stages), dead)) break;
+      const uint32_t kst = base + C::off_k + j % C::stages * C::k, vst = base + C::off_v + j % C::stages * C::v;
+      if (ct < 4) scales[(j & 3) * 4 + ct] = sc;
 #pragma unroll
       for (int u = 0; u < KU; u++) {
         const int n = ct + 128 * u, key = n / (D / 16), c = n % (D / 16);  // values 16c .. : chunks 2c and 2c + 1
-        const uint32_t at = base + C::off_k + b * C::k + (c / 4) * (kKeys * 128) + key * 128;
+        const uint32_t at = kst + (c / 4) * (kKeys * 128) + key * 128;
         const int swap = D == 128 ? c >> 2 & 1 : key & 1;  // neighbours write different banks
-        const uint32_t w[4] = {kr[u].x, kr[u].y, kr[u].z, kr[u].w};
+        const uint32_t w[4] = {kc[u].x, kc[u].y, kc[u].z, kc[u].w};
 #pragma unroll
         for (int e = 0; e < 2; e++) {
           const int s = e ^ swap;
@@ -368,21 +403,20 @@ __global__ void __launch_bounds__(288, 1)
 #pragma unroll
       for (int u = 0; u < VU; u++) {
         const int n = ct + 128 * u, grp = n / (D / 4), w = n % (D / 4);
-        const uint32_t at = base + C::off_v + b * C::v + 4 * w * 128;
+        const uint32_t at = vst + 4 * w * 128;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const int v = (e + (w >> 1)) & 3;  // the order in which neighbours write different banks
           const uint32_t pick = v | (4 + v) << 8;
           uint32_t y[4];
 #pragma unroll
-          for (int m = 0; m < 4; m++) y[m] = to_f16(__byte_perm(vr[u][2 * m], vr[u][2 * m + 1], pick) & 0x00ff00ffu);
+          for (int m = 0; m < 4; m++) y[m] = to_f16(__byte_perm(vc[u][2 * m], vc[u][2 * m + 1], pick) & 0x00ff00ffu);
           sts16(at + v * 128 + (grp ^ ((4 * w + v) & 7)) * 16, y[0], y[1], y[2], y[3]);
         }
       }
-      if (j + 1 < nt) load(j + 1);
       fence_async();
       __syncwarp();
-      if (lane == 0) bar_arrive(conv(b));
+      if (lane == 0) bar_arrive(conv(j));
     }
   } else {
     // ---- the rows
@@ -398,7 +432,7 @@ __global__ void __launch_bounds__(288, 1)
     bool ok = true;
     for (int j = 0; j < nt; j++) {
       const int b = j & 1, key0 = (tb + j) * kKeys;
-      ok = bar_wait(conv(b), (j >> 1) & 1, dead) && bar_wait(scored(b), (j >> 1) & 1, dead);
+      ok = bar_wait(conv(j), of4(j), dead) && bar_wait(scored(j), of2(j), dead);
       if (!ok) break;
       fence_after();
       uint32_t s[kKeys];
@@ -408,7 +442,7 @@ __global__ void __launch_bounds__(288, 1)
       bool gone = false;
 #pragma unroll
       for (int u = 0; u < 4; u++) {
-        const float2 c = scales[b * 4 + u];
+        const float2 c = scales[(j & 3) * 4 + u];
         gone = gone || c.x == ninf();
         sk[u] = c.x;
         sv[u] = c.y;
@@ -452,7 +486,7 @@ __global__ void __launch_bounds__(288, 1)
           k = __fmul_rn(k, up);
         }
         if (j > 0) {
-          ok = bar_wait(added(b ^ 1), ((j - 1) >> 1) & 1, dead);
+          ok = bar_wait(added(j - 1), of4(j - 1), dead);
           if (!ok) break;
           fence_after();
 #pragma unroll 1
@@ -488,7 +522,7 @@ __global__ void __launch_bounds__(288, 1)
           if (key0 + e < lo || key0 + e > p || sk[e / 16] == ninf()) x[e] = 0.f;
       }
       if (j > 1) {
-        ok = bar_wait(added(b), ((j - 2) >> 1) & 1, dead);  // P b is free
+        ok = bar_wait(added(j - 2), of4(j - 2), dead);  // P b is free
         if (!ok) break;
       }
 #pragma unroll
@@ -507,9 +541,9 @@ __global__ void __launch_bounds__(288, 1)
       wait_st();
       fence_before();
       __syncwarp();
-      if (lane == 0) bar_arrive(weighed(b));
+      if (lane == 0) bar_arrive(weighed(j));
     }
-    if (ok && nt > 0) ok = bar_wait(added((nt - 1) & 1), ((nt - 1) >> 1) & 1, dead);
+    if (ok && nt > 0) ok = bar_wait(added(nt - 1), of4(nt - 1), dead);
     if (ok) {
       fence_after();
       const float inv = l == 0.f ? 0.f : __fdiv_rn(W, l);
