@@ -4,27 +4,25 @@
 //
 // A block takes 128 query rows (token by token, the heads of a group side by
 // side) against tiles of 64 keys, one pass with the running maximum and sum:
-//  * warps 4-7 turn a tile's bytes into float16 operands (exact): the keys as
-//    they lie, [key][value], the values turned, [value][key], both in the
+//  * warps 8-15 turn a tile's bytes into float16 operands (exact): the keys
+//    as they lie, [key][value], the values turned, [value][key], both in the
 //    128-byte swizzle that the tensor core reads; the next tile's bytes come
 //    into registers meanwhile;
-//  * warp 8 issues the products: scores S = Q·Kᵀ into one of two TMEM tiles,
+//  * warp 16 issues the products: scores S = Q·Kᵀ into one of two TMEM tiles,
 //    Q being the sum of two float16s of a row scaled to 2^14 (22 bits and
 //    more: 32-bit scores), and O += P·V with P from TMEM, one float16 for
 //    16-bit outputs and the sum of two for float32 ones. The scores of tile
 //    j + 1 are issued ahead of the outputs of tile j;
-//  * warps 0-3, a row a thread: a row's 64 scores from TMEM, weights
+//  * warps 0-7, two threads a row: 32 of a row's 64 scores from TMEM, weights
 //    p·s_v/W, written back as P. The maximum moves only when a score passes
 //    it by 2^8; then, and when a larger value scale comes, the row of O in
-//    TMEM is multiplied.
+//    TMEM is multiplied. The two threads of a row exchange their maxima in
+//    shared memory.
 // Blocks with the most keys start first. Every wait is bounded (about a
 // second of clocks); one that runs out sets the block's `dead` word, every
 // role leaves its loop, the block frees its TMEM, and the status word gets
 // GRX_ETIMEDOUT.
 //
-// What bounds it is the exponentials and the rows' instructions between two
-// tiles' products (64 of each a thread and tile); the products take about
-// 800 clocks a tile of 128 x 64 at 128 values.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -127,6 +125,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t* d) {
       "r"(d[28]), "r"(d[29]), "r"(d[30]), "r"(d[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* d) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(at),
+      "r"(d[0]), "r"(d[1]), "r"(d[2]), "r"(d[3]), "r"(d[4]), "r"(d[5]), "r"(d[6]), "r"(d[7]), "r"(d[8]), "r"(d[9]),
+      "r"(d[10]), "r"(d[11]), "r"(d[12]), "r"(d[13]), "r"(d[14]), "r"(d[15])
+      : "memory");
+}
 __device__ __forceinline__ uint32_t to_f16(uint32_t u) {
   uint32_t d;
   asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(u ^ 0x64806480u), "r"(0xe480e480u));
@@ -139,12 +144,13 @@ __device__ __forceinline__ void sts16(uint32_t at, uint32_t a, uint32_t b, uint3
 // NP: float16s of a weight.
 template <int D, int NP>
 struct Prompt {
-  static constexpr int threads = 288;
+  static constexpr int threads = 544;
   // shared memory: bytes of the two halves of Q, of a tile's keys and values
   static constexpr int q = kRows * D * 2, k = kKeys * D * 2, v = D * kKeys * 2;
   static constexpr int stages = 3;  // tiles of operands
   static constexpr int off_k = 2 * q, off_v = off_k + stages * k, off_s = off_v + stages * v;  // scales: [4][4] pairs
-  static constexpr int off_f = off_s + 4 * 4 * 8, off_bar = off_f + kRows * 4, used = off_bar + 12 * 8 + 16;
+  static constexpr int off_f = off_s + 4 * 4 * 8, off_x = off_f + kRows * 4;  // rows' factors; exchanged [2][2][rows]
+  static constexpr int off_bar = off_x + 4 * kRows * 4, used = off_bar + 20 * 8 + 16;
   // TMEM columns: two score tiles, two weight tiles, the outputs
   static constexpr int c_p = 2 * kKeys, c_o = c_p + 2 * NP * kKeys / 2, columns = c_o + D <= 256 ? 256 : 512;
   // Blocks that share an SM fit in its 512 columns together: one, or two.
@@ -153,7 +159,7 @@ struct Prompt {
 };
 
 template <int D, int NP>
-__global__ void __launch_bounds__(288, 1)
+__global__ void __launch_bounds__(544, 1)
     k_kv8_prompt(Kv8Args a, Kv8Attend t, int type, int qtiles, bool vec, bool ovec) {
   using C = Prompt<D, NP>;
   constexpr int H2 = D / 64;
@@ -162,6 +168,7 @@ __global__ void __launch_bounds__(288, 1)
   uint8_t* mem = raw_smem + (base - raw);
   float2* scales = reinterpret_cast<float2*>(mem + C::off_s);  // [tile & 3][sixteen keys]
   float* rowf = reinterpret_cast<float*>(mem + C::off_f);
+  float* tops = reinterpret_cast<float*>(mem + C::off_x);  // [tile & 1][half][row]
   const uint32_t bars = base + C::off_bar;
   // Barriers of tile j, and the parity that they end with: its operands and
   // scales are in shared memory; its scores in S j & 1; its weights in P j & 1;
@@ -172,8 +179,9 @@ __global__ void __launch_bounds__(288, 1)
   const auto weighed = [&](int j) { return bars + 8 * (10 + (j & 1)); };
   const auto of4 = [](int j) { return uint32_t(j >> 2) & 1u; };
   const auto of2 = [](int j) { return uint32_t(j >> 1) & 1u; };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mem + C::off_bar + 96);
-  volatile int* dead = reinterpret_cast<volatile int*>(mem + C::off_bar + 100);
+  const auto pair = [&](int q, int j) { return bars + 8 * (12 + 2 * q + (j & 1)); };  // both halves of rows 32q ..
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mem + C::off_bar + 160);
+  volatile int* dead = reinterpret_cast<volatile int*>(mem + C::off_bar + 164);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   // heads of one tile side by side, the last queries (the most keys) first
@@ -195,16 +203,17 @@ __global__ void __launch_bounds__(288, 1)
   if (tid == 0) {
     *dead = 0;
     for (int j = 0; j < 4; j++) {
-      bar_init(conv(j), 4);
+      bar_init(conv(j), 8);
       bar_init(added(j), 1);
     }
     for (int j = 0; j < 2; j++) {
       bar_init(scored(j), 1);
-      bar_init(weighed(j), 4);
+      bar_init(weighed(j), 8);
+      for (int q = 0; q < 4; q++) bar_init(pair(q, j), 2);
     }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  if (warp == 8) {
+  if (warp == 16) {
     asm volatile(
         "tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n"
         "tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::"r"(smem_at(tmem_slot)),
@@ -213,11 +222,11 @@ __global__ void __launch_bounds__(288, 1)
   }
 
   // --- the queries: rotated, scaled, as the sum of two float16s; four lanes
-  // to a row, warps 0-7 eight rows at a time ---
-  if (warp < 8) {
+  // to a row, eight rows to a warp ---
+  const auto queries = [&]() {
     const int g = lane >> 2, tg = lane & 3;
-#pragma unroll 1
-    for (int r = warp * 8 + g; r < kRows; r += 64) {
+    {
+      const int r = warp * 8 + g;
       const bool there = r < nrow;
       const int tq = there ? (r0 + r) / group : 0, hq = h * group + (there ? (r0 + r) % group : 0);
       float x[H2][16];
@@ -262,13 +271,18 @@ __global__ void __launch_bounds__(288, 1)
         rowf[r] = __fmul_rn(__fmul_rn(amax, 256.f / kQueryUnits), __fmul_rn(t.scale, 1.44269504f));
     }
     fence_async();
-  }
-  fence_before();
-  __syncthreads();
-  fence_after();
-  const uint32_t tmem = *tmem_slot;
+  };
+  // the set-up is done: barriers, TMEM, queries
+  uint32_t tmem = 0;
+  const auto ready = [&]() {
+    fence_before();
+    __syncthreads();
+    fence_after();
+    tmem = *tmem_slot;
+  };
 
-  if (warp == 8) {
+  if (warp == 16) {
+    ready();
     // ---- the products
     const uint32_t idesc_s = (1u << 4) | (uint32_t(kKeys >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
     const uint32_t idesc_o = (1u << 4) | (uint32_t(D >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
@@ -312,11 +326,11 @@ __global__ void __launch_bounds__(288, 1)
       while (clock64() - t0 < (1LL << 24)) {
       }
     }
-  } else if (warp >= 4) {
+  } else if (warp >= 8) {
     // ---- a tile's operands
-    const int ct = tid - 128;  // 0 .. 127
-    constexpr int KU = D / 32;  // sixteen-byte units of keys a thread
-    constexpr int VU = D / 64;  // units of eight tokens by four values
+    const int ct = tid - 256;  // 0 .. 255
+    constexpr int KU = D / 64;  // sixteen-byte units of keys a thread
+    const bool turns = D == 128 || ct < 128;  // has a unit of eight tokens by four values
     const int64_t pbytes = int64_t(a.heads << a.plog) * D;
     const int8_t* kh = a.k + (int64_t(h) << a.plog) * D;
     const int8_t* vh = a.v + (int64_t(h) << a.plog) * D;
@@ -332,66 +346,55 @@ __global__ void __launch_bounds__(288, 1)
     };
     int c0 = tb * 4, page = page_of(c0 + lane), ahead = page_of(c0 + 32 + lane);
     if (page < 0 && c0 + lane < plast && c0 + lane <= pmax >> 4) report(a);
-    float2 scale = scale_of(page), next_scale = scale;
-    int64_t at16[4];  // where the next tile's four groups of sixteen keys lie (some page's bytes where there is none)
-    uint4 kr[KU];
-    uint32_t vr[VU][8];
-    float2 sc;
-    const auto load = [&](int j) {
+    float2 scale = scale_of(page), scale_ahead = scale;
+    struct Bytes {
+      uint4 k[KU];
+      uint32_t v[8];
+      float2 scale;
+    } one, two;  // two tiles' bytes are under way: a tile takes less than a load's way to memory
+    const auto load = [&](int j, Bytes& to) {
+      int64_t at16[4];  // where the tile's four groups of sixteen keys lie (some page's bytes where there is none)
       const int c = (tb + j) * 4;
       if (c - c0 == 32) {
         c0 += 32;
         page = ahead;
         if (page < 0 && c0 + lane < plast && c0 + lane <= pmax >> 4) report(a);
-        scale = scale_of(page);
+        scale = scale_ahead;
         ahead = page_of(c0 + 32 + lane);
       }
+      if (c - c0 == 16) scale_ahead = scale_of(ahead);
 #pragma unroll
       for (int u = 0; u < 4; u++) {
         const int pg = __shfl_sync(FULL, page, c - c0 + u);
         at16[u] = int64_t(max(pg, 0)) * pbytes + ((c + u) * 16 & ((1 << a.plog) - 1)) * D;
       }
-      next_scale.x = __shfl_sync(FULL, scale.x, c - c0 + (lane & 3));
-      next_scale.y = __shfl_sync(FULL, scale.y, c - c0 + (lane & 3));
+      to.scale.x = __shfl_sync(FULL, scale.x, c - c0 + (lane & 3));
+      to.scale.y = __shfl_sync(FULL, scale.y, c - c0 + (lane & 3));
 #pragma unroll
       for (int u = 0; u < KU; u++) {
-        const int n = ct + 128 * u, key = n / (D / 16);  // unit: key, sixteen values n % (D/16)
-        // (128·u keys on: the group is known when this is compiled, but for D = 64's two)
-        const int64_t at = D == 128 ? at16[u] : key & 16 ? at16[2 * u + 1] : at16[2 * u];
-        kr[u] = __ldg(reinterpret_cast<const uint4*>(kh + at + (key & 15) * D + n % (D / 16) * 16));
-      }
-#pragma unroll
-      for (int u = 0; u < VU; u++) {
-        const int n = ct + 128 * u, grp = n / (D / 4);  // unit: tokens 8·grp .., values 4·(n % (D/4)) ..
-        const int g16 = grp >> 1;
+        const int n = ct + 256 * u, key = n / (D / 16), g16 = key >> 4;  // unit: key, sixteen values n % (D/16)
         const int64_t at = D == 128 ? (g16 & 1 ? at16[2 * u + 1] : at16[2 * u])
                                     : (g16 & 2 ? (g16 & 1 ? at16[3] : at16[2]) : (g16 & 1 ? at16[1] : at16[0]));
-        const int8_t* from = vh + at + (grp & 1) * 8 * D + n % (D / 4) * 4;
+        to.k[u] = __ldg(reinterpret_cast<const uint4*>(kh + at + (key & 15) * D + n % (D / 16) * 16));
+      }
+      if (turns) {
+        const int grp = ct / (D / 4), g16 = grp >> 1;  // unit: tokens 8·grp .., values 4·(ct % (D/4)) ..
+        const int64_t at = g16 & 2 ? (g16 & 1 ? at16[3] : at16[2]) : (g16 & 1 ? at16[1] : at16[0]);
+        const int8_t* from = vh + at + (grp & 1) * 8 * D + ct % (D / 4) * 4;
 #pragma unroll
-        for (int e = 0; e < 8; e++) vr[u][e] = __ldg(reinterpret_cast<const uint32_t*>(from + e * D));
+        for (int e = 0; e < 8; e++) to.v[e] = __ldg(reinterpret_cast<const uint32_t*>(from + e * D));
       }
     };
-    if (nt > 0) load(0);
-    for (int j = 0; j < nt; j++) {
-      uint4 kc[KU];
-      uint32_t vc[VU][8];
-#pragma unroll
-      for (int u = 0; u < KU; u++) kc[u] = kr[u];
-#pragma unroll
-      for (int u = 0; u < VU; u++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) vc[u][e] = vr[u][e];
-      sc = next_scale;
-      if (j + 1 < nt) load(j + 1);
-      if (j >= C::stages && !bar_wait(added(j - C::stages), of4(j - C::stages), dead)) break;
+    const auto turn = [&](int j, Bytes& in) {
+      if (j >= C::stages && !bar_wait(added(j - C::stages), of4(j - C::stages), dead)) return false;
       const uint32_t kst = base + C::off_k + j % C::stages * C::k, vst = base + C::off_v + j % C::stages * C::v;
-      if (ct < 4) scales[(j & 3) * 4 + ct] = sc;
+      if (ct < 4) scales[(j & 3) * 4 + ct] = in.scale;
 #pragma unroll
       for (int u = 0; u < KU; u++) {
-        const int n = ct + 128 * u, key = n / (D / 16), c = n % (D / 16);  // values 16c .. : chunks 2c and 2c + 1
+        const int n = ct + 256 * u, key = n / (D / 16), c = n % (D / 16);  // values 16c .. : chunks 2c and 2c + 1
         const uint32_t at = kst + (c / 4) * (kKeys * 128) + key * 128;
         const int swap = D == 128 ? c >> 2 & 1 : key & 1;  // neighbours write different banks
-        const uint32_t w[4] = {kc[u].x, kc[u].y, kc[u].z, kc[u].w};
+        const uint32_t w[4] = {in.k[u].x, in.k[u].y, in.k[u].z, in.k[u].w};
 #pragma unroll
         for (int e = 0; e < 2; e++) {
           const int s = e ^ swap;
@@ -400,9 +403,8 @@ __global__ void __launch_bounds__(288, 1)
                 to_f16(__byte_perm(x, 0, 0x4342)), to_f16(__byte_perm(y, 0, 0x4140)), to_f16(__byte_perm(y, 0, 0x4342)));
         }
       }
-#pragma unroll
-      for (int u = 0; u < VU; u++) {
-        const int n = ct + 128 * u, grp = n / (D / 4), w = n % (D / 4);
+      if (turns) {
+        const int grp = ct / (D / 4), w = ct % (D / 4);
         const uint32_t at = vst + 4 * w * 128;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -410,66 +412,73 @@ __global__ void __launch_bounds__(288, 1)
           const uint32_t pick = v | (4 + v) << 8;
           uint32_t y[4];
 #pragma unroll
-          for (int m = 0; m < 4; m++) y[m] = to_f16(__byte_perm(vc[u][2 * m], vc[u][2 * m + 1], pick) & 0x00ff00ffu);
+          for (int m = 0; m < 4; m++) y[m] = to_f16(__byte_perm(in.v[2 * m], in.v[2 * m + 1], pick) & 0x00ff00ffu);
           sts16(at + v * 128 + (grp ^ ((4 * w + v) & 7)) * 16, y[0], y[1], y[2], y[3]);
         }
       }
       fence_async();
       __syncwarp();
       if (lane == 0) bar_arrive(conv(j));
-    }
+      if (j + 2 < nt) load(j + 2, in);
+      return true;
+    };
+    if (nt > 0) load(0, one);
+    if (nt > 1) load(1, two);
+    queries();
+    ready();
+    for (int j = 0; j < nt; j += 2)
+      if (!turn(j, one) || (j + 1 < nt && !turn(j + 1, two))) break;
   } else {
-    // ---- the rows
-    const int r = tid;
+    // ---- the rows: a thread has half of a row's keys, and of its outputs
+    queries();
+    ready();
+    const int quarter = warp & 3, half = warp >> 2, r = quarter * 32 + lane;
     const bool there = r < nrow;
     const int tq = there ? (r0 + r) / group : 0, hq = h * group + (there ? (r0 + r) % group : 0);
     const int p = there ? p0 + tq : pmax;
     const int lo = max(first, t.window > 0 ? p - t.window + 1 : 0);  // sees lo .. p
     const int in_lo = max(first, t.window > 0 ? pmax - t.window + 1 : 0);
     const float f = rowf[r];
-    const uint32_t lanes = tmem + (uint32_t(warp * 32) << 16);
+    constexpr int N = kKeys / 2;  // a thread's keys
+    const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16), mine = lanes + C::c_o + half * (D / 2);
     float ref = ninf(), l = 0.f, W = 0.f, toW = 0.f;
     bool ok = true;
     for (int j = 0; j < nt; j++) {
-      const int b = j & 1, key0 = (tb + j) * kKeys;
+      const int b = j & 1, key0 = (tb + j) * kKeys + half * N;
       ok = bar_wait(conv(j), of4(j), dead) && bar_wait(scored(j), of2(j), dead);
       if (!ok) break;
       fence_after();
-      uint32_t s[kKeys];
-      tmem_ld32(lanes + b * kKeys, s);
-      tmem_ld32(lanes + b * kKeys + 32, s + 32);
-      float sk[4], sv[4];
-      bool gone = false;
-#pragma unroll
-      for (int u = 0; u < 4; u++) {
-        const float2 c = scales[(j & 3) * 4 + u];
-        gone = gone || c.x == ninf();
-        sk[u] = c.x;
-        sv[u] = c.y;
-      }
+      uint32_t s[N];
+      tmem_ld32(lanes + b * kKeys + half * N, s);
+      const float2 c0 = scales[(j & 3) * 4 + 2 * half], c1 = scales[(j & 3) * 4 + 2 * half + 1];
+      const float2 d0 = scales[(j & 3) * 4 + 2 - 2 * half], d1 = scales[(j & 3) * 4 + 3 - 2 * half];
+      const float wide = fmaxf(fmaxf(c0.y, c1.y), fmaxf(d0.y, d1.y));
+      const bool edge = c0.x == ninf() || c1.x == ninf() || key0 < in_lo || key0 + N - 1 > pmin;
       wait_ld();
-      const bool edge = gone || key0 < in_lo || key0 + kKeys - 1 > pmin;
       f2* x2 = reinterpret_cast<f2*>(s);
       float* x = reinterpret_cast<float*>(s);
+      const f2 f0 = f2dup(__fmul_rn(f, c0.x)), f1 = f2dup(__fmul_rn(f, c1.x));
 #pragma unroll
-      for (int u = 0; u < 4; u++) {
-        const f2 c = f2dup(__fmul_rn(f, sk[u]));
-#pragma unroll
-        for (int e = 0; e < 8; e++) x2[8 * u + e] = f2mul(x2[8 * u + e], c);
-      }
+      for (int e = 0; e < N / 2; e++) x2[e] = f2mul(x2[e], e < N / 4 ? f0 : f1);
       if (edge) {
 #pragma unroll
-        for (int e = 0; e < kKeys; e++)
-          if (key0 + e < lo || key0 + e > p || sk[e / 16] == ninf()) x[e] = ninf();
+        for (int e = 0; e < N; e++)
+          if (key0 + e < lo || key0 + e > p || (e < N / 2 ? c0.x : c1.x) == ninf()) x[e] = ninf();
       }
       float top = x[0];
 #pragma unroll
-      for (int e = 1; e < kKeys; e++) top = fmaxf(top, x[e]);
-      float wide = sv[0];
-#pragma unroll
-      for (int u = 1; u < 4; u++) wide = fmaxf(wide, sv[u]);
+      for (int e = 1; e < N; e++) top = fmaxf(top, x[e]);
+      {
+        float* at = tops + (b * 2) * kRows + r;
+        at[half * kRows] = top;
+        __syncwarp();
+        if (lane == 0) bar_arrive(pair(quarter, j));
+        ok = bar_wait(pair(quarter, j), of2(j), dead);
+        if (!ok) break;
+        top = fmaxf(top, at[(half ^ 1) * kRows]);
+      }
       // the references move: a score 2^8 above the row's (any, before its
-      // first key), a larger value scale
+      // first key), a larger value scale; both halves alike
       const bool over = top > __fadd_rn(ref, 8.f);
       if (__any_sync(FULL, over) || wide > W) {
         float k = 1.f;
@@ -490,13 +499,13 @@ __global__ void __launch_bounds__(288, 1)
           if (!ok) break;
           fence_after();
 #pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
+          for (int c = 0; c < D / 2; c += 32) {
             uint32_t o[32];
-            tmem_ld32(lanes + C::c_o + c, o);
+            tmem_ld32(mine + c, o);
             wait_ld();
 #pragma unroll
             for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__fmul_rn(__uint_as_float(o[e]), k));
-            tmem_st32(lanes + C::c_o + c, o);
+            tmem_st32(mine + c, o);
           }
           wait_st();
         }
@@ -504,22 +513,19 @@ __global__ void __launch_bounds__(288, 1)
       const f2 m = f2dup(ref == ninf() ? 0.f : -ref);
       f2 sum = 0;
 #pragma unroll
-      for (int e = 0; e < kKeys / 2; e++) {
+      for (int e = 0; e < N / 2; e++) {
         const f2 y = f2add(x2[e], m);
         x2[e] = f2make(ex2(f2lo(y)), ex2(f2hi(y)));
         sum = f2add(sum, x2[e]);
       }
       l = __fadd_rn(l, __fadd_rn(f2lo(sum), f2hi(sum)));
+      const f2 w0 = f2dup(__fmul_rn(c0.y, toW)), w1 = f2dup(__fmul_rn(c1.y, toW));
 #pragma unroll
-      for (int u = 0; u < 4; u++) {
-        const f2 c = f2dup(__fmul_rn(sv[u], toW));
-#pragma unroll
-        for (int e = 0; e < 8; e++) x2[8 * u + e] = f2mul(x2[8 * u + e], c);
-      }
+      for (int e = 0; e < N / 2; e++) x2[e] = f2mul(x2[e], e < N / 4 ? w0 : w1);
       if (edge) {  // what is not seen counts nothing, whatever its page's scale
 #pragma unroll
-        for (int e = 0; e < kKeys; e++)
-          if (key0 + e < lo || key0 + e > p || sk[e / 16] == ninf()) x[e] = 0.f;
+        for (int e = 0; e < N; e++)
+          if (key0 + e < lo || key0 + e > p || (e < N / 2 ? c0.x : c1.x) == ninf()) x[e] = 0.f;
       }
       if (j > 1) {
         ok = bar_wait(added(j - 2), of4(j - 2), dead);  // P b is free
@@ -527,16 +533,16 @@ __global__ void __launch_bounds__(288, 1)
       }
 #pragma unroll
       for (int n = 0; n < NP; n++) {
-        uint32_t w[kKeys / 2];
+        uint32_t w[N / 2];
 #pragma unroll
-        for (int e = 0; e < kKeys / 2; e++) {
+        for (int e = 0; e < N / 2; e++) {
           w[e] = pack_f16(x[2 * e], x[2 * e + 1]);
           if (n + 1 < NP) {
             x[2 * e] = __fsub_rn(x[2 * e], __half2float(__ushort_as_half(w[e] & 0xffff)));
             x[2 * e + 1] = __fsub_rn(x[2 * e + 1], __half2float(__ushort_as_half(w[e] >> 16)));
           }
         }
-        tmem_st32(lanes + C::c_p + (b * NP + n) * (kKeys / 2), w);
+        tmem_st16(lanes + C::c_p + (b * NP + n) * (kKeys / 2) + half * (N / 2), w);
       }
       wait_st();
       fence_before();
@@ -545,11 +551,19 @@ __global__ void __launch_bounds__(288, 1)
     }
     if (ok && nt > 0) ok = bar_wait(added(nt - 1), of4(nt - 1), dead);
     if (ok) {
+      // the halves' sums together, by way of the maxima's place
+      tops[((nt & 1) * 2 + half) * kRows + r] = l;
+      __syncwarp();
+      if (lane == 0) bar_arrive(pair(quarter, nt));
+      ok = bar_wait(pair(quarter, nt), of2(nt), dead);
+    }
+    if (ok) {
       fence_after();
+      l = __fadd_rn(tops[(nt & 1) * 2 * kRows + r], tops[((nt & 1) * 2 + 1) * kRows + r]);
       const float inv = l == 0.f ? 0.f : __fdiv_rn(W, l);
       const int64_t at = int64_t(sp.row + tq) * t.out.row + int64_t(hq) * t.out.head;
 #pragma unroll 1
-      for (int c = 0; c < D; c += 32) {
+      for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
         uint32_t o[32];
         if (nt > 0) {
           tmem_ld32(lanes + C::c_o + c, o);
@@ -591,12 +605,12 @@ __global__ void __launch_bounds__(288, 1)
           t.q8s[to / QK] = make_float2(quant_scale(most), quant_scale(most));
         }
       }
-      if (there && t.lse) t.lse[int64_t(sp.row + tq) * t.heads + hq] = lse_of(ref, l);
+      if (there && half == 0 && t.lse) t.lse[int64_t(sp.row + tq) * t.heads + hq] = lse_of(ref, l);
     }
   }
   fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 16) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(C::columns) : "memory");
   }
