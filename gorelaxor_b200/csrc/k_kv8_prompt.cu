@@ -12,12 +12,13 @@
 //    Q being the sum of two float16s of a row scaled to 2^14 (22 bits and
 //    more: 32-bit scores), and O += P·V with P from TMEM, one float16 for
 //    16-bit outputs and the sum of two for float32 ones. The scores of tile
-//    j + 1 are issued ahead of the outputs of tile j;
-//  * warps 0-7, two threads a row: 32 of a row's 64 scores from TMEM, weights
-//    p·s_v/W, written back as P. The maximum moves only when a score passes
-//    it by 2^8; then, and when a larger value scale comes, the row of O in
-//    TMEM is multiplied. The two threads of a row exchange their maxima in
-//    shared memory.
+//    j + 2 are issued ahead of the outputs of tile j;
+//  * warps 0-3 take the even tiles and warps 4-7 the odd ones, a thread to a
+//    row and with a maximum, a sum and an O of their own, joined at the end:
+//    the scores' maximum from TMEM, the scores again, weights p·s_v/W,
+//    written back as P. The maximum moves only when a score passes it by 2^8;
+//    then, and when a larger value scale comes, the row of O in TMEM is
+//    multiplied. So one half's exponentials run while the other half waits.
 // Blocks with the most keys start first. Every wait is bounded (about a
 // second of clocks); one that runs out sets the block's `dead` word, every
 // role leaves its loop, the block frees its TMEM, and the status word gets
@@ -147,12 +148,12 @@ struct Prompt {
   static constexpr int threads = 544;
   // shared memory: bytes of the two halves of Q, of a tile's keys and values
   static constexpr int q = kRows * D * 2, k = kKeys * D * 2, v = D * kKeys * 2;
-  static constexpr int stages = 3;  // tiles of operands
+  static constexpr int stages = 4;  // tiles of operands
   static constexpr int off_k = 2 * q, off_v = off_k + stages * k, off_s = off_v + stages * v;  // scales: [4][4] pairs
-  static constexpr int off_f = off_s + 4 * 4 * 8, off_x = off_f + kRows * 4;  // rows' factors; exchanged [2][2][rows]
-  static constexpr int off_bar = off_x + 4 * kRows * 4, used = off_bar + 20 * 8 + 16;
+  static constexpr int off_f = off_s + 4 * 4 * 8, off_x = off_f + kRows * 4;  // rows' factors; the halves' {maximum, sum, W}
+  static constexpr int off_bar = off_x + 2 * 3 * kRows * 4, used = off_bar + 14 * 8 + 16;
   // TMEM columns: two score tiles, two weight tiles, the outputs
-  static constexpr int c_p = 2 * kKeys, c_o = c_p + 2 * NP * kKeys / 2, columns = c_o + D <= 256 ? 256 : 512;
+  static constexpr int c_p = 2 * kKeys, c_o = c_p + 2 * NP * kKeys / 2, columns = 512;
   // Blocks that share an SM fit in its 512 columns together: one, or two.
   static constexpr int room = columns == 512 ? 116 * 1024 : 78 * 1024;
   static constexpr int smem = 1024 + (used > room ? used : room);
@@ -168,7 +169,7 @@ __global__ void __launch_bounds__(544, 1)
   uint8_t* mem = raw_smem + (base - raw);
   float2* scales = reinterpret_cast<float2*>(mem + C::off_s);  // [tile & 3][sixteen keys]
   float* rowf = reinterpret_cast<float*>(mem + C::off_f);
-  float* tops = reinterpret_cast<float*>(mem + C::off_x);  // [tile & 1][half][row]
+  float* halves = reinterpret_cast<float*>(mem + C::off_x);  // [half][3][row]
   const uint32_t bars = base + C::off_bar;
   // Barriers of tile j, and the parity that they end with: its operands and
   // scales are in shared memory; its scores in S j & 1; its weights in P j & 1;
@@ -177,11 +178,11 @@ __global__ void __launch_bounds__(544, 1)
   const auto added = [&](int j) { return bars + 8 * (4 + (j & 3)); };
   const auto scored = [&](int j) { return bars + 8 * (8 + (j & 1)); };
   const auto weighed = [&](int j) { return bars + 8 * (10 + (j & 1)); };
+  const auto taken = [&](int j) { return bars + 8 * (12 + (j & 1)); };  // scores read for the last time
   const auto of4 = [](int j) { return uint32_t(j >> 2) & 1u; };
   const auto of2 = [](int j) { return uint32_t(j >> 1) & 1u; };
-  const auto pair = [&](int q, int j) { return bars + 8 * (12 + 2 * q + (j & 1)); };  // both halves of rows 32q ..
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mem + C::off_bar + 160);
-  volatile int* dead = reinterpret_cast<volatile int*>(mem + C::off_bar + 164);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mem + C::off_bar + 112);
+  volatile int* dead = reinterpret_cast<volatile int*>(mem + C::off_bar + 116);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   // heads of one tile side by side, the last queries (the most keys) first
@@ -208,8 +209,8 @@ __global__ void __launch_bounds__(544, 1)
     }
     for (int j = 0; j < 2; j++) {
       bar_init(scored(j), 1);
-      bar_init(weighed(j), 8);
-      for (int q = 0; q < 4; q++) bar_init(pair(q, j), 2);
+      bar_init(weighed(j), 4);
+      bar_init(taken(j), 4);
     }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
@@ -293,15 +294,15 @@ __global__ void __launch_bounds__(544, 1)
       for (int n = 0; n < NP; n++)
 #pragma unroll
         for (int kk = 0; kk < kKeys / 16; kk++)
-          mma_ts(tmem + C::c_o, tmem + C::c_p + (b * NP + n) * (kKeys / 2) + kk * 8,
-                 operand(base + C::off_v + j % C::stages * C::v + kk * 32), idesc_o, j > 0 || n > 0 || kk > 0);
+          mma_ts(tmem + C::c_o + b * D, tmem + C::c_p + (b * NP + n) * (kKeys / 2) + kk * 8,
+                 operand(base + C::off_v + j % C::stages * C::v + kk * 32), idesc_o, j > 1 || n > 0 || kk > 0);
       commit(added(j));
     };
     int done = 0;
     bool ok = true;
     for (int j = 0; j < nt && ok; j++) {
       const int b = j & 1;
-      ok = bar_wait(conv(j), of4(j), dead);
+      ok = bar_wait(conv(j), of4(j), dead) && (j < 2 || bar_wait(taken(j - 2), of2(j - 2), dead));
       if (!ok) break;
       fence_after();
 #pragma unroll
@@ -313,12 +314,15 @@ __global__ void __launch_bounds__(544, 1)
                  idesc_s,
                  n > 0 || kk > 0);
       commit(scored(j));
-      if (j > 0) {
-        ok = bar_wait(weighed(j - 1), of2(j - 1), dead);
-        if (ok) outputs(j - 1), done = j;
+      if (j > 1) {
+        ok = bar_wait(weighed(j - 2), of2(j - 2), dead);
+        if (ok) outputs(j - 2), done = j - 1;
       }
     }
-    if (ok && nt > 0 && bar_wait(weighed(nt - 1), of2(nt - 1), dead)) outputs(nt - 1), done = nt;
+    for (int j = max(nt - 2, 0); j < nt && ok; j++) {
+      ok = bar_wait(weighed(j), of2(j), dead);
+      if (ok) outputs(j), done = j + 1;
+    }
     if (done < nt && nt > 0) {
       // given up: what was issued ends before the TMEM is released
       commit(added(0));
@@ -429,7 +433,7 @@ __global__ void __launch_bounds__(544, 1)
     for (int j = 0; j < nt; j += 2)
       if (!turn(j, one) || (j + 1 < nt && !turn(j + 1, two))) break;
   } else {
-    // ---- the rows: a thread has half of a row's keys, and of its outputs
+    // ---- the rows: a half of the tiles each
     queries();
     ready();
     const int quarter = warp & 3, half = warp >> 2, r = quarter * 32 + lane;
@@ -439,46 +443,58 @@ __global__ void __launch_bounds__(544, 1)
     const int lo = max(first, t.window > 0 ? p - t.window + 1 : 0);  // sees lo .. p
     const int in_lo = max(first, t.window > 0 ? pmax - t.window + 1 : 0);
     const float f = rowf[r];
-    constexpr int N = kKeys / 2;  // a thread's keys
-    const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16), mine = lanes + C::c_o + half * (D / 2);
+    const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
+    const uint32_t my_s = lanes + half * kKeys, my_o = lanes + C::c_o + half * D;
+    const uint32_t my_p = lanes + C::c_p + half * NP * (kKeys / 2);
     float ref = ninf(), l = 0.f, W = 0.f, toW = 0.f;
     bool ok = true;
-    for (int j = 0; j < nt; j++) {
-      const int b = j & 1, key0 = (tb + j) * kKeys + half * N;
+    for (int j = half; j < nt; j += 2) {
+      const int key0 = (tb + j) * kKeys;
       ok = bar_wait(conv(j), of4(j), dead) && bar_wait(scored(j), of2(j), dead);
       if (!ok) break;
       fence_after();
-      uint32_t s[N];
-      tmem_ld32(lanes + b * kKeys + half * N, s);
-      const float2 c0 = scales[(j & 3) * 4 + 2 * half], c1 = scales[(j & 3) * 4 + 2 * half + 1];
-      const float2 d0 = scales[(j & 3) * 4 + 2 - 2 * half], d1 = scales[(j & 3) * 4 + 3 - 2 * half];
-      const float wide = fmaxf(fmaxf(c0.y, c1.y), fmaxf(d0.y, d1.y));
-      const bool edge = c0.x == ninf() || c1.x == ninf() || key0 < in_lo || key0 + N - 1 > pmin;
-      wait_ld();
+      float2 c[4];
+      float wide = 0.f;
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        c[g] = scales[(j & 3) * 4 + g];
+        wide = fmaxf(wide, c[g].y);
+      }
+      const bool edge = c[0].x == ninf() || c[1].x == ninf() || c[2].x == ninf() || c[3].x == ninf() || key0 < in_lo ||
+                        key0 + kKeys - 1 > pmin;
+      const auto hidden = [&](int e) { return key0 + e < lo || key0 + e > p || c[e / 16].x == ninf(); };
+      uint32_t s[32];
       f2* x2 = reinterpret_cast<f2*>(s);
       float* x = reinterpret_cast<float*>(s);
-      const f2 f0 = f2dup(__fmul_rn(f, c0.x)), f1 = f2dup(__fmul_rn(f, c1.x));
+      // the largest score: a group's largest product times its factor, which
+      // is not negative
+      float top = ninf();
 #pragma unroll
-      for (int e = 0; e < N / 2; e++) x2[e] = f2mul(x2[e], e < N / 4 ? f0 : f1);
-      if (edge) {
+      for (int u = 0; u < 2; u++) {
+        tmem_ld32(my_s + 32 * u, s);
+        wait_ld();
+        if (edge) {
 #pragma unroll
-        for (int e = 0; e < N; e++)
-          if (key0 + e < lo || key0 + e > p || (e < N / 2 ? c0.x : c1.x) == ninf()) x[e] = ninf();
+          for (int e = 0; e < 32; e++)
+            if (hidden(32 * u + e)) x[e] = ninf();
+        }
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+          float m[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            m[e] = fmaxf(fmaxf(x[16 * g + e], x[16 * g + 4 + e]), fmaxf(x[16 * g + 8 + e], x[16 * g + 12 + e]));
+          const float y = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+          top = fmaxf(top, y == ninf() ? y : __fmul_rn(y, __fmul_rn(f, c[2 * u + g].x)));
+        }
       }
-      float top = x[0];
-#pragma unroll
-      for (int e = 1; e < N; e++) top = fmaxf(top, x[e]);
-      {
-        float* at = tops + (b * 2) * kRows + r;
-        at[half * kRows] = top;
-        __syncwarp();
-        if (lane == 0) bar_arrive(pair(quarter, j));
-        ok = bar_wait(pair(quarter, j), of2(j), dead);
+      if (j > 1) {
+        ok = bar_wait(added(j - 2), of4(j - 2), dead);  // P is free, O as it was left
         if (!ok) break;
-        top = fmaxf(top, at[(half ^ 1) * kRows]);
+        fence_after();
       }
       // the references move: a score 2^8 above the row's (any, before its
-      // first key), a larger value scale; both halves alike
+      // first key), a larger value scale
       const bool over = top > __fadd_rn(ref, 8.f);
       if (__any_sync(FULL, over) || wide > W) {
         float k = 1.f;
@@ -494,18 +510,14 @@ __global__ void __launch_bounds__(544, 1)
           l = __fmul_rn(l, up);
           k = __fmul_rn(k, up);
         }
-        if (j > 0) {
-          ok = bar_wait(added(j - 1), of4(j - 1), dead);
-          if (!ok) break;
-          fence_after();
+        if (j > 1) {
 #pragma unroll 1
-          for (int c = 0; c < D / 2; c += 32) {
-            uint32_t o[32];
-            tmem_ld32(mine + c, o);
+          for (int n = 0; n < D; n += 32) {
+            tmem_ld32(my_o + n, s);
             wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__fmul_rn(__uint_as_float(o[e]), k));
-            tmem_st32(mine + c, o);
+            for (int e = 0; e < 32; e++) x[e] = __fmul_rn(x[e], k);
+            tmem_st32(my_o + n, s);
           }
           wait_st();
         }
@@ -513,66 +525,83 @@ __global__ void __launch_bounds__(544, 1)
       const f2 m = f2dup(ref == ninf() ? 0.f : -ref);
       f2 sum = 0;
 #pragma unroll
-      for (int e = 0; e < N / 2; e++) {
-        const f2 y = f2add(x2[e], m);
-        x2[e] = f2make(ex2(f2lo(y)), ex2(f2hi(y)));
-        sum = f2add(sum, x2[e]);
+      for (int u = 0; u < 2; u++) {
+        tmem_ld32(my_s + 32 * u, s);
+        wait_ld();
+        if (u == 1) {  // the tile after next may come into their place
+          fence_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(taken(j));
+        }
+        const float2 c0 = c[2 * u], c1 = c[2 * u + 1];
+        const f2 f0 = f2dup(__fmul_rn(f, c0.x)), f1 = f2dup(__fmul_rn(f, c1.x));
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          const f2 y = f2fma(x2[e], e < 8 ? f0 : f1, m);
+          x2[e] = f2make(ex2(f2lo(y)), ex2(f2hi(y)));
+        }
+        if (edge) {
+#pragma unroll
+          for (int e = 0; e < 32; e++)
+            if (hidden(32 * u + e)) x[e] = 0.f;
+        }
+        const f2 w0 = f2dup(__fmul_rn(c0.y, toW)), w1 = f2dup(__fmul_rn(c1.y, toW));
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          sum = f2add(sum, x2[e]);
+          x2[e] = f2mul(x2[e], e < 8 ? w0 : w1);
+        }
+        if (edge) {  // what is not seen counts nothing, whatever its page's scale
+#pragma unroll
+          for (int e = 0; e < 32; e++)
+            if (hidden(32 * u + e)) x[e] = 0.f;
+        }
+#pragma unroll
+        for (int n = 0; n < NP; n++) {
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            w[e] = pack_f16(x[2 * e], x[2 * e + 1]);
+            if (n + 1 < NP) {
+              x[2 * e] = __fsub_rn(x[2 * e], __half2float(__ushort_as_half(w[e] & 0xffff)));
+              x[2 * e + 1] = __fsub_rn(x[2 * e + 1], __half2float(__ushort_as_half(w[e] >> 16)));
+            }
+          }
+          tmem_st16(my_p + n * (kKeys / 2) + 16 * u, w);
+        }
       }
       l = __fadd_rn(l, __fadd_rn(f2lo(sum), f2hi(sum)));
-      const f2 w0 = f2dup(__fmul_rn(c0.y, toW)), w1 = f2dup(__fmul_rn(c1.y, toW));
-#pragma unroll
-      for (int e = 0; e < N / 2; e++) x2[e] = f2mul(x2[e], e < N / 4 ? w0 : w1);
-      if (edge) {  // what is not seen counts nothing, whatever its page's scale
-#pragma unroll
-        for (int e = 0; e < N; e++)
-          if (key0 + e < lo || key0 + e > p || (e < N / 2 ? c0.x : c1.x) == ninf()) x[e] = 0.f;
-      }
-      if (j > 1) {
-        ok = bar_wait(added(j - 2), of4(j - 2), dead);  // P b is free
-        if (!ok) break;
-      }
-#pragma unroll
-      for (int n = 0; n < NP; n++) {
-        uint32_t w[N / 2];
-#pragma unroll
-        for (int e = 0; e < N / 2; e++) {
-          w[e] = pack_f16(x[2 * e], x[2 * e + 1]);
-          if (n + 1 < NP) {
-            x[2 * e] = __fsub_rn(x[2 * e], __half2float(__ushort_as_half(w[e] & 0xffff)));
-            x[2 * e + 1] = __fsub_rn(x[2 * e + 1], __half2float(__ushort_as_half(w[e] >> 16)));
-          }
-        }
-        tmem_st16(lanes + C::c_p + (b * NP + n) * (kKeys / 2) + half * (N / 2), w);
-      }
       wait_st();
       fence_before();
       __syncwarp();
       if (lane == 0) bar_arrive(weighed(j));
     }
+    // the halves together; a half without a tile has no O
     if (ok && nt > 0) ok = bar_wait(added(nt - 1), of4(nt - 1), dead);
-    if (ok) {
-      // the halves' sums together, by way of the maxima's place
-      tops[((nt & 1) * 2 + half) * kRows + r] = l;
-      __syncwarp();
-      if (lane == 0) bar_arrive(pair(quarter, nt));
-      ok = bar_wait(pair(quarter, nt), of2(nt), dead);
-    }
+    if (ok && nt > 1) ok = bar_wait(added(nt - 2), of4(nt - 2), dead);
+    halves[(half * 3 + 0) * kRows + r] = ref;
+    halves[(half * 3 + 1) * kRows + r] = l;
+    halves[(half * 3 + 2) * kRows + r] = W;
+    asm volatile("bar.sync 1, 256;\n" ::: "memory");
     if (ok) {
       fence_after();
-      l = __fadd_rn(tops[(nt & 1) * 2 * kRows + r], tops[((nt & 1) * 2 + 1) * kRows + r]);
-      const float inv = l == 0.f ? 0.f : __fdiv_rn(W, l);
+      const float ref0 = halves[r], ref1 = halves[3 * kRows + r], l0 = halves[kRows + r], l1 = halves[4 * kRows + r];
+      ref = fmaxf(ref0, ref1);
+      const float k0 = ref0 == ref ? 1.f : ex2(__fsub_rn(ref0, ref)), k1 = ref1 == ref ? 1.f : ex2(__fsub_rn(ref1, ref));
+      l = __fadd_rn(__fmul_rn(l0, k0), __fmul_rn(l1, k1));
+      const float inv0 = __fdiv_rn(__fmul_rn(halves[2 * kRows + r], k0), l);
+      const float inv1 = __fdiv_rn(__fmul_rn(halves[5 * kRows + r], k1), l);
       const int64_t at = int64_t(sp.row + tq) * t.out.row + int64_t(hq) * t.out.head;
 #pragma unroll 1
       for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
-        uint32_t o[32];
-        if (nt > 0) {
-          tmem_ld32(lanes + C::c_o + c, o);
-          wait_ld();
-        }
+        uint32_t o[32], o1[32] = {};
+        if (nt > 0) tmem_ld32(lanes + C::c_o + c, o);
+        if (nt > 1) tmem_ld32(lanes + C::c_o + D + c, o1);
+        wait_ld();
         float y[32], most = 0.f;
 #pragma unroll
         for (int e = 0; e < 32; e++) {
-          y[e] = l == 0.f ? 0.f : __fmul_rn(__uint_as_float(o[e]), inv);
+          y[e] = l == 0.f ? 0.f : __fadd_rn(__fmul_rn(__uint_as_float(o[e]), inv0), __fmul_rn(__uint_as_float(o1[e]), inv1));
           most = fmaxf(most, fabsf(y[e]));
         }
         if (!there) continue;
