@@ -738,21 +738,7 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
     const int pos = p0 + tq;
     float x[H2][16];
     const int64_t off = int64_t(sp.row + tq) * t.q.row + int64_t(hq) * t.q.head + 16 * tg;
-#pragma unroll
-    for (int j = 0; j < H2; j++)
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const int64_t o = off + 64 * j + e;
-        if (!there) {
-          x[j][e] = x[j][e + 1] = x[j][e + 2] = x[j][e + 3] = 0.f;
-        } else if (type == 0) {
-          load4(static_cast<const float*>(t.q.p) + o, vec, &x[j][e]);
-        } else if (type == 1) {
-          load4(static_cast<const __half*>(t.q.p) + o, vec, &x[j][e]);
-        } else {
-          load4(static_cast<const __nv_bfloat16*>(t.q.p) + o, vec, &x[j][e]);
-        }
-      }
+    load_row<D>(t.q.p, off, type, vec, there, x);
     rotate16<D>(x, a, pos, tg);
     const float amax = group_amax<D>(x, FULL);  // NaN where a value is none
     const float to = lift_row<D>(x, amax);
@@ -1162,18 +1148,7 @@ __global__ void __launch_bounds__(32 * Shape1<D, WU>::warps, Shape1<D, WU>::bloc
   {
     float x[H2][16];
     const int64_t off = int64_t(sp.row) * t.q.row + int64_t(h) * t.q.head + 16 * tg;
-#pragma unroll
-    for (int j = 0; j < H2; j++)
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const int64_t o = off + 64 * j + e;
-        if (type == 0)
-          load4(static_cast<const float*>(t.q.p) + o, vec, &x[j][e]);
-        else if (type == 1)
-          load4(static_cast<const __half*>(t.q.p) + o, vec, &x[j][e]);
-        else
-          load4(static_cast<const __nv_bfloat16*>(t.q.p) + o, vec, &x[j][e]);
-      }
+    load_row<D>(t.q.p, off, type, vec, true, x);
     rotate16<D>(x, a, p, tg);
     const float amax = group_amax<D>(x, FULL);  // NaN where a value is none
     const float to = lift_row<D>(x, amax);

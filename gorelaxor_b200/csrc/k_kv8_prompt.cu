@@ -232,20 +232,7 @@ __global__ void __launch_bounds__(544, 1)
       const int tq = there ? (r0 + r) / group : 0, hq = h * group + (there ? (r0 + r) % group : 0);
       float x[H2][16];
       const int64_t off = int64_t(sp.row + tq) * t.q.row + int64_t(hq) * t.q.head + 16 * tg;
-#pragma unroll
-      for (int j = 0; j < H2; j++)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          const int64_t o = off + 64 * j + e;
-          if (!there)
-            x[j][e] = x[j][e + 1] = x[j][e + 2] = x[j][e + 3] = 0.f;
-          else if (type == 0)
-            load4(static_cast<const float*>(t.q.p) + o, vec, &x[j][e]);
-          else if (type == 1)
-            load4(static_cast<const __half*>(t.q.p) + o, vec, &x[j][e]);
-          else
-            load4(static_cast<const __nv_bfloat16*>(t.q.p) + o, vec, &x[j][e]);
-        }
+      load_row<D>(t.q.p, off, type, vec, there, x);
       rotate16<D>(x, a, p0 + tq, tg);
       const float amax = group_amax<D>(x, FULL);
       const float to = __fmul_rn(lift_row<D>(x, amax), kTo14);
@@ -462,7 +449,19 @@ __global__ void __launch_bounds__(544, 1)
       }
       const bool edge = c[0].x == ninf() || c[1].x == ninf() || c[2].x == ninf() || c[3].x == ninf() || key0 < in_lo ||
                         key0 + kKeys - 1 > pmin;
-      const auto hidden = [&](int e) { return key0 + e < lo || key0 + e > p || c[e / 16].x == ninf(); };
+      // bit e: this row sees key e of the tile
+      uint64_t seen = ~0ull;
+      bool none = false;  // some value scale is no number
+      if (edge) {
+        const int from = max(lo - key0, 0), to = min(p - key0, kKeys - 1);
+        seen = from > to ? 0 : (~0ull >> (kKeys - 1 - to)) >> from << from;
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+          if (c[g].x == ninf()) seen &= ~(0xffffull << (16 * g));
+          none = none || isnan(c[g].y);
+        }
+      }
+      const auto hidden = [&](int e) { return !(uint32_t(e < 32 ? seen : seen >> 32) >> (e & 31) & 1); };
       uint32_t s[32];
       f2* x2 = reinterpret_cast<f2*>(s);
       float* x = reinterpret_cast<float*>(s);
@@ -551,7 +550,7 @@ __global__ void __launch_bounds__(544, 1)
           sum = f2add(sum, x2[e]);
           x2[e] = f2mul(x2[e], e < 8 ? w0 : w1);
         }
-        if (edge) {  // what is not seen counts nothing, whatever its page's scale
+        if (none) {  // what is not seen counts nothing, whatever its page's scale
 #pragma unroll
           for (int e = 0; e < 32; e++)
             if (hidden(32 * u + e)) x[e] = 0.f;
@@ -589,43 +588,28 @@ __global__ void __launch_bounds__(544, 1)
       ref = fmaxf(ref0, ref1);
       const float k0 = ref0 == ref ? 1.f : ex2(__fsub_rn(ref0, ref)), k1 = ref1 == ref ? 1.f : ex2(__fsub_rn(ref1, ref));
       l = __fadd_rn(__fmul_rn(l0, k0), __fmul_rn(l1, k1));
-      const float inv0 = __fdiv_rn(__fmul_rn(halves[2 * kRows + r], k0), l);
-      const float inv1 = __fdiv_rn(__fmul_rn(halves[5 * kRows + r], k1), l);
-      const int64_t at = int64_t(sp.row + tq) * t.out.row + int64_t(hq) * t.out.head;
+      // a row without keys has an O of zeros or none
+      const float inv0 = l == 0.f ? 0.f : __fdiv_rn(__fmul_rn(halves[2 * kRows + r], k0), l);
+      const float inv1 = l == 0.f ? 0.f : __fdiv_rn(__fmul_rn(halves[5 * kRows + r], k1), l);
 #pragma unroll 1
       for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
-        uint32_t o[32], o1[32] = {};
+        uint32_t o[32] = {}, o1[32] = {};
         if (nt > 0) tmem_ld32(lanes + C::c_o + c, o);
         if (nt > 1) tmem_ld32(lanes + C::c_o + D + c, o1);
         wait_ld();
-        float y[32], most = 0.f;
+        float* y = reinterpret_cast<float*>(o);
 #pragma unroll
-        for (int e = 0; e < 32; e++) {
-          y[e] = l == 0.f ? 0.f : __fadd_rn(__fmul_rn(__uint_as_float(o[e]), inv0), __fmul_rn(__uint_as_float(o1[e]), inv1));
-          most = fmaxf(most, fabsf(y[e]));
-        }
-        if (!there) continue;
-        if (t.out.p && ovec && type == 0) {
-          float4* op = reinterpret_cast<float4*>(static_cast<float*>(const_cast<void*>(t.out.p)) + at + c);
+        for (int e = 0; e < 32; e++) y[e] = __fadd_rn(__fmul_rn(y[e], inv0), __fmul_rn(__uint_as_float(o1[e]), inv1));
+        // into the place of Q, chunks of 16 bytes in an order that keeps banks apart
 #pragma unroll
-          for (int e = 0; e < 8; e++) op[e] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
-        } else if (t.out.p && ovec) {
-          uint32_t hy[16];
-#pragma unroll
-          for (int e = 0; e < 16; e++)
-            hy[e] = type == 1 ? pack_f16(y[2 * e], y[2 * e + 1])
-                              : uint32_t(__bfloat16_as_ushort(__float2bfloat16_rn(y[2 * e]))) |
-                                    uint32_t(__bfloat16_as_ushort(__float2bfloat16_rn(y[2 * e + 1]))) << 16;
-          uint4* op = reinterpret_cast<uint4*>(static_cast<uint16_t*>(const_cast<void*>(t.out.p)) + at + c);
-#pragma unroll
-          for (int e = 0; e < 4; e++) op[e] = make_uint4(hy[4 * e], hy[4 * e + 1], hy[4 * e + 2], hy[4 * e + 3]);
-        } else if (t.out.p) {
-#pragma unroll
-          for (int e = 0; e < 32; e++) put(t, type, at + c + e, y[e]);
-        }
-        if (t.q8) {  // one Q8_0 block
+        for (int e = 0; e < 8; e++)
+          sts16(base + r * (D * 4) + ((c / 4 + e) ^ (r & 7)) * 16, o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        if (t.q8 && there) {  // one Q8_0 block
           const int64_t to = (int64_t(sp.row + tq) * t.heads + hq) * D + c;
+          float most = 0.f;
           uint32_t w[8] = {};
+#pragma unroll
+          for (int e = 0; e < 32; e++) most = fmaxf(most, fabsf(y[e]));
 #pragma unroll
           for (int e = 0; e < 32; e++) w[e / 4] |= uint32_t(uint8_t(quant_val(y[e], most))) << (8 * (e % 4));
           uint4* op = reinterpret_cast<uint4*>(t.q8 + to);
@@ -635,6 +619,40 @@ __global__ void __launch_bounds__(544, 1)
         }
       }
       if (there && half == 0 && t.lse) t.lse[int64_t(sp.row + tq) * t.heads + hq] = lse_of(ref, l);
+    }
+    asm volatile("bar.sync 1, 256;\n" ::: "memory");
+    if (ok && t.out.p) {
+      // whole rows to memory, sixteen to a warp
+      constexpr int E = NP == 2 ? 4 : 8, L = D / E;  // values a lane, lanes a row
+      const float* stage = reinterpret_cast<const float*>(mem);
+      const int own = warp * 16 + (lane & 15), n = min(r0 + own, r0 + nrow - 1);
+      const int64_t to = int64_t(sp.row + n / group) * t.out.row + int64_t(h * group + n % group) * t.out.head;
+#pragma unroll 1
+      for (int i16 = 0; i16 < 16; i16 += 32 / L) {
+        const int row = warp * 16 + i16 + lane / L, c = lane % L * E;
+        const int64_t at = __shfl_sync(FULL, to, i16 + lane / L) + c;
+        if (row >= nrow) continue;
+        float y[E];
+#pragma unroll
+        for (int e = 0; e < E; e += 4)
+          *reinterpret_cast<float4*>(y + e) =
+              *reinterpret_cast<const float4*>(stage + row * D + ((c + e) / 4 ^ (row & 7)) * 4);
+        if (!ovec) {
+#pragma unroll
+          for (int e = 0; e < E; e++) put(t, type, at + e, y[e]);
+        } else if (NP == 2) {
+          *reinterpret_cast<float4*>(static_cast<float*>(const_cast<void*>(t.out.p)) + at) = *reinterpret_cast<float4*>(y);
+        } else {
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            w[e] = type == 1 ? pack_f16(y[2 * e % E], y[(2 * e + 1) % E])
+                             : uint32_t(__bfloat16_as_ushort(__float2bfloat16_rn(y[2 * e % E]))) |
+                                   uint32_t(__bfloat16_as_ushort(__float2bfloat16_rn(y[(2 * e + 1) % E]))) << 16;
+          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(const_cast<void*>(t.out.p)) + at) =
+              make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
     }
   }
   fence_before();
