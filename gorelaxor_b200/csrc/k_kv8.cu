@@ -480,15 +480,20 @@ cudaError_t read_t(const Kv8Args& a, const Kv8Rows& k, const Kv8Rows& v, cudaStr
 // outputs (2^-11 of each weight, what a float16 output is rounded by) and the
 // sum of two for float32 ones (2^-25 of the largest weight).
 //
-// Layout. A warp takes sixteen tokens at a time, straight from global
-// memory into the registers of the product's operands: a key row's bytes
-// are spread over four lanes, sixteen consecutive ones each, a value row's
-// over eight. No shared memory in the loop and no synchronisation: WU warps
-// of a block, and the blocks of a cluster, take separate stretches of the
-// keys and are joined at the end through (distributed) shared memory; with
-// WU = 1 each warp has a unit of its own and writes it out. The maximum
-// moves only when a score passes it by 2^8 (the weights stay far from
-// overflow), so most steps need no exchange between lanes.
+// Layout. A warp takes sixteen tokens at a time from a ring of its own in
+// shared memory (Ring, below): a key row's bytes are spread over four lanes,
+// sixteen consecutive ones each, a value row's over eight. No block-wide
+// synchronisation in the loop: WU warps of a block, and the blocks of a
+// cluster, take separate stretches of the keys and are joined at the end
+// through (distributed) shared memory; with WU = 1 each warp has a unit of
+// its own and writes it out. The maximum moves only when a score passes it
+// by 2^8 (the weights stay far from overflow), so most steps need no
+// exchange between lanes.
+//
+// Bound by the arithmetic of the digits and weights: 48 sequences of 1 to
+// 12001 tokens, 4 heads of 128 with 4 queries each, float16: 70 us, 3.4 TB/s
+// of the cache. One sequence of 32768 tokens, 8 heads with 4 queries each:
+// 33 us, 2.0 TB/s, on the 128 blocks that clusters of 16 give.
 
 __device__ __forceinline__ void mma_s8(int* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
@@ -1075,27 +1080,23 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
 //    permutations for sixteen bytes) and no conversion.
 // Sums are exact integers until the reference moves (a score 2^1 above it,
 // a larger value scale) or 32768 keys have gone by; then they go into
-// float32 sums. About 60 instructions for sixteen tokens where eight columns
-// of queries take 260: bound by the cache's bytes.
+// float32 sums. 256 sequences of 65 to 576 tokens, 16 heads of 64: 37 us,
+// 4.6 TB/s of the cache, 10 us of it the launch and the join; sequences of
+// thousands of tokens read at 6.2 to 6.4 TB/s.
 __device__ __forceinline__ void mma_s8u8(int* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-#ifndef KV8_STEPS64
-#define KV8_STEPS64 3
-#define KV8_WARPS64 16
-#endif
-#ifndef KV8_STEPS128
-#define KV8_STEPS128 2
-#define KV8_WARPS128 12
-#endif
+// Steps of a warp's ring and warps an SM shall hold, by shared memory: heads
+// of 64 took 1 to 3 % longer with 2 steps and 16 or 20 warps and with 4 steps
+// and 12.
 template <int D, int WU>
 struct Shape1 {
   static constexpr int warps = WU == 1 ? 4 : WU;
-  static constexpr int ring = D == 64 ? KV8_STEPS64 : KV8_STEPS128;  // steps of 32 tokens
-  static constexpr int per_sm = D == 64 ? KV8_WARPS64 : KV8_WARPS128;  // warps, by registers and rings
+  static constexpr int ring = D == 64 ? 3 : 2;  // steps of 32 tokens
+  static constexpr int per_sm = D == 64 ? 16 : 12;  // warps, by registers and rings
   static constexpr int blocks = per_sm / warps < 1 ? 1 : per_sm / warps;
   static constexpr size_t rings = size_t(warps) * ring * 2 * Ring<D>::tile;
   static constexpr size_t smem = rings;  // the joined outputs, smaller, take their place
@@ -1472,10 +1473,14 @@ cudaError_t attend_d(const Kv8Args& a, int type, const Kv8Attend& t, cudaStream_
   const int64_t rows = int64_t(a.max_new) * (t.heads / a.heads);  // queries that share a head's keys
   if (rows == 1) return attend1_d<D>(a, type, t, st);
   if (rows <= 8) return attend_t<D, 1, NP>(a, type, t, st);
-  // Many queries go to the 5th-generation tensor core, 128 a block, unless
-  // few blocks would have long stretches of keys that these kernels split.
+  // More than 16 queries go to the 5th-generation tensor core, 128 a block,
+  // unless few blocks would have long stretches of keys that these kernels
+  // split. Heads of 128, bfloat16, us here and there: 36 queries of 16 x 4
+  // heads over 512 keys 29 and 24, over 2048 100 and 45; of 4 x 4 heads over
+  // 2048 46 and 45, of 1 x 4 over 8192 34 and 140. 16 queries of 256 x 4 heads
+  // over 2048 keys: 168 and 302.
   const int64_t blocks = int64_t(a.n) * a.heads * ((rows + 127) / 128);
-  if (rows > 32 && (blocks >= kSMs / 4 || a.max_len <= 1024)) return launch_kv8_prompt(a, D, type, t, st);
+  if (rows > 16 && (blocks >= kSMs / 4 || a.max_len <= 1024)) return launch_kv8_prompt(a, D, type, t, st);
   if (rows <= 16) return attend_t<D, 2, NP>(a, type, t, st);
   return attend_t<D, 4, NP>(a, type, t, st);
 }

@@ -157,7 +157,9 @@ typedef struct grx_kv8 {
  * and len allow, a len past table_width pages or rope_positions, a page that
  * is none of the cache's) touch no memory: the sequence, or the page's
  * tokens, are left out, and *status, if given (device memory), becomes
- * GRX_ERANGE. It is never cleared by a call. */
+ * GRX_ERANGE. It is never cleared by a call. The kernel for prompts waits
+ * between its parts for about a second at most; a wait that runs out leaves
+ * rows of outputs unwritten and makes *status GRX_ETIMEDOUT. */
 #define GRX_ROPE_NONE 0
 #define GRX_ROPE_PAIRS 1
 #define GRX_ROPE_HALVES 2
@@ -182,8 +184,8 @@ typedef struct grx_kv8_seqs {
  * scale s' = max(s, a/127), a the largest magnitude among the new values
  * and s the scale so far (0 when the page's first token is among the new);
  * where s' > s, the bytes it held become rne(q·s/s'); the new ones are
- * rne(x/s'). Quotients and roundings are done in 64 bits, so the bytes do
- * not depend on how tokens of one call are spread over threads; a value
+ * rne(x/s'). Rotations, quotients and roundings come out as in 64 bits, so
+ * the bytes do not depend on how a call's tokens are spread over threads; a value
  * that is not finite makes its page's scale NaN, until the page begins
  * anew. A page that is written must belong to one sequence of the call
  * (grx_kv8_check finds out). Work is queued on `stream` and not waited for;
@@ -201,8 +203,9 @@ int grx_kv8_read(const grx_kv8* kv, const grx_kv8_seqs* s, int type, void* k, in
  * window > 0, the last `window` of them. out = softmax(scale·q·k)·v, sums in
  * 32 bits; the queries are rotated as the keys were. lse [rows][heads] (may
  * be NULL) gets log Σ e^(scale·q·k). A query that sees no key answers zeros
- * and −inf; one that is not finite, or sees a page whose scale is not,
- * answers NaN. Results do not depend on timing. Queued on `stream`. */
+ * and −inf; one that is not finite, or sees a page whose scale is not (or
+ * whose values' scale is below 0), answers NaN. out must not overlap q.
+ * Results do not depend on timing. Queued on `stream`. */
 int grx_kv8_attend(const grx_kv8* kv, const grx_kv8_seqs* s, int type, int heads, const void* q, int64_t q_row,
                    int64_t q_head, float scale, int window, void* out, int64_t out_row, int64_t out_head, float* lse,
                    void* stream);
