@@ -5,10 +5,12 @@
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "host.h"
@@ -194,8 +196,9 @@ int grx_kv8_check(const grx_kv8* kv, const grx_kv8_seqs* s, int writes) {
   auto bad = [](int i, const std::string& what) {
     return fail(GRX_ERANGE, "grx_kv8_check: sequence " + std::to_string(i) + ": " + what);
   };
-  std::vector<int> owner(writes ? size_t(a.pages) : 0, -1);  // the sequence that appends to a page
-  auto pages_of = [&](const Kv8Span& sp) { return (sp.len + (1 << a.plog) - 1) >> a.plog; };
+  const auto begins = [&](const Kv8Span& sp) { return (sp.len - sp.T) >> a.plog; };  // the first page it appends to
+  const auto pages_of = [&](const Kv8Span& sp) { return (sp.len + (1 << a.plog) - 1) >> a.plog; };
+  std::vector<std::pair<int, int>> written;  // pages that are appended to, and by which sequence
   for (int i = 0; i < a.n; i++) {
     const Kv8Span sp = kv8_span(a, i);
     if (!sp.ok)
@@ -207,21 +210,25 @@ int grx_kv8_check(const grx_kv8* kv, const grx_kv8_seqs* s, int writes) {
       if (p < 0)
         return bad(i, "its page " + std::to_string(b) + " is " + std::to_string(a.table[int64_t(i) * a.width + b]) +
                           " of " + std::to_string(a.pages));
-      if (writes && sp.len >= sp.T && sp.T > 0 && b >= (sp.len - sp.T) >> a.plog) {
-        if (owner[size_t(p)] >= 0) return bad(i, "appends to page " + std::to_string(p) + ", as sequence " +
-                                                     std::to_string(owner[size_t(p)]) + " does");
-        owner[size_t(p)] = i;
-      }
+      if (writes && sp.len >= sp.T && sp.T > 0 && b >= begins(sp)) written.emplace_back(p, i);
     }
   }
-  if (writes)
+  std::sort(written.begin(), written.end());
+  for (size_t j = 1; j < written.size(); j++)
+    if (written[j].first == written[j - 1].first)
+      return bad(written[j].second, "appends to page " + std::to_string(written[j].first) + ", as sequence " +
+                                        std::to_string(written[j - 1].second) + " does");
+  if (!written.empty())
     for (int i = 0; i < a.n; i++) {
       const Kv8Span sp = kv8_span(a, i);
-      const int whole = sp.T > 0 && sp.len >= sp.T ? (sp.len - sp.T) >> a.plog : pages_of(sp);
-      for (int b = 0; b < whole; b++)
-        if (owner[size_t(kv8_page(a, i, b))] >= 0)
-          return bad(i, "holds page " + std::to_string(kv8_page(a, i, b)) + ", which sequence " +
-                            std::to_string(owner[size_t(kv8_page(a, i, b))]) + " appends to");
+      const int whole = sp.T > 0 && sp.len >= sp.T ? begins(sp) : pages_of(sp);
+      for (int b = 0; b < whole; b++) {
+        const int p = kv8_page(a, i, b);
+        const auto w = std::lower_bound(written.begin(), written.end(), std::make_pair(p, 0));
+        if (w != written.end() && w->first == p)
+          return bad(i, "holds page " + std::to_string(p) + ", which sequence " + std::to_string(w->second) +
+                            " appends to");
+      }
     }
   return GRX_OK;
 }

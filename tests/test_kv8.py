@@ -56,6 +56,13 @@ def test_check_refuses(table, lens, kw, word):
     refused(lambda: cache().check(np.array(table), lens, **kw), ERANGE, word)
 
 
+def test_check_of_a_vast_cache():
+    """The check's memory goes by the table, not by what pages could be."""
+    kv = cache(pages=2**31 - 1)
+    kv.check(np.array([[5, 2**31 - 2], [7, 8]]), [20, 20], writes=True)
+    refused(lambda: kv.check(np.array([[5, 2**31 - 2], [7, 2**31 - 2]]), [20, 20], writes=True), ERANGE, "appends")
+
+
 def seqs(**kw):
     a = dict(n=2, d_table=4096, table_width=2, d_len=4096, max_len=32)
     return g.KV8Seqs(**{**a, **kw})
