@@ -1151,7 +1151,7 @@ static int streams_text_one(grx_streams* q, const int* ids, const int* off, floa
   float2* xs = ar.alloc<float2>(size_t(R) * (d / 32), &rc);  // a scale per 32-value block
   int8_t* fq = ar.alloc<int8_t>(size_t(R) * ff, &rc);
   float2* fs = ar.alloc<float2>(size_t(R) * (ff / 32), &rc);
-  int* dint = ar.alloc<int>(size_t(3) * R + size_t(5) * ns + 2 * size_t(n) + 1, &rc);
+  int* dint = ar.alloc<int>(size_t(3) * R + size_t(5) * ns + 2 * size_t(n) + 2, &rc);
   float* qkv = q->kv8.page ? ar.alloc<float>(size_t(R) * 3 * d, &rc) : nullptr;
   float* lo = out ? ar.alloc<float>(size_t(ns) * d, &rc) : nullptr;
   float* lrow = out ? ar.alloc<float>(size_t(ns) * d, &rc) : nullptr;
@@ -1164,10 +1164,12 @@ static int streams_text_one(grx_streams* q, const int* ids, const int* off, floa
   std::vector<int> hint;
   for (const auto* v : {&row_id, &row_slot, &row_pos, &c_row0, &c_T, &c_pos0, &c_slot, &last_row, &row0, &len})
     hint.insert(hint.end(), v->begin(), v->end());
+  hint.push_back(0);
   CK(cudaMemcpyAsync(dint, hint.data(), sizeof(int) * hint.size(), cudaMemcpyHostToDevice, q->st));
   const int *d_id = dint, *d_slot = dint + R, *d_pos = dint + 2 * R, *d_row0 = dint + 3 * R, *d_T = d_row0 + ns,
             *d_pos0 = d_T + ns, *d_cslot = d_pos0 + ns, *d_last = d_cslot + ns, *d_rows = d_last + ns,
             *d_len = d_rows + n + 1;
+  int* d_status = dint + hint.size() - 1;  // of the attention over 8-bit caches
   cudaStream_t st = q->st;
   if (d_xin)  // the rows themselves (voice conditioning), in row order
     CK(cudaMemcpyAsync(x, d_xin, sizeof(float) * size_t(R) * d, cudaMemcpyDeviceToDevice, st));
@@ -1195,6 +1197,7 @@ static int streams_text_one(grx_streams* q, const int* ids, const int* off, floa
       a.max_new = tmax;
       a.len = d_len;
       a.len_add = 0;
+      a.status = d_status;
       CK(kv8_attention(a, qkv, d, xq, xs, st));
     } else {
       EpiArgs e;
@@ -1260,8 +1263,11 @@ static int streams_text_one(grx_streams* q, const int* ids, const int* off, floa
     for (int i = 0; i < ns; i++)
       std::memcpy(out + size_t(c_slot[size_t(i)]) * d, h.data() + size_t(i) * d, sizeof(float) * size_t(d));
   }
+  int status = 0;
+  if (q->kv8.page) CK(cudaMemcpyAsync(&status, d_status, sizeof status, cudaMemcpyDeviceToHost, st));
   CK(cudaStreamSynchronize(st));
   CK(cudaGetLastError());
+  if (status) return fail(status, "grx_streams_text: the attention over the 8-bit caches gave up");
   return GRX_OK;
 }
 

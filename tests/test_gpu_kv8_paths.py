@@ -142,6 +142,39 @@ def test_steps_device_runs_and_texts_agree(have_gpu):
     assert bits_equal(st.kv(131), last)
 
 
+@pytest.mark.parametrize("page", [16, 64])
+def test_long_texts_near_the_float_set(have_gpu, page):
+    """Texts from none to hundreds of tokens in one call: the first layer's
+    caches are the float32 set's within a step; and the last token's output
+    is that of a float32 set whose voice is what the 8-bit caches hold of the
+    tokens before it, within the 2 % that a frame's is (the two differ in the
+    one token's own key and value)."""
+    cfg, gm = model(seed=4)
+    lens = [0, 1, 20, 70, 150, 17, 64, 201]
+    n = len(lens)
+    vs = voices(cfg, gm, n, lambda i: 10 + 9 * i)
+    ids = [[(11 * i + 3 * j) % cfg.text_vocab for j in range(m)] for i, m in enumerate(lens)]
+    a, b = g.Streams(gm, vs, 210), g.Streams(gm, vs, 210, kv8_page=page)
+    a.text(ids)
+    tb = b.text(ids)
+    for i, m in enumerate(lens):
+        assert b.pos(i) == a.pos(i) == 10 + 9 * i + m
+        if m:
+            c = g.Streams(gm, [gm.voice(np.ascontiguousarray(b.kv(i)[:, :, :-1]))], 4)
+            tc = c.text([ids[i][-1:]])[0]
+            assert np.sqrt(np.mean((tc - tb[i]) ** 2)) <= 0.02 * np.sqrt(np.mean(tc**2)), i
+        x, y = a.kv(i)[0].astype(np.float64), b.kv(i)[0].astype(np.float64)
+        for lo in range(0, x.shape[1], page):
+            u, v = x[:, lo:lo + page], y[:, lo:lo + page]
+            for j in range(2):
+                for h in range(cfg.heads):
+                    c = slice(h * 64, h * 64 + 64)
+                    # a page that the voice began was rounded once before its scale rose
+                    assert np.abs(u[j, :, c] - v[j, :, c]).max() <= np.abs(u[j, :, c]).max() / 127 * (1 + 1e-5)
+    again = g.Streams(gm, vs, 210, kv8_page=page)
+    assert bits_equal(again.text(ids), tb)
+
+
 def test_what_streams_refuse(have_gpu):
     cfg, gm = model()
     v = voices(cfg, gm, 1)
