@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(256, G == D / 8 ? 4 : 3)
     k_kv8_append(Kv8Args a, Kv8Rows kin, Kv8Rows vin, int blocks, int per, bool vec) {
   constexpr int C = D / 8;                // items a token
   constexpr int N = G == C ? 1 : kItems;  // items a thread
-  __shared__ uint32_t red[16];
+  __shared__ uint32_t red[4 * 8];
   const int tid = threadIdx.x % G;
   const uint32_t group = (blockIdx.x * 256u + threadIdx.x) / G;  // the launch has fewer than 2^31 units
   const uint32_t parts = (2 * a.heads + per - 1) / per, rest = group / parts;
@@ -215,7 +215,9 @@ __global__ void __launch_bounds__(256, G == D / 8 ? 4 : 3)
     items = held = 0;
   }
   // the unit's largest of numbers that are not negative, as their bits
-  // compare (NaN above all); `round` picks the place of its exchange
+  // compare (NaN above all). `round` picks the place of its exchange: two for
+  // a head and others for the next, since a head may have one exchange alone,
+  // and a warp is then past it while another reads
   auto largest = [&](float m, int round) {
     uint32_t v = __float_as_uint(m) & 0x7fffffffu;
     if constexpr (G < 32) {
@@ -272,7 +274,8 @@ __global__ void __launch_bounds__(256, G == D / 8 ? 4 : 3)
       for (int j = 0; j < 8; j++) most = max_nan(most, fabsf(y[u][j]));
     }
     if (hh + 1 < he) load(hh + 1);
-    const float top = largest(most, 0);
+    const int turn = 2 * (hh & 1);
+    const float top = largest(most, turn);
     bool slow = !(top < kHuge) || (top > 0.f && top < kTiny);
     float mine = 0.f;  // a/127 as stored, of this thread's candidates
     const float bound = slow ? 0.f : __fmul_rn(top, 1.f - 0x1p-19f);
@@ -295,7 +298,7 @@ __global__ void __launch_bounds__(256, G == D / 8 ? 4 : 3)
     }
     // what is not rotated is exact as it is (and a 32-bit number over 127 is
     // never near the middle of two others: its digits repeat every seven bits)
-    const float fresh = mode == ROPE_NONE && !slow ? __fdiv_rn(top, 127.f) : largest(mine, 1);
+    const float fresh = mode == ROPE_NONE && !slow ? __fdiv_rn(top, 127.f) : largest(mine, turn + 1);
     const float scale = isnan(old) || isnan(fresh) ? __int_as_float(0x7fc00000) : fmaxf(old, fresh);
     const bool some = scale > 0.f;  // not 0, and a number
     slow = slow || scale < kTiny;

@@ -149,6 +149,22 @@ def test_append_ragged(have_gpu, dtype, d, page, heads):
     assert s.status.item() == 0
 
 
+@pytest.mark.parametrize("mode", ["none", "halves"])
+@pytest.mark.parametrize("new", [(64, 64), (20, 150)])
+def test_append_heads_in_turn(have_gpu, mode, new):
+    """So many pages that a block takes several heads of one after another;
+    values of very different sizes from head to head."""
+    rng = np.random.default_rng(5)
+    n = 100
+    lens = rng.integers(150, 260, n)
+    s = Side(lens.tolist(), rng.integers(new[0], new[1] + 1, n).tolist(), heads=8, d=64, page=64, mode=mode, seed=1)
+    kv = s.rng.normal(0, 1, (s.rows, 2, 8, 64)).astype(np.float32) * (4.0 ** np.arange(8, dtype=np.float32))[:, None]
+    for _ in range(2):
+        s.append(kv[..., ::-1, :].copy())
+    s.same()
+    assert s.status.item() == 0
+
+
 def test_append_strides_and_offsets(have_gpu):
     """Heads outermost, and rows that begin off every wide boundary."""
     s = Side([40, 21], [17, 9], heads=3, d=64, mode="pairs", seed=5)
