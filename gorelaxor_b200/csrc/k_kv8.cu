@@ -1073,7 +1073,7 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
 //    middle in odd ones, the highest added to odd ones), so every lane has
 //    the digits of four keys and takes one of them: one score, one
 //    exponential and one weight a lane for 32 keys;
-//  * the weight is a whole number of 2^-22 of the reference weight, whose
+//  * the weight is a whole number of 2^-23 of the reference weight, whose
 //    three bytes are taken as they lie in the float n + 2^23; one 8x8
 //    transposition brings the bytes of all 32 keys to the columns of an
 //    integer product with the values' bytes (m16n8k32, unsigned weights):
@@ -1081,8 +1081,8 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
 //    highest digits in one product, middle ones in another;
 //  * the values' bytes need a 4x4 byte transposition (eight byte
 //    permutations for sixteen bytes) and no conversion.
-// Sums are exact integers until the reference moves (a score 2^1 above it,
-// a larger value scale) or 32768 keys have gone by; then they go into
+// Sums are exact integers until the reference moves (a larger score, a
+// larger value scale) or 32768 keys have gone by; then they go into
 // float32 sums. 256 sequences of 65 to 576 tokens, 16 heads of 64: 37 us,
 // 4.6 TB/s of the cache, 10 us of it the launch and the join; sequences of
 // thousands of tokens read at 6.2 to 6.4 TB/s.
@@ -1109,7 +1109,7 @@ template <int D, int WU>
 __global__ void __launch_bounds__(32 * Shape1<D, WU>::warps, Shape1<D, WU>::blocks)
     k_kv8_attend1(Kv8Args a, Kv8Attend t, int type, int S, int units, bool vec) {
   constexpr int H2 = D / 64, M = D / 16, WV = D / 32, R = Shape1<D, WU>::ring;
-  constexpr float kOne = 4194303.f;  // of a weight of 1; weights go to 2
+  constexpr float kOne = 8388592.f;  // of a weight of 1, with room for a product's roundings below 2^23
   extern __shared__ __align__(16) uint8_t smem[];
   float* part = reinterpret_cast<float*>(smem);  // [WU][D + 2], and the block's, when the rings are done
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tg = lane & 3;
@@ -1228,14 +1228,14 @@ __global__ void __launch_bounds__(32 * Shape1<D, WU>::warps, Shape1<D, WU>::bloc
       if (hide) x = ninf(), sv = 0.f;
     }
     // The reference moves: a larger value scale (an eighth above it, to move
-    // less often), or a score 2 above (any, before the first key).
+    // less often), or a larger score.
     if (wide > W) {
       const float w = fminf(fmaxf(__fmul_rn(1.125f, wide), 1.17549435e-38f), 3.4e38f);
       flush(__fdiv_rn(W, w));
       W = w;
       toW = __fdiv_rn(1.f, w);
     }
-    if (__any_sync(FULL, x > 1.f)) {
+    if (__any_sync(FULL, x > 0.f)) {
       float m = hide ? ninf() : __fmul_rn(s, fs);
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, d));
@@ -1246,7 +1246,7 @@ __global__ void __launch_bounds__(32 * Shape1<D, WU>::warps, Shape1<D, WU>::bloc
       l = __fmul_rn(l, r);
       x = hide ? ninf() : __fmaf_rn(s, fs, -m);
     }
-    const float w = ex2(x);
+    const float w = x > 0.f ? 1.f : ex2(x);  // above 0 by the rounding of the reference
     l = __fadd_rn(l, __fmaf_rn(0.f, sv, w));  // a scale that is no number makes the sum none
     // n + 2^23: the bytes of n as they lie
     const uint32_t y = __float_as_uint(__fmaf_rn(__fmul_rn(w, __fmul_rn(sv, toW)), kOne, 8388608.f));
