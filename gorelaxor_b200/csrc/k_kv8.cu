@@ -1397,7 +1397,17 @@ inline int64_t stretches(const Kv8Args& a, int64_t units, int warps_per_sm, int 
   const int64_t tiles = (std::max(a.max_len, 1) + 15) / 16, most = std::max<int64_t>(1, tiles / 2);
   return std::min(most, std::max((tiles + longest - 1) / longest, (int64_t(kSMs) * warps_per_sm + units - 1) / units));
 }
-
+// Blocks of `warps` warps to a cluster that shares a unit's keys: as many as
+// the parts ask for, of those that run at once (what
+// cudaOccupancyMaxActiveClusters says of one or two blocks an SM). A second
+// wave costs more than shorter stretches give: 4 sequences of 8192 tokens,
+// 8 heads of 64 with 4 queries each, 36 us on clusters of 16 and 21 of 8.
+inline int blocks_of(int64_t units, int64_t parts, int warps, int per_sm) {
+  static constexpr int at_once[2][5] = {{148, 74, 33, 15, 7}, {296, 148, 71, 33, 14}};  // of 1, 2, 4, 8, 16
+  int n = 0;
+  while (n < 4 && (int64_t(warps) << n) < parts && units <= at_once[per_sm - 1][n + 1]) n++;
+  return 1 << n;
+}
 
 template <int D, int NQ, int NP, int WU>
 cudaError_t attend_launch(const Kv8Args& a, int type, const Kv8Attend& t, int64_t units, int qtiles, int S,
@@ -1430,14 +1440,12 @@ cudaError_t attend_t(const Kv8Args& a, int type, const Kv8Attend& t, cudaStream_
   const int64_t units = int64_t(a.n) * a.heads * qtiles;
   const int64_t parts = stretches(a, units, 16, 64);
   if (parts == 1) return attend_launch<D, NQ, NP, 1>(a, type, t, units, qtiles, 1, st);
-  int S = 1;
   if constexpr (NQ == 1) {
     constexpr int WU = kWide<D>;
-    if (parts > 4 && units <= kSMs) {
-      while (S < 16 && S * WU < parts) S *= 2;
-      return attend_launch<D, NQ, NP, WU>(a, type, t, units, qtiles, S, st);
-    }
+    if (parts > 4 && units <= kSMs)
+      return attend_launch<D, NQ, NP, WU>(a, type, t, units, qtiles, blocks_of(units, parts, WU, 2), st);
   }
+  int S = 1;
   while (S < 16 && S * 4 < parts) S *= 2;
   return attend_launch<D, NQ, NP, 4>(a, type, t, units, qtiles, S, st);
 }
@@ -1466,9 +1474,7 @@ cudaError_t attend1_d(const Kv8Args& a, int type, const Kv8Attend& t, cudaStream
   const int64_t units = int64_t(a.n) * a.heads, parts = stretches(a, units, Shape1<D, 1>::per_sm, 64);
   if (parts == 1) return attend1_launch<D, 1>(a, type, t, 1, st);
   if (parts <= 4) return attend1_launch<D, 4>(a, type, t, 1, st);
-  int S = 1;
-  while (S < 16 && S * 8 < parts) S *= 2;
-  return attend1_launch<D, 8>(a, type, t, S, st);
+  return attend1_launch<D, 8>(a, type, t, blocks_of(units, parts, 8, Shape1<D, 8>::blocks), st);
 }
 
 template <int D, int NP>
