@@ -564,22 +564,20 @@ cudaError_t rows_t(const LogpArgs& a, cudaStream_t st) {
 
 template <class T, int NE>
 void warp_rows(const LogpArgs& a, cudaStream_t st) {
-  k_logp_warp<T, NE><<<unsigned((a.rows + kRowsPerBlock - 1) / kRowsPerBlock), 32 * kRowsPerBlock, 0, st>>>(a);
+  k_logp_warp<T, NE><<<unsigned((int64_t(a.rows) + kRowsPerBlock - 1) / kRowsPerBlock), 32 * kRowsPerBlock, 0, st>>>(a);
 }
 
-template <class T>
+// Rows of up to 2048 values: a warp each, with the least multiple of 8 values
+// a lane that holds one.
+template <class T, int NE = 8>
 cudaError_t logp_t(const LogpArgs& a, cudaStream_t st) {
-  if (a.vocab <= 32 * 16)
-    warp_rows<T, 16>(a, st);
-  else if (a.vocab <= 32 * 34)
-    warp_rows<T, 34>(a, st);
-  else if (a.vocab <= 32 * 48)
-    warp_rows<T, 48>(a, st);
-  else if (a.vocab <= 32 * 64)
-    warp_rows<T, 64>(a, st);
-  else
+  if constexpr (NE <= 64) {
+    if (a.vocab > 32 * NE) return logp_t<T, NE + 8>(a, st);
+    warp_rows<T, NE>(a, st);
+    return cudaGetLastError();
+  } else {
     return rows_t<T, kBlock>(a, st);
-  return cudaGetLastError();
+  }
 }
 
 }  // namespace
