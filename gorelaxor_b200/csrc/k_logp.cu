@@ -240,10 +240,10 @@ __device__ __forceinline__ V peer(const V* p, uint32_t rank) {
 // memory. Three blocks of 512 threads an SM: 107 us for 2048 rows of 100003
 // bfloat16 logits (two blocks with four vectors a turn 121, five of 256
 // threads 123).
-constexpr int kCand = 1024, kBlock = 512;
+constexpr int kCand = 1024, kBlock = 512, kSmallBlock = 128;
 
 template <class T, int NT>
-__global__ void __launch_bounds__(NT, 3) k_logp(LogpArgs a, int S) {
+__global__ void __launch_bounds__(NT, 1536 / NT) k_logp(LogpArgs a, int S) {
   constexpr int V = 16 / sizeof(T), U = 2, NW = NT / 32;
   __shared__ float wm[NW], wn[NW], wz[NW], wt[NW];
   __shared__ u64 wk[NW];
@@ -576,7 +576,12 @@ cudaError_t logp_t(const LogpArgs& a, cudaStream_t st) {
     warp_rows<T, NE>(a, st);
     return cudaGetLastError();
   } else {
-    return rows_t<T, kBlock>(a, st);
+    // A block's exchanges take about 6 us whatever the row's length: many
+    // short rows go to more, smaller blocks. 4000 rows of float32 values, us
+    // with 512 threads and with 128: of 4000 values 64 and 27, of 16000 89
+    // and 68, of 32000 123 and 125. 400 rows of 4000: 12 and 11, of 32000 15
+    // and 19; up to 32 rows 512 threads are the faster at any length.
+    return a.vocab <= 24 * 1024 && a.rows >= 2 * kSMs ? rows_t<T, kSmallBlock>(a, st) : rows_t<T, kBlock>(a, st);
   }
 }
 

@@ -99,6 +99,24 @@ def test_sizes(have_gpu, rows, vocab, dtype, top):
     check(x, rng.integers(0, vocab, rows), min(top, vocab), dtype=dtype)
 
 
+@pytest.mark.parametrize("vocab", [2049, 4100, 9001, 24576, 24577])
+@pytest.mark.parametrize("dtype,top", [("f32", 5), ("f16", 32), ("bf16", 0), ("f32", 32), ("bf16", 1)])
+def test_many_rows(have_gpu, vocab, dtype, top):
+    """Enough rows that smaller blocks take them, around the longest that do;
+    a few with equal values, masked values or none that is a number."""
+    rng = np.random.default_rng(vocab + top)
+    rows = 310 if vocab < 9001 else 297
+    x = rng.normal(0, 3, (rows, vocab)).astype(np.float32)
+    x[3] = 1.5                        # all alike
+    x[4, 10:] = -np.inf
+    x[5] = np.round(x[5])             # many alike
+    x[6, 7], x[7, vocab - 1] = np.nan, np.inf
+    x[8] = -np.inf
+    x[9, vocab - 1] = 60000.0
+    with np.errstate(invalid="ignore"):
+        check(x, rng.integers(0, vocab, rows), top, dtype=dtype, stride=vocab + 3, offset=1)
+
+
 @pytest.mark.parametrize("vocab", [50, 1030, 3001, 40000])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_strides_and_offsets(have_gpu, vocab, dtype):
