@@ -27,6 +27,31 @@ def test_rows_and_tiles(have_gpu, d, page, heads, kv_heads, mode, dtype, new):
     assert s.status.item() == 0
 
 
+@pytest.mark.parametrize("heads,kv_heads,d", [(20, 1, 64), (68, 2, 128), (130, 1, 64), (17, 1, 128)])
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_many_query_heads_to_a_key_head(have_gpu, heads, kv_heads, d, dtype):
+    """Single tokens whose key heads serve more than 16 query heads, slots
+    without tokens among them."""
+    lens = [1, 0, 64, 65, 300, 0, 17]
+    s = Side(lens, [1] * len(lens), heads=kv_heads, d=d, page=16, mode="pairs", seed=heads)
+    q = s.rng.normal(0, 1.5, (len(lens), heads, d)).astype(np.float32)
+    dt = getattr(torch, TORCH[dtype])
+    dq, out = up(q).to(dt), torch.full((len(lens), heads, d), 7.0, dtype=dt, device=DEV)
+    lse = torch.full((len(lens), heads), 7.0, device=DEV)
+    s.kv.attend(s.seqs(d_row0=None), heads, dq.data_ptr(), out.data_ptr(), dtype=dtype, d_lse=lse.data_ptr(),
+                stream=stream())
+    got, gl, qs = out.float().cpu().numpy(), lse.cpu().numpy(), dq.float().cpu().numpy()
+    for i, m in enumerate(lens):
+        if m == 0:
+            assert (got[i] == 0).all() and np.isneginf(gl[i]).all()
+            continue
+        want, wl, tol = attend(s.ref, s.table[i], m, qs[i:i + 1], s.rope, "pairs", half=dtype != "f32")
+        tol = tol[..., None] + 2.0**-11 * np.abs(want) * (dtype == "f16") + 2.0**-24 * (dtype == "f16")
+        assert (np.abs(got[i:i + 1] - want) <= tol).all(), i
+        assert (np.abs(gl[i] - wl[0]) <= 2.0**-19 * (np.abs(wl[0]) + 8)).all()
+    assert s.status.item() == 0
+
+
 @pytest.mark.parametrize("d,heads,kv_heads", [(64, 2, 2), (128, 8, 2)])
 def test_long_sequences_of_many_blocks(have_gpu, d, heads, kv_heads):
     s = Side([1500, 1101] + [20] * 20, [18, 3] + [18] * 20, heads=kv_heads, d=d, page=64, mode="halves", seed=d)
