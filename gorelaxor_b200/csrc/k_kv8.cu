@@ -1444,10 +1444,7 @@ cudaError_t attend_t(const Kv8Args& a, int type, const Kv8Attend& t, cudaStream_
   const int qtiles = int((int64_t(a.max_new) * group + 8 * NQ - 1) / (8 * NQ));
   const int64_t units = int64_t(a.n) * a.heads * qtiles;
   const int64_t parts = stretches(a, units, 16, 64);
-  // one part: many units with few keys, which with more than 16 queries are
-  // the tensor-core kernel's
-  if constexpr (NQ < 4)
-    if (parts == 1) return attend_launch<D, NQ, NP, 1>(a, type, t, units, qtiles, 1, st);
+  if (parts == 1) return attend_launch<D, NQ, NP, 1>(a, type, t, units, qtiles, 1, st);
   // few units: wide blocks, two an SM; with more of them narrower ones are
   // the faster (48 sequences of 2000 keys and 4 heads: 40 us, wide ones 48)
   if constexpr (NQ == 1) {
@@ -1455,8 +1452,12 @@ cudaError_t attend_t(const Kv8Args& a, int type, const Kv8Attend& t, cudaStream_
     if (parts > 4 && units <= kSMs)
       return attend_launch<D, NQ, NP, WU>(a, type, t, units, qtiles, blocks_of(units, parts, WU, 2), st);
   }
-  int S = 1;
-  while (S < 16 && S * 4 < parts) S *= 2;
+  // several queries: one wave again (16 sequences of 8192 keys, 4 heads, 16
+  // queries: 53 us, with clusters of all the parts 101); one query a column,
+  // whose blocks are smaller, gains from more (ragged: 70 us, one wave 123)
+  int S = NQ > 1 ? blocks_of(units, parts, 4, 2) : 1;
+  if (NQ == 1)
+    while (S < 16 && S * 4 < parts) S *= 2;
   return attend_launch<D, NQ, NP, 4>(a, type, t, units, qtiles, S, st);
 }
 
@@ -1492,14 +1493,17 @@ cudaError_t attend_d(const Kv8Args& a, int type, const Kv8Attend& t, cudaStream_
   const int64_t rows = int64_t(a.max_new) * (t.heads / a.heads);  // queries that share a head's keys
   if (rows == 1) return attend1_d<D>(a, type, t, st);
   if (rows <= 8) return attend_t<D, 1, NP>(a, type, t, st);
-  // More than 16 queries go to the 5th-generation tensor core, 128 a block,
+  // More than 32 queries go to the 5th-generation tensor core, 128 a block,
   // unless few blocks would have long stretches of keys that these kernels
-  // split. Heads of 128, bfloat16, us here and there: 36 queries of 16 x 4
-  // heads over 512 keys 29 and 24, over 2048 100 and 45; of 4 x 4 heads over
-  // 2048 46 and 45, of 1 x 4 over 8192 34 and 140. 16 queries of 256 x 4 heads
-  // over 2048 keys: 168 and 302.
+  // split; more than 16 where one wave of blocks has few keys. 4 heads of 128,
+  // bfloat16, us here and there: 64 queries of 16 sequences over 2048 keys 58
+  // and 45, of 4 over 2048 31 and 45, over 512 26 and 23; 128 of 48 over 2048
+  // 214 and 94; 32 of 16 over 512 29 and 24, over 2048 40 and 45, of 128 over
+  // 512 67 and 72.
   const int64_t blocks = int64_t(a.n) * a.heads * ((rows + 127) / 128);
-  if (rows > 16 && (blocks >= kSMs / 4 || a.max_len <= 1024)) return launch_kv8_prompt(a, D, type, t, st);
+  const bool brief = a.max_len <= 512;
+  if (rows > 32 ? brief || blocks >= kSMs / 4 : rows > 16 && brief && blocks <= kSMs)
+    return launch_kv8_prompt(a, D, type, t, st);
   if (rows <= 16) return attend_t<D, 2, NP>(a, type, t, st);
   return attend_t<D, 4, NP>(a, type, t, st);
 }
@@ -1528,6 +1532,7 @@ void attend_init() {
   attend_attrs<D, 1, NP, kWide<D>>();
   attend_attrs<D, 2, NP, 1>();
   attend_attrs<D, 2, NP, 4>();
+  attend_attrs<D, 4, NP, 1>();
   attend_attrs<D, 4, NP, 4>();
 }
 
