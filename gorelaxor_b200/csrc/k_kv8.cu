@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(256, G == D / 8 ? 4 : 3)
   constexpr int N = G == C ? 1 : kItems;  // items a thread
   __shared__ uint32_t red[4 * 8];
   const int tid = threadIdx.x % G;
-  const uint32_t group = (blockIdx.x * 256u + threadIdx.x) / G;  // the launch has fewer than 2^31 units
+  const uint32_t group = kv8_append_group(blockIdx.x, threadIdx.x, G);
   const uint32_t parts = (2 * a.heads + per - 1) / per, rest = group / parts;
   const int hb = int(group - rest * parts) * per, he = min(hb + per, 2 * a.heads);
   const int i = min(int(rest / blocks), a.n), b = int(rest % blocks);
@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(256) k_kv8_copy_pages(Kv8Args a, int bytes, co
 template <int D, class T>
 cudaError_t append_t(const Kv8Args& a, const Kv8Rows& k, const Kv8Rows& v, cudaStream_t st) {
   const int page = 1 << a.plog;
-  const int blocks = (a.max_new + page - 2) / page + 1;  // pages that max_new tokens can touch
+  const int blocks = int(kv8_append_pages(a.max_new, page));
   const int64_t units = int64_t(a.n) * blocks * 2 * a.heads;
   const bool vec = aligned<T>(k, 4) && aligned<T>(v, 4);
   // One token to a sequence: as many threads as hold it. A warp while its
@@ -446,8 +446,7 @@ cudaError_t append_t(const Kv8Args& a, const Kv8Rows& k, const Kv8Rows& v, cudaS
   // there are blocks enough without.
   int per = 1;
   const auto grid = [&](int g) {
-    const int64_t groups = int64_t(a.n) * blocks * ((2 * a.heads + per - 1) / per);
-    return unsigned((groups * g + 255) / 256);
+    return kv8_append_grid(int64_t(a.n) * blocks * ((2 * a.heads + per - 1) / per), g);
   };
   if (a.max_new == 1) {
     k_kv8_append<D, D / 8, T><<<grid(D / 8), 256, 0, st>>>(a, k, v, blocks, per, vec);

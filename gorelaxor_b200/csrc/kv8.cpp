@@ -136,8 +136,7 @@ int grx_kv8_append(const grx_kv8* kv, const grx_kv8_seqs* s, int type, const voi
   if (rc) return rc;
   if (nothing(a)) return GRX_OK;
   if (!k || !v) return fail(GRX_EINVAL, "grx_kv8_append: null keys or values");
-  const int64_t blocks = (int64_t(a.max_new) + kv->page_tokens - 2) / kv->page_tokens + 1;
-  if (a.n * blocks * 2 * a.heads > INT32_MAX)
+  if (a.n * kv8_append_pages(a.max_new, kv->page_tokens) * 2 * a.heads > INT32_MAX)
     return fail(GRX_ERANGE, "grx_kv8_append: too many pages for one call; append fewer tokens at a time");
   const OnDevice on(kv->device);
   if (on.rc) return on.rc;

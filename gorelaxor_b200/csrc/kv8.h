@@ -62,6 +62,19 @@ KV8_FN int kv8_page(const Kv8Args& a, int i, int b) {
   return p >= 0 && p < a.pages ? p : -1;
 }
 
+// Pages that max_new tokens of a sequence can touch.
+KV8_FN int64_t kv8_append_pages(int max_new, int page) { return (int64_t(max_new) + page - 2) / page + 1; }
+// The group of `threads` threads that thread `thread` of block `block` (of
+// 256 threads) belongs to. Groups are fewer than 2^31 (the entry point
+// refuses more); their threads need not be, so those are never counted.
+KV8_FN uint32_t kv8_append_group(uint32_t block, uint32_t thread, int threads) {
+  return block * uint32_t(256 / threads) + thread / uint32_t(threads);
+}
+// Blocks of 256 threads for `groups` groups of `threads` threads.
+KV8_FN uint32_t kv8_append_grid(int64_t groups, int threads) {
+  return uint32_t((groups + 256 / threads - 1) / (256 / threads));
+}
+
 // Rows of keys, values or queries in memory: element e of head h of row r
 // is at r·row + h·head + e.
 struct Kv8Rows {

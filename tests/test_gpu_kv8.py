@@ -453,3 +453,51 @@ def test_offsets_past_32_bits(have_gpu):
     s.same()
     s.attend(8)
     assert s.status.item() == 0
+
+
+@pytest.mark.parametrize("heads,d,page,new", [(1, 128, 16, 4096), (4, 64, 16, 4096)])
+def test_append_of_more_blocks_than_2_to_the_24(have_gpu, heads, d, page, new):
+    """One long prompt among 65534 single tokens: so many groups of threads
+    that a count of their threads passes 32 bits. Every sequence's token is
+    appended once, the first ones' and the last ones' too. (The numbering
+    itself is tested in test_kv8_host.py.)"""
+    n = 65535
+    rng = np.random.default_rng(heads)
+    lens = np.full(n, 2, np.int32)
+    lens[n // 2] = new
+    row0 = np.concatenate([[0], np.cumsum(np.where(lens == new, new, 1))]).astype(np.int32)
+    rows, width = int(row0[-1]), new // page
+    table = torch.full((n, width), -1, dtype=torch.int32)
+    table[:, 0] = torch.arange(n, dtype=torch.int32)
+    table[n // 2] = torch.arange(n, n + width, dtype=torch.int32)
+    table[n - 1, 0] = n // 2  # the page that the long one does not use
+    t, ln, r0 = table.to(DEV), up(lens), up(row0)
+    pools = [torch.randint(-127, 128, (n + width, heads, page, d), dtype=torch.int8, device=DEV) for _ in range(2)]
+    scale = torch.full((n + width, heads, 2), 1 / 254, device=DEV)
+    held = [p[:, :, 0].clone() for p in pools]
+    kv = torch.from_numpy(rng.normal(0, 1, (rows, 2, heads, d)).astype(np.float32)).to(DEV)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    c = g.KV8(pools[0].data_ptr(), pools[1].data_ptr(), scale.data_ptr(), n + width, page, heads, d)
+    seqs = g.KV8Seqs(n, t.data_ptr(), width, ln.data_ptr(), new, d_row0=r0.data_ptr(), rows=rows, max_new=new,
+                     d_status=status.data_ptr())
+    hd = heads * d
+    c.append(seqs, kv.data_ptr(), kv.data_ptr() + 4 * hd, k_strides=(2 * hd, d), v_strides=(2 * hd, d), stream=stream())
+    assert status.item() == 0
+    # the single tokens: slot 1 of their pages, whose slot 0 is rounded to the new scale once
+    at = torch.cat([torch.arange(n // 2), torch.arange(n // 2 + 1, n - 1), torch.tensor([n // 2])]).to(DEV)
+    x = torch.cat([kv[:n // 2], kv[n // 2 + new:]])
+    for j in range(2):
+        amax = x[:, j].abs().amax(-1).double() / 127
+        want = torch.maximum(amax.float(), torch.tensor(1 / 254, device=DEV))
+        assert torch.equal(scale[at, :, j], want)
+        q = (x[:, j].double() / want.double()[..., None]).round().clamp(-127, 127).to(torch.int8)
+        assert torch.equal(pools[j][at, :, 1], q)
+        old = (held[j][at].double() * float(np.float32(1 / 254)) / want.double()[..., None]).round().to(torch.int8)
+        assert torch.equal(pools[j][at, :, 0], old)
+    # the long prompt
+    y = kv[n // 2:n // 2 + new].view(width, page, 2, heads, d)
+    for j in range(2):
+        want = (y[:, :, j].abs().amax((1, -1)).double() / 127).float()
+        assert torch.equal(scale[n:, :, j], want)
+        q = (y[:, :, j].double() / want.double()[:, None, :, None]).round().clamp(-127, 127).to(torch.int8)
+        assert torch.equal(pools[j][n:].transpose(1, 2), q)
