@@ -219,7 +219,8 @@ __global__ void __launch_bounds__(256, G == D / 8 ? 4 : 3)
     items = held = 0;
   }
   // the unit's largest of numbers that are not negative, as their bits
-  // compare (NaN above all). `round` picks the place of its exchange: two for
+  // compare (NaN above all). Every lane of a warp is here (a group of fewer
+  // than 32 threads has one unit, so its warp's lanes take the same steps). `round` picks the place of its exchange: two for
   // a head and others for the next, since a head may have one exchange alone,
   // and a warp is then past it while another reads
   auto largest = [&](float m, int round) {
@@ -302,7 +303,11 @@ __global__ void __launch_bounds__(256, G == D / 8 ? 4 : 3)
     }
     // what is not rotated is exact as it is (and a 32-bit number over 127 is
     // never near the middle of two others: its digits repeat every seven bits)
-    const float fresh = mode == ROPE_NONE && !slow ? __fdiv_rn(top, 127.f) : largest(mine, turn + 1);
+    const bool exact = mode == ROPE_NONE && !slow;
+    float fresh = 0.f;
+    // a warp of several units makes the exchange in step, whichever need it
+    if (G < 32 || !exact) fresh = largest(mine, turn + 1);
+    if (exact) fresh = __fdiv_rn(top, 127.f);
     const float scale = isnan(old) || isnan(fresh) ? __int_as_float(0x7fc00000) : fmaxf(old, fresh);
     const bool some = scale > 0.f;  // not 0, and a number
     slow = slow || scale < kTiny;

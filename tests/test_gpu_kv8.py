@@ -501,3 +501,21 @@ def test_append_of_more_blocks_than_2_to_the_24(have_gpu, heads, d, page, new):
         assert torch.equal(scale[n:, :, j], want)
         q = (y[:, :, j].double() / want.double()[:, None, :, None]).round().clamp(-127, 127).to(torch.int8)
         assert torch.equal(pools[j][n:].transpose(1, 2), q)
+
+
+@pytest.mark.parametrize("heads", [1, 2, 3, 5])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("mode", ["none", "pairs", "halves"])
+def test_append_units_of_one_warp_that_differ(have_gpu, heads, d, mode):
+    """Single tokens, several units (a head's keys or values) to a warp: keys
+    that are rotated beside values that are not, and ordinary numbers beside
+    tiny, huge and non-finite ones in every order of sequences and heads."""
+    n = 24
+    s = Side(list(range(1, n + 1)), [1] * n, heads=heads, d=d, mode=mode, seed=heads)
+    kv = s.rng.normal(0, 1, (n, 2, heads, d)).astype(np.float32)
+    by = np.array([1, 1e-36, 1, 1e37, 1, 1e-42, 0, 1], np.float32)
+    kv *= by[s.rng.integers(0, 8, (n, 2, heads))][..., None]
+    kv[5, 0, 0, 3], kv[11, 1, heads - 1, d - 1] = np.inf, np.nan
+    s.append(kv, d_row0=None)
+    s.same()
+    assert np.isnan(s.ref.scale).sum() == 2 and s.status.item() == 0
