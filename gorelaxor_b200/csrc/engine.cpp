@@ -1479,8 +1479,9 @@ static int kv8_setup(grx_streams* s, const grx_voice* const* voices, int page) {
     for (int u = 0; u < nv; u++)
       for (int j = 0; j < 2; j++) {
         const size_t P = size_t(len[size_t(u)]) * d;
-        CK(cudaMemcpy(rows + j * R * d + size_t(row0[size_t(u)]) * d, &each[size_t(u)]->kv[(size_t(l) * 2 + j) * P],
-                      sizeof(float) * P, cudaMemcpyHostToDevice));
+        // behind the append of the layer before, whose rows these replace
+        CK(cudaMemcpyAsync(rows + j * R * d + size_t(row0[size_t(u)]) * d, &each[size_t(u)]->kv[(size_t(l) * 2 + j) * P],
+                           sizeof(float) * P, cudaMemcpyHostToDevice, s->st));
       }
     Kv8Args a = kv8_layer(s, l);
     a.n = nv;
@@ -1498,8 +1499,8 @@ static int kv8_setup(grx_streams* s, const grx_voice* const* voices, int page) {
     k.row = v.row = d;
     k.head = v.head = 64;
     CK(launch_kv8_append(a, 64, GRX_F32, k, v, s->st));
-    CK(cudaStreamSynchronize(s->st));
   }
+  CK(cudaStreamSynchronize(s->st));
   return GRX_OK;
 }
 
@@ -1602,6 +1603,7 @@ static int streams_create_one(grx_flowlm* m, int n, const grx_voice* const* voic
   CK(cudaMemcpy(s->pos0, p0.data(), sizeof(int) * size_t(n), cudaMemcpyHostToDevice));
   rc = page ? kv8_setup(s.get(), voices, page) : frame1_setup(s.get());
   if (rc) return rc;
+  CK(copies_done());
   rc = grx_streams_reset(s.get());
   if (rc) return rc;
   rc = build_graph(s.get());

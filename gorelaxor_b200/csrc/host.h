@@ -20,6 +20,13 @@ const std::string& last_error_message();
 // Once per device: kernel attributes (dynamic shared memory opt-ins).
 int device_init(int dev);
 
+// Waits for the current device's legacy stream. cudaMemcpy from pageable
+// memory, cudaMemcpy on the device and cudaMemset may return before the
+// device's memory is written, and nothing orders them before work on the
+// models' and sets' own (non-blocking) streams: whoever uses them calls this
+// before that work.
+inline cudaError_t copies_done() { return cudaStreamSynchronize(cudaStreamLegacy); }
+
 // Device allocations of one owner, freed together on its device.
 struct Arena {
   int dev = 0;
@@ -42,7 +49,7 @@ struct Arena {
   template <class T>
   T* upload(const T* h, size_t n, int* rc) {
     T* p = alloc<T>(n, rc);
-    if (p && cudaMemcpy(p, h, n * sizeof(T), cudaMemcpyHostToDevice) != cudaSuccess)
+    if (p && (cudaMemcpy(p, h, n * sizeof(T), cudaMemcpyHostToDevice) != cudaSuccess || copies_done() != cudaSuccess))
       *rc = fail(GRX_ECUDA, "upload failed");
     return p;
   }

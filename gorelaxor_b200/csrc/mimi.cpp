@@ -609,6 +609,7 @@ int set_init(grx_mimi_streams* s, const MimiSizes& z, size_t positions, const MC
       h[R + 2 * N + i] = int(i);
     }
     CK(cudaMemcpy(stat, h.data(), sizeof(int) * h.size(), cudaMemcpyHostToDevice));
+    CK(copies_done());
     s->rowslot = stat;
     s->crow0 = stat + R;
     s->cT = stat + R + N;

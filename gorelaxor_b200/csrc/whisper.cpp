@@ -452,7 +452,7 @@ int ws1_check(grx_whisper_batch* b) {
   int e = 0;
   CK(cudaMemcpy(&e, b->ws1_err, sizeof e, cudaMemcpyDeviceToHost));
   if (!e) return GRX_OK;
-  CK(cudaMemset(b->ws1_err, 0, sizeof(int)));
+  CK(cudaMemsetAsync(b->ws1_err, 0, sizeof(int), b->st));
   return fail(GRX_ETIMEDOUT, "the persistent Whisper step gave up on a grid barrier after its one-second limit");
 }
 
@@ -740,6 +740,7 @@ int grx_whisper_load(const void* bytes, size_t len, int device, grx_whisper** ou
   v.exact_rows = m->ar.alloc<unsigned long long>(1, &rc);
   if (rc) return rc;
   CK(cudaMemset(v.exact_rows, 0, sizeof(unsigned long long)));
+  CK(copies_done());
   *out = m.release();
   return GRX_OK;
 }
@@ -830,6 +831,7 @@ int grx_whisper_batch_create(grx_whisper* m, int n, grx_whisper_batch** out) {
   r.row_tok = b->row_tok;
   rc = ws1_setup(b.get());
   if (rc) return rc;
+  CK(copies_done());
   *out = b.release();
   return GRX_OK;
 }
@@ -1189,7 +1191,7 @@ static int run(grx_whisper_batch* b, int steps) {
   if (b->ws1) {  // the whole run in one launch
     if (b->ws1_out != b->run_out) {
       CK(cudaStreamSynchronize(b->st));
-      CK(cudaMemcpy(&b->ws1_args->out, &b->run_out, sizeof(int*), cudaMemcpyHostToDevice));
+      CK(cudaMemcpyAsync(&b->ws1_args->out, &b->run_out, sizeof(int*), cudaMemcpyHostToDevice, b->st));
       b->ws1_out = b->run_out;
     }
     CK(cudaMemsetAsync(b->ws1_bar, 0, sizeof(unsigned), b->st));
@@ -1253,14 +1255,14 @@ int grx_whisper_watchdog_test(grx_whisper_batch* b) {
   const int one = 1, zero = 0;
   CK(cudaStreamSynchronize(b->st));
   if (b->ws1_out != b->run_out) {
-    CK(cudaMemcpy(&b->ws1_args->out, &b->run_out, sizeof(int*), cudaMemcpyHostToDevice));
+    CK(cudaMemcpyAsync(&b->ws1_args->out, &b->run_out, sizeof(int*), cudaMemcpyHostToDevice, b->st));
     b->ws1_out = b->run_out;
   }
-  CK(cudaMemcpy(&b->ws1_args->stall, &one, sizeof one, cudaMemcpyHostToDevice));
-  CK(cudaMemset(b->ws1_bar, 0, sizeof(unsigned)));
+  CK(cudaMemcpyAsync(&b->ws1_args->stall, &one, sizeof one, cudaMemcpyHostToDevice, b->st));
+  CK(cudaMemsetAsync(b->ws1_bar, 0, sizeof(unsigned), b->st));
   const cudaError_t e = launch_wstep1(b->ws1_args, b->ws1_grid, b->ws1_smem, b->pos, 1, b->st);
   const cudaError_t e2 = cudaStreamSynchronize(b->st);
-  CK(cudaMemcpy(&b->ws1_args->stall, &zero, sizeof zero, cudaMemcpyHostToDevice));
+  CK(cudaMemcpyAsync(&b->ws1_args->stall, &zero, sizeof zero, cudaMemcpyHostToDevice, b->st));
   CK(e);
   CK(e2);
   return ws1_check(b);

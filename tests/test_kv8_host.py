@@ -1,9 +1,13 @@
 """The host's side of the 8-bit paged cache's calls, without a GPU: the index
-arithmetic that kernels and host share, compiled here."""
+arithmetic that kernels and host share, compiled here; and calls on a CUDA
+runtime that writes launches down instead of running them (fake_cuda.c)."""
 
 import os
 import subprocess
+import sys
 from pathlib import Path
+
+import pytest
 
 ROOT = Path(__file__).resolve().parents[1]
 
@@ -42,3 +46,98 @@ def test_append_groups_past_2_to_the_24_blocks(tmp_path):
     for (int64_t t : {int64_t(1), int64_t(2), int64_t(page), int64_t(page) + 1, int64_t(4096), int64_t(2147483647)})
       if (kv8_append_pages(int(t), page) != (page - 1 + t - 1) / page + 1) std::puts("pages");""")
     assert out == []
+
+
+HEAD = """
+import ctypes as C
+import dataclasses, sys
+import numpy as np
+import gorelaxor_b200 as g
+from gorelaxor_b200 import synth
+from tests.helpers import SMALL, voice_kv
+fake = C.CDLL(None)
+fake.fake_first_unordered.restype = C.c_char_p
+
+def launched():
+    name, grid, out = C.create_string_buffer(400), (C.c_uint * 3)(), []
+    for i in range(fake.fake_launches()):
+        fake.fake_launch(i, name, 400, grid)
+        out.append((name.value.decode(), tuple(grid)))
+    return out
+
+def flow(n=3, positions=lambda i: 5 + 11 * i):
+    cfg = synth.FlowLMConfig(**SMALL)
+    gm = g.FlowLM(synth.flowlm_gguf(cfg, synth.flowlm_tensors(cfg, 0)))
+    return cfg, gm, [gm.voice(voice_kv(cfg, positions(i), 1 + i)) for i in range(n)]
+"""
+
+
+@pytest.fixture(scope="session")
+def fake(tmp_path_factory):
+    so = tmp_path_factory.mktemp("fake") / "libfakecuda.so"
+    subprocess.run(["gcc", "-shared", "-fPIC", "-O1", "-Wall", "-o", str(so), str(ROOT / "tests/fake_cuda.c")], check=True)
+
+    def run(body):
+        env = {**os.environ, "LD_PRELOAD": str(so), "PYTHONPATH": str(ROOT)}
+        r = subprocess.run([sys.executable, "-c", HEAD + body], capture_output=True, text=True, cwd=ROOT, env=env,
+                           timeout=120)
+        assert r.returncode == 0, r.stdout + r.stderr
+        return r.stdout.split("\n")
+
+    return run
+
+
+SETS = {
+    "flow lm, 8 bits": """
+cfg, gm, vs = flow()
+for page in (16, 64):
+    st = g.Streams(gm, vs + vs[:1], 20, kv8_page=page)
+    st.text([[1, 2, 3], [], [4], [5] * 9])
+    st.step(np.zeros((4, cfg.ldim), np.float32))
+    st.kv(2)
+    st.reset()
+""",
+    "flow lm": """
+cfg, gm, vs = flow()
+for n in (1, 3):
+    st = g.Streams(gm, vs[:n], 20)
+    st.text([[1, 2, 3]] * n)
+    st.step(np.zeros((n, cfg.ldim), np.float32))
+    st.kv(n - 1)
+    st.reset()
+st = g.Streams(gm, (vs * 50)[:130], 20)
+st.step(np.zeros((130, cfg.ldim), np.float32))
+""",
+    "whisper": """
+cfg = synth.WhisperConfig(n_state=128, n_head=2, n_text_layer=2, n_text_ctx=64)
+gm = g.Whisper(synth.whisper_ggml(cfg, synth.whisper_tensors(cfg, 0), synth.whisper_words(cfg)))
+for n in (1, 3):
+    b = g.WhisperBatch(gm, n)
+    b.set_audio(np.stack([synth.whisper_encoder_out(1 + i, cfg) for i in range(n)]))
+    b.prompt([gm.prev, 100, 200, gm.sot], 3)
+    b.run(2)
+    b.score([1] * n, 3)
+    b.run(7)
+""",
+    "mimi": """
+mc = synth.MimiConfig()
+gm = g.Mimi(synth.flowlm_gguf(synth.FlowLMConfig(ldim=32), synth.mimi_tensors(mc, 32, 0), mimi=mc))
+s = g.MimiStreams(gm, 2, max_frames=4)
+s.decode(np.zeros((2, 32), np.float32))
+""",
+    "tdt": """
+cfg = synth.TDTConfig(H=128, V=65, J=96, D=128)
+gm = g.TDT(synth.tdt_gguf(cfg, synth.tdt_tensors(cfg, 0)))
+b = g.TDTBatch(gm, 2, 8, 256)
+b.decode(np.zeros((2, 8, 128), np.float32), [8, 8])
+""",
+}
+
+
+@pytest.mark.parametrize("what", list(SETS))
+def test_set_up_copies_are_waited_for(fake, what):
+    """Copies that the legacy stream orders alone (from pageable memory, on
+    the device) are waited for before a set's own streams use what they
+    brought."""
+    n, first = fake(SETS[what] + "print(fake.fake_unordered()); print(fake.fake_first_unordered().decode())")[:2]
+    assert (int(n), first) == (0, "")
