@@ -222,8 +222,9 @@ cudaError_t kv8_attention(const Kv8Args& a, const float* qkv, int d, int8_t* q8,
 
 // The kernel sequence of one frame for all streams (see grx.h): flowLM.step
 // (lm.go:185-195 → nn.go:142-182) then flowHead.sample (lm.go:108-160).
-// Returns the number of kernels launched.
-int enqueue_frame(grx_streams* s) {
+// Returns the number of kernels launched; *refused becomes the first error of
+// a launch that says so itself (the others leave theirs as the last error).
+int enqueue_frame(grx_streams* s, cudaError_t* refused) {
   grx_flowlm* m = s->m;
   const int M = s->n, d = m->d, fd = m->fd;
   cudaStream_t st = s->st;
@@ -258,7 +259,8 @@ int enqueue_frame(grx_streams* s) {
       e.y = s->kv8.qkv;
       e.ldy = 3 * d;
       launch_q8_product(s->xq, s->xs, M, ly.qkv, e, st);
-      kv8_attention(kv8_layer(s, l), s->kv8.qkv, d, s->xq, s->xs, st);
+      const cudaError_t e8 = kv8_attention(kv8_layer(s, l), s->kv8.qkv, d, s->xq, s->xs, st);
+      if (*refused == cudaSuccess) *refused = e8;
       k++;
     } else {
       EpiArgs e;
@@ -606,10 +608,18 @@ int build_graph(grx_streams* s) {
   for (int n : {1, kGraphFrames}) {
     CK(cudaStreamBeginCapture(s->st, cudaStreamCaptureModeThreadLocal));
     int k = 0;
-    for (int f = 0; f < n; f++) k = enqueue_frame(s);
+    cudaError_t refused = cudaSuccess;
+    cudaGetLastError();  // the calls up to here have been checked
+    for (int f = 0; f < n; f++) k = enqueue_frame(s, &refused);
     cudaGraph_t g = nullptr;
     cudaError_t e = cudaStreamEndCapture(s->st, &g);
-    if (e != cudaSuccess) return fail(GRX_ECUDA, std::string("graph capture: ") + cudaGetErrorString(e));
+    // a refused launch leaves no node: the frame without it must not be replayed
+    const cudaError_t last = cudaGetLastError();
+    if (e == cudaSuccess) e = refused != cudaSuccess ? refused : last;
+    if (e != cudaSuccess) {
+      if (g) cudaGraphDestroy(g);
+      return fail(GRX_ECUDA, std::string("graph capture of a frame: ") + cudaGetErrorString(e));
+    }
     if (n == 1) {
       s->graph = g;
       CK(cudaGraphInstantiate(&s->exec, g, 0));

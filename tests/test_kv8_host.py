@@ -141,3 +141,42 @@ def test_set_up_copies_are_waited_for(fake, what):
     brought."""
     n, first = fake(SETS[what] + "print(fake.fake_unordered()); print(fake.fake_first_unordered().decode())")[:2]
     assert (int(n), first) == (0, "")
+
+
+@pytest.mark.parametrize("page", [None, 16])
+@pytest.mark.parametrize("kernel,nth", [("k_ln", 0), ("k_q8", 1), ("k_kv8_append", 0), ("k_kv8_append", 9),
+                                        ("k_kv8_attend", 1), ("k_flin", 3)])
+def test_a_refused_launch_fails_the_set(fake, page, kernel, nth):
+    """A launch that the runtime refuses while a frame is captured leaves no
+    node in its graph: the set is not made. (Appends before the capture, of
+    the voice's two layers, are refused at once.)"""
+    if page is None and "kv8" in kernel:
+        pytest.skip("float32 caches have no such kernel")
+    out = fake(f"""
+cfg, gm, vs = flow(2)
+fake.fake_fail(b"{kernel}", {nth})
+try:
+    g.Streams(gm, vs, 20, kv8_page={page})
+    print("made")
+except g.GrxError as e:
+    print(e.code, e)
+fake.fake_fail(b"", -1)
+st = g.Streams(gm, vs, 20, kv8_page={page})  # nothing is left of the refusal
+st.step(np.zeros((2, cfg.ldim), np.float32))
+""")
+    assert out[0].startswith("-4 ") and "invalid configuration" in out[0], out
+
+
+def test_a_refused_launch_fails_a_text(fake):
+    out = fake("""
+cfg, gm, vs = flow(2)
+st = g.Streams(gm, vs, 20, kv8_page=16)
+for kernel, nth in (("k_q8", 0), ("k_kv8_append", 1), ("k_kv8_attend", 0)):
+    fake.fake_fail(kernel.encode(), nth)
+    try:
+        st.text([[1, 2], [3]])
+        print("ok")
+    except g.GrxError as e:
+        print(e.code)
+""")
+    assert out[:3] == ["-4"] * 3
