@@ -469,8 +469,10 @@ cudaError_t read_t(const Kv8Args& a, const Kv8Rows& k, const Kv8Rows& v, cudaStr
   const bool vec = (!k.p || aligned<T>(k, 16 / sizeof(T))) && (!v.p || aligned<T>(v, 16 / sizeof(T)));
   int xlog = 4;  // threads over a token
   while (xlog < 8 && 1 << xlog < 2 * a.heads * (D / int(16 / sizeof(T)))) xlog++;
-  const int tokens = kReads * (256 >> xlog);
-  k_kv8_read<D, T><<<dim3(unsigned((a.max_new - 1) / tokens + 1), a.n), 256, 0, st>>>(a, k, v, xlog, vec);
+  // no sequence has more tokens than its row of the table has room for, at
+  // most 2^31 − 64: the kernel's token numbers stay in 32 bits with any max_new
+  const int most = int(std::min<int64_t>(a.max_new, int64_t(a.width) << a.plog)), tokens = kReads * (256 >> xlog);
+  k_kv8_read<D, T><<<dim3(unsigned((most - 1) / tokens + 1), a.n), 256, 0, st>>>(a, k, v, xlog, vec);
   return cudaGetLastError();
 }
 

@@ -519,3 +519,14 @@ def test_append_units_of_one_warp_that_differ(have_gpu, heads, d, mode):
     s.append(kv, d_row0=None)
     s.same()
     assert np.isnan(s.ref.scale).sum() == 2 and s.status.item() == 0
+
+
+def test_read_with_the_largest_bounds(have_gpu):
+    """rows and max_new are bounds: with the largest numbers there the same
+    tokens are read."""
+    s = Side([5, 50, 33], [5, 17, 20], heads=2, d=64, seed=2)
+    got = [torch.zeros(s.rows, 2, 64, device=DEV) for _ in range(4)]
+    s.kv.read(s.seqs(), got[0].data_ptr(), got[1].data_ptr(), stream=stream())
+    s.kv.read(s.seqs(rows=2**31 - 1, max_new=2**31 - 1), got[2].data_ptr(), got[3].data_ptr(), stream=stream())
+    assert torch.equal(got[0], got[2]) and torch.equal(got[1], got[3]) and got[0].abs().sum() > 0
+    assert s.status.item() == 0

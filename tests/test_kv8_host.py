@@ -180,3 +180,19 @@ for kernel, nth in (("k_q8", 0), ("k_kv8_append", 1), ("k_kv8_attend", 0)):
         print(e.code)
 """)
     assert out[:3] == ["-4"] * 3
+
+
+@pytest.mark.parametrize("width,max_new", [(2, 2**31 - 1), (2**25 - 1, 2**31 - 1), (2**25 - 1, 100), (2, 1)])
+def test_reads_of_any_max_new(fake, width, max_new):
+    """max_new may be any bound, the largest number too: the blocks go no
+    further than the table's tokens, so the last block's token numbers have 32
+    bits."""
+    out = fake(f"""
+c = g.KV8(4096, 4096, 4096, 8, 64, 2, 64)
+s = g.KV8Seqs(2, 4096, {width}, 4096, 32, d_row0=4096, rows=2**31 - 1, max_new={max_new})
+c.read(s, 4096, 4096)
+print(launched()[0][1][0])
+""")
+    per, most = 16, min(max_new, 64 * width)  # tokens a block: 64 threads to a token of two heads' float32
+    assert int(out[0]) == -(-most // per)
+    assert int(out[0]) * per < 2**31
