@@ -243,14 +243,15 @@ __global__ void __launch_bounds__(544, 1)
       load_row<D>(t.q.p, off, type, vec, there, x);
       rotate16<D>(x, a, p0 + tq, tg);
       const float amax = group_amax<D>(x, FULL);
-      const float to = __fmul_rn(lift_row<D>(x, amax), kTo14);
+      // the sign of the scale goes into the query, so that the row's factor has none
+      const float to = __fmul_rn(lift_row<D>(x, amax), t.scale < 0.f ? -kTo14 : kTo14);
 #pragma unroll
       for (int j = 0; j < H2; j++) {
         uint32_t hi[8], lo[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           // a row that is no number: 0 here, and its factor is none
-          const float y0 = to > 0.f ? __fmul_rn(x[j][2 * e], to) : 0.f, y1 = to > 0.f ? __fmul_rn(x[j][2 * e + 1], to) : 0.f;
+          const float y0 = to != 0.f ? __fmul_rn(x[j][2 * e], to) : 0.f, y1 = to != 0.f ? __fmul_rn(x[j][2 * e + 1], to) : 0.f;
           hi[e] = pack_f16(y0, y1);
           lo[e] = pack_f16(__fsub_rn(y0, __half2float(__ushort_as_half(hi[e] & 0xffff))),
                            __fsub_rn(y1, __half2float(__ushort_as_half(hi[e] >> 16))));
@@ -264,7 +265,7 @@ __global__ void __launch_bounds__(544, 1)
         }
       }
       if (tg == 0)
-        rowf[r] = __fmul_rn(__fmul_rn(amax, 256.f / kQueryUnits), __fmul_rn(t.scale, 1.44269504f));
+        rowf[r] = __fmul_rn(__fmul_rn(amax, 256.f / kQueryUnits), __fmul_rn(fabsf(t.scale), 1.44269504f));
     }
     fence_async();
   };
@@ -450,11 +451,25 @@ __global__ void __launch_bounds__(544, 1)
       fence_after();
       float2 c[4];
       float wide = 0.f;
+      uint32_t turned = 0;  // groups of sixteen keys whose scale is below 0: their products change sign, the scale has none
 #pragma unroll
       for (int g = 0; g < 4; g++) {
         c[g] = scales[(j & 3) * 4 + g];
         wide = fmaxf(wide, c[g].y);
+        if (c[g].x < 0.f && c[g].x != ninf()) {
+          turned |= 1u << g;
+          c[g].x = -c[g].x;
+        }
       }
+      // the 32 products of half u of the tile
+      const auto turn = [&](int u, float* x) {
+#pragma unroll
+        for (int g = 0; g < 2; g++)
+          if (turned >> (2 * u + g) & 1) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) x[16 * g + e] = -x[16 * g + e];
+          }
+      };
       const bool edge = c[0].x == ninf() || c[1].x == ninf() || c[2].x == ninf() || c[3].x == ninf() || key0 < in_lo ||
                         key0 + kKeys - 1 > pmin;
       // bit e: this row sees key e of the tile
@@ -473,13 +488,14 @@ __global__ void __launch_bounds__(544, 1)
       uint32_t s[32];
       f2* x2 = reinterpret_cast<f2*>(s);
       float* x = reinterpret_cast<float*>(s);
-      // the largest score: a group's largest product times its factor, which
-      // is not negative
+      // the largest score: a group's largest product times its factor, from
+      // which every sign has been taken
       float top = ninf();
 #pragma unroll
       for (int u = 0; u < 2; u++) {
         tmem_ld32(my_s + 32 * u, s);
         wait_ld();
+        if (turned) turn(u, x);
         if (edge) {
 #pragma unroll
           for (int e = 0; e < 32; e++)
@@ -540,6 +556,7 @@ __global__ void __launch_bounds__(544, 1)
           __syncwarp();
           if (lane == 0) bar_arrive(taken(j));
         }
+        if (turned) turn(u, x);
         const float2 c0 = c[2 * u], c1 = c[2 * u + 1];
         const f2 f0 = f2dup(__fmul_rn(f, c0.x)), f1 = f2dup(__fmul_rn(f, c1.x));
 #pragma unroll
