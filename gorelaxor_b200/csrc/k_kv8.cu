@@ -661,11 +661,9 @@ struct Pages {
     ahead = of(c0 + 32 + lane);
   }
   __device__ __forceinline__ int of(int c) const { return c < c1 ? kv8_page(a, i, c >> (a.plog - 4)) : -1; }
-  // A scale that is not finite (or, of values, below 0) as NaN; no page: 0.
+  // No page: 0.
   __device__ __forceinline__ float2 scale_of(int p) const {
-    if (p < 0) return make_float2(0.f, 0.f);
-    const float2 s = scales[int64_t(p) * a.heads];
-    return make_float2(isfinite(s.x) ? s.x : qnan(), s.y >= 0.f && isfinite(s.y) ? s.y : qnan());
+    return p < 0 ? make_float2(0.f, 0.f) : sound_scales(scales[int64_t(p) * a.heads]);
   }
   __device__ __forceinline__ void move(int lane) {  // to the next 32 tiles
     base += 32;
@@ -1257,7 +1255,7 @@ __global__ void __launch_bounds__(32 * Shape1<D, WU>::warps, Shape1<D, WU>::bloc
       x = hide ? ninf() : __fmaf_rn(s, fs, -m);
     }
     const float w = x > 0.f ? 1.f : ex2(x);  // above 0 by the rounding of the reference
-    l = __fadd_rn(l, __fmaf_rn(0.f, sv, w));  // a scale that is no number makes the sum none
+    l = __fadd_rn(l, w);
     // n + 2^23: the bytes of n as they lie
     const uint32_t y = __float_as_uint(__fmaf_rn(__fmul_rn(w, __fmul_rn(sv, toW)), kOne, 8388608.f));
     const uint32_t yt = transpose8(y);

@@ -338,11 +338,10 @@ __global__ void __launch_bounds__(544, 1)
     // tiles at a time, and the pages of the next eight
     const int plast = (sp.len + 15) >> 4;
     const auto page_of = [&](int c) { return c < plast ? kv8_page(a, i, c >> (a.plog - 4)) : -1; };
-    // −inf where there is no page, NaN for what is no scale
+    // −inf where there is no page
     const auto scale_of = [&](int page) {
       if (page < 0) return make_float2(ninf(), 0.f);
-      const float2 s = reinterpret_cast<const float2*>(a.scale)[int64_t(page) * a.heads + h];
-      return make_float2(isfinite(s.x) ? s.x : qnan(), s.y >= 0.f && isfinite(s.y) ? s.y : qnan());
+      return sound_scales(reinterpret_cast<const float2*>(a.scale)[int64_t(page) * a.heads + h]);
     };
     int c0 = tb * 4, page = page_of(c0 + lane), ahead = page_of(c0 + 32 + lane);
     if (page < 0 && c0 + lane < plast && c0 + lane <= pmax >> 4) report(a);

@@ -82,6 +82,13 @@ __device__ __forceinline__ void load_row(const void* p, int64_t off, int type, b
 
 __device__ __forceinline__ float ninf() { return __int_as_float(0xff800000); }
 __device__ __forceinline__ float qnan() { return __int_as_float(0x7fc00000); }
+// A page's scales of keys and values, both NaN where one is not finite or the
+// values' is below 0: then a query that sees the page has a sum, and with it
+// an output and a log-sum-exp, that are no numbers.
+__device__ __forceinline__ float2 sound_scales(float2 s) {
+  const bool sound = isfinite(s.x) && isfinite(s.y) && s.y >= 0.f;
+  return sound ? s : make_float2(qnan(), qnan());
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -204,7 +204,8 @@ int grx_kv8_read(const grx_kv8* kv, const grx_kv8_seqs* s, int type, void* k, in
  * 32 bits; the queries are rotated as the keys were. lse [rows][heads] (may
  * be NULL) gets log Σ e^(scale·q·k). A query that sees no key answers zeros
  * and −inf; one that is not finite, or sees a page whose scale is not (or
- * whose values' scale is below 0), answers NaN. out must not overlap q.
+ * whose values' scale is below 0), answers NaN, output and log-sum-exp both.
+ * out must not overlap q.
  * Results do not depend on timing. Queued on `stream`. */
 int grx_kv8_attend(const grx_kv8* kv, const grx_kv8_seqs* s, int type, int heads, const void* q, int64_t q_row,
                    int64_t q_head, float scale, int window, void* out, int64_t out_row, int64_t out_head, float* lse,

@@ -530,3 +530,26 @@ def test_read_with_the_largest_bounds(have_gpu):
     s.kv.read(s.seqs(rows=2**31 - 1, max_new=2**31 - 1), got[2].data_ptr(), got[3].data_ptr(), stream=stream())
     assert torch.equal(got[0], got[2]) and torch.equal(got[1], got[3]) and got[0].abs().sum() > 0
     assert s.status.item() == 0
+
+
+@pytest.mark.parametrize("heads,new", [(1, 1), (4, 1), (4, 3), (1, 50)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("bad", [(np.nan, 1.0), (1.0, np.nan), (1.0, np.inf), (1.0, -0.5), (-np.inf, 1.0)])
+def test_attend_unsound_scales_reach_output_and_lse(have_gpu, heads, new, dtype, bad):
+    """A page whose keys' or values' scale is not finite, or whose values' is
+    below 0: output and log-sum-exp of who sees it are NaN, in each kernel,
+    and those of who does not are not."""
+    s = Side([90, 90], [new, new], heads=1, d=64, page=16, seed=6)
+    s.ref.scale[s.table[1][2], 0] = bad  # positions 32 .. 47 of the second sequence
+    s.upload()
+    q = s.rng.normal(0, 1, (s.rows, heads, 64)).astype(np.float32)
+    dt = getattr(torch, TORCH[dtype])
+    dq, out, lse = up(q).to(dt), torch.zeros(s.rows, heads, 64, dtype=dt, device=DEV), torch.zeros(s.rows, heads, device=DEV)
+    for window, sees in ((0, lambda p: p >= 32), (10, lambda p: 32 <= p < 57)):
+        s.kv.attend(s.seqs(), heads, dq.data_ptr(), out.data_ptr(), dtype=dtype, window=window, d_lse=lse.data_ptr(),
+                    stream=stream())
+        want = np.array([False] * new + [sees(90 - new + r) for r in range(new)])
+        assert np.array_equal(torch.isnan(out).all(-1).all(-1).cpu().numpy(), want)
+        assert np.array_equal(torch.isnan(out).any(-1).any(-1).cpu().numpy(), want)
+        assert np.array_equal(torch.isnan(lse).all(-1).cpu().numpy(), want)
+        assert np.array_equal(torch.isnan(lse).any(-1).cpu().numpy(), want)
