@@ -488,10 +488,16 @@ cudaError_t read_t(const Kv8Args& a, const Kv8Rows& k, const Kv8Rows& v, cudaStr
 // loaded: no conversion of a key, and 32-bit scores. (Two digits would do
 // for 16-bit outputs, not for lse.)
 // Values. A byte is exact in float16: below 0x64 its bits ^ 0x80 are the
-// number 1024 + 128 + byte, and one subtraction leaves it. The weight
-// w = p·s_v/W, with W the largest value scale so far, is a float16 for 16-bit
-// outputs (2^-11 of each weight, what a float16 output is rounded by) and the
-// sum of two for float32 ones (2^-25 of the largest weight).
+// number 1024 + 128 + byte, and one subtraction leaves it. The weight is
+// w = 2^11·p·s_v/W, with W a power of two of each query's own, at least a
+// sixteenth of its largest p·s_v so far: a float16 for 16-bit outputs (off by
+// 2^-12 of itself, half of what a float16 output is rounded by) and the sum of
+// two for float32 ones (2^-22), or by 2^-36 W where that is more. So
+// thousands of small weights beside a large one are not lost, and pages of
+// large values that a query hardly looks at cost it nothing. (With W the
+// largest value scale of the sequence and no 2^11 both were: 2e-3 of 32768
+// keys 16.6 nats below another.) A query's maximum and W move together, when
+// a score passes the one by 2^8 or a weight the other by 2^4.
 //
 // Layout. A warp takes sixteen tokens at a time from a ring of its own in
 // shared memory (Ring, below): a key row's bytes are spread over four lanes,
@@ -499,9 +505,8 @@ cudaError_t read_t(const Kv8Args& a, const Kv8Rows& k, const Kv8Rows& v, cudaStr
 // synchronisation in the loop: WU warps of a block, and the blocks of a
 // cluster, take separate stretches of the keys and are joined at the end
 // through (distributed) shared memory; with WU = 1 each warp has a unit of
-// its own and writes it out. The maximum moves only when a score passes it
-// by 2^8 (the weights stay far from overflow), so most steps need no
-// exchange between lanes.
+// its own and writes it out. The references move seldom, so most steps need
+// no exchange between lanes.
 //
 // Bound by the arithmetic of the digits and weights: 48 sequences of 1 to
 // 12001 tokens, 4 heads of 128 with 4 queries each, float16: 70 us, 3.4 TB/s
@@ -781,13 +786,17 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
 
   // --- the pass over the keys ---
   float o[NQ][D / 16][4] = {};
-  float ref[NQ][2], l[NQ][2] = {}, f[NQ][2];
-  float W = 0.f, toW = 0.f;  // the value scales' reference, and 1/W
+  // a query's largest score (about), sum, score factor, the exponent field of
+  // its W, and log2 of 2^4·W
+  float ref[NQ][2], l[NQ][2] = {}, f[NQ][2], most[NQ][2];
+  int wexp[NQ][2];
 #pragma unroll
   for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
     for (int j = 0; j < 2; j++) {
       ref[nq][j] = ninf();
+      wexp[nq][j] = 12;
+      most[nq][j] = ninf();
       f[nq][j] = qf[nq * 8 + 2 * tg + j];
     }
   // tiles that every query of the unit sees whole
@@ -797,20 +806,8 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
     const int page = __shfl_sync(FULL, pages.page, j);
     const float bsk = __shfl_sync(FULL, pages.scale.x, j), bsv = __shfl_sync(FULL, pages.scale.y, j);
     const bool edge = page < 0 || c * 16 < in_lo || c * 16 + 15 > in_hi;
-    if (bsv > W) {  // a larger scale, in every lane alike: twice it, to move less often
-      const float w = fminf(fmaxf(__fmul_rn(2.f, bsv), 1.17549435e-38f), 3.4e38f), k = __fdiv_rn(W, w);
-      W = w;
-      toW = __fdiv_rn(1.f, w);
-#pragma unroll
-      for (int nq = 0; nq < NQ; nq++)
-#pragma unroll
-        for (int mt = 0; mt < D / 16; mt++)
-#pragma unroll
-          for (int j = 0; j < 4; j++) o[nq][mt][j] = __fmul_rn(o[nq][mt][j], k);
-    }
     uint4 bk[2][H2];
     ring.keys(n, bk);
-    const float sv = __fmul_rn(bsv, toW);
     uint32_t pw[NQ][NP][2];  // the weights, transposed: queries in rows
 #pragma unroll
     for (int nq = 0; nq < NQ; nq++) {
@@ -845,8 +842,16 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
           if (hide[j]) x[j] = ninf();
         }
       }
+      // (A scale far above W has a term of 0, or as far below 1: no infinity
+      // here, and none for what is hidden, whose term is 0 whatever its page's
+      // scale. Where that is no number, the terms of what is seen are none.)
+      float sv[2];
+#pragma unroll
+      for (int j = 0; j < 2; j++) sv[j] = fminf(__fmul_rn(bsv, pow2(265 - wexp[nq][j])), 3.4e38f);
+      const float heavy = lg2(bsv);
       // before its first key a query's reference is −inf, and any score above
-      if (__any_sync(FULL, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > 8.f)) {
+      if (__any_sync(FULL, fmaxf(x[0], x[2]) > fminf(8.f, __fsub_rn(most[nq][0], heavy)) ||
+                               fmaxf(x[1], x[3]) > fminf(8.f, __fsub_rn(most[nq][1], heavy)))) {
 #pragma unroll
         for (int j = 0; j < 2; j++) {
           float m = fmaxf(hide[j] ? ninf() : __fmul_rn(s[j], fs[j]), hide[j + 2] ? ninf() : __fmul_rn(s[j + 2], fs[j]));
@@ -856,13 +861,23 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
           const float r = ref[nq][j] == m ? 1.f : ex2(__fsub_rn(ref[nq][j], m));
           ref[nq][j] = m;
           l[nq][j] = __fmul_rn(l[nq][j], r);
-#pragma unroll
-          for (int mt = 0; mt < D / 16; mt++) {
-            o[nq][mt][j] = __fmul_rn(o[nq][mt][j], r);
-            o[nq][mt][j + 2] = __fmul_rn(o[nq][mt][j + 2], r);
-          }
           x[j] = hide[j] ? ninf() : __fmaf_rn(s[j], fs[j], -m);
           x[j + 2] = hide[j + 2] ? ninf() : __fmaf_rn(s[j + 2], fs[j], -m);
+          // the largest weight, hidden keys' of an unsound scale aside
+          float u = fmaxf(__fmul_rn(ex2(x[j]), bsv), __fmul_rn(ex2(x[j + 2]), bsv));
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) u = fmaxf(u, __shfl_xor_sync(FULL, u, d));
+          const float W = __fmul_rn(pow2(wexp[nq][j]), r);  // what o's unit is worth now
+          const int e = unit_of(fmaxf(u, W));
+          wexp[nq][j] = e;
+          most[nq][j] = float(e - 123);
+          sv[j] = fminf(__fmul_rn(bsv, pow2(265 - e)), 3.4e38f);
+          const float k = __fmul_rn(W, pow2(254 - e));
+#pragma unroll
+          for (int mt = 0; mt < D / 16; mt++) {
+            o[nq][mt][j] = __fmul_rn(o[nq][mt][j], k);
+            o[nq][mt][j + 2] = __fmul_rn(o[nq][mt][j + 2], k);
+          }
         }
       }
       float w[4];
@@ -870,12 +885,7 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
       for (int j = 0; j < 4; j++) {
         const float p = ex2(x[j]);
         l[nq][j & 1] = __fadd_rn(l[nq][j & 1], p);
-        w[j] = __fmul_rn(p, sv);
-      }
-      if (edge) {  // what is not seen counts nothing, whatever its page's scale
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-          if (hide[j]) w[j] = 0.f;
+        w[j] = __fmul_rn(p, sv[j & 1]);
       }
 #pragma unroll
       for (int n = 0; n < NP; n++)
@@ -946,12 +956,12 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
         const int r = nq * 8 + 2 * tg + j;
         const bool there = r < nrow;
         const int tq = there ? (r0 + r) / group : 0, hq = h * group + (there ? (r0 + r) % group : 0);
-        const float inv = l[nq][j] == 0.f ? 0.f : __fdiv_rn(W, l[nq][j]);
+        const float inv = l[nq][j] == 0.f ? 0.f : __fdiv_rn(pow2(wexp[nq][j]), l[nq][j]);
         float y[E];
 #pragma unroll
         for (int mt = 0; mt < D / 16; mt++) {
-          y[2 * mt] = __fmul_rn(o[nq][mt][j], inv);
-          y[2 * mt + 1] = __fmul_rn(o[nq][mt][j + 2], inv);
+          y[2 * mt] = __fmul_rn(__fmul_rn(o[nq][mt][j], 1.f / 2048.f), inv);
+          y[2 * mt + 1] = __fmul_rn(__fmul_rn(o[nq][mt][j + 2], 1.f / 2048.f), inv);
         }
         if (t.q8) {
           // blocks of 32 values: over 32/E of the eight lanes of a query
@@ -1010,10 +1020,11 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
           wl[warp * NR + r] = l[nq][j];
         }
         float* dst = wo + (warp * NR + r) * D + g * (D / 8);
+        const float W = pow2(wexp[nq][j]);
 #pragma unroll
         for (int mt = 0; mt < D / 16; mt++)
-          *reinterpret_cast<float2*>(dst + 2 * mt) =
-              make_float2(__fmul_rn(o[nq][mt][j], W), __fmul_rn(o[nq][mt][j + 2], W));
+          *reinterpret_cast<float2*>(dst + 2 * mt) = make_float2(__fmul_rn(__fmul_rn(o[nq][mt][j], 1.f / 2048.f), W),
+                                                                 __fmul_rn(__fmul_rn(o[nq][mt][j + 2], 1.f / 2048.f), W));
       }
     __syncthreads();
     // Item: 32 values of one row, a lane each. The weight of a share is
@@ -1081,17 +1092,20 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
 //    middle in odd ones, the highest added to odd ones), so every lane has
 //    the digits of four keys and takes one of them: one score, one
 //    exponential and one weight a lane for 32 keys;
-//  * the weight is a whole number of 2^-23 of the reference weight, whose
-//    three bytes are taken as they lie in the float n + 2^23; one 8x8
-//    transposition brings the bytes of all 32 keys to the columns of an
-//    integer product with the values' bytes (m16n8k32, unsigned weights):
-//    the four keys of a row group in columns of their own, lowest and
-//    highest digits in one product, middle ones in another;
+//  * the weight, a key's softmax term times its page's value scale, is a
+//    whole number of 2^-32 of a reference W, a power of two above the largest
+//    such product so far and at most twice it; one 8x8 transposition brings its four bytes for all 32
+//    keys to the columns of integer products with the values' bytes
+//    (m16n8k32, unsigned weights): the four keys of a row group in columns of
+//    their own, the bytes 0 and 2 in one product, 1 and 3 in another. So a
+//    weight has all of a float's bits down to 2^-8 of W, and below that half
+//    a step of 2^-33 W: thousands of small ones beside a large one are not
+//    lost (whole numbers of 2^-23 of the largest value scale lost them, and
+//    what stood beside pages of large values that the query did not look at);
 //  * the values' bytes need a 4x4 byte transposition (eight byte
 //    permutations for sixteen bytes) and no conversion.
-// Sums are exact integers until the reference moves (a larger score, a
-// larger value scale) or 32768 keys have gone by; then they go into
-// float32 sums. 256 sequences of 65 to 576 tokens, 16 heads of 64: 38 us,
+// Sums are exact integers until the references move (a larger score, a larger
+// weight) or 32768 keys have gone by; then they go into float32 sums. 256 sequences of 65 to 576 tokens, 16 heads of 64: 38 us,
 // 4.5 TB/s of the cache; sequences of thousands of tokens in such numbers are
 // read at 6.2 to 6.4 TB/s.
 __device__ __forceinline__ void mma_s8u8(int* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -1117,7 +1131,7 @@ template <int D, int WU>
 __global__ void __launch_bounds__(32 * Shape1<D, WU>::warps, Shape1<D, WU>::blocks)
     k_kv8_attend1(Kv8Args a, Kv8Attend t, int type, int S, int units, bool vec) {
   constexpr int H2 = D / 64, M = D / 16, WV = D / 32, R = Shape1<D, WU>::ring;
-  constexpr float kOne = 8388592.f;  // of a weight of 1, with room for a product's roundings below 2^23
+  constexpr float kOne = 4294967296.f;  // of a weight of W; just below it at most
   extern __shared__ __align__(16) uint8_t smem[];
   float* part = reinterpret_cast<float*>(smem);  // [WU][D + 2], and the block's, when the rings are done
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tg = lane & 3;
@@ -1179,10 +1193,10 @@ __global__ void __launch_bounds__(32 * Shape1<D, WU>::warps, Shape1<D, WU>::bloc
 
   // --- the pass over the keys: lane (g, tg) has key g + 8·(tg & 1) of tile tg >> 1 ---
   const uint32_t at0 = column_bytes(g, 0, 0x20), at1 = column_bytes(g, 1, 0x20);
-  const uint32_t mid0 = g & 1 ? 0x4444 : column_bytes(g, 0, 0x31), mid1 = g & 1 ? 0x4444 : column_bytes(g, 1, 0x31);
-  int lh[M][4] = {}, md[M][4] = {};  // lowest (even columns) and highest (odd) digits; middle ones
+  const uint32_t odd0 = column_bytes(g, 0, 0x31), odd1 = column_bytes(g, 1, 0x31);
+  int ev[M][4] = {}, od[M][4] = {};  // sums over the weights' bytes 0 (even columns) and 2 (odd), 1 and 3
   float o[M][2] = {};
-  float ref = ninf(), l = 0.f, W = 0.f, toW = 0.f;
+  float ref = ninf(), l = 0.f, W = pow2(12), toW = pow2(242), most = ninf();  // 1/W; log2 of W
   int held = 0;  // steps in the integer sums
   // the integer sums into the float ones, and these times r
   auto flush = [&](float r) {
@@ -1190,9 +1204,10 @@ __global__ void __launch_bounds__(32 * Shape1<D, WU>::warps, Shape1<D, WU>::bloc
     for (int mt = 0; mt < M; mt++)
 #pragma unroll
       for (int e = 0; e < 2; e++) {
-        const float lo = __fmaf_rn(256.f, float(md[mt][2 * e]), float(lh[mt][2 * e]));
-        o[mt][e] = __fmul_rn(r, __fadd_rn(o[mt][e], __fmaf_rn(65536.f, float(lh[mt][2 * e + 1]), lo)));
-        lh[mt][2 * e] = lh[mt][2 * e + 1] = md[mt][2 * e] = 0;
+        const float lo = __fmaf_rn(256.f, float(od[mt][2 * e]), float(ev[mt][2 * e]));
+        const float hi = __fmaf_rn(256.f, float(od[mt][2 * e + 1]), float(ev[mt][2 * e + 1]));
+        o[mt][e] = __fmul_rn(r, __fadd_rn(o[mt][e], __fmaf_rn(65536.f, hi, lo)));
+        ev[mt][2 * e] = ev[mt][2 * e + 1] = od[mt][2 * e] = od[mt][2 * e + 1] = 0;
       }
     held = 0;
   };
@@ -1202,7 +1217,6 @@ __global__ void __launch_bounds__(32 * Shape1<D, WU>::warps, Shape1<D, WU>::bloc
     const float sva = __shfl_sync(FULL, pages.scale.y, j), svb = __shfl_sync(FULL, pages.scale.y, j + 1);
     const float fs = __fmul_rn(f, __shfl_sync(FULL, pages.scale.x, j + (tg >> 1)));
     float sv = tg < 2 ? sva : svb;
-    const float wide = fmaxf(sva, svb);
     const bool edge = (pa | pb) < 0 || c * 16 < first || c * 16 + 31 > p;
     // the highest digit's sums, then the lower ones' on top: even columns
     // the lowest digit, odd ones 256·highest + middle (below 2^31)
@@ -1235,32 +1249,34 @@ __global__ void __launch_bounds__(32 * Shape1<D, WU>::warps, Shape1<D, WU>::bloc
       hide = key > p || key < first || (tg < 2 ? pa : pb) < 0;
       if (hide) x = ninf(), sv = 0.f;
     }
-    // The reference moves: a larger value scale (an eighth above it, to move
-    // less often), or a larger score.
-    if (wide > W) {
-      const float w = fminf(fmaxf(__fmul_rn(1.125f, wide), 1.17549435e-38f), 3.4e38f);
-      flush(__fdiv_rn(W, w));
-      W = w;
-      toW = __fdiv_rn(1.f, w);
-    }
-    if (__any_sync(FULL, x > 0.f)) {
+    // The references move: a larger score, or a larger weight.
+    if (__any_sync(FULL, x > fminf(0.f, __fsub_rn(most, lg2(sv))))) {
       float m = hide ? ninf() : __fmul_rn(s, fs);
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, d));
       m = fmaxf(m, ref);
       const float r = ref == m ? 1.f : ex2(__fsub_rn(ref, m));
-      flush(r);
       ref = m;
       l = __fmul_rn(l, r);
+      W = __fmul_rn(W, r);
       x = hide ? ninf() : __fmaf_rn(s, fs, -m);
+      float u = __fmul_rn(ex2(x), sv);
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) u = fmaxf(u, __shfl_xor_sync(FULL, u, d));
+      // the power of two above the largest weight, or what W is worth now
+      const int e = unit_of(fmaxf(__fadd_rn(u, u), W));
+      toW = pow2(254 - e);
+      flush(__fmul_rn(W, toW));
+      W = pow2(e);
+      most = float(e - 127);
     }
     const float w = x > 0.f ? 1.f : ex2(x);  // above 0 by the rounding of the reference
     l = __fadd_rn(l, w);
-    // n + 2^23: the bytes of n as they lie
-    const uint32_t y = __float_as_uint(__fmaf_rn(__fmul_rn(w, __fmul_rn(sv, toW)), kOne, 8388608.f));
+    // a scale far above W has a term of 0, or as far below 1: no infinity here
+    const uint32_t y = __float2uint_rn(__fmul_rn(__fmul_rn(w, fminf(__fmul_rn(sv, toW), 3.4e38f)), kOne));
     const uint32_t yt = transpose8(y);
     const uint32_t b0 = __byte_perm(yt, 0, at0), b1 = __byte_perm(yt, 0, at1);
-    const uint32_t m0 = __byte_perm(yt, 0, mid0), m1 = __byte_perm(yt, 0, mid1);
+    const uint32_t m0 = __byte_perm(yt, 0, odd0), m1 = __byte_perm(yt, 0, odd1);
     uint32_t v[2][4][WV];
     ring.values(2 * n, v[0]);
     ring.values(2 * n + 1, v[1]);
@@ -1282,8 +1298,8 @@ __global__ void __launch_bounds__(32 * Shape1<D, WU>::warps, Shape1<D, WU>::bloc
 #pragma unroll
       for (int e = 0; e < 2; e++) {
         const uint32_t av[4] = {d[0][2 * e], d[0][2 * e + 1], d[1][2 * e], d[1][2 * e + 1]};
-        mma_s8u8(lh[2 * wd + e], av, b0, b1);
-        mma_s8u8(md[2 * wd + e], av, m0, m1);
+        mma_s8u8(ev[2 * wd + e], av, b0, b1);
+        mma_s8u8(od[2 * wd + e], av, m0, m1);
       }
     }
     if (++held == 1024) flush(1.f);  // 32768 keys: 255·128·32768 < 2^31
@@ -1322,14 +1338,13 @@ __global__ void __launch_bounds__(32 * Shape1<D, WU>::warps, Shape1<D, WU>::bloc
   // lane (g, tg) goes on with D/32 of row group g's D/8 values
   constexpr int E = D / 32;
   float y[E];
-  const float unit_w = __fmul_rn(W, 1.f / kOne);
 #pragma unroll
   for (int e = 0; e < E; e++) {
     float v = o[e / 2][e % 2];
 #pragma unroll
     for (int n = 1; n < 4; n++)
       if (tg == n) v = o[(n * E + e) / 2][e % 2];
-    y[e] = __fmul_rn(v, unit_w);
+    y[e] = __fmul_rn(__fmul_rn(v, 1.f / kOne), W);  // W is 0 where there was no key
   }
   const int d0 = g * (D / 8) + tg * E;
   auto finish = [&](float top, float sum, const float* val) {

@@ -15,10 +15,13 @@
 //    j + 2 are issued ahead of the outputs of tile j;
 //  * warps 0-3 take the even tiles and warps 4-7 the odd ones, a thread to a
 //    row and with a maximum, a sum and an O of their own, joined at the end:
-//    the scores' maximum from TMEM, the scores again, weights p·s_v/W,
-//    written back as P. The maximum moves only when a score passes it by 2^8;
-//    then, and when a larger value scale comes, the row of O in TMEM is
-//    multiplied. So one half's exponentials run while the other half waits.
+//    the scores' maximum from TMEM, the scores again, weights 2^11·p·s_v/W,
+//    written back as P, W being a power of two of the row's own, at least a
+//    sixteenth of its largest p·s_v so far: a weight is off by 2^-12 of itself (2^-22 as the sum of
+//    two), or by 2^-36 W where that is more. The maximum moves only when a
+//    score passes it by 2^8; when a weight passes W by 2^4, the row of O in
+//    TMEM is multiplied. So one half's exponentials run while the other half
+//    waits.
 // Blocks with the most keys start first. Every wait is bounded (about a
 // second of clocks); one that runs out sets the block's `dead` word, every
 // role leaves its loop, the block frees its TMEM, and the status word gets
@@ -441,7 +444,8 @@ __global__ void __launch_bounds__(544, 1)
     const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
     const uint32_t my_s = lanes + half * kKeys, my_o = lanes + C::c_o + half * D;
     const uint32_t my_p = lanes + C::c_p + half * NP * (kKeys / 2);
-    float ref = ninf(), l = 0.f, W = 0.f, toW = 0.f;
+    float ref = ninf(), l = 0.f, most = ninf();  // log2 of 2^4·W
+    int unit = 12;                               // W's exponent field
     bool ok = true;
     for (int j = half; j < nt; j += 2) {
       const int key0 = (tb + j) * kKeys;
@@ -449,12 +453,10 @@ __global__ void __launch_bounds__(544, 1)
       if (!ok) break;
       fence_after();
       float2 c[4];
-      float wide = 0.f;
       uint32_t turned = 0;  // groups of sixteen keys whose scale is below 0: their products change sign, the scale has none
 #pragma unroll
       for (int g = 0; g < 4; g++) {
         c[g] = scales[(j & 3) * 4 + g];
-        wide = fmaxf(wide, c[g].y);
         if (c[g].x < 0.f && c[g].x != ninf()) {
           turned |= 1u << g;
           c[g].x = -c[g].x;
@@ -473,14 +475,12 @@ __global__ void __launch_bounds__(544, 1)
                         key0 + kKeys - 1 > pmin;
       // bit e: this row sees key e of the tile
       uint64_t seen = ~0ull;
-      bool none = false;  // some value scale is no number
       if (edge) {
         const int from = max(lo - key0, 0), to = min(p - key0, kKeys - 1);
         seen = from > to ? 0 : (~0ull >> (kKeys - 1 - to)) >> from << from;
 #pragma unroll
         for (int g = 0; g < 4; g++) {
           if (c[g].x == ninf()) seen &= ~(0xffffull << (16 * g));
-          none = none || isnan(c[g].y);
         }
       }
       const auto hidden = [&](int e) { return !(uint32_t(e < 32 ? seen : seen >> 32) >> (e & 31) & 1); };
@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(544, 1)
       float* x = reinterpret_cast<float*>(s);
       // the largest score: a group's largest product times its factor, from
       // which every sign has been taken
-      float top = ninf();
+      float top = ninf(), heavy = ninf();  // and the largest of log2 of a weight, from the same
 #pragma unroll
       for (int u = 0; u < 2; u++) {
         tmem_ld32(my_s + 32 * u, s);
@@ -506,8 +506,10 @@ __global__ void __launch_bounds__(544, 1)
 #pragma unroll
           for (int e = 0; e < 4; e++)
             m[e] = fmaxf(fmaxf(x[16 * g + e], x[16 * g + 4 + e]), fmaxf(x[16 * g + 8 + e], x[16 * g + 12 + e]));
-          const float y = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-          top = fmaxf(top, y == ninf() ? y : __fmul_rn(y, __fmul_rn(f, c[2 * u + g].x)));
+          float y = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+          if (y != ninf()) y = __fmul_rn(y, __fmul_rn(f, c[2 * u + g].x));
+          top = fmaxf(top, y);
+          heavy = fmaxf(heavy, __fadd_rn(y, lg2(c[2 * u + g].y)));
         }
       }
       if (j > 1) {
@@ -516,22 +518,19 @@ __global__ void __launch_bounds__(544, 1)
         fence_after();
       }
       // the references move: a score 2^8 above the row's (any, before its
-      // first key), a larger value scale
+      // first key), a weight 2^4 above W
       const bool over = top > __fadd_rn(ref, 8.f);
-      if (__any_sync(FULL, over) || wide > W) {
-        float k = 1.f;
-        if (wide > W) {
-          const float w = fminf(fmaxf(__fmul_rn(2.f, wide), 1.17549435e-38f), 3.4e38f);
-          k = __fdiv_rn(W, w);
-          W = w;
-          toW = __fdiv_rn(1.f, w);
-        }
+      if (__any_sync(FULL, over || __fsub_rn(heavy, ref) > most)) {
+        float W = pow2(unit);
         if (over) {
           const float up = ex2(__fsub_rn(ref, top));
           ref = top;
           l = __fmul_rn(l, up);
-          k = __fmul_rn(k, up);
+          W = __fmul_rn(W, up);  // what O's unit is worth now
         }
+        unit = unit_of(fmaxf(W, ex2(__fsub_rn(heavy, ref))));
+        most = float(unit - 123);
+        const float k = __fmul_rn(W, pow2(254 - unit));
         if (j > 1) {
 #pragma unroll 1
           for (int n = 0; n < D; n += 32) {
@@ -568,16 +567,13 @@ __global__ void __launch_bounds__(544, 1)
           for (int e = 0; e < 32; e++)
             if (hidden(32 * u + e)) x[e] = 0.f;
         }
-        const f2 w0 = f2dup(__fmul_rn(c0.y, toW)), w1 = f2dup(__fmul_rn(c1.y, toW));
+        // (a scale far above W has terms of 0, or as far below 1: no infinity here)
+        const float toW = pow2(265 - unit);
+        const f2 w0 = f2dup(fminf(__fmul_rn(c0.y, toW), 3.4e38f)), w1 = f2dup(fminf(__fmul_rn(c1.y, toW), 3.4e38f));
 #pragma unroll
         for (int e = 0; e < 16; e++) {
           sum = f2add(sum, x2[e]);
           x2[e] = f2mul(x2[e], e < 8 ? w0 : w1);
-        }
-        if (none) {  // what is not seen counts nothing, whatever its page's scale
-#pragma unroll
-          for (int e = 0; e < 32; e++)
-            if (hidden(32 * u + e)) x[e] = 0.f;
         }
 #pragma unroll
         for (int n = 0; n < NP; n++) {
@@ -604,7 +600,7 @@ __global__ void __launch_bounds__(544, 1)
     if (ok && nt > 1) ok = bar_wait(added(nt - 2), of4(nt - 2), dead);
     halves[(half * 3 + 0) * kRows + r] = ref;
     halves[(half * 3 + 1) * kRows + r] = l;
-    halves[(half * 3 + 2) * kRows + r] = W;
+    halves[(half * 3 + 2) * kRows + r] = pow2(unit);
     asm volatile("bar.sync 1, 256;\n" ::: "memory");
     if (ok) {
       fence_after();
@@ -613,8 +609,8 @@ __global__ void __launch_bounds__(544, 1)
       const float k0 = ref0 == ref ? 1.f : ex2(__fsub_rn(ref0, ref)), k1 = ref1 == ref ? 1.f : ex2(__fsub_rn(ref1, ref));
       l = __fadd_rn(__fmul_rn(l0, k0), __fmul_rn(l1, k1));
       // a row without keys has an O of zeros or none
-      const float inv0 = l == 0.f ? 0.f : __fdiv_rn(__fmul_rn(halves[2 * kRows + r], k0), l);
-      const float inv1 = l == 0.f ? 0.f : __fdiv_rn(__fmul_rn(halves[5 * kRows + r], k1), l);
+      const float inv0 = l == 0.f ? 0.f : __fmul_rn(1.f / 2048.f, __fdiv_rn(__fmul_rn(halves[2 * kRows + r], k0), l));
+      const float inv1 = l == 0.f ? 0.f : __fmul_rn(1.f / 2048.f, __fdiv_rn(__fmul_rn(halves[5 * kRows + r], k1), l));
 #pragma unroll 1
       for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
         uint32_t o[32] = {}, o1[32] = {};

@@ -94,6 +94,16 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Weights are counted in units of a power of two W = 2^(e − 127), kept as its
+// exponent field e: of the number `most` (not below 0), within the range in
+// which W, 1/W and 2^11/W are normal numbers.
+__device__ __forceinline__ int unit_of(float most) { return min(max(int(__float_as_uint(most) >> 23), 12), 253); }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float(uint32_t(e) << 23); }  // 2^(e − 127)
 // Two floats as float16s, lo in the low half.
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t y;

@@ -200,8 +200,12 @@ int grx_kv8_read(const grx_kv8* kv, const grx_kv8_seqs* s, int type, void* k, in
 /* Attention of the rows' queries over their sequences: heads query heads, a
  * multiple of kv_heads (query head h reads key head h·kv_heads/heads), each
  * query seeing the keys up to its own position, from first[i] on and, with
- * window > 0, the last `window` of them. out = softmax(scale·q·k)·v, sums in
- * 32 bits; the queries are rotated as the keys were. lse [rows][heads] (may
+ * window > 0, the last `window` of them. out = softmax(scale·q·k)·v; the
+ * queries are rotated as the keys were. Scores are 32 bits (a query's values
+ * to 2^-23 of its largest), and so are all sums. A weight, a key's softmax term
+ * times its page's value scale, is held to 2^-22 of itself where outputs are
+ * float32 and to 2^-12 (a float16) where they have 16 bits, or, where that is
+ * more, to 2^-32 of the query's largest. lse [rows][heads] (may
  * be NULL) gets log Σ e^(scale·q·k). A query that sees no key answers zeros
  * and −inf; one that is not finite, or sees a page whose scale is not (or
  * whose values' scale is below 0), answers NaN, output and log-sum-exp both.
