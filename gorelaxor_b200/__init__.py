@@ -316,8 +316,9 @@ class _KV8Seqs(C.Structure):  # grx_kv8_seqs
 class KV8Seqs:
     """The sequences of a call (grx_kv8_seqs), as device addresses: the page
     table [n][table_width], the lengths d_len [n] (this call's tokens among
-    them), the row numbers d_row0 [n + 1] (None: one row for each sequence).
-    Make it once and use it for every layer of a step, and for every step
+    them), the row numbers d_row0 [n + 1] (None: one row for each sequence)
+    and their bounds: rows (None: n, also with d_row0) and max_new, past which
+    a sequence is left out. Make it once and use it for every layer of a step, and for every step
     while the addresses and bounds stay."""
 
     def __init__(self, n: int, d_table: int, table_width: int, d_len: int, max_len: int, d_row0: int | None = None,
@@ -373,17 +374,22 @@ class KV8:
         if rc < 0:
             _check(rc)
 
-    def check(self, table: np.ndarray, lens, row0=None, rows: int | None = None, max_new: int = 1,
+    def check(self, table: np.ndarray, lens, row0=None, rows: int | None = None, max_new: int | None = None,
               rope_positions: int | None = None, writes: bool = False) -> None:
         """grx_kv8_check on host copies of a call's arrays; raises GrxError
-        with what does not fit."""
+        with what does not fit. rows and max_new are the call's bounds, by
+        default what row0 itself says (one row for each sequence without)."""
         t = np.ascontiguousarray(table, np.int32)
         ln = np.ascontiguousarray(lens, np.int32)
         r0 = None if row0 is None else np.ascontiguousarray(row0, np.int32)
         n = ln.size
         if t.ndim != 2 or t.shape[0] != n or (r0 is not None and r0.size != n + 1):
             raise ValueError(f"check: a table of shape {t.shape} and {n} lengths")
-        s = _KV8Seqs(n, t.shape[1], n if rows is None else rows, max_new, int(ln.max(initial=0)) if n else 0,
+        if rows is None:
+            rows = n if r0 is None else int(r0[-1])
+        if max_new is None:
+            max_new = 1 if r0 is None else max(0, int(np.diff(r0.astype(np.int64)).max(initial=0)))
+        s = _KV8Seqs(n, t.shape[1], rows, max_new, int(ln.max(initial=0)) if n else 0,
                      t.ctypes.data, ln.ctypes.data, None if r0 is None else r0.ctypes.data, None, None,
                      rope_positions or 0, 0 if rope_positions is None else 1, None)
         _check(self._lib.grx_kv8_check(self._p, C.byref(s), int(writes)))

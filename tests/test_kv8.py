@@ -160,3 +160,16 @@ def test_reference_cache_rounds_as_defined():
     step = c.scale[[2, 0, 1]][np.arange(40) // 16, :, 0]
     assert (np.abs(got - x[:, 0]).max(-1) <= (0.5 + 0.5 * grown) * step * (1 + 1e-6)).all()
     assert rope_table(3, 64).shape == (3, 32, 2)
+
+
+def test_bounds_of_ragged_calls():
+    """A check of a ragged call takes the bounds that it is not given from the
+    rows."""
+    kv, t = cache(), np.array([[0, 1], [2, 3], [4, 5]])
+    kv.check(t, [20, 30, 7], row0=[0, 20, 25, 25])
+    kv.check(t, [20, 30, 7], row0=[0, 0, 0, 0], writes=True)
+    kv.check(t, [1, 30, 7], writes=True)
+    refused(lambda: kv.check(t, [20, 30, 7], row0=[0, 20, 25, 25], rows=24), ERANGE, "rows 20 to 25")
+    refused(lambda: kv.check(t, [20, 30, 7], row0=[0, 20, 25, 25], max_new=19), ERANGE, "rows 0 to 20")
+    refused(lambda: kv.check(t, [20, 4, 7], row0=[0, 20, 25, 25]), ERANGE, "rows 20 to 25")
+    refused(lambda: kv.check(t, [20, 30, 7], row0=[0, 20, 15, 25]), ERANGE, "rows 20 to 15")
