@@ -1580,8 +1580,11 @@ cudaError_t launch_kv8_read(const Kv8Args& a, int head_dim, int type, const Kv8R
 }
 
 cudaError_t launch_kv8_attend(const Kv8Args& a, int head_dim, int type, const Kv8Attend& t, cudaStream_t st) {
-  if (head_dim == 64) return type == 0 ? attend_d<64, 2>(a, type, t, st) : attend_d<64, 1>(a, type, t, st);
-  return type == 0 ? attend_d<128, 2>(a, type, t, st) : attend_d<128, 1>(a, type, t, st);
+  const cudaError_t e = head_dim == 64
+                            ? (type == 0 ? attend_d<64, 2>(a, type, t, st) : attend_d<64, 1>(a, type, t, st))
+                            : (type == 0 ? attend_d<128, 2>(a, type, t, st) : attend_d<128, 1>(a, type, t, st));
+  if (e != cudaSuccess) cudaGetLastError();  // returned: a later launch must not find it as its own
+  return e;
 }
 
 cudaError_t launch_kv8_copy_pages(const Kv8Args& a, int head_dim, int layers, const int* from, const int* to, int count,

@@ -588,9 +588,11 @@ cudaError_t logp_t(const LogpArgs& a, cudaStream_t st) {
 }  // namespace
 
 cudaError_t launch_logp(const LogpArgs& a, int type, cudaStream_t st) {
-  return type == 0   ? logp_t<float>(a, st)
-         : type == 1 ? logp_t<__half>(a, st)
-                     : logp_t<__nv_bfloat16>(a, st);
+  const cudaError_t e = type == 0   ? logp_t<float>(a, st)
+                        : type == 1 ? logp_t<__half>(a, st)
+                                    : logp_t<__nv_bfloat16>(a, st);
+  if (e != cudaSuccess) cudaGetLastError();  // returned: a later launch must not find it as its own
+  return e;
 }
 
 }  // namespace grx

@@ -178,6 +178,7 @@ for kernel, nth in (("k_q8", 0), ("k_kv8_append", 1), ("k_kv8_attend", 0)):
         print("ok")
     except g.GrxError as e:
         print(e.code)
+    st.text([[1, 2], [3]])  # reported once
 """)
     assert out[:3] == ["-4"] * 3
 
@@ -196,3 +197,29 @@ print(launched()[0][1][0])
     per, most = 16, min(max_new, 64 * width)  # tokens a block: 64 threads to a token of two heads' float32
     assert int(out[0]) == -(-most // per)
     assert int(out[0]) * per < 2**31
+
+
+def test_a_refused_launch_is_reported_once(fake):
+    """An attention or a scoring that the runtime refuses says so; the append
+    and the read behind it are queued and say nothing."""
+    out = fake("""
+c = g.KV8(4096, 4096, 4096, 8, 16, 2, 64)
+s = g.KV8Seqs(2, 4096, 2, 4096, 32)
+many = g.KV8Seqs(2, 4096, 9, 4096, 99, d_row0=4096, rows=99, max_new=90)
+calls = [("k_kv8_attend", lambda: c.attend(s, 2, 4096, 4096)), ("k_kv8_attend", lambda: c.attend(s, 8, 4096, 4096)),
+         ("k_kv8_prompt", lambda: c.attend(many, 2, 4096, 4096)), ("k_kv8_append", lambda: c.append(s, 4096, 4096)),
+         ("k_kv8_read", lambda: c.read(s, 4096, 4096)), ("k_logp", lambda: g.logprobs(4096, 3, 100, d_entropy=4096)),
+         ("k_logp", lambda: g.logprobs(4096, 3, 99999, d_entropy=4096))]
+for name, call in calls:
+    fake.fake_fail(name.encode(), 0)
+    try:
+        call()
+        print("queued")
+    except g.GrxError as e:
+        print(e.code)
+    c.append(s, 4096, 4096)
+    c.read(s, 4096, 4096)
+    call()
+print(fake.cudaPeekAtLastError())
+""")
+    assert out[:8] == ["-4"] * 7 + ["0"]
