@@ -489,10 +489,10 @@ cudaError_t read_t(const Kv8Args& a, const Kv8Rows& k, const Kv8Rows& v, cudaStr
 // for 16-bit outputs, not for lse.)
 // Values. A byte is exact in float16: below 0x64 its bits ^ 0x80 are the
 // number 1024 + 128 + byte, and one subtraction leaves it. The weight is
-// w = 2^11·p·s_v/W, with W a power of two of each query's own, at least a
-// sixteenth of its largest p·s_v so far: a float16 for 16-bit outputs (off by
-// 2^-12 of itself, half of what a float16 output is rounded by) and the sum of
-// two for float32 ones (2^-22), or by 2^-36 W where that is more. So
+// w = 2^11·p·s_v/W, with W of each query's own, at least a sixteenth of its
+// largest p·s_v so far: a float16 for 16-bit outputs (off by 2^-12 of itself,
+// half of what a float16 output is rounded by) and the sum of two for float32
+// ones (2^-22), or by 2^-36 W where that is more. So
 // thousands of small weights beside a large one are not lost, and pages of
 // large values that a query hardly looks at cost it nothing. (With W the
 // largest value scale of the sequence and no 2^11 both were: 2e-3 of 32768
@@ -786,16 +786,14 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
 
   // --- the pass over the keys ---
   float o[NQ][D / 16][4] = {};
-  // a query's largest score (about), sum, score factor, the exponent field of
-  // its W, and log2 of 2^4·W
-  float ref[NQ][2], l[NQ][2] = {}, f[NQ][2], most[NQ][2];
-  int wexp[NQ][2];
+  // a query's largest score (about), sum, score factor, 2^11/W, and log2 of 2^4·W
+  float ref[NQ][2], l[NQ][2] = {}, f[NQ][2], toW[NQ][2], most[NQ][2];
 #pragma unroll
   for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
     for (int j = 0; j < 2; j++) {
       ref[nq][j] = ninf();
-      wexp[nq][j] = 12;
+      toW[nq][j] = pow2(253);
       most[nq][j] = ninf();
       f[nq][j] = qf[nq * 8 + 2 * tg + j];
     }
@@ -847,7 +845,7 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
       // scale. Where that is no number, the terms of what is seen are none.)
       float sv[2];
 #pragma unroll
-      for (int j = 0; j < 2; j++) sv[j] = fminf(__fmul_rn(bsv, pow2(265 - wexp[nq][j])), 3.4e38f);
+      for (int j = 0; j < 2; j++) sv[j] = fminf(__fmul_rn(bsv, toW[nq][j]), 3.4e38f);
       const float heavy = lg2(bsv);
       // before its first key a query's reference is −inf, and any score above
       if (__any_sync(FULL, fmaxf(x[0], x[2]) > fminf(8.f, __fsub_rn(most[nq][0], heavy)) ||
@@ -867,12 +865,10 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
           float u = fmaxf(__fmul_rn(ex2(x[j]), bsv), __fmul_rn(ex2(x[j + 2]), bsv));
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) u = fmaxf(u, __shfl_xor_sync(FULL, u, d));
-          const float W = __fmul_rn(pow2(wexp[nq][j]), r);  // what o's unit is worth now
-          const int e = unit_of(fmaxf(u, W));
-          wexp[nq][j] = e;
-          most[nq][j] = float(e - 123);
-          sv[j] = fminf(__fmul_rn(bsv, pow2(265 - e)), 3.4e38f);
-          const float k = __fmul_rn(W, pow2(254 - e));
+          const float unit = __fmul_rn(inverse<NP>(toW[nq][j]), r);  // what o's unit, 2^-11 W, is worth now
+          toW[nq][j] = weight_scale<NP>(fmaxf(u, __fmul_rn(unit, 2048.f)), &most[nq][j]);
+          sv[j] = fminf(__fmul_rn(bsv, toW[nq][j]), 3.4e38f);
+          const float k = __fmul_rn(unit, toW[nq][j]);
 #pragma unroll
           for (int mt = 0; mt < D / 16; mt++) {
             o[nq][mt][j] = __fmul_rn(o[nq][mt][j], k);
@@ -956,12 +952,12 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
         const int r = nq * 8 + 2 * tg + j;
         const bool there = r < nrow;
         const int tq = there ? (r0 + r) / group : 0, hq = h * group + (there ? (r0 + r) % group : 0);
-        const float inv = l[nq][j] == 0.f ? 0.f : __fdiv_rn(pow2(wexp[nq][j]), l[nq][j]);
+        const float inv = l[nq][j] == 0.f ? 0.f : __fdiv_rn(inverse<NP>(toW[nq][j]), l[nq][j]);
         float y[E];
 #pragma unroll
         for (int mt = 0; mt < D / 16; mt++) {
-          y[2 * mt] = __fmul_rn(__fmul_rn(o[nq][mt][j], 1.f / 2048.f), inv);
-          y[2 * mt + 1] = __fmul_rn(__fmul_rn(o[nq][mt][j + 2], 1.f / 2048.f), inv);
+          y[2 * mt] = __fmul_rn(o[nq][mt][j], inv);
+          y[2 * mt + 1] = __fmul_rn(o[nq][mt][j + 2], inv);
         }
         if (t.q8) {
           // blocks of 32 values: over 32/E of the eight lanes of a query
@@ -1020,11 +1016,11 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
           wl[warp * NR + r] = l[nq][j];
         }
         float* dst = wo + (warp * NR + r) * D + g * (D / 8);
-        const float W = pow2(wexp[nq][j]);
+        const float unit = inverse<NP>(toW[nq][j]);
 #pragma unroll
         for (int mt = 0; mt < D / 16; mt++)
-          *reinterpret_cast<float2*>(dst + 2 * mt) = make_float2(__fmul_rn(__fmul_rn(o[nq][mt][j], 1.f / 2048.f), W),
-                                                                 __fmul_rn(__fmul_rn(o[nq][mt][j + 2], 1.f / 2048.f), W));
+          *reinterpret_cast<float2*>(dst + 2 * mt) =
+              make_float2(__fmul_rn(o[nq][mt][j], unit), __fmul_rn(o[nq][mt][j + 2], unit));
       }
     __syncthreads();
     // Item: 32 values of one row, a lane each. The weight of a share is

@@ -16,8 +16,8 @@
 //  * warps 0-3 take the even tiles and warps 4-7 the odd ones, a thread to a
 //    row and with a maximum, a sum and an O of their own, joined at the end:
 //    the scores' maximum from TMEM, the scores again, weights 2^11·p·s_v/W,
-//    written back as P, W being a power of two of the row's own, at least a
-//    sixteenth of its largest p·s_v so far: a weight is off by 2^-12 of itself (2^-22 as the sum of
+//    written back as P, W being the row's own, at least a sixteenth of its
+//    largest p·s_v so far: a weight is off by 2^-12 of itself (2^-22 as the sum of
 //    two), or by 2^-36 W where that is more. The maximum moves only when a
 //    score passes it by 2^8; when a weight passes W by 2^4, the row of O in
 //    TMEM is multiplied. So one half's exponentials run while the other half
@@ -444,8 +444,7 @@ __global__ void __launch_bounds__(544, 1)
     const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
     const uint32_t my_s = lanes + half * kKeys, my_o = lanes + C::c_o + half * D;
     const uint32_t my_p = lanes + C::c_p + half * NP * (kKeys / 2);
-    float ref = ninf(), l = 0.f, most = ninf();  // log2 of 2^4·W
-    int unit = 12;                               // W's exponent field
+    float ref = ninf(), l = 0.f, toW = pow2(253), most = ninf();  // 2^11/W, log2 of 2^4·W
     bool ok = true;
     for (int j = half; j < nt; j += 2) {
       const int key0 = (tb + j) * kKeys;
@@ -521,16 +520,15 @@ __global__ void __launch_bounds__(544, 1)
       // first key), a weight 2^4 above W
       const bool over = top > __fadd_rn(ref, 8.f);
       if (__any_sync(FULL, over || __fsub_rn(heavy, ref) > most)) {
-        float W = pow2(unit);
+        float unit = inverse<NP>(toW);  // O's, 2^-11 W
         if (over) {
           const float up = ex2(__fsub_rn(ref, top));
           ref = top;
           l = __fmul_rn(l, up);
-          W = __fmul_rn(W, up);  // what O's unit is worth now
+          unit = __fmul_rn(unit, up);  // what it is worth now
         }
-        unit = unit_of(fmaxf(W, ex2(__fsub_rn(heavy, ref))));
-        most = float(unit - 123);
-        const float k = __fmul_rn(W, pow2(254 - unit));
+        toW = weight_scale<NP>(fmaxf(__fmul_rn(unit, 2048.f), ex2(__fsub_rn(heavy, ref))), &most);
+        const float k = __fmul_rn(unit, toW);
         if (j > 1) {
 #pragma unroll 1
           for (int n = 0; n < D; n += 32) {
@@ -568,7 +566,6 @@ __global__ void __launch_bounds__(544, 1)
             if (hidden(32 * u + e)) x[e] = 0.f;
         }
         // (a scale far above W has terms of 0, or as far below 1: no infinity here)
-        const float toW = pow2(265 - unit);
         const f2 w0 = f2dup(fminf(__fmul_rn(c0.y, toW), 3.4e38f)), w1 = f2dup(fminf(__fmul_rn(c1.y, toW), 3.4e38f));
 #pragma unroll
         for (int e = 0; e < 16; e++) {
@@ -600,7 +597,7 @@ __global__ void __launch_bounds__(544, 1)
     if (ok && nt > 1) ok = bar_wait(added(nt - 2), of4(nt - 2), dead);
     halves[(half * 3 + 0) * kRows + r] = ref;
     halves[(half * 3 + 1) * kRows + r] = l;
-    halves[(half * 3 + 2) * kRows + r] = pow2(unit);
+    halves[(half * 3 + 2) * kRows + r] = inverse<NP>(toW);
     asm volatile("bar.sync 1, 256;\n" ::: "memory");
     if (ok) {
       fence_after();
@@ -609,8 +606,8 @@ __global__ void __launch_bounds__(544, 1)
       const float k0 = ref0 == ref ? 1.f : ex2(__fsub_rn(ref0, ref)), k1 = ref1 == ref ? 1.f : ex2(__fsub_rn(ref1, ref));
       l = __fadd_rn(__fmul_rn(l0, k0), __fmul_rn(l1, k1));
       // a row without keys has an O of zeros or none
-      const float inv0 = l == 0.f ? 0.f : __fmul_rn(1.f / 2048.f, __fdiv_rn(__fmul_rn(halves[2 * kRows + r], k0), l));
-      const float inv1 = l == 0.f ? 0.f : __fmul_rn(1.f / 2048.f, __fdiv_rn(__fmul_rn(halves[5 * kRows + r], k1), l));
+      const float inv0 = l == 0.f ? 0.f : __fdiv_rn(__fmul_rn(halves[2 * kRows + r], k0), l);
+      const float inv1 = l == 0.f ? 0.f : __fdiv_rn(__fmul_rn(halves[5 * kRows + r], k1), l);
 #pragma unroll 1
       for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
         uint32_t o[32] = {}, o1[32] = {};

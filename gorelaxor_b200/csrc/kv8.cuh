@@ -104,6 +104,26 @@ __device__ __forceinline__ float lg2(float x) {
 // which W, 1/W and 2^11/W are normal numbers.
 __device__ __forceinline__ int unit_of(float most) { return min(max(int(__float_as_uint(most) >> 23), 12), 253); }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(uint32_t(e) << 23); }  // 2^(e − 127)
+// 1/x of a unit of weights: powers of two for two float16s a weight, exact; for
+// one any number (the largest weight itself is then exact), off by 2^-23.
+template <int NP>
+__device__ __forceinline__ float inverse(float x) {
+  if (NP == 2) return __uint_as_float((254u << 23) - __float_as_uint(x));
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 2^11/W for weights as NP float16s, W being about `most`, the largest weight:
+// that itself for one (which is then exact, as it is where it comes again), the
+// power of two below it for two (whose sums then move exactly). *slack: log2 of
+// 2^4·W, where W moves again.
+template <int NP>
+__device__ __forceinline__ float weight_scale(float most, float* slack) {
+  const float W = fminf(fmaxf(most, 0x1p-115f), 0x1p126f);
+  *slack = __fadd_rn(lg2(W), 4.f);
+  return NP == 1 ? __fmul_rn(2048.f, inverse<1>(W)) : pow2(265 - unit_of(W));
+}
 // Two floats as float16s, lo in the low half.
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t y;
