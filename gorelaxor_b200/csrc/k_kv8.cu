@@ -509,7 +509,7 @@ cudaError_t read_t(const Kv8Args& a, const Kv8Rows& k, const Kv8Rows& v, cudaStr
 // no exchange between lanes.
 //
 // Bound by the arithmetic of the digits and weights: 48 sequences of 1 to
-// 12001 tokens, 4 heads of 128 with 4 queries each, float16: 70 us, 3.4 TB/s
+// 12001 tokens, 4 heads of 128 with 4 queries each, float16: 69 us, 3.4 TB/s
 // of the cache. One sequence of 32768 tokens, 8 heads with 4 queries each:
 // 33 us, 2.0 TB/s, on the 128 blocks that clusters of 16 give.
 
@@ -1101,9 +1101,9 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
 //  * the values' bytes need a 4x4 byte transposition (eight byte
 //    permutations for sixteen bytes) and no conversion.
 // Sums are exact integers until the references move (a larger score, a larger
-// weight) or 32768 keys have gone by; then they go into float32 sums. 256 sequences of 65 to 576 tokens, 16 heads of 64: 38 us,
-// 4.5 TB/s of the cache; sequences of thousands of tokens in such numbers are
-// read at 6.2 to 6.4 TB/s.
+// weight) or 32768 keys have gone by; then they go into float32 sums. 256
+// sequences of 65 to 576 tokens, 16 heads of 64: 38 us, 4.5 TB/s of the cache;
+// as many of 8192 tokens 623 us, 6.9 TB/s, and 64 of 16384 336 us, 6.4 TB/s.
 __device__ __forceinline__ void mma_s8u8(int* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
@@ -1412,14 +1412,15 @@ __global__ void __launch_bounds__(32 * Shape1<D, WU>::warps, Shape1<D, WU>::bloc
 // Blocks and warps for a unit's keys: the stretches that they are cut into
 // give the GPU enough warps, at most `longest` tiles of sixteen keys to one
 // and at least two. With 64 tiles 48 ragged sequences of up to 12001 keys take
-// 70 us, with 32 76, with 20 116: clusters grow that short sequences leave idle.
+// 69 us, with 32 76, with 20 116: clusters grow that short sequences leave idle.
 inline int64_t stretches(const Kv8Args& a, int64_t units, int warps_per_sm, int longest) {
   const int64_t tiles = (std::max(a.max_len, 1) + 15) / 16, most = std::max<int64_t>(1, tiles / 2);
   return std::min(most, std::max((tiles + longest - 1) / longest, (int64_t(kSMs) * warps_per_sm + units - 1) / units));
 }
 // Blocks of `warps` warps to a cluster that shares a unit's keys: as many as
 // the parts ask for, of those that run at once (what
-// cudaOccupancyMaxActiveClusters says of one or two blocks an SM). A second
+// cudaOccupancyMaxActiveClusters says on a B200, the only GPU that this is
+// built for, of blocks of which an SM holds one or two). A second
 // wave costs more than shorter stretches give: 4 sequences of 8192 tokens,
 // 8 heads of 64 with 4 queries each, 36 us on clusters of 16 and 21 of 8.
 inline int blocks_of(int64_t units, int64_t parts, int warps, int per_sm) {
@@ -1469,7 +1470,7 @@ cudaError_t attend_t(const Kv8Args& a, int type, const Kv8Attend& t, cudaStream_
   }
   // several queries: one wave again (16 sequences of 8192 keys, 4 heads, 16
   // queries: 53 us, with clusters of all the parts 101); one query a column,
-  // whose blocks are smaller, gains from more (ragged: 70 us, one wave 123)
+  // whose blocks are smaller, gains from more (ragged: 69 us, one wave 123)
   int S = NQ > 1 ? blocks_of(units, parts, 4, 2) : 1;
   if (NQ == 1)
     while (S < 16 && S * 4 < parts) S *= 2;

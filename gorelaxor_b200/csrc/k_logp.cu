@@ -444,6 +444,12 @@ __global__ void __launch_bounds__(NT, 1536 / NT) k_logp(LogpArgs a, int S) {
 }
 
 // ---- short rows: a warp each, the row in its registers ----
+//
+// The bound is what `top` lanes' largest values reach. From 28 alternatives on
+// the search for it stops at the first bit that all 32 lanes reach, which
+// half of a usual row passes: the list is then too short and the row is scanned
+// `top` times. 24000 rows of 1030 float32 values: 25 us for one alternative, 77
+// for 24, 495 for 28.
 constexpr int kWarpCand = 128, kRowsPerBlock = 8;
 
 template <class T, int NE>

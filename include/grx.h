@@ -145,7 +145,8 @@ typedef struct grx_kv8 {
  *
  * rows bounds the row numbers, max_new a sequence's rows in the call (1 with
  * row0 NULL). max_len is about how long the longest sequence is: it decides
- * how the work is split, and no result depends on it. Rows behind the last
+ * how attention is split and which kernel takes it. The same bounds hold for
+ * its results with any max_len, but not the same last bits. Rows behind the last
  * sequence's are left as they are.
  *
  * The rotation, if rope is given: the pair of values (a, b) of a row at the
