@@ -120,7 +120,8 @@ int grx_linear_q8_static(const grx_weight* w, const float* d_x, int m, const flo
  * token at position p lies in the page table[i·table_width + p/page_tokens]
  * at the slot p % page_tokens; pages of a common beginning may stand in
  * several rows of the table. A page and head has two scales, one for its
- * keys and one for its values, and a byte q stands for q·scale.
+ * keys and one for its values, and a byte q stands for q·scale (scales up to
+ * the largest float32 over 127, which is what appending writes at most).
  *
  * Device memory is the caller's: k and v [pages][kv_heads][page_tokens]
  * [head_dim] int8 from 16-byte boundaries, scale [pages][kv_heads][2]
