@@ -492,11 +492,11 @@ cudaError_t read_t(const Kv8Args& a, const Kv8Rows& k, const Kv8Rows& v, cudaStr
 // w = 2^11·p·s_v/W, with W of each query's own, at least a sixteenth of its
 // largest p·s_v so far: a float16 for 16-bit outputs (off by 2^-12 of itself,
 // half of what a float16 output is rounded by) and the sum of two for float32
-// ones (2^-22), or by 2^-36 W where that is more. So
-// thousands of small weights beside a large one are not lost, and pages of
-// large values that a query hardly looks at cost it nothing. (With W the
-// largest value scale of the sequence and no 2^11 both were: 2e-3 of 32768
-// keys 16.6 nats below another.) A query's maximum and W move together, when
+// ones (2^-22), or by 2^-36 W where that is more. So thousands of small
+// weights beside a large one are not lost, and pages of large values that a
+// query hardly looks at cost it nothing. (With W the largest value scale of
+// the sequence and no 2^11 the one lost 2e-3 of the output, 32768 keys 16.6
+// nats below another, and the other the ratio of the values in bits.) A query's maximum and W move together, when
 // a score passes the one by 2^8 or a weight the other by 2^4.
 //
 // Layout. A warp takes sixteen tokens at a time from a ring of its own in
@@ -1090,12 +1090,12 @@ __global__ void __launch_bounds__(32 * Shape<D, NQ, WU>::warps, Shape<D, NQ, WU>
 //    exponential and one weight a lane for 32 keys;
 //  * the weight, a key's softmax term times its page's value scale, is a
 //    whole number of 2^-32 of a reference W, a power of two above the largest
-//    such product so far and at most twice it; one 8x8 transposition brings its four bytes for all 32
-//    keys to the columns of integer products with the values' bytes
-//    (m16n8k32, unsigned weights): the four keys of a row group in columns of
-//    their own, the bytes 0 and 2 in one product, 1 and 3 in another. So a
-//    weight has all of a float's bits down to 2^-8 of W, and below that half
-//    a step of 2^-33 W: thousands of small ones beside a large one are not
+//    such product so far and at most twice it; one 8x8 transposition brings
+//    its four bytes for all 32 keys to the columns of integer products with
+//    the values' bytes (m16n8k32, unsigned weights): the four keys of a row
+//    group in columns of their own, the bytes 0 and 2 in one product, 1 and 3
+//    in another. So a weight has all of a float's bits down to 2^-8 of W, and
+//    below that it is off by 2^-33 W at most: thousands of small ones beside a large one are not
 //    lost (whole numbers of 2^-23 of the largest value scale lost them, and
 //    what stood beside pages of large values that the query did not look at);
 //  * the values' bytes need a 4x4 byte transposition (eight byte

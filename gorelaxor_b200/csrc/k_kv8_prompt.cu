@@ -17,8 +17,8 @@
 //    row and with a maximum, a sum and an O of their own, joined at the end:
 //    the scores' maximum from TMEM, the scores again, weights 2^11·p·s_v/W,
 //    written back as P, W being the row's own, at least a sixteenth of its
-//    largest p·s_v so far: a weight is off by 2^-12 of itself (2^-22 as the sum of
-//    two), or by 2^-36 W where that is more. The maximum moves only when a
+//    largest p·s_v so far: a weight is off by 2^-12 of itself (2^-22 as the
+//    sum of two), or by 2^-36 W where that is more. The maximum moves only when a
 //    score passes it by 2^8; when a weight passes W by 2^4, the row of O in
 //    TMEM is multiplied. So one half's exponentials run while the other half
 //    waits.
